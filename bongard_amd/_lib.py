@@ -9,7 +9,7 @@ from ctypes import c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p, POINTE
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libbongard_fp8.so")
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 # name -> (restype, argtypes); mirrors include/bongard_fp8.h one to one.
 SIGNATURES = {
@@ -73,6 +73,21 @@ SIGNATURES = {
     "bf8_quantize_mx_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p,
                                      c_void_p, c_void_p, c_void_p]),
     "bf8_gemm_mx_workspace": (c_size_t, [c_int64, c_int64, c_int64]),
+    "bf8_quantize_mxfp4_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p]),
+    "bf8_dequant_mxfp4": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "bf8_gemm_mxfp4_workspace": (c_size_t, [c_int64, c_int64, c_int64]),
+    "bf8_gemm_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                               c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p,
+                               c_size_t, c_void_p]),
+    "bf8_rmsnorm_residual_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                          c_void_p, c_float, c_float, c_int, c_void_p, c_void_p,
+                                          c_void_p]),
+    "bf8_rmsnorm_residual_bwd_workspace": (c_size_t, [c_int64, c_int64]),
+    "bf8_rmsnorm_residual_bwd_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                              c_int64, c_void_p, c_void_p, c_void_p, c_float,
+                                              c_float, c_int, c_void_p, c_void_p, c_void_p,
+                                              c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "bf8_quantize_nvfp4_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_void_p]),
     "bf8_quantize_nvfp4_partials_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64,

@@ -29,10 +29,10 @@ import torch
 from . import linear as _linear
 from . import ops as _ops
 from . import scaling as _scaling
-from .te_linear import (RECIPES, _is_blocked, _is_mx, _is_nvfp4, _make_recipe, _new_scaling,
-                        _pad_rows, _ScalingExtraState, present)
+from .te_linear import (RECIPES, _is_blocked, _is_mx, _is_mxfp4, _is_nvfp4, _make_recipe,
+                        _new_scaling, _pad_rows, _ScalingExtraState, present)
 
-__all__ = ["RECIPES", "FusedMLP", "enable_fused_mlp", "hf_state_dict"]
+__all__ = ["RECIPES", "FusedMLP", "enable_fused_mlp", "hf_state_dict", "residual_norm"]
 
 
 def _rms_norm(x, weight, eps):
@@ -61,6 +61,43 @@ class _FusedRMSNorm(torch.autograd.Function):
                                        need_dx=ctx.needs_input_grad[0],
                                        need_dw=ctx.needs_input_grad[1])
         return dx, dw, None, None
+
+
+class _ResidualNorm(torch.autograd.Function):
+    """The kernels behind :func:`residual_norm`."""
+
+    @staticmethod
+    def forward(ctx, h, residual, post_weight, pre_weight, gate, eps, residual_scale):
+        out, y = _ops.rmsnorm_residual(h, residual, post_weight, pre_weight, eps, gate=gate,
+                                       residual_scale=residual_scale, zero_centered=True)
+        ctx.eps, ctx.residual_scale = eps, residual_scale
+        ctx.save_for_backward(h, out, post_weight, pre_weight, gate)
+        ctx.set_materialize_grads(False)
+        return out, y
+
+    @staticmethod
+    def backward(ctx, dout, dy):
+        h, out, post_weight, pre_weight, gate = ctx.saved_tensors
+        if dout is None and dy is None:
+            return (None,) * 7
+        grads = _ops.rmsnorm_residual_backward(
+            h, out, dout, dy, post_weight, pre_weight, ctx.eps, gate=gate,
+            residual_scale=ctx.residual_scale, zero_centered=True,
+            needs=ctx.needs_input_grad[:5])
+        return (*grads, None, None)
+
+
+@torch.compiler.disable
+def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
+                  residual_scale=1.0):
+    """What a T5Gemma2 layer does between two blocks, in one kernel each way: the post-block norm
+    of ``h`` (zero-centred ``post_weight``), its addition to ``residual`` and the pre-block norm
+    (``pre_weight``) of the sum. bf16 [..., hidden] tensors; returns ``(the new residual, the
+    next block's input)``, differentiable in every tensor. ``gate`` (bf16 [hidden]) multiplies
+    the normed h, ``residual_scale`` (a number) the old residual. The sum is formed in fp32 and
+    rounded to bf16 once; the second norm is that of the rounded sum."""
+    return _ResidualNorm.apply(h, residual, post_weight, pre_weight, gate, float(eps),
+                               float(residual_scale))
 
 
 class FusedMLP(_ScalingExtraState, torch.nn.Module):
@@ -142,8 +179,12 @@ class FusedMLP(_ScalingExtraState, torch.nn.Module):
         mx = _is_mx(self.recipe)
         if _is_nvfp4(self.recipe):
             return self._nvfp4_forward(x, flat, length, first)
+        mxfp4 = _is_mxfp4(self.recipe)
         if first:
-            if mx:
+            if mxfp4:
+                self._fp8_weights = (_linear.quantize_weight_mxfp4(self.fc1_weight),
+                                     _linear.quantize_weight_mxfp4(self.fc2_weight))
+            elif mx:
                 self._fp8_weights = (_linear.quantize_weight_mx(self.fc1_weight, scale_rows=False),
                                      _linear.quantize_weight_mx(self.fc2_weight, scale_rows=False))
             elif fc1 is not None:
@@ -159,7 +200,7 @@ class FusedMLP(_ScalingExtraState, torch.nn.Module):
                     _linear.quantize_weight(self.fc2_weight))
         gu_q, down_q = self._fp8_weights
         flat = _linear.dense_rows(flat.to(torch.bfloat16))
-        if mx:
+        if mx or mxfp4:
             # block scales need no tensor-wide amax: the norm's partials go unused
             if _ops.rmsnorm_supported(flat.shape[1]):
                 parts = torch.empty(_ops.rmsnorm_partials_count(flat.shape[0]),
@@ -167,8 +208,9 @@ class FusedMLP(_ScalingExtraState, torch.nn.Module):
                 normed = _FusedRMSNorm.apply(flat, self.layer_norm_weight, self.eps, parts)
             else:
                 normed = _rms_norm(flat, self.layer_norm_weight, self.eps)
-            out = _linear.Fp8GegluMlpMxFunction.apply(normed, self.fc1_weight, self.fc2_weight,
-                                                      gu_q, down_q, self.intermediate_size)
+            mlp = _linear.Mxfp4GegluMlpFunction if mxfp4 else _linear.Fp8GegluMlpMxFunction
+            out = mlp.apply(normed, self.fc1_weight, self.fc2_weight, gu_q, down_q,
+                            self.intermediate_size)
             # sliced only if padded: a slice's backward fills and copies the whole gradient
             return (out if length == flat.shape[0] else out[:length]).reshape_as(x)
         count = _ops.rmsnorm_partials_count(flat.shape[0])

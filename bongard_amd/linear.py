@@ -496,6 +496,104 @@ class Fp8GegluMlpMxFunction(_Fp8Function):
         return dx, dgu, dd, None, None, None
 
 
+def quantize_weight_mxfp4(weight, *, transpose=True):
+    """MXFP4 copy of a weight [N, K]: blocks along K (forward), and with ``transpose`` the
+    columnwise copy with blocks along N (the input-gradient GEMM's operand)."""
+    return ops.quantize_mxfp4(dense_rows(weight.detach()), rowwise=True, colwise=transpose)
+
+
+def _check_mxfp4(who, *dims):
+    bad = [d for d in dims if d % 32]
+    if bad:
+        raise ValueError(f"{who}: MXFP4 blocks need feature sizes that are multiples of 32 "
+                         f"(got {list(dims)})")
+
+
+class Mxfp4LinearFunction(_Fp8Function):
+    """y = x @ W^T with every tensor in MXFP4 (e2m1 codes in blocks of 32 under a power of two,
+    gradients included; round to nearest even) on the FP4 MFMA; x: bf16 [M, K], any M; W [N, K],
+    K a multiple of 32, N of 8 (of 32 for gradients). ``wq``: a cached MXFP4 weight
+    (:func:`quantize_weight_mxfp4`) or None.
+
+      forward  y  = X4 . W4^T           blocks along K on both
+      dgrad    dX = dY4 . (W^T)4^T      dY blocks along N, W's columnwise copy
+      wgrad    dW = (dY^T)4 . (X^T)4^T  columnwise copies of dY and X (blocks along M, the last
+                                        one filled up with zeros)
+
+    Beside the 4-bit recipe of bongard/te_linear.py:17,38 (NVFP4, whose blocks gfx950 has no MFMA
+    for); the reference has no counterpart."""
+
+    @staticmethod
+    def forward(ctx, x, weight, wq):
+        need_dx, need_dw = _forward_needs(ctx, 2)
+        _check_mxfp4("mxfp4 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
+        xq = ops.quantize_mxfp4(dense_rows(x), rowwise=True, colwise=need_dw)
+        if wq is None or (need_dx and wq.data_t is None):
+            wq = quantize_weight_mxfp4(weight, transpose=need_dx)
+        y = ops.gemm_mxfp4(xq.data, xq.planes, wq.data, wq.planes)
+        ctx.save_for_backward(xq.data_t, xq.planes_t, wq.data_t if need_dx else None,
+                              wq.planes_t if need_dx else None)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x4t, xpt, w4t, wpt = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        dyq = ops.quantize_mxfp4(dense_rows(dy), rowwise=need_dx, colwise=need_dw)
+        dx = dw = None
+        if need_dx:
+            dx = ops.gemm_mxfp4(dyq.data, dyq.planes, w4t, wpt)
+        if need_dw:
+            dw = ops.gemm_mxfp4(dyq.data_t, dyq.planes_t, x4t, xpt)
+        return dx, dw, None
+
+
+class Mxfp4GegluMlpFunction(_Fp8Function):
+    """The gated MLP of :class:`Fp8GegluMlpFunction` with every tensor in MXFP4: the gate/up
+    product with the gated GELU and H's quantization, the down product; backward through dH, the
+    gelu chain's dGU and the dgrad/wgrad products on the columnwise copies. x: bf16 [M, K], any
+    M; w_gu [2I, K], w_down [K_out, I], K and K_out multiples of 32, I of 128. ``gu_q`` /
+    ``down_q``: optional cached MXFP4 weights. TEMLP / FusedMLP under 'mxfp4'
+    (bongard/te_linear.py:98-103, bongard/fused_mlp.py:25-33 for the chain)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gu, w_down, gu_q, down_q, intermediate):
+        I = int(intermediate)
+        need_dx, need_dgu, need_dd = _forward_needs(ctx, 3)
+        train = need_dx or need_dgu or need_dd
+        _check_mxfp4("mxfp4 gated MLP", x.shape[-1], *([w_down.shape[0]] if train else []))
+        xq = ops.quantize_mxfp4(dense_rows(x), rowwise=True, colwise=need_dgu)
+        if gu_q is None or (need_dx and gu_q.data_t is None):
+            gu_q = quantize_weight_mxfp4(w_gu, transpose=need_dx)
+        hq, GU = ops.gemm_geglu_mxfp4(xq.data, xq.planes, gu_q.data, gu_q.planes, I,
+                                      colwise=need_dd, keep_gu=need_dx or need_dgu)
+        if down_q is None or ((need_dx or need_dgu) and down_q.data_t is None):
+            down_q = quantize_weight_mxfp4(w_down, transpose=need_dx or need_dgu)
+        y = ops.gemm_mxfp4(hq.data, hq.planes, down_q.data, down_q.planes)
+        keep = need_dx or need_dgu
+        ctx.save_for_backward(GU, xq.data_t, xq.planes_t, hq.data_t, hq.planes_t,
+                              gu_q.data_t if need_dx else None, gu_q.planes_t if need_dx else None,
+                              down_q.data_t if keep else None, down_q.planes_t if keep else None)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        GU, x4t, xpt, h4t, hpt, gu4t, gupt, d4t, dpt = ctx.saved_tensors
+        need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]
+        dyq = ops.quantize_mxfp4(dense_rows(dy), rowwise=need_dx or need_dgu, colwise=need_dd)
+        dx = dgu = dd = None
+        if need_dd:
+            dd = ops.gemm_mxfp4(dyq.data_t, dyq.planes_t, h4t, hpt)
+        if need_dx or need_dgu:
+            dH = ops.gemm_mxfp4(dyq.data, dyq.planes, d4t, dpt)
+            dq = ops.geglu_bwd_mxfp4(dH, GU, rowwise=need_dx, colwise=need_dgu)
+            if need_dx:
+                dx = ops.gemm_mxfp4(dq.data, dq.planes, gu4t, gupt)
+            if need_dgu:
+                dgu = ops.gemm_mxfp4(dq.data_t, dq.planes_t, x4t, xpt)
+        return dx, dgu, dd, None, None, None
+
+
 def mlp_forward(x, w_gu, w_down, gu_q, down_q, intermediate, split_scales, scaling, x_amax,
                 needs):
     """Forward of the FP8 gated MLP (see Fp8GegluMlpFunction): ``(y, saved)`` with saved =

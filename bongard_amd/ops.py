@@ -1256,3 +1256,279 @@ def gemm_nvfp4(a_data, a_scales, a_meta, b_data, b_scales, b_meta, *, out_dtype=
     a = a_deq if a_deq is not None else dequant_nvfp4(a_data, a_scales)
     b = b_deq if b_deq is not None else dequant_nvfp4(b_data, b_scales)
     return gemm_bf16(a, b, a_meta[2:3], b_meta[2:3], out_dtype=out_dtype)
+
+
+# ---- MXFP4: e2m1 codes in blocks of 32 under a power of two ---------------------------------
+def _one_device(who, *tensors):
+    """The HIP device of the tensors (None among them is skipped), which must be one."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        _require_gpu(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{who}: tensors on different devices ({dev} and {t.device})")
+    return dev
+
+
+class _On:
+    """Makes ``device`` the current one for a call where it is not (launches go to the current
+    device; the caller's stream of ``device`` is what they are queued on)."""
+
+    __slots__ = ("idx", "prev")
+
+    def __init__(self, device):
+        self.idx = device.index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.idx is not None and self.prev != self.idx:
+            torch.cuda.set_device(self.idx)
+
+    def __exit__(self, *exc):
+        if self.idx is not None and self.prev != self.idx:
+            torch.cuda.set_device(self.prev)
+
+
+def _call_workspace(nbytes, device):
+    """``(workspace or None, its bytes)`` of a call: the stream's shared one, or while a graph is
+    captured one of the graph's own (two graphs captured on a stream may replay side by side)."""
+    if not nbytes:
+        return None, 0
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    else:
+        ws = gemm_workspace(nbytes, device)
+    return ws, ws.numel()
+
+
+def _aligned(t):
+    """``t`` on 16-byte alignment: copied where a view starts off it."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@dataclass
+class Mxfp4Tensor:
+    """An MXFP4 tensor of x [rows, cols] (32-element blocks of e2m1 codes under one E8M0 scale):
+    ``data`` uint8 [rows, cols / 2] (two codes a byte, the even element in the low nibble) with
+    ``planes`` int32 [ceil(cols / 128), rows] (blocks along rows), and/or ``data_t`` uint8
+    [cols, R / 2] with ``planes_t`` int32 [ceil(rows / 128), cols] (blocks along columns of x,
+    stored transposed; R is ``rows`` rounded up to 32, the codes past ``rows`` 0). A plane holds
+    a dword of four scale bytes for every row."""
+
+    data: Optional[torch.Tensor]
+    planes: Optional[torch.Tensor]
+    data_t: Optional[torch.Tensor]
+    planes_t: Optional[torch.Tensor]
+    rows: int
+    cols: int
+
+
+def _new_mxfp4(rows, cols, rowwise, colwise, device):
+    out = pl = out_t = pl_t = None
+    if rowwise:
+        if cols % 32:
+            raise ValueError(f"MXFP4 blocks along rows need cols % 32 == 0 (got {cols})")
+        out = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
+        pl = _new_planes(cols, rows, device)
+    if colwise:
+        out_t = torch.empty((cols, (rows + 31) // 32 * 16), dtype=torch.uint8, device=device)
+        pl_t = _new_planes(rows, cols, device)
+    return Mxfp4Tensor(out, pl, out_t, pl_t, rows, cols)
+
+
+def quantize_mxfp4(x, *, rowwise=True, colwise=False):
+    """MXFP4 quantization of a bf16 tensor (flattened to [rows, cols]) as a :class:`Mxfp4Tensor`:
+    per block of 32 the smallest power of two s with max|x| <= 6 s, the values x / s rounded to
+    the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code). ``rowwise``: blocks
+    along rows (cols a multiple of 32); ``colwise``: along columns, any number of rows (cols a
+    multiple of 8). Both copies come from one pass over x."""
+    who = "quantize_mxfp4"
+    dev = _one_device(who, x)
+    x = _aligned(_bf16_2d(x))
+    rows, cols = x.shape
+    if not (rowwise or colwise):
+        raise ValueError(f"{who}: nothing requested")
+    q = _new_mxfp4(rows, cols, rowwise, colwise, dev)
+    if not x.numel():
+        return q
+    with _On(dev):
+        _lib.check(_lib.lib().bf8_quantize_mxfp4_bf16(
+            _ptr(x), rows, cols, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t), _ptr(q.planes_t),
+            _stream(dev)), "bf8_quantize_mxfp4_bf16")
+    return q
+
+
+def _mxfp4_operand(who, name, codes, planes, rows=None):
+    """Checks an MXFP4 operand [rows, K] and returns (rows, K)."""
+    if codes.dtype != torch.uint8:
+        raise TypeError(f"{who}: {name} must be uint8 codes (got {codes.dtype})")
+    _byte_matrix(who, **{name: codes})
+    R, K = codes.shape[0], 2 * codes.shape[1]
+    if rows is not None and R != rows:
+        raise ValueError(f"{who}: {name} must have {rows} rows (got {R})")
+    _mx_planes(who, {f"{name}_planes": R}, K, **{f"{name}_planes": planes})
+    return R, K
+
+
+def dequant_mxfp4(q, *, transpose=False):
+    """The values of a :class:`Mxfp4Tensor` as bf16 [rows, cols], or with ``transpose`` those of
+    its columnwise copy, [cols, rows] (a view of rows padded to 32 where rows is not a multiple).
+    Exact: a code times its block's power of two is a bf16 value."""
+    who = "dequant_mxfp4"
+    codes, planes = (q.data_t, q.planes_t) if transpose else (q.data, q.planes)
+    if codes is None:
+        raise ValueError(f"{who}: the tensor has no {'columnwise' if transpose else 'rowwise'} copy")
+    dev = _one_device(who, codes, planes)
+    rows, cols = _mxfp4_operand(who, "codes", codes, planes)
+    codes = codes.contiguous()
+    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=dev)
+    with _On(dev):
+        _lib.check(_lib.lib().bf8_dequant_mxfp4(_ptr(codes), _ptr(planes), rows, cols, _ptr(out),
+                                                _stream(dev)), "bf8_dequant_mxfp4")
+    return out[:, :q.rows] if transpose and q.rows != cols else out
+
+
+@functools.lru_cache(maxsize=4096)
+def _gemm_mxfp4_ws_cached(M, N, K, override):
+    return int(_lib.lib().bf8_gemm_mxfp4_workspace(M, N, K))
+
+
+def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16, out=None):
+    """``C = A @ B.T (+ bias)`` of MXFP4 operands A [M, K] and B [N, K] (codes and scale planes as
+    :func:`quantize_mxfp4` writes them) on the block-scaled FP4 MFMA, sums in fp32."""
+    who = "gemm_mxfp4"
+    dev = _one_device(who, a, a_planes, b, b_planes, bias, out)
+    M, K = _mxfp4_operand(who, "a", a, a_planes)
+    N, Kb = _mxfp4_operand(who, "b", b, b_planes)
+    if K != Kb:
+        raise ValueError(f"{who}: inner dims differ ({K} vs {Kb})")
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"{who}: out_dtype must be bfloat16 or float32")
+    if out is None:
+        out = torch.empty((M, N), dtype=out_dtype, device=dev)
+    _out_matrix(who, out, (M, N), out_dtype)
+    if bias is not None:
+        if bias.dtype != torch.bfloat16 or bias.numel() != N:
+            raise ValueError(f"{who}: bias must be bfloat16 [{N}] (got {bias.dtype} {tuple(bias.shape)})")
+        bias = _aligned(bias.contiguous())
+    if K == 0:  # an empty sum
+        return out.zero_() if bias is None else out.copy_(bias.expand(M, N))
+    ws, ws_bytes = _call_workspace(_gemm_mxfp4_ws_cached(M, N, K, _tile_override()), dev)
+    with _On(dev):
+        _lib.check(_lib.lib().bf8_gemm_mxfp4(
+            _ptr(a), a.stride(0), _ptr(a_planes), _ptr(b), b.stride(0), _ptr(b_planes), M, N, K,
+            _ptr(bias), _ptr(out), OUT_BF16 if out_dtype == torch.bfloat16 else OUT_F32,
+            out.stride(0), _ptr(ws), ws_bytes, _stream(dev)), "bf8_gemm_mxfp4")
+    return out
+
+
+def gemm_geglu_mxfp4(x, x_planes, w, w_planes, intermediate, *, colwise=False, keep_gu=False):
+    """Gate/up product of MXFP4 operands X [M, K] and W [2I, K] (gate rows then up rows) with the
+    gated GELU: ``(hq, GU or None)``, ``hq`` the :class:`Mxfp4Tensor` of H = gelu_tanh(gate) *
+    up [M, I] (gate, up, the activation and H rounded to bf16, as :func:`geglu` does; with
+    ``colwise`` the columnwise copy as well) and ``GU`` the bf16 pre-activations when
+    ``keep_gu``. I must be a multiple of 128."""
+    who = "gemm_geglu_mxfp4"
+    dev = _one_device(who, x, x_planes, w, w_planes)
+    I = int(intermediate)
+    M, K = _mxfp4_operand(who, "x", x, x_planes)
+    _, Kw = _mxfp4_operand(who, "w", w, w_planes, 2 * I)
+    if K != Kw:
+        raise ValueError(f"{who}: inner dims differ ({K} vs {Kw})")
+    if I % 128:
+        raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
+    GU = gemm_mxfp4(x, x_planes, w, w_planes)
+    with _On(dev):
+        H, _ = geglu(GU)
+    return quantize_mxfp4(H, colwise=colwise), GU if keep_gu else None
+
+
+def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
+    """:func:`geglu_bwd` and the :func:`quantize_mxfp4` of its dGU [M, 2I]."""
+    dev = _one_device("geglu_bwd_mxfp4", dH, GU)
+    with _On(dev):
+        dGU, _ = geglu_bwd(dH, GU)
+    return quantize_mxfp4(dGU, rowwise=rowwise, colwise=colwise)
+
+
+# ---- the norms on either side of a residual connection ---------------------------------------
+RESIDUAL_NORM_MAX_COLS = 16384
+
+
+def _residual_norm_args(who, rows_of, post_weight, pre_weight, gate):
+    """The row tensors (None kept) as contiguous 2-D bf16 of one shape and the weights, checked."""
+    dev = _one_device(who, *rows_of.values(), post_weight, pre_weight, gate)
+    shape, rows = None, {}
+    for name, t in rows_of.items():
+        if t is not None:
+            if shape is not None and tuple(t.shape) != shape:
+                raise ValueError(f"{who}: {name} must be {shape} (got {tuple(t.shape)})")
+            shape = tuple(t.shape)
+            t = _aligned(_bf16_2d(t))
+        rows[name] = t
+    cols = shape[-1]
+    weights = []
+    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("gate", gate)):
+        if t is not None:
+            if t.dtype != torch.bfloat16 or tuple(t.shape) != (cols,):
+                raise ValueError(f"{who}: {name} must be bf16 [{cols}] (got {t.dtype} {tuple(t.shape)})")
+            t = _aligned(t.contiguous())
+        weights.append(t)
+    return dev, shape, rows, weights
+
+
+def rmsnorm_residual(h, residual, post_weight, pre_weight, eps, *, gate=None, residual_scale=1.0,
+                     zero_centered=True):
+    """The norm of a block's output ``h``, its addition to the residual stream and the norm of the
+    sum for the next block, in one kernel (bf16 tensors [..., cols], fp32 arithmetic):
+    ``out = residual_scale * residual + gate * rmsnorm(h, post_weight)`` and
+    ``y = rmsnorm(out, pre_weight)``; returns ``(out, y)``. ``gate``: bf16 [cols] or None (1)."""
+    who = "rmsnorm_residual"
+    dev, shape, t, (post, pre, gate) = _residual_norm_args(
+        who, {"h": h, "residual": residual}, post_weight, pre_weight, gate)
+    h, residual = t["h"], t["residual"]
+    rows, cols = h.shape
+    out, y = torch.empty_like(h), torch.empty_like(h)
+    with _On(dev):
+        _lib.check(_lib.lib().bf8_rmsnorm_residual_bf16(
+            _ptr(h), _ptr(residual), rows, cols, _ptr(post), _ptr(pre), _ptr(gate),
+            float(residual_scale), float(eps), int(bool(zero_centered)), _ptr(out), _ptr(y),
+            _stream(dev)), "bf8_rmsnorm_residual_bf16")
+    return out.reshape(shape), y.reshape(shape)
+
+
+def rmsnorm_residual_backward(h, out, dout, dy, post_weight, pre_weight, eps, *, gate=None,
+                              residual_scale=1.0, zero_centered=True,
+                              needs=(True, True, True, True, True)):
+    """Gradients ``(dh, dresidual, dpost, dpre, dgate)`` of :func:`rmsnorm_residual` from its ``h``
+    and ``out`` and the gradients ``dout`` and ``dy`` of its results (one of them may be None: zero).
+    ``needs``: which to compute (the others are None; ``dgate`` is None without a gate)."""
+    who = "rmsnorm_residual_backward"
+    if dout is None and dy is None:
+        raise ValueError(f"{who}: no gradient given")
+    dev, shape, t, (post, pre, gate) = _residual_norm_args(
+        who, {"h": h, "out": out, "dout": dout, "dy": dy}, post_weight, pre_weight, gate)
+    h, out, dout, dy = t["h"], t["out"], t["dout"], t["dy"]
+    rows, cols = h.shape
+    needs = tuple(needs[:4]) + (bool(needs[4]) and gate is not None,)
+    grads = [torch.empty_like(h) if n else None for n in needs[:2]]
+    grads += [torch.empty(cols, dtype=torch.bfloat16, device=dev) if n else None for n in needs[2:]]
+    if any(needs):
+        if rows == 0:
+            for g in grads[2:]:
+                if g is not None:
+                    g.zero_()
+        else:
+            L = _lib.lib()
+            nbytes = int(L.bf8_rmsnorm_residual_bwd_workspace(rows, cols)) if any(needs[2:]) else 0
+            ws, nbytes = _call_workspace(nbytes, dev)
+            with _On(dev):
+                _lib.check(L.bf8_rmsnorm_residual_bwd_bf16(
+                    _ptr(h), _ptr(out), _ptr(dout), _ptr(dy), rows, cols, _ptr(post), _ptr(pre),
+                    _ptr(gate), float(residual_scale), float(eps), int(bool(zero_centered)),
+                    *[_ptr(g) for g in grads], _ptr(ws), nbytes, _stream(dev)),
+                    "bf8_rmsnorm_residual_bwd_bf16")
+    return tuple(g.reshape(shape) if g is not None and i < 2 else g for i, g in enumerate(grads))

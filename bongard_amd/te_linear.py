@@ -28,7 +28,10 @@ Hadamard transform, stochastic rounding and 2-D weight blocks are not built). gf
 MFMA for e4m3-scaled FP4 blocks, so the blocks are dequantized exactly to bf16 and multiplied
 on the bf16 MFMA (bongard_amd.linear.Fp8LinearNvfp4Function), the gated GELU in the fused
 gate_up GEMM's epilogue (GegluGateUpNvfp4Function; the split projections use the elementwise
-GegluFunction); stateless, like 'mxfp8'.
+GegluFunction); stateless, like 'mxfp8'. 'mxfp4' (an addition to the reference's names) is the
+4-bit format that gfx950 multiplies itself: every tensor in e2m1 blocks of 32 under a power of
+two, round to nearest even (bongard_amd.linear.Mxfp4LinearFunction / Mxfp4GegluMlpFunction), any
+number of rows unpadded; stateless.
 """
 
 import os
@@ -42,7 +45,7 @@ from . import linear as _linear
 from . import scaling as _scaling
 from .scaling import LinearScaling
 
-RECIPES = ('nvfp4', 'mxfp8', 'fp8', 'fp8_delayed')
+RECIPES = ('nvfp4', 'mxfp8', 'fp8', 'fp8_delayed', 'mxfp4')
 ATTENTION_PROJECTIONS = ('q_proj', 'k_proj', 'v_proj', 'o_proj')
 
 
@@ -80,6 +83,15 @@ class NVFP4BlockScaling:
     block_size: int = 16
 
 
+@dataclass(frozen=True)
+class MXFP4BlockScaling:
+    """OCP MXFP4: e2m1 values in 32-element blocks with E8M0 scales, for every tensor (round to
+    nearest even; no Hadamard transform, no stochastic rounding)."""
+
+    fp4_format: str = "E2M1"
+    block_size: int = 32
+
+
 def _make_recipe(name):
     if name == 'fp8':
         return Float8CurrentScaling()
@@ -89,6 +101,8 @@ def _make_recipe(name):
         return MXFP8BlockScaling()
     if name == 'nvfp4':
         return NVFP4BlockScaling()
+    if name == 'mxfp4':
+        return MXFP4BlockScaling()
     raise ValueError(f'TE recipe must be one of {RECIPES}')
 
 
@@ -100,8 +114,13 @@ def _is_nvfp4(recipe):
     return isinstance(recipe, NVFP4BlockScaling)
 
 
+def _is_mxfp4(recipe):
+    return isinstance(recipe, MXFP4BlockScaling)
+
+
 def _is_blocked(recipe):
-    """Whether a recipe quantizes blocks along the rows (the columnwise copies)."""
+    """Whether a recipe's kernels need whole blocks of 32 rows (the columnwise copies; MXFP4's
+    quantizer fills up the last block itself)."""
     return _is_mx(recipe) or _is_nvfp4(recipe)
 
 
@@ -203,6 +222,8 @@ class TELinear(_ScalingExtraState, torch.nn.Module):
             elif _is_nvfp4(self.recipe):
                 q = _linear.quantize_weight_nvfp4(self.weight, transpose=True,
                                                   cache_dequant=is_first_microbatch is not None)
+            elif _is_mxfp4(self.recipe):
+                q = _linear.quantize_weight_mxfp4(self.weight, transpose=True)
             else:
                 q = _linear.quantize_weight(self.weight,
                                             scaler=self.scaling and self.scaling.weight)
@@ -257,6 +278,9 @@ class TELinear(_ScalingExtraState, torch.nn.Module):
             out = _linear.Fp8LinearNvfp4Function.apply(flat, self.weight,
                                                        self.fp8_weight(first_microbatch),
                                                        x_partials)
+        elif _is_mxfp4(self.recipe):
+            out = _linear.Mxfp4LinearFunction.apply(flat, self.weight,
+                                                    self.fp8_weight(first_microbatch))
         else:
             out = _linear.Fp8LinearFunction.apply(flat, self.weight, None,
                                                   self.fp8_weight(first_microbatch), self.scaling)
@@ -327,7 +351,7 @@ class TEMLP(torch.nn.Module):
                                          first or self.gate_up._fp8_weight is None,
                                          down_first or self.down._fp8_weight is None)
         down_q = self.down.fp8_weight(down_first)
-        if _is_mx(self.down.recipe):
+        if _is_mx(self.down.recipe) or _is_mxfp4(self.down.recipe):
             return self._mx_forward(x, flat, length, aligned, down_q)
         if self.fused_gate_up:
             first = self.gate_up._note_microbatch()
@@ -381,24 +405,28 @@ class TEMLP(torch.nn.Module):
         return out.reshape(*x.shape[:-1], out.shape[-1])
 
     def _mx_forward(self, x, flat, length, aligned, down_q):
-        """MXFP8: blocks along K never straddle gate and up rows, so the stacked weight's
-        MX copy is the two projections' copies side by side (fused or split alike)."""
+        """MXFP8 and MXFP4: blocks along K never straddle gate and up rows, so the stacked
+        weight's copy is the two projections' copies side by side (fused or split alike)."""
         I = self.intermediate_size
+        mxfp4 = _is_mxfp4(self.down.recipe)
         if self.fused_gate_up:
             first = self.gate_up._note_microbatch()
             if first or self.gate_up._fp8_weight is None:
-                self.gate_up._fp8_weight = _linear.quantize_weight_mx(self.gate_up.weight)
+                self.gate_up._fp8_weight = (_linear.quantize_weight_mxfp4 if mxfp4 else
+                                            _linear.quantize_weight_mx)(self.gate_up.weight)
             gu_q = self.gate_up._fp8_weight
             w_gu = self.gate_up.weight
         else:
             first_g = self.gate_proj._note_microbatch()
             first_u = self.up_proj._note_microbatch()
             if first_g or first_u or self._split_cache is None:
-                self._split_cache = _linear.quantize_weight_mx(
-                    torch.cat([self.gate_proj.weight, self.up_proj.weight], 0), scale_rows=False)
+                stacked = torch.cat([self.gate_proj.weight, self.up_proj.weight], 0)
+                self._split_cache = (_linear.quantize_weight_mxfp4(stacked) if mxfp4 else
+                                     _linear.quantize_weight_mx(stacked, scale_rows=False))
             gu_q = self._split_cache
             w_gu = _SplitGateUp.apply(self.gate_proj.weight, self.up_proj.weight)
-        out = _linear.Fp8GegluMlpMxFunction.apply(flat, w_gu, self.down.weight, gu_q, down_q, I)
+        mlp = _linear.Mxfp4GegluMlpFunction if mxfp4 else _linear.Fp8GegluMlpMxFunction
+        out = mlp.apply(flat, w_gu, self.down.weight, gu_q, down_q, I)
         if aligned != length:
             out = out[:length]
         return out.reshape(*x.shape[:-1], out.shape[-1])

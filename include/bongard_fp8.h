@@ -540,6 +540,65 @@ int bf8_gemm_geglu_mx_planes(const uint8_t* X, int64_t ldx, const uint32_t* X_pl
                              uint32_t* H8_planes, uint8_t* H8t, uint32_t* H8t_planes, void* GU,
                              void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * MXFP4: 32-element blocks of e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6; sign in bit 3; two codes a
+ * byte, the even element in the low nibble) under one E8M0 scale, the 4-bit format whose product
+ * gfx950 has an MFMA for. Beside the 4-bit recipe of bongard/te_linear.py:17,38 ('nvfp4', whose
+ * e4m3 scales per 16 values the MFMA does not take); the reference has no counterpart.
+ * Per block: 2^(e - 127) is the smallest power of two with max |x| <= 6 * 2^(e - 127) (e >= 0; a
+ * block that holds inf: e = 254; NaN: e = 255, codes 0), code = e2m1(x * 2^(127 - e)), to
+ * nearest, ties to the even code. Scales lie in planes, uint32 [(K + 127) / 128][rows]: plane g
+ * holds the bytes of blocks 4 g .. 4 g + 3 of every row (absent blocks 127).
+ * ------------------------------------------------------------------------------- */
+
+/* x: bf16 [rows, cols], cols % 8 == 0. out [rows, cols / 2] with out_planes: blocks along rows,
+ * cols % 32 == 0. out_t [cols, R / 2] with out_t_planes [(rows + 127) / 128][cols]: blocks
+ * along columns, stored transposed, R = rows rounded up to 32 and the codes past rows 0. Either
+ * pair may be NULL (not both). x and out_t 16-byte, the others 4-byte aligned. */
+int bf8_quantize_mxfp4_bf16(const void* x, int64_t rows, int64_t cols, uint8_t* out,
+                            uint32_t* out_planes, uint8_t* out_t, uint32_t* out_t_planes,
+                            void* stream);
+
+/* out: bf16 [rows, cols] = e2m1(code) * 2^(e - 127), exact (inf past bf16's range, NaN where e =
+ * 255); cols % 32 == 0. */
+int bf8_dequant_mxfp4(const uint8_t* codes, const uint32_t* planes, int64_t rows, int64_t cols,
+                      void* out, void* stream);
+
+/* C [M, N] = A . B^T (+ bias[n]) on MXFP4 operands A [M, K], B [N, K] (row strides lda, ldb in
+ * bytes, multiples of 16), sums in fp32; K % 32 == 0, N % 8 == 0, ldc % 4 == 0. ws:
+ * bf8_gemm_mxfp4_workspace(M, N, K) bytes, 256-byte aligned, or fewer (a slower plan). */
+size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
+int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
+                   int64_t ldb, const uint32_t* B_planes, int64_t M, int64_t N, int64_t K,
+                   const void* bias, void* C, int out_dtype, int64_t ldc, void* ws,
+                   size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * The norms on either side of a residual connection in one kernel (HF T5Gemma2's layer:
+ * post-block norm, addition, pre-block norm of the next block; the two norms around
+ * bongard/te_linear.py's and bongard/fused_mlp.py:84-98's converted modules). Per row, in fp32:
+ *   out = bf16(residual_scale * residual + gate * (h / rms(h)) * (z + post)),
+ *   y   = bf16((out / rms(out)) * (z + pre)),    rms(v) = sqrt(mean(v^2) + eps)
+ * z = 1 when zero_centered, else 0; gate bf16 [cols] or NULL (1). All tensors bf16 and 16-byte
+ * aligned, [rows, cols] row-major, cols % 8 == 0 and <= 16384; post, pre [cols].
+ * ------------------------------------------------------------------------------- */
+int bf8_rmsnorm_residual_bf16(const void* h, const void* residual, int64_t rows, int64_t cols,
+                              const void* post, const void* pre, const void* gate,
+                              float residual_scale, float eps, int zero_centered, void* out,
+                              void* y, void* stream);
+
+/* Its backward from the forward's h and out: gradients dout and dy of out and y (either may be
+ * NULL: zero). dh, dresidual [rows, cols], dpost, dpre, dgate [cols], each optional (at least
+ * one); the last three need ws: bf8_rmsnorm_residual_bwd_workspace(rows, cols) bytes of block
+ * partials, added in a fixed order. rows > 0. */
+size_t bf8_rmsnorm_residual_bwd_workspace(int64_t rows, int64_t cols);
+int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* dout, const void* dy,
+                                  int64_t rows, int64_t cols, const void* post, const void* pre,
+                                  const void* gate, float residual_scale, float eps,
+                                  int zero_centered, void* dh, void* dresidual, void* dpost,
+                                  void* dpre, void* dgate, void* ws, size_t ws_bytes,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif
