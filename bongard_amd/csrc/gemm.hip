@@ -960,7 +960,7 @@ static int gemm_mx_args(const char* who, int64_t M, int64_t N, int64_t K, const 
 static int gemm_mx_launch(const uint8_t* A, int64_t lda, MxScales a_sc, const uint8_t* B,
                           int64_t ldb, MxScales b_sc, int64_t M, int64_t N, int64_t K,
                           const void* bias, void* C, int out_dtype, int64_t ldc, void* ws,
-                          size_t ws_bytes, void* stream) {
+                          size_t ws_bytes, void* stream, int fmt = BF8_E4M3) {
   GemmParams p{};
   p.A = A; p.B = B; p.lda = lda; p.ldb = ldb;
   p.M = (int)M; p.N = (int)N; p.K = (int)K; p.I = 0;
@@ -969,8 +969,7 @@ static int gemm_mx_launch(const uint8_t* A, int64_t lda, MxScales a_sc, const ui
   for (int s = 0; s < 4; ++s) p.seg_end[s] = (int)N;
   p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
   const Plan pl = choose_plan(M, N, K, false, ws ? ws_bytes : 0, true);
-  return launch_plan(pl, p, EPI_LINEAR, out_dtype, BF8_E4M3, BF8_E4M3, ws, as_stream(stream),
-                     true);
+  return launch_plan(pl, p, EPI_LINEAR, out_dtype, fmt, fmt, ws, as_stream(stream), true);
 }
 
 int bf8_gemm_mx(const uint8_t* A, int64_t lda, const uint8_t* A_scales, int64_t lda_sc,
@@ -1001,6 +1000,37 @@ int bf8_gemm_mx_planes(const uint8_t* A, int64_t lda, const uint32_t* A_planes, 
   if (rc) return rc;
   return gemm_mx_launch(A, lda, plane_scales(A_planes, M), B, ldb, plane_scales(B_planes, N), M, N,
                         K, bias, C, out_dtype, ldc, ws, ws_bytes, stream);
+}
+
+// ---- MXFP4 ---------------------------------------------------------------------------
+// The MX GEMM on FP4 codes: K, lda and ldb in bytes, two planes of scales per K step.
+static int check_mx4_operand(const char* who, const char* what, const uint8_t* q, int64_t ld,
+                             const uint32_t* planes, int64_t rows, int64_t K) {
+  BF8_CHECK(q && planes, "%s: %s or its scale planes are NULL", who, what);
+  BF8_CHECK(ld % 16 == 0 && 2 * ld >= K && ((uintptr_t)q & 15) == 0,
+            "%s: %s needs a 16-byte aligned base and a row stride >= K / 2 bytes", who, what);
+  BF8_CHECK(((uintptr_t)planes & 3) == 0, "%s: %s scale planes need 4-byte alignment", who, what);
+  BF8_CHECK(rows * ld < (1LL << 31), "%s: %s larger than 2 GiB", who, what);
+  return BF8_OK;
+}
+
+size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
+  return bf8_gemm_mx_workspace(M, N, K / 2);  // plans are made on K bytes
+}
+
+int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
+                   int64_t ldb, const uint32_t* B_planes, int64_t M, int64_t N, int64_t K,
+                   const void* bias, void* C, int out_dtype, int64_t ldc, void* ws,
+                   size_t ws_bytes, void* stream) {
+  const char* who = "bf8_gemm_mxfp4";
+  int rc = gemm_mx_args(who, M, N, K, bias, C, out_dtype, ldc, ws, ws_bytes);
+  if (rc || M == 0 || N == 0) return rc;
+  rc = check_mx4_operand(who, "A", A, lda, A_planes, M, K);
+  if (rc) return rc;
+  rc = check_mx4_operand(who, "B", B, ldb, B_planes, N, K);
+  if (rc) return rc;
+  return gemm_mx_launch(A, lda, plane_scales(A_planes, M), B, ldb, plane_scales(B_planes, N), M, N,
+                        K / 2, bias, C, out_dtype, ldc, ws, ws_bytes, stream, kFmtFp4);
 }
 
 // The MX gate/up GEMM + gated GELU; H8 (with H8t) set: H quantized in the epilogue.

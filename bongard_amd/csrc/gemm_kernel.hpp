@@ -12,6 +12,9 @@ enum GemmEpi { EPI_LINEAR = 0, EPI_GEGLU = 1 };
 // Operand format of a bf16 GEMM (both operands bf16: 64 K-values per 128-byte step, so K,
 // lda and ldb are passed in bytes); the FP8 formats are BF8_E4M3 (0) and BF8_E5M2 (1).
 constexpr int kFmtBf16 = 2;
+// MXFP4 operands (both; the code the FP4 MFMA names them by): 256 K-values per 128-byte step, K, lda and ldb
+// in bytes, block scales in planes.
+constexpr int kFmtFp4 = 4;
 
 struct MxScales {
   uint8_t* p;

@@ -70,6 +70,13 @@ constexpr int extra_lds(int epi, bool late) { return epi == EPI_GEGLU && !late ?
 // planes (FP8 416.5; the four-wave tile 523.5 from rows), (4096, 2560, 10240) 121.2 -> 94.5 us on
 // the 256x160 tile.
 constexpr int kMxStageBytes = 2048;
+// MXFP4: a step of 256 K-values takes two dwords a tile row, from two planes: [A plane 0 | B
+// plane 0 | A plane 1 | B plane 1], each operand's rows rounded up to the 64 of a wave's load (no more:
+// with 256 rows each the 128x64 tile's third stage would not fit two workgroups' LDS).
+constexpr int f4_rows(int rows) { return (rows + 63) / 64 * 64; }
+constexpr int mx_stage_bytes(int bm, int bn, bool f4) {
+  return f4 ? 8 * (f4_rows(bm) + f4_rows(bn)) : kMxStageBytes;
+}
 
 // Buffer resource (4 SGPRs): base, stride 0, `bytes` valid bytes (offsets at or beyond
 // read as zero), raw-buffer flags of gfx9/gfx950.
@@ -180,6 +187,16 @@ template <int FA, int FB, int OPSEL>
 __device__ __forceinline__ v16f mfma_mx(v8i a, v8i b, v16f c, uint32_t sa, uint32_t sb) {
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, OPSEL, (int)sa, OPSEL,
                                                          (int)sb);
+}
+
+// The FP4 form: 16 bytes a lane, the 32 K-values of block lane >> 5 of 64. At twice the FP8
+// rate, so the two of a 64-byte sub-step take an FP8 MFMA's time.
+template <int OPSEL>
+__device__ __forceinline__ v16f mfma_f4(v4u a, v4u b, v16f c, uint32_t sa, uint32_t sb) {
+  const v8i av = __builtin_bit_cast(v8i, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));
+  const v8i bv = __builtin_bit_cast(v8i, __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1));
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(av, bv, c, kFmtFp4, kFmtFp4, OPSEL,
+                                                         (int)sa, OPSEL, (int)sb);
 }
 
 // Swizzled position of logical 16-byte chunk c in tile row r (128-byte rows).
@@ -464,11 +481,16 @@ gemm_kernel(GemmParams p) {
   // MX: each stage also holds the E8M0 block scales of its K step: one dword (4 blocks of
   // 32) per tile row, A rows at kData + 4 r, B rows at kData + 1024 + 4 r (r < 256).
   constexpr bool MX8 = MX && NW == 8;
+  // MXFP4: the layout of its scales is mx_stage_bytes's
+  constexpr bool F4 = FA == kFmtFp4;
+  static_assert(!F4 || (MX && FB == kFmtFp4), "FP4 operands: both, with block scales");
+  constexpr int RA = F4 ? f4_rows(BM) : 256, RB = F4 ? f4_rows(BN) : 256;  // scale rows per plane
   constexpr int kData = (BM + BN) * kBK;
-  constexpr int kStage = kData + (MX ? kMxStageBytes : 0);  // [A tile | B tile | scales]
+  constexpr int kStage = kData + (MX ? mx_stage_bytes(BM, BN, F4) : 0);  // [A tile | B tile | scales]
   constexpr int DA = BM / (8 * NW), DB = BN / (8 * NW);  // 1 KB DMA blocks per wave per stage
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole 1 KB blocks per wave");
-  constexpr int ND = DA + DB + (MX ? (MX8 ? 1 : 2) : 0);  // loads per wave per stage
+  constexpr int NSC = MX ? (MX8 ? 1 : 2) * (F4 ? 2 : 1) : 0;  // of scales
+  constexpr int ND = DA + DB + NSC;  // loads per wave per stage
   constexpr int NM = FM * FN;                // MFMAs per sub-step
   constexpr int NH = 2 * (FM + FN);          // 16-byte fragment halves per sub-step
   static_assert(EPI != EPI_GEGLU || FN % 2 == 0 || (T::WN == 1 && BN % 16 == 0 && BN % 64 != 0),
@@ -592,15 +614,22 @@ gemm_kernel(GemmParams p) {
   // read as zero.
   i32x4 srd_sa = {0, 0, 0, 0}, srd_sb = {0, 0, 0, 0};
   uint32_t sa_off = kOob, sb_off = kOob, sa_gs = 0, sb_gs = 0;
+  // FP4: the waves past an operand's last 64 rows load its first ones again, so that every wave
+  // issues the same number of loads
+  const int sc_wave = MX8 ? wid & 3 : wid;
+  const int sa_wave = F4 ? sc_wave % (RA / 64) : sc_wave;
+  const int sb_wave = F4 ? sc_wave % (RB / 64) : sc_wave;
+  const int ngroups = F4 ? (p.K + 63) / 64 : ksteps;  // groups of 128 K-values
   if constexpr (MX) {
     auto sc_srd = [&](const MxScales& m, int rows) {
-      const int64_t by_row = rows * m.rs, by_group = ksteps * m.gs;  // whichever is the outer
+      const int64_t by_row = rows * m.rs, by_group = ngroups * m.gs;  // whichever is the outer
       return make_srd(m.p, (uint32_t)(by_row > by_group ? by_row : by_group));
     };
-    const int r = (MX8 ? wid & 3 : wid) * 64 + lane;
+    const int r = sa_wave * 64 + lane, rb = sb_wave * 64 + lane;
     uint32_t oa = kOob, ob = kOob;
     if (r < BM && m0 + r < p.M) oa = (uint32_t)((int64_t)(m0 + r) * p.a_sc.rs);
-    if (r < BN) {
+    if (rb < BN) {
+      const int r = rb;
       int bn;
       bool bvalid;
       if (EPI == EPI_GEGLU) {
@@ -646,7 +675,17 @@ gemm_kernel(GemmParams p) {
         off = (dead ? kOob : b_off) + b_str[j];
       dma16(rb, lds_addr(bdst) + (j * NW + wid) * 1024, off, BKM ? k0 * (uint32_t)p.ldb : k0);
     }
-    else if (x == DA + DB)
+    else if constexpr (F4) {
+      // eight waves: plane x (of A, or of B in the upper four); four: A and B of plane 0, of plane 1
+      const int pl = MX8 ? x - (DA + DB) : (x - (DA + DB)) >> 1;
+      const bool b = MX8 ? false : ((x - (DA + DB)) & 1) != 0;
+      const int group = (int)(k0 / (kBK / 2)) + pl;
+      const bool dead = kill_sc || group >= ngroups;
+      const uint32_t lds = base + kData + pl * 4 * (RA + RB) +
+                           ((MX8 ? wid >= 4 : b) ? 4 * RA + 256 * sb_wave : 256 * sa_wave);
+      dma4(b ? srd_sb : srd_sa, lds, dead ? kOob : b ? sb_off : sa_off,
+           dead ? 0u : (uint32_t)group * (b ? sb_gs : sa_gs));
+    } else if (x == DA + DB)
       dma4(srd_sa, base + kData + wid * 256, kill_sc ? kOob : sa_off, (k0 / kBK) * sa_gs);
     else
       dma4(srd_sb, base + kData + 1024 + wid * 256, kill_sc ? kOob : sb_off, (k0 / kBK) * sb_gs);
@@ -711,22 +750,23 @@ gemm_kernel(GemmParams p) {
   // MX scales of the current stage (per fragment: the row's four block scales, shifted
   // so that byte 2 kk holds block 2 kk + (lane >> 5)) and of the next one.
   uint32_t scA[MX ? FM : 1], scB[MX ? FN : 1], scA_n[MX ? FM : 1], scB_n[MX ? FN : 1];
-  // the scale dword of A fragment j / B fragment i of a stage, unshifted
-  auto read_sa = [&](const uint8_t* stage, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const uint32_t*>(stage + kData +
+  // the scale dword of A fragment j / B fragment i of a stage (FP4: of its plane pl), unshifted
+  auto read_sa = [&](const uint8_t* stage, int j, int pl = 0) __attribute__((always_inline)) {
+    return *reinterpret_cast<const uint32_t*>(stage + kData + pl * 4 * (RA + RB) +
                                               (wave_m0 + j * 32 + (lane & 31)) * 4);
   };
-  auto read_sb = [&](const uint8_t* stage, int i) __attribute__((always_inline)) {
-    return *reinterpret_cast<const uint32_t*>(stage + kData + 1024 + (brow[i] + (lane & 31)) * 4);
+  auto read_sb = [&](const uint8_t* stage, int i, int pl = 0) __attribute__((always_inline)) {
+    return *reinterpret_cast<const uint32_t*>(stage + kData + pl * 4 * (RA + RB) + 4 * RA +
+                                              (brow[i] + (lane & 31)) * 4);
   };
   auto read_scales = [&](const uint8_t* stage, uint32_t* sa_, uint32_t* sb_)
       __attribute__((always_inline)) {
     if constexpr (MX) {
-      const int sh = (lane >> 5) * 8;
+      const int sh = MX8 || F4 ? 0 : (lane >> 5) * 8;
 #pragma unroll
-      for (int j = 0; j < FM; ++j) sa_[j] = read_sa(stage, j) >> (MX8 ? 0 : sh);
+      for (int j = 0; j < FM; ++j) sa_[j] = read_sa(stage, j) >> sh;
 #pragma unroll
-      for (int i = 0; i < FN; ++i) sb_[i] = read_sb(stage, i) >> (MX8 ? 0 : sh);
+      for (int i = 0; i < FN; ++i) sb_[i] = read_sb(stage, i) >> sh;
     }
   };
   auto mma_one = [&](const Frags<NH>& f, int x, auto kk_tag) __attribute__((always_inline)) {
@@ -734,13 +774,26 @@ gemm_kernel(GemmParams p) {
     const int i = x / FM, j = x % FM;
     const int hb = i == 0 ? 0 : 2 * (FM + i);
     const int ha = 2 * (1 + j);
+    if constexpr (F4) {
+      // the sub-step's scale dwords (plane kk: scA / scB for kk 0, their _n for 1), read raw in the
+      // previous half-step: byte 2 h becomes the block of the lane half's 16-byte half h
+      uint32_t& sa = kk == 0 ? scA[j] : scA_n[j];
+      uint32_t& sb = kk == 0 ? scB[i] : scB_n[i];
+      if (i == 0) sa >>= (lane >> 5) * 8;
+      if (j == 0) sb >>= (lane >> 5) * 8;
+      acc[i][j] = mfma_f4<0>(f.h[hb], f.h[ha], acc[i][j], sb, sa);
+      acc[i][j] = mfma_f4<2>(f.h[hb + 1], f.h[ha + 1], acc[i][j], sb, sa);
+      return;
+    }
     if constexpr (MX8 && kk == 0) {
       // the step's scale dwords, read raw in the previous half-step: byte 2 kk becomes the
       // lane half's own block
       if (i == 0) scA[j] >>= (lane >> 5) * 8;
       if (j == 0) scB[i] >>= (lane >> 5) * 8;
     }
-    if constexpr (MX)
+    if constexpr (F4)
+      ;
+    else if constexpr (MX)
       acc[i][j] = mfma_mx<FB, FA, 2 * kk>(join(f.h[hb], f.h[hb + 1]), join(f.h[ha], f.h[ha + 1]),
                                          acc[i][j], scB[i], scA[j]);
     else
@@ -817,6 +870,10 @@ gemm_kernel(GemmParams p) {
 #pragma unroll
     for (int x = 0; x < NM; ++x) {
       mma_one(f0, x, std::integral_constant<int, 0>{});
+      if constexpr (F4) {  // this step's second plane, for the second half
+        if (x < FM) scA_n[x] = read_sa(cur, x, 1);
+        if (x < FN) scB_n[x] = read_sb(cur, x, 1);
+      }
 #pragma unroll
       for (int h = x * NH / NR; h < (x + 1) * NH / NR && h < NH; ++h)
         read_one(f1, cur, curb, 1, h);
@@ -839,11 +896,14 @@ gemm_kernel(GemmParams p) {
     const bool killnb_end = kstep(ls + NSB) >= nsteps;
     // step niters - 2 leaves slot 0 to the gelu table; the last step's mid-step wait covers it
     if constexpr (extra == EXTRA_TABLE) load_table();
-    if constexpr (!MX8) read_scales(nxt, scA_n, scB_n);
+    if constexpr (!MX8 && !F4) read_scales(nxt, scA_n, scB_n);
 #pragma unroll
     for (int x = 0; x < NM; ++x) {
       mma_one(f1, x, std::integral_constant<int, 1>{});
-      if constexpr (MX8) {  // each scale register takes the next step's dword after its last use
+      if constexpr (F4) {  // the next step's first plane
+        if (x < FM) scA[x] = read_sa(nxt, x);
+        if (x < FN) scB[x] = read_sb(nxt, x);
+      } else if constexpr (MX8) {  // each scale register takes the next step's dword after its last use
         if (x % FM == FM - 1) scB[x / FM] = read_sb(nxt, x / FM);
         if (x / FM == FN - 1) scA[x % FM] = read_sa(nxt, x % FM);
       }
@@ -860,7 +920,7 @@ gemm_kernel(GemmParams p) {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (MX && !MX8) {
+    if constexpr (MX && !MX8 && !F4) {
 #pragma unroll
       for (int j = 0; j < FM; ++j) scA[j] = scA_n[j];
 #pragma unroll
@@ -1272,9 +1332,10 @@ int launch_typed(const GemmParams& p, int fa, int fb, hipStream_t s) {
 // A gated-GELU tile cut to two stages keeps a third slot for B tiles alone when it fits
 // (the 256x160 tile of skinny gate/up GEMMs, whose B rows stream from HBM: B then loads
 // two steps ahead).
-template <class T, int EPI, bool MX>
+template <class T, int EPI, bool MX, bool F4 = false>
 struct FitTile {
-  static constexpr int kStageBytes = (T::BM + T::BN) * kBK + (MX ? kMxStageBytes : 0);
+  static constexpr int kStageBytes =
+      (T::BM + T::BN) * kBK + (MX ? mx_stage_bytes(T::BM, T::BN, F4) : 0);
   static constexpr int bytes(int ns, int xb = 0) {
     return (ns * kStageBytes + xb * T::BN * kBK +
             extra_lds(EPI, late_table(EPI, ns, xb, T::KG, kStageBytes))) * T::OCC;
@@ -1289,6 +1350,19 @@ struct FitTile {
                                            kXB>>;
   static_assert(bytes(type::NS, type::XB) <= kLimit, "stages do not fit the LDS");
 };
+
+// The linear MXFP4 GEMM on tile T.
+template <class T>
+int launch_f4(const GemmParams& p, int out_dtype, hipStream_t s) {
+  const dim3 grid(grid_blocks(p)), block(tile_threads<T>());
+  if (out_dtype == BF8_OUT_BF16)
+    hipLaunchKernelGGL((gemm_kernel<T, kFmtFp4, kFmtFp4, EPI_LINEAR, BF8_OUT_BF16, true>), grid,
+                       block, 0, s, p);
+  else
+    hipLaunchKernelGGL((gemm_kernel<T, kFmtFp4, kFmtFp4, EPI_LINEAR, BF8_OUT_F32, true>), grid,
+                       block, 0, s, p);
+  return launch_status("gemm_kernel(mxfp4)");
+}
 
 template <class T>
 int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int fmt_b,
@@ -1312,6 +1386,7 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
     }
     if (mx) {
       if constexpr (T::BM == 128 && T::BN == 128) {
+        if (fmt_a == kFmtFp4) return launch_f4<T>(p, out_dtype, stream);
         if (out_dtype == BF8_OUT_BF16)
           hipLaunchKernelGGL((gemm_kernel<T, 0, 0, EPI_LINEAR, BF8_OUT_BF16, true>), grid, block,
                              0, stream, p);
@@ -1380,6 +1455,8 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
   }
   if (mx) {
     if constexpr (T::NW == 4 || (T::BM == 256 && T::BN == 256)) {
+      if (fmt_a == kFmtFp4)
+        return launch_f4<typename FitTile<T, EPI_LINEAR, true, true>::type>(p, out_dtype, stream);
       // MX block scales (e4m3 operands) beside the stages
       using TM = typename FitTile<T, EPI_LINEAR, true>::type;
       if (out_dtype == BF8_OUT_BF16)

@@ -1,6 +1,6 @@
 // MXFP4 for gfx950: the quantizer of bf16 tensors into blocks of 32 e2m1 codes under one power of
-// two (OCP Microscaling Formats v1.0, section 5), their exact read-back, and the product of two
-// such operands on the block-scaled FP4 MFMA.
+// two (OCP Microscaling Formats v1.0, section 5) and their exact read-back. The products are
+// gemm.hip's.
 //
 // The scale of a block is the smallest power of two 2^k with max |x| <= 6 * 2^k (e = k + 127), so no
 // value is clipped: the specification's own floor(log2(max)) - 2 would clip the magnitudes between
@@ -63,52 +63,6 @@ __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint8_t* __restr
   }
 }
 
-typedef int v8i __attribute__((ext_vector_type(8)));
-typedef float v16f __attribute__((ext_vector_type(16)));
-
-// C [M, N] = A . B^T of MXFP4 operands, one 32 x 32 tile a wave straight from memory: lane l of the
-// FP4 MFMA supplies the 32 K-values (16 bytes) of row l & 31, block l >> 5 of the step of 64, with
-// that block's scale.
-template <int OUT>
-__global__ __launch_bounds__(64) void mx4_gemm_kernel(
-    const uint8_t* __restrict__ A, int64_t lda, const uint32_t* __restrict__ pa,
-    const uint8_t* __restrict__ B, int64_t ldb, const uint32_t* __restrict__ pb, int64_t M,
-    int64_t N, int64_t K, const uint16_t* __restrict__ bias, void* __restrict__ C, int64_t ldc) {
-  const int lane = threadIdx.x, half = lane >> 5;
-  const int64_t tiles_n = (N + 31) / 32;
-  const int64_t m = blockIdx.x / tiles_n * 32 + (lane & 31), n = blockIdx.x % tiles_n * 32 + (lane & 31);
-  v16f acc;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) acc[i] = 0.0f;
-  auto load = [&](const uint8_t* q, int64_t ld, const uint32_t* p, int64_t rows, int64_t row,
-                  int64_t blk, v8i& f, int& s) {
-    const bool in = row < rows && 32 * blk < K;
-    const uint4 d = in ? *reinterpret_cast<const uint4*>(q + row * ld + 16 * blk)
-                       : make_uint4(0u, 0u, 0u, 0u);
-    s = in ? (int)((p[(blk >> 2) * rows + row] >> (8 * (blk & 3))) & 0xFFu) : (int)kMxPadScale;
-    f[0] = (int)d.x; f[1] = (int)d.y; f[2] = (int)d.z; f[3] = (int)d.w;
-    f[4] = f[5] = f[6] = f[7] = 0;
-  };
-  for (int64_t k = 0; k < K; k += 64) {
-    v8i a, b;
-    int sa, sb;
-    load(A, lda, pa, M, m, (k >> 5) + half, a, sa);
-    load(B, ldb, pb, N, n, (k >> 5) + half, b, sb);
-    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b, a, acc, 4, 4, 0, sb, 0, sa);
-  }
-  if (m >= M) return;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t col = n - (lane & 31) + 8 * (i >> 2) + 4 * half + (i & 3);
-    if (col >= N) continue;
-    const float v = acc[i] + (bias ? bf16_lo(bias[col]) : 0.0f);
-    if (OUT == BF8_OUT_BF16)
-      reinterpret_cast<uint16_t*>(C)[m * ldc + col] = (uint16_t)f32_to_bf16_bits(v);
-    else
-      reinterpret_cast<float*>(C)[m * ldc + col] = v;
-  }
-}
-
 template <int LPR, int W>
 int mx4_launch(const uint16_t* x, const Mx4Out& p, hipStream_t s) {
   using T = Mx4Tile<LPR, W>;
@@ -165,44 +119,6 @@ int bf8_dequant_mxfp4(const uint8_t* codes, const uint32_t* planes, int64_t rows
   hipLaunchKernelGGL(mx4_dequant_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)),
                      dim3(256), 0, as_stream(stream), codes, planes, rows, cols, (uint16_t*)out);
   return launch_status("mx4_dequant_kernel");
-}
-
-size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) { return 0; }
-
-int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
-                   int64_t ldb, const uint32_t* B_planes, int64_t M, int64_t N, int64_t K,
-                   const void* bias, void* C, int out_dtype, int64_t ldc, void* ws,
-                   size_t ws_bytes, void* stream) {
-  const char* who = "bf8_gemm_mxfp4";
-  BF8_CHECK(out_dtype == BF8_OUT_BF16 || out_dtype == BF8_OUT_F32, "%s: bad out_dtype", who);
-  BF8_CHECK(M >= 0 && N >= 0 && K >= 0, "%s: negative shape", who);
-  BF8_CHECK(K % 32 == 0, "%s: K must be a multiple of the 32-element block (got %lld)", who,
-            (long long)K);
-  BF8_CHECK(N % 8 == 0 && ldc >= N && ldc % 4 == 0, "%s: need N %% 8 == 0, ldc >= N, ldc %% 4 == 0",
-            who);
-  BF8_CHECK(((uintptr_t)C & 15) == 0 && ((uintptr_t)bias & 7) == 0,
-            "%s: C must be 16-byte, bias 8-byte aligned", who);
-  BF8_CHECK(ws_bytes == 0 || (ws && ((uintptr_t)ws & 255) == 0),
-            "%s: workspace must be 256-byte aligned", who);
-  if (M == 0 || N == 0) return BF8_OK;
-  BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
-  BF8_CHECK(A && A_planes && B && B_planes && C, "%s: NULL pointer", who);
-  BF8_CHECK(lda % 16 == 0 && ldb % 16 == 0 && 2 * lda >= K && 2 * ldb >= K &&
-                (((uintptr_t)A | (uintptr_t)B) & 15) == 0,
-            "%s: A and B need 16-byte aligned bases and row strides >= K / 2 bytes", who);
-  BF8_CHECK((((uintptr_t)A_planes | (uintptr_t)B_planes) & 3) == 0,
-            "%s: scale planes need 4-byte alignment", who);
-  BF8_CHECK(M * lda < (1LL << 31) && N * ldb < (1LL << 31), "%s: operand larger than 2 GiB", who);
-  const int64_t tiles = ((M + 31) / 32) * ((N + 31) / 32);
-  BF8_CHECK(tiles < (1LL << 31), "%s: output too large", who);
-  hipStream_t s = as_stream(stream);
-  if (out_dtype == BF8_OUT_BF16)
-    hipLaunchKernelGGL(mx4_gemm_kernel<BF8_OUT_BF16>, dim3((unsigned)tiles), dim3(64), 0, s, A, lda,
-                       A_planes, B, ldb, B_planes, M, N, K, (const uint16_t*)bias, C, ldc);
-  else
-    hipLaunchKernelGGL(mx4_gemm_kernel<BF8_OUT_F32>, dim3((unsigned)tiles), dim3(64), 0, s, A, lda,
-                       A_planes, B, ldb, B_planes, M, N, K, (const uint16_t*)bias, C, ldc);
-  return launch_status("mx4_gemm_kernel");
 }
 
 }  // extern "C"

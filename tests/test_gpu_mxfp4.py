@@ -462,3 +462,34 @@ def test_refusals(gpu):
     with pytest.raises(ValueError, match="multiples of 32"):
         linear.Mxfp4LinearFunction.apply(x, torch.zeros(40, 64, dtype=torch.bfloat16, device=gpu,
                                                         requires_grad=True), None)
+
+
+TILES = ["256x256", "256x160", "160x256", "128x128", "192x256", "128x64", "64x128", "256x128",
+         "256x256w8", "128x128o2", "128x64:3", "256x256w8:2"]
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("M,N,K", [(5, 24, 32), (300, 328, 1312), (517, 1040, 4128)])
+def test_product_on_every_tile(gpu, monkeypatch, tile, M, N, K):
+    """Every tile's FP4 variant: partial tiles, a last step of 32, 160 and 32 K-values, one step and
+    many, K pieces."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    a, ra = _operand(M, K, M + K, gpu)
+    b, rb = _operand(N, K, N + K, gpu, spread=False)
+    ref, mag = mx4.mm(ra, rb)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=dtype)
+        _check_product(y, ref, mag, K, dtype)
+
+
+def test_tail_split(gpu, monkeypatch):
+    """Whole tiles in full rounds, the last round's tiles in K pieces."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", "256x256w8:t")
+    M, N, K = 4160, 3848, 4128
+    a, ra = _operand(M, K, 1, gpu, spread=False)
+    b, rb = _operand(N, K, 2, gpu, spread=False)
+    y = ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=torch.float32)
+    rows = torch.cat([torch.arange(0, 64), torch.arange(M - 80, M)])
+    ref = mx4.values(ra[0][rows], ra[1][rows]) @ mx4.values(*rb).t()
+    mag = mx4.values(ra[0][rows], ra[1][rows]).abs() @ mx4.values(*rb).abs().t()
+    _check_product(y[rows.to(gpu)], ref, mag, K, torch.float32)

@@ -81,8 +81,8 @@ def _calls(L):
         (deq, (p, p, 4, 32, odd, null), "16-byte"),
         (g, (p, 16, p, p, 16, p, 4, 8, 48, null, p, 0, 8, null, 0, null), "32-element"),
         (g, (p, 16, p, p, 16, p, 4, 9, 32, null, p, 0, 12, null, 0, null), "N % 8"),
-        (g, (p, 16, p, p, 16, p, 4, 8, 64, null, p, 0, 8, null, 0, null), "row strides"),
-        (g, (p, 24, p, p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "row strides"),
+        (g, (p, 16, p, p, 16, p, 4, 8, 64, null, p, 0, 8, null, 0, null), "row stride"),
+        (g, (p, 24, p, p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "row stride"),
         (g, (odd, 16, p, p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "16-byte"),
         (g, (p, 16, ctypes.c_void_p(4098), p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "planes"),
         (g, (p, 16, null, p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "NULL"),
