@@ -80,6 +80,11 @@ SIGNATURES = {
     "bf8_gemm_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
                                c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p,
                                c_size_t, c_void_p]),
+    "bf8_gemm_geglu_mxfp4": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p,
+                                     c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_void_p]),
+    "bf8_geglu_bwd_mxfp4": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p]),
     "bf8_rmsnorm_residual_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
                                           c_void_p, c_float, c_float, c_int, c_void_p, c_void_p,
                                           c_void_p]),

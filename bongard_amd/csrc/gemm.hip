@@ -1055,7 +1055,7 @@ static int geglu_mx_args(const char* who, int64_t M, int64_t I, int64_t K, const
 static int geglu_mx_launch(const uint8_t* X, int64_t ldx, MxScales x_sc, const uint8_t* W,
                            int64_t ldw, MxScales w_sc, int64_t M, int64_t I, int64_t K, void* H,
                            int64_t ldh, uint8_t* H8, MxScales h8_sc, uint8_t* H8t,
-                           MxScales h8t_sc, void* GU, void* stream) {
+                           MxScales h8t_sc, void* GU, void* stream, int fmt = BF8_E4M3) {
   GemmParams p{};
   p.A = X; p.B = W; p.lda = ldx; p.ldb = ldw;
   p.M = (int)M; p.N = (int)(2 * I); p.K = (int)K; p.I = (int)I;
@@ -1065,8 +1065,7 @@ static int geglu_mx_launch(const uint8_t* X, int64_t ldx, MxScales x_sc, const u
   p.h8 = H8; p.h8_sc = h8_sc;
   p.h8t = H8t; p.h8t_sc = h8t_sc;
   Plan pl = choose_plan(M, 2 * I, K, true, 0, true);
-  return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, BF8_E4M3, BF8_E4M3, nullptr,
-                     as_stream(stream), true);
+  return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, fmt, fmt, nullptr, as_stream(stream), true);
 }
 
 static int geglu_mx_entry(const char* who, const uint8_t* X, int64_t ldx, const uint8_t* X_scales,
@@ -1128,6 +1127,32 @@ int bf8_gemm_geglu_mx_planes(const uint8_t* X, int64_t ldx, const uint32_t* X_pl
   return geglu_mx_launch(X, ldx, plane_scales(X_planes, M), W, ldw, plane_scales(W_planes, 2 * I),
                          M, I, K, H, ldh, H8, plane_scales(H8_planes, M), H8t,
                          plane_scales(H8t_planes, I), GU, stream);
+}
+
+int bf8_gemm_geglu_mxfp4(const uint8_t* X, int64_t ldx, const uint32_t* X_planes, const uint8_t* W,
+                         int64_t ldw, const uint32_t* W_planes, int64_t M, int64_t I, int64_t K,
+                         uint8_t* H4, uint32_t* H4_planes, uint8_t* H4t, uint32_t* H4t_planes,
+                         void* GU, void* stream) {
+  const char* who = "bf8_gemm_geglu_mxfp4";
+  BF8_CHECK(M >= 0 && I >= 0 && K >= 0, "%s: negative shape", who);
+  BF8_CHECK(I % 128 == 0, "%s: I must be a multiple of 128 (got %lld)", who, (long long)I);
+  BF8_CHECK(K % 32 == 0, "%s: K must be a multiple of the 32-element block (got %lld)", who,
+            (long long)K);
+  BF8_CHECK((H4t == nullptr) == (H4t_planes == nullptr), "%s: H4t needs its scale planes", who);
+  BF8_CHECK((((uintptr_t)GU | (uintptr_t)H4t) & 15) == 0 &&
+                (((uintptr_t)H4 | (uintptr_t)H4_planes | (uintptr_t)H4t_planes) & 3) == 0,
+            "%s: GU, H4t 16-byte, H4 and scale planes 4-byte aligned", who);
+  BF8_CHECK(M * I < (1LL << 31), "%s: H larger than 2 Gi elements", who);
+  if (M == 0 || I == 0) return BF8_OK;
+  BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
+  BF8_CHECK(H4 && H4_planes, "%s: H4 or its scale planes are NULL", who);
+  int rc = check_mx4_operand(who, "X", X, ldx, X_planes, M, K);
+  if (rc) return rc;
+  rc = check_mx4_operand(who, "W", W, ldw, W_planes, 2 * I, K);
+  if (rc) return rc;
+  return geglu_mx_launch(X, ldx, plane_scales(X_planes, M), W, ldw, plane_scales(W_planes, 2 * I),
+                         M, I, K / 2, nullptr, I, H4, plane_scales(H4_planes, M), H4t,
+                         plane_scales(H4t_planes, I), GU, stream, kFmtFp4);
 }
 
 }  // extern "C"

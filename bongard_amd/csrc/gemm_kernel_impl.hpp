@@ -26,6 +26,7 @@
 
 #include "gelu.hpp"
 #include "gemm_kernel.hpp"
+#include "mxfp4.hpp"
 
 namespace bf8 {
 namespace {
@@ -72,10 +73,12 @@ constexpr int extra_lds(int epi, bool late) { return epi == EPI_GEGLU && !late ?
 constexpr int kMxStageBytes = 2048;
 // MXFP4: a step of 256 K-values takes two dwords a tile row, from two planes: [A plane 0 | B
 // plane 0 | A plane 1 | B plane 1], each operand's rows rounded up to the 64 of a wave's load (no more:
-// with 256 rows each the 128x64 tile's third stage would not fit two workgroups' LDS).
+// with 256 rows each the 128x64 tile's third stage would not fit two workgroups' LDS), 2 KB at least, which
+// takes the 64x128 tile's stage to the gelu table's 26 KB.
 constexpr int f4_rows(int rows) { return (rows + 63) / 64 * 64; }
 constexpr int mx_stage_bytes(int bm, int bn, bool f4) {
-  return f4 ? 8 * (f4_rows(bm) + f4_rows(bn)) : kMxStageBytes;
+  const int b = 8 * (f4_rows(bm) + f4_rows(bn));
+  return f4 && b > kMxStageBytes ? b : kMxStageBytes;
 }
 
 // Buffer resource (4 SGPRs): base, stride 0, `bytes` valid bytes (offsets at or beyond
@@ -372,6 +375,83 @@ __device__ __forceinline__ void mx_h_epilogue(const GemmParams& p, const uint8_t
     r1[(gm >> 5) & 3] = (uint8_t)e1;
     if ((gm >> 5) == nblk - 1) {
       // the column's last block also pads its last dword of scales
+      for (int pb = nblk; pb < sc_pad_end; ++pb) {
+        r0[pb & 3] = (uint8_t)kMxPadScale;
+        r1[pb & 3] = (uint8_t)kMxPadScale;
+      }
+    }
+  }
+}
+
+// The same in MXFP4 (h8: codes [M, I / 2], h8t: [I, R / 2] with R = M rounded up to 32; the rows past
+// M are zeros here, their operand rows having read as zero).
+template <int ROWS, int CH, bool FINITE>
+__device__ __forceinline__ void mx4_h_epilogue(const GemmParams& p, const uint8_t* wbuf, int lane,
+                                               int gm0, int h0) {
+#pragma unroll 4
+  for (int it = 0; it < ROWS * CH / 64; ++it) {
+    const int idx = it * 64 + lane;
+    const int row = idx / CH, c = idx % CH;  // lanes 4j .. 4j+3: one block of one row
+    const uint4 d = stage_get<CH>(wbuf, row, c);
+    const uint32_t k2 = pk_max_u16(pk_max_u16(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu),
+                                   pk_max_u16(d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu));
+    uint32_t k = max(k2 & 0xFFFFu, k2 >> 16);
+    k = max(k, (uint32_t)__builtin_amdgcn_mov_dpp((int)k, 0xB1, 0xF, 0xF, true));
+    k = max(k, (uint32_t)__builtin_amdgcn_mov_dpp((int)k, 0x4E, 0xF, 0xF, true));
+    const int gm = gm0 + row;
+    if (gm < p.M) {
+      const int n = h0 + c * 8;
+      const uint32_t e = FINITE ? mx4_exponent_finite(k) : mx4_exponent(k);
+      uint32_t q = 0;
+      q = mx4_pack2<0, FINITE>(q, d.x, e);
+      q = mx4_pack2<1, FINITE>(q, d.y, e);
+      q = mx4_pack2<2, FINITE>(q, d.z, e);
+      q = mx4_pack2<3, FINITE>(q, d.w, e);
+      *reinterpret_cast<uint32_t*>(p.h8 + (((int64_t)gm * p.I + n) >> 1)) = q;
+      if ((c & 3) == 0)
+        p.h8_sc.p[(int64_t)gm * p.h8_sc.rs + (n >> 7) * p.h8_sc.gs + ((n >> 5) & 3)] = (uint8_t)e;
+    }
+  }
+  if (p.h8t == nullptr) return;
+  constexpr int CP = CH * 4;              // column pairs per staged row
+  constexpr int ITEMS = (ROWS / 32) * CP;  // (32-row block, column pair) items
+  const int nblk = (p.M + 31) >> 5;
+  const int sc_pad_end = ((p.M + 127) >> 7) << 2;
+#pragma unroll 1
+  for (int item = lane; item < ITEMS; item += 64) {
+    const int blk = item / CP, cp = item % CP;
+    const int gm = gm0 + blk * 32;
+    if (gm >= p.M) continue;
+    uint32_t v[32];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      v[i] = stage_get_pair<CH>(wbuf, blk * 32 + i, 2 * cp);
+      top = pk_max_u16(top, v[i] & 0x7FFF7FFFu);
+    }
+    const uint32_t k0 = top & 0xFFFFu, k1 = top >> 16;
+    const uint32_t e0 = FINITE ? mx4_exponent_finite(k0) : mx4_exponent(k0);
+    const uint32_t e1 = FINITE ? mx4_exponent_finite(k1) : mx4_exponent(k1);
+    uint32_t q0[4] = {}, q1[4] = {};
+    static_for<4>([&](auto w_tag) __attribute__((always_inline)) {
+      constexpr int w = decltype(w_tag)::value;
+      static_for<4>([&](auto b_tag) __attribute__((always_inline)) {
+        constexpr int b = decltype(b_tag)::value;
+        const uint32_t x = v[8 * w + 2 * b], y = v[8 * w + 2 * b + 1];
+        q0[w] = mx4_pack2<b, FINITE>(q0[w], __byte_perm(x, y, 0x5410), e0);
+        q1[w] = mx4_pack2<b, FINITE>(q1[w], __byte_perm(x, y, 0x7632), e1);
+      });
+    });
+    const int n = h0 + 2 * cp;
+    const int64_t ldt = (int64_t)nblk * 16;
+    *reinterpret_cast<uint4*>(p.h8t + n * ldt + (gm >> 1)) = make_uint4(q0[0], q0[1], q0[2], q0[3]);
+    *reinterpret_cast<uint4*>(p.h8t + (n + 1) * ldt + (gm >> 1)) =
+        make_uint4(q1[0], q1[1], q1[2], q1[3]);
+    uint8_t* r0 = p.h8t_sc.p + (int64_t)n * p.h8t_sc.rs + (gm >> 7) * p.h8t_sc.gs;
+    uint8_t* r1 = r0 + p.h8t_sc.rs;
+    r0[(gm >> 5) & 3] = (uint8_t)e0;
+    r1[(gm >> 5) & 3] = (uint8_t)e1;
+    if ((gm >> 5) == nblk - 1) {
       for (int pb = nblk; pb < sc_pad_end; ++pb) {
         r0[pb & 3] = (uint8_t)kMxPadScale;
         r1[pb & 3] = (uint8_t)kMxPadScale;
@@ -1229,7 +1309,12 @@ gemm_kernel(GemmParams p) {
           // every value this wave quantizes is one it staged: with none of them inf or NaN
           // (and a finite scale) no product can be NaN, so the NaN patch is skipped
           const bool finite = !__any(hmax >= 0x7F800000u) && (MX || hs < INFINITY);
-          if constexpr (MX) {
+          if constexpr (F4) {
+            if (finite)
+              mx4_h_epilogue<ROWS, CH, true>(p, wbuf, lane, m0 + wave_m0, wave_h0);
+            else
+              mx4_h_epilogue<ROWS, CH, false>(p, wbuf, lane, m0 + wave_m0, wave_h0);
+          } else if constexpr (MX) {
             if (finite)
               mx_h_epilogue<ROWS, CH, true>(p, wbuf, lane, m0 + wave_m0, wave_h0);
             else
@@ -1415,6 +1500,12 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
     if constexpr (T::FN % 2 == 0) {
       if (mx) {
         if constexpr (T::NW == 4 || (T::BM == 256 && T::BN == 256)) {
+          if (fmt_a == kFmtFp4) {
+            using TF = typename FitTile<T, EPI_GEGLU, true, true>::type;
+            hipLaunchKernelGGL((gemm_kernel<TF, kFmtFp4, kFmtFp4, EPI_GEGLU, BF8_OUT_BF16, true>),
+                               grid, block, 0, stream, p);
+            return launch_status("gemm_kernel(geglu, mxfp4)");
+          }
           using TG = typename FitTile<T, EPI_GEGLU, true>::type;
           hipLaunchKernelGGL((gemm_kernel<TG, 0, 0, EPI_GEGLU, BF8_OUT_BF16, true>), grid, block,
                              0, stream, p);

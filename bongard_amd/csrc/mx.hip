@@ -255,45 +255,6 @@ __device__ __forceinline__ void mx_tiles(const MxTile& p, int64_t blk, int64_t n
   }
 }
 
-// d_g (G) or d_u of 8 elements: the chain of geglu_bwd8, one half of it.
-template <bool G>
-__device__ __forceinline__ uint4 geglu_bwd8_half(uint4 dh, uint4 g, uint4 u, const uint16_t* ta,
-                                                 const uint32_t* tf) {
-  const uint32_t dw[4] = {dh.x, dh.y, dh.z, dh.w}, gw[4] = {g.x, g.y, g.z, g.w};
-  const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
-  uint32_t outside = 0, ix[4], t[8], o[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w)
-    ix[w] = G ? gelu_factor_index2(gw[w], outside) : gelu_index2(gw[w], outside);
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    t[2 * w] = G ? tf[ix[w] & 0xFFFFu] : ta[ix[w] & 0xFFFFu];
-    t[2 * w + 1] = G ? tf[ix[w] >> 16] : ta[ix[w] >> 16];
-  }
-  if (__builtin_expect(__any(outside != 0), 0)) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      t[2 * w] = G ? gelu_factor_finish(gw[w], t[2 * w]) : gelu_finish(gw[w], t[2 * w]);
-      t[2 * w + 1] = G ? gelu_factor_finish(gw[w] >> 16, t[2 * w + 1])
-                       : gelu_finish(gw[w] >> 16, t[2 * w + 1]);
-    }
-  }
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float d0 = bf16_lo(dw[w]), d1 = bf16_hi(dw[w]);
-    if constexpr (G) {
-      const uint32_t da = pack_bf16x2(d0 * bf16_lo(uw[w]), d1 * bf16_hi(uw[w]));
-      o[w] = pack_bf16x2(bf16_lo(da) * __uint_as_float(t[2 * w]),
-                         bf16_hi(da) * __uint_as_float(t[2 * w + 1]));
-    } else {
-      const uint32_t a = t[2 * w] | (t[2 * w + 1] << 16);
-      o[w] = pack_bf16x2(d0 * bf16_lo(a), d1 * bf16_hi(a));
-    }
-    o[w] = nan_ffff_bf16x2(o[w]);
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
 // d_g or d_u of the lane's eight rows 4 k of a tile, in two batches of loads.
 template <bool G>
 __device__ __forceinline__ void geglu_bwd_rows(const uint16_t* dp, const uint16_t* gp, int64_t I,

@@ -11,6 +11,7 @@
 
 #include <algorithm>
 
+#include "gelu.hpp"
 #include "mxfp4.hpp"
 
 namespace bf8 {
@@ -37,6 +38,60 @@ __global__ __launch_bounds__(64 * W) void mx4_tile_kernel(const uint16_t* __rest
         v[k] = *reinterpret_cast<const uint4*>(x + (r + k) * p.cols + c);
     }
     mx4_tile_finish<LPR, W>(p, r0, c0, v, sh, wid, lane);
+  }
+}
+
+// d_g (G) or d_u of the lane's RL rows of a tile, four rows' loads at a time.
+template <bool G, int RL>
+__device__ __forceinline__ void geglu_bwd_rows(const uint16_t* dp, const uint16_t* gp, int64_t I,
+                                               int64_t rows_left, const uint16_t* ta,
+                                               const uint32_t* tf, uint4 (&v)[RL]) {
+#pragma unroll
+  for (int q = 0; q < RL / 4; ++q) {
+    uint4 d[4], g[4], u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int row = 4 * q + k;
+      d[k] = g[k] = u[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (row < rows_left) {
+        d[k] = *reinterpret_cast<const uint4*>(dp + row * I);
+        g[k] = *reinterpret_cast<const uint4*>(gp + row * 2 * I);
+        if (G) u[k] = *reinterpret_cast<const uint4*>(gp + row * 2 * I + I);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[4 * q + k] = geglu_bwd8_half<G>(d[k], g[k], u[k], ta, tf);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
+// The gated-GELU backward and the quantization of its dGU [M, 2I] (p: rows M, cols 2I) from
+// dH [M, I] and GU [M, 2I], I % 128 == 0: dGU goes from registers to its copies. The first half of
+// a block's waves take the d_g tile of 32 W x 8 LPR elements of H, the others its d_u tile.
+template <int LPR, int W>
+__global__ __launch_bounds__(128 * W) void geglu_bwd_mx4_kernel(const uint16_t* __restrict__ dH,
+                                                                const uint16_t* __restrict__ GU,
+                                                                int64_t I, Mx4Out p) {
+  using T = Mx4Tile<LPR, W>;
+  __shared__ __attribute__((aligned(16))) uint16_t ta[kGeluABytes / 2];
+  __shared__ __attribute__((aligned(16))) uint32_t tf[kGeluFBytes / 4];
+  __shared__ typename T::Shared sh[2];
+  load_gelu_tables<128 * W>(ta, tf);
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wid = w % W, half = w / W;
+  const int64_t tiles_c = I / T::kCols, tiles_r = (p.rows + T::kRows - 1) / T::kRows;
+  for (int64_t t = blockIdx.x; t < tiles_c * tiles_r; t += gridDim.x) {
+    const int64_t r0 = (t / tiles_c) * T::kRows, c0 = (t % tiles_c) * T::kCols;
+    const int64_t r = r0 + 32 * wid + T::RL * (lane / LPR);
+    const uint16_t* dp = dH + r * I + c0 + 8 * (lane % LPR);
+    const uint16_t* gp = GU + r * 2 * I + c0 + 8 * (lane % LPR);
+    uint4 v[T::RL];
+    if (half == 0)
+      geglu_bwd_rows<true, T::RL>(dp, gp, I, p.rows - r, ta, tf, v);
+    else
+      geglu_bwd_rows<false, T::RL>(dp, gp, I, p.rows - r, ta, tf, v);
+    mx4_tile_finish<LPR, W>(p, r0, half * I + c0, v, sh[half], wid, lane);
   }
 }
 
@@ -119,6 +174,24 @@ int bf8_dequant_mxfp4(const uint8_t* codes, const uint32_t* planes, int64_t rows
   hipLaunchKernelGGL(mx4_dequant_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20)),
                      dim3(256), 0, as_stream(stream), codes, planes, rows, cols, (uint16_t*)out);
   return launch_status("mx4_dequant_kernel");
+}
+
+int bf8_geglu_bwd_mxfp4(const void* dH, const void* GU, int64_t M, int64_t I, uint8_t* out,
+                        uint32_t* out_planes, uint8_t* out_t, uint32_t* out_t_planes,
+                        void* stream) {
+  const char* who = "bf8_geglu_bwd_mxfp4";
+  BF8_CHECK(I % 128 == 0, "%s: need I %% 128 == 0 (got %lld)", who, (long long)I);
+  const Mx4Out p{M, 2 * I, out, out_planes, out_t, out_t_planes};
+  if (const int rc = check_mx4_out(who, p)) return rc;
+  if (M == 0 || I == 0) return BF8_OK;
+  BF8_CHECK(dH && GU && (((uintptr_t)dH | (uintptr_t)GU) & 15) == 0,
+            "%s: dH and GU must be given, 16-byte aligned", who);
+  const auto* d = (const uint16_t*)dH;
+  const auto* g = (const uint16_t*)GU;
+  const int64_t tiles = ((M + 127) / 128) * (I / 128);
+  hipLaunchKernelGGL((geglu_bwd_mx4_kernel<16, 4>), dim3((unsigned)std::min<int64_t>(tiles, 512)),
+                     dim3(512), 0, as_stream(stream), d, g, I, p);
+  return launch_status("geglu_bwd_mx4_kernel");
 }
 
 }  // extern "C"

@@ -1440,18 +1440,39 @@ def gemm_geglu_mxfp4(x, x_planes, w, w_planes, intermediate, *, colwise=False, k
         raise ValueError(f"{who}: inner dims differ ({K} vs {Kw})")
     if I % 128:
         raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
-    GU = gemm_mxfp4(x, x_planes, w, w_planes)
+    if K == 0:
+        raise ValueError(f"{who}: K must not be 0")
+    hq = _new_mxfp4(M, I, True, colwise, dev)
+    GU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dev) if keep_gu else None
+    if M == 0:
+        return hq, GU
     with _On(dev):
-        H, _ = geglu(GU)
-    return quantize_mxfp4(H, colwise=colwise), GU if keep_gu else None
+        _lib.check(_lib.lib().bf8_gemm_geglu_mxfp4(
+            _ptr(x), x.stride(0), _ptr(x_planes), _ptr(w), w.stride(0), _ptr(w_planes), M, I, K,
+            _ptr(hq.data), _ptr(hq.planes), _ptr(hq.data_t), _ptr(hq.planes_t), _ptr(GU),
+            _stream(dev)), "bf8_gemm_geglu_mxfp4")
+    return hq, GU
 
 
 def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
-    """:func:`geglu_bwd` and the :func:`quantize_mxfp4` of its dGU [M, 2I]."""
-    dev = _one_device("geglu_bwd_mxfp4", dH, GU)
-    with _On(dev):
-        dGU, _ = geglu_bwd(dH, GU)
-    return quantize_mxfp4(dGU, rowwise=rowwise, colwise=colwise)
+    """:func:`geglu_bwd` and the :func:`quantize_mxfp4` of its dGU [M, 2I] in one pass (the same
+    codes and planes; the bf16 dGU is not written). I must be a multiple of 128."""
+    who = "geglu_bwd_mxfp4"
+    dev = _one_device(who, dH, GU)
+    dH = _aligned(_bf16_2d(dH))
+    M, I = dH.shape
+    GU = _aligned(_gu_operand(who, GU, M, I))
+    if not (rowwise or colwise):
+        raise ValueError(f"{who}: nothing requested")
+    if I % 128:
+        raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
+    q = _new_mxfp4(M, 2 * I, rowwise, colwise, dev)
+    if M:
+        with _On(dev):
+            _lib.check(_lib.lib().bf8_geglu_bwd_mxfp4(
+                _ptr(dH), _ptr(GU), M, I, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t),
+                _ptr(q.planes_t), _stream(dev)), "bf8_geglu_bwd_mxfp4")
+    return q
 
 
 # ---- the norms on either side of a residual connection ---------------------------------------

@@ -573,6 +573,22 @@ int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, cons
                    const void* bias, void* C, int out_dtype, int64_t ldc, void* ws,
                    size_t ws_bytes, void* stream);
 
+/* The gate/up product of MXFP4 operands X [M, K], W [2 I, K] (gate rows then up rows) with the
+ * gated GELU and the quantization of H [M, I] in its epilogue (bongard/te_linear.py:98-103's
+ * chain): g, u rounded to bf16, H = bf16(bf16(gelu_tanh(g)) * u), H4 [M, I / 2] with H4_planes and
+ * optionally H4t [I, R / 2] with H4t_planes, the bytes bf8_quantize_mxfp4_bf16 gives for that H
+ * (which is not written). GU: bf16 [M, 2 I] pre-activations or NULL. I % 128 == 0. */
+int bf8_gemm_geglu_mxfp4(const uint8_t* X, int64_t ldx, const uint32_t* X_planes, const uint8_t* W,
+                         int64_t ldw, const uint32_t* W_planes, int64_t M, int64_t I, int64_t K,
+                         uint8_t* H4, uint32_t* H4_planes, uint8_t* H4t, uint32_t* H4t_planes,
+                         void* GU, void* stream);
+
+/* bf8_geglu_bwd and the MXFP4 quantization of its dGU [M, 2 I] in one pass: the bytes and planes
+ * of bf8_quantize_mxfp4_bf16 of that dGU, which is not written. I % 128 == 0. */
+int bf8_geglu_bwd_mxfp4(const void* dH, const void* GU, int64_t M, int64_t I, uint8_t* out,
+                        uint32_t* out_planes, uint8_t* out_t, uint32_t* out_t_planes,
+                        void* stream);
+
 /* ---------------------------------------------------------------------------------
  * The norms on either side of a residual connection in one kernel (HF T5Gemma2's layer:
  * post-block norm, addition, pre-block norm of the next block; the two norms around

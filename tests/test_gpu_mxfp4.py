@@ -493,3 +493,22 @@ def test_tail_split(gpu, monkeypatch):
     ref = mx4.values(ra[0][rows], ra[1][rows]) @ mx4.values(*rb).t()
     mag = mx4.values(ra[0][rows], ra[1][rows]).abs() @ mx4.values(*rb).abs().t()
     _check_product(y[rows.to(gpu)], ref, mag, K, torch.float32)
+
+
+@pytest.mark.parametrize("tile", ["256x256w8", "256x256", "160x256", "192x256", "128x128", "64x128", "256x128"])
+@pytest.mark.parametrize("M,K,I", [(1, 32, 128), (45, 288, 256), (290, 544, 640)])
+def test_gated_product_on_every_tile(gpu, monkeypatch, tile, M, K, I):
+    """The gated-GELU epilogue of every tile: H's copies from its own GU, one K step and several, ragged
+    rows, a NaN and an inf among the inputs of the last case."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    x, w, _, _ = _mlp_inputs(M, K, I, M + K + I, gpu)
+    if M == 290:
+        x[M - 1, 5], x[7, 40] = float("nan"), 3e38
+    xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    hq, GU = ops.gemm_geglu_mxfp4(xq.data, xq.planes, wq.data, wq.planes, I, colwise=True, keep_gu=True)
+    rows = [i for i in range(M) if M != 290 or i not in (7, M - 1)]
+    ref, mag = mx4.mm(mx4.quantize(x.cpu()), mx4.quantize(w.cpu()))
+    _check_product(GU[rows], ref[rows], mag[rows], K, torch.bfloat16)
+    want = ops.quantize_mxfp4(ops.geglu(GU)[0], colwise=True)
+    assert torch.equal(hq.planes, want.planes) and torch.equal(hq.data, want.data)
+    assert torch.equal(hq.planes_t, want.planes_t) and torch.equal(hq.data_t, want.data_t)

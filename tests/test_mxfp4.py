@@ -67,7 +67,21 @@ def _calls(L):
     q, g = L.bf8_quantize_mxfp4_bf16, L.bf8_gemm_mxfp4
     n, b = L.bf8_rmsnorm_residual_bf16, L.bf8_rmsnorm_residual_bwd_bf16
     deq = L.bf8_dequant_mxfp4
+    h, d = L.bf8_gemm_geglu_mxfp4, L.bf8_geglu_bwd_mxfp4
     return [
+        (h, (p, 16, p, p, 16, p, 4, 96, 32, p, p, null, null, null, null), "multiple of 128"),
+        (h, (p, 16, p, p, 16, p, 4, 128, 48, p, p, null, null, null, null), "32-element"),
+        (h, (p, 16, p, p, 16, p, 4, 128, 0, p, p, null, null, null, null), "K == 0"),
+        (h, (p, 16, p, p, 16, p, 4, 128, 32, null, p, null, null, null, null), "NULL"),
+        (h, (p, 16, p, p, 16, p, 4, 128, 32, p, p, p, null, null, null), "H4t needs"),
+        (h, (p, 16, p, p, 16, p, 4, 128, 32, p, p, null, null, odd, null), "16-byte"),
+        (h, (p, 16, null, p, 16, p, 4, 128, 32, p, p, null, null, null, null), "X or its scale"),
+        (h, (p, 16, p, p, 8, p, 4, 128, 32, p, p, null, null, null, null), "row stride"),
+        (h, (p, 16, p, p, 16, p, 1 << 20, 1 << 12, 32, p, p, null, null, null, null), "2 Gi"),
+        (d, (p, p, 4, 64, p, p, null, null, null), "I % 128"),
+        (d, (p, p, 4, 128, null, null, null, null, null), "give out"),
+        (d, (odd, p, 4, 128, p, p, null, null, null), "16-byte"),
+        (d, (p, null, 4, 128, p, p, null, null, null), "must be given"),
         (q, (p, 32, 40, p, p, null, null, null), "cols % 32"),
         (q, (p, 32, 12, null, null, p, p, null), "cols % 8"),
         (q, (p, -1, 32, p, p, null, null, null), "negative"),
