@@ -1259,53 +1259,52 @@ def gemm_nvfp4(a_data, a_scales, a_meta, b_data, b_scales, b_meta, *, out_dtype=
 
 
 # ---- MXFP4: e2m1 codes in blocks of 32 under a power of two ---------------------------------
-def _one_device(who, *tensors):
-    """The HIP device of the tensors (None among them is skipped), which must be one."""
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        _require_gpu(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{who}: tensors on different devices ({dev} and {t.device})")
-    return dev
+# The ops below run in training steps and decoding loops of small tensors, where a call's host time is
+# what it takes: their checks read the tensors' fields once, and tensors that are as the
+# kernels want them (2-D, contiguous, aligned) pass without a call.
+def _index_of(who, first, *rest):
+    """The device index of the tensors (None among ``rest`` is skipped), which must be one."""
+    idx = first.get_device()
+    for t in rest:
+        if t is not None and t.get_device() != idx:
+            _require_gpu(first, t)
+            raise ValueError(f"{who}: tensors on different devices ({first.device} and {t.device})")
+    if idx < 0:
+        _require_gpu(first)
+    return idx
 
 
-class _On:
-    """Makes ``device`` the current one for a call where it is not (launches go to the current
-    device; the caller's stream of ``device`` is what they are queued on)."""
-
-    __slots__ = ("idx", "prev")
-
-    def __init__(self, device):
-        self.idx = device.index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.idx is not None and self.prev != self.idx:
-            torch.cuda.set_device(self.idx)
-
-    def __exit__(self, *exc):
-        if self.idx is not None and self.prev != self.idx:
-            torch.cuda.set_device(self.prev)
-
-
-def _call_workspace(nbytes, device):
-    """``(workspace or None, its bytes)`` of a call: the stream's shared one, or while a graph is
-    captured one of the graph's own (two graphs captured on a stream may replay side by side)."""
-    if not nbytes:
-        return None, 0
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+def _call(what, idx, fn, *args):
+    """Calls a library entry on the current stream of device ``idx`` (made the current one for the
+    launch where it is not) and checks its status."""
+    if idx == torch._C._cuda_getDevice():
+        rc = fn(*args, _stream_of(idx))
     else:
-        ws = gemm_workspace(nbytes, device)
+        with torch.cuda.device(idx):
+            rc = fn(*args, _stream_of(idx))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _stream_of(idx):
+    return _raw_stream(idx) if _raw_stream is not None else torch.cuda.current_stream(idx).cuda_stream
+
+
+def _call_workspace(nbytes, like):
+    """``(workspace, its bytes)`` of a call: the stream's shared one, or while a graph is captured
+    one of the graph's own (two graphs captured on a stream may replay side by side)."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    else:
+        ws = gemm_workspace(nbytes, like.device)
     return ws, ws.numel()
 
 
-def _aligned(t):
-    """``t`` on 16-byte alignment: copied where a view starts off it."""
+def _rows_bf16(t):
+    """``t`` as the kernels read it: bf16 [rows, cols], contiguous and 16-byte aligned, copied or
+    flattened where it is not."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 2 or not t.is_contiguous():
+        t = _bf16_2d(t)
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -1332,10 +1331,10 @@ def _new_mxfp4(rows, cols, rowwise, colwise, device):
         if cols % 32:
             raise ValueError(f"MXFP4 blocks along rows need cols % 32 == 0 (got {cols})")
         out = torch.empty((rows, cols // 2), dtype=torch.uint8, device=device)
-        pl = _new_planes(cols, rows, device)
+        pl = torch.empty(((cols + 127) // 128, rows), dtype=torch.int32, device=device)
     if colwise:
         out_t = torch.empty((cols, (rows + 31) // 32 * 16), dtype=torch.uint8, device=device)
-        pl_t = _new_planes(rows, cols, device)
+        pl_t = torch.empty(((rows + 127) // 128, cols), dtype=torch.int32, device=device)
     return Mxfp4Tensor(out, pl, out_t, pl_t, rows, cols)
 
 
@@ -1345,32 +1344,29 @@ def quantize_mxfp4(x, *, rowwise=True, colwise=False):
     the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (ties to the even code). ``rowwise``: blocks
     along rows (cols a multiple of 32); ``colwise``: along columns, any number of rows (cols a
     multiple of 8). Both copies come from one pass over x."""
-    who = "quantize_mxfp4"
-    dev = _one_device(who, x)
-    x = _aligned(_bf16_2d(x))
+    idx = _index_of("quantize_mxfp4", x)
+    x = _rows_bf16(x)
     rows, cols = x.shape
     if not (rowwise or colwise):
-        raise ValueError(f"{who}: nothing requested")
-    q = _new_mxfp4(rows, cols, rowwise, colwise, dev)
-    if not x.numel():
-        return q
-    with _On(dev):
-        _lib.check(_lib.lib().bf8_quantize_mxfp4_bf16(
-            _ptr(x), rows, cols, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t), _ptr(q.planes_t),
-            _stream(dev)), "bf8_quantize_mxfp4_bf16")
+        raise ValueError("quantize_mxfp4: nothing requested")
+    q = _new_mxfp4(rows, cols, rowwise, colwise, x.device)
+    if rows and cols:
+        _call("bf8_quantize_mxfp4_bf16", idx, _lib.lib().bf8_quantize_mxfp4_bf16, x.data_ptr(), rows,
+              cols, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t), _ptr(q.planes_t))
     return q
 
 
-def _mxfp4_operand(who, name, codes, planes, rows=None):
-    """Checks an MXFP4 operand [rows, K] and returns (rows, K)."""
-    if codes.dtype != torch.uint8:
+def _mxfp4_operand(who, name, codes, planes):
+    """(rows, K) of an MXFP4 operand, checked."""
+    if codes.dtype is not torch.uint8:
         raise TypeError(f"{who}: {name} must be uint8 codes (got {codes.dtype})")
-    _byte_matrix(who, **{name: codes})
-    R, K = codes.shape[0], 2 * codes.shape[1]
-    if rows is not None and R != rows:
-        raise ValueError(f"{who}: {name} must have {rows} rows (got {R})")
-    _mx_planes(who, {f"{name}_planes": R}, K, **{f"{name}_planes": planes})
-    return R, K
+    if codes.dim() != 2 or (codes.stride(1) != 1 and codes.shape[1] > 1):
+        _byte_matrix(who, **{name: codes})
+    rows, half = codes.shape
+    if (planes.dtype is not torch.int32 or planes.shape != ((half + 63) // 64, rows)
+            or not planes.is_contiguous()):
+        _mx_planes(who, {f"{name}_planes": rows}, 2 * half, **{f"{name}_planes": planes})
+    return rows, 2 * half
 
 
 def dequant_mxfp4(q, *, transpose=False):
@@ -1381,13 +1377,13 @@ def dequant_mxfp4(q, *, transpose=False):
     codes, planes = (q.data_t, q.planes_t) if transpose else (q.data, q.planes)
     if codes is None:
         raise ValueError(f"{who}: the tensor has no {'columnwise' if transpose else 'rowwise'} copy")
-    dev = _one_device(who, codes, planes)
+    idx = _index_of(who, codes, planes)
     rows, cols = _mxfp4_operand(who, "codes", codes, planes)
     codes = codes.contiguous()
-    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=dev)
-    with _On(dev):
-        _lib.check(_lib.lib().bf8_dequant_mxfp4(_ptr(codes), _ptr(planes), rows, cols, _ptr(out),
-                                                _stream(dev)), "bf8_dequant_mxfp4")
+    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=codes.device)
+    if rows and cols:
+        _call("bf8_dequant_mxfp4", idx, _lib.lib().bf8_dequant_mxfp4, codes.data_ptr(),
+              planes.data_ptr(), rows, cols, out.data_ptr())
     return out[:, :q.rows] if transpose and q.rows != cols else out
 
 
@@ -1400,28 +1396,33 @@ def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16,
     """``C = A @ B.T (+ bias)`` of MXFP4 operands A [M, K] and B [N, K] (codes and scale planes as
     :func:`quantize_mxfp4` writes them) on the block-scaled FP4 MFMA, sums in fp32."""
     who = "gemm_mxfp4"
-    dev = _one_device(who, a, a_planes, b, b_planes, bias, out)
+    idx = _index_of(who, a, a_planes, b, b_planes, bias, out)
     M, K = _mxfp4_operand(who, "a", a, a_planes)
     N, Kb = _mxfp4_operand(who, "b", b, b_planes)
     if K != Kb:
         raise ValueError(f"{who}: inner dims differ ({K} vs {Kb})")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
         raise TypeError(f"{who}: out_dtype must be bfloat16 or float32")
     if out is None:
-        out = torch.empty((M, N), dtype=out_dtype, device=dev)
-    _out_matrix(who, out, (M, N), out_dtype)
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=a.device), N
+    else:
+        _out_matrix(who, out, (M, N), out_dtype)
+        ldc = out.stride(0)
     if bias is not None:
         if bias.dtype != torch.bfloat16 or bias.numel() != N:
             raise ValueError(f"{who}: bias must be bfloat16 [{N}] (got {bias.dtype} {tuple(bias.shape)})")
-        bias = _aligned(bias.contiguous())
+        bias = bias.contiguous()
+        if bias.data_ptr() % 8:
+            bias = bias.clone()
     if K == 0:  # an empty sum
-        return out.zero_() if bias is None else out.copy_(bias.expand(M, N))
-    ws, ws_bytes = _call_workspace(_gemm_mxfp4_ws_cached(M, N, K, _tile_override()), dev)
-    with _On(dev):
-        _lib.check(_lib.lib().bf8_gemm_mxfp4(
-            _ptr(a), a.stride(0), _ptr(a_planes), _ptr(b), b.stride(0), _ptr(b_planes), M, N, K,
-            _ptr(bias), _ptr(out), OUT_BF16 if out_dtype == torch.bfloat16 else OUT_F32,
-            out.stride(0), _ptr(ws), ws_bytes, _stream(dev)), "bf8_gemm_mxfp4")
+        return out.zero_() if bias is None else out.copy_(bias.reshape(1, N).expand(M, N))
+    ws = None
+    ws_bytes = _gemm_mxfp4_ws_cached(M, N, K, _tile_override())
+    if ws_bytes:
+        ws, ws_bytes = _call_workspace(ws_bytes, a)
+    _call("bf8_gemm_mxfp4", idx, _lib.lib().bf8_gemm_mxfp4, a.data_ptr(), a.stride(0),
+          a_planes.data_ptr(), b.data_ptr(), b.stride(0), b_planes.data_ptr(), M, N, K, _ptr(bias),
+          out.data_ptr(), OUT_BF16 if out_dtype is torch.bfloat16 else OUT_F32, ldc, _ptr(ws), ws_bytes)
     return out
 
 
@@ -1432,25 +1433,22 @@ def gemm_geglu_mxfp4(x, x_planes, w, w_planes, intermediate, *, colwise=False, k
     ``colwise`` the columnwise copy as well) and ``GU`` the bf16 pre-activations when
     ``keep_gu``. I must be a multiple of 128."""
     who = "gemm_geglu_mxfp4"
-    dev = _one_device(who, x, x_planes, w, w_planes)
+    idx = _index_of(who, x, x_planes, w, w_planes)
     I = int(intermediate)
     M, K = _mxfp4_operand(who, "x", x, x_planes)
-    _, Kw = _mxfp4_operand(who, "w", w, w_planes, 2 * I)
-    if K != Kw:
-        raise ValueError(f"{who}: inner dims differ ({K} vs {Kw})")
+    N, Kw = _mxfp4_operand(who, "w", w, w_planes)
+    if N != 2 * I or K != Kw:
+        raise ValueError(f"{who}: w must have {2 * I} rows of {K} values (got {N} of {Kw})")
     if I % 128:
         raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
     if K == 0:
         raise ValueError(f"{who}: K must not be 0")
-    hq = _new_mxfp4(M, I, True, colwise, dev)
-    GU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dev) if keep_gu else None
-    if M == 0:
-        return hq, GU
-    with _On(dev):
-        _lib.check(_lib.lib().bf8_gemm_geglu_mxfp4(
-            _ptr(x), x.stride(0), _ptr(x_planes), _ptr(w), w.stride(0), _ptr(w_planes), M, I, K,
-            _ptr(hq.data), _ptr(hq.planes), _ptr(hq.data_t), _ptr(hq.planes_t), _ptr(GU),
-            _stream(dev)), "bf8_gemm_geglu_mxfp4")
+    hq = _new_mxfp4(M, I, True, colwise, x.device)
+    GU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=x.device) if keep_gu else None
+    if M and I:
+        _call("bf8_gemm_geglu_mxfp4", idx, _lib.lib().bf8_gemm_geglu_mxfp4, x.data_ptr(), x.stride(0),
+              x_planes.data_ptr(), w.data_ptr(), w.stride(0), w_planes.data_ptr(), M, I, K,
+              hq.data.data_ptr(), hq.planes.data_ptr(), _ptr(hq.data_t), _ptr(hq.planes_t), _ptr(GU))
     return hq, GU
 
 
@@ -1458,20 +1456,18 @@ def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
     """:func:`geglu_bwd` and the :func:`quantize_mxfp4` of its dGU [M, 2I] in one pass (the same
     codes and planes; the bf16 dGU is not written). I must be a multiple of 128."""
     who = "geglu_bwd_mxfp4"
-    dev = _one_device(who, dH, GU)
-    dH = _aligned(_bf16_2d(dH))
+    idx = _index_of(who, dH, GU)
+    dH = _rows_bf16(dH)
     M, I = dH.shape
-    GU = _aligned(_gu_operand(who, GU, M, I))
+    GU = _rows_bf16(_gu_operand(who, GU, M, I))
     if not (rowwise or colwise):
         raise ValueError(f"{who}: nothing requested")
     if I % 128:
         raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
-    q = _new_mxfp4(M, 2 * I, rowwise, colwise, dev)
-    if M:
-        with _On(dev):
-            _lib.check(_lib.lib().bf8_geglu_bwd_mxfp4(
-                _ptr(dH), _ptr(GU), M, I, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t),
-                _ptr(q.planes_t), _stream(dev)), "bf8_geglu_bwd_mxfp4")
+    q = _new_mxfp4(M, 2 * I, rowwise, colwise, dH.device)
+    if M and I:
+        _call("bf8_geglu_bwd_mxfp4", idx, _lib.lib().bf8_geglu_bwd_mxfp4, dH.data_ptr(), GU.data_ptr(),
+              M, I, _ptr(q.data), _ptr(q.planes), _ptr(q.data_t), _ptr(q.planes_t))
     return q
 
 
@@ -1479,26 +1475,12 @@ def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
 RESIDUAL_NORM_MAX_COLS = 16384
 
 
-def _residual_norm_args(who, rows_of, post_weight, pre_weight, gate):
-    """The row tensors (None kept) as contiguous 2-D bf16 of one shape and the weights, checked."""
-    dev = _one_device(who, *rows_of.values(), post_weight, pre_weight, gate)
-    shape, rows = None, {}
-    for name, t in rows_of.items():
-        if t is not None:
-            if shape is not None and tuple(t.shape) != shape:
-                raise ValueError(f"{who}: {name} must be {shape} (got {tuple(t.shape)})")
-            shape = tuple(t.shape)
-            t = _aligned(_bf16_2d(t))
-        rows[name] = t
-    cols = shape[-1]
-    weights = []
+def _norm_weights(who, cols, post_weight, pre_weight, gate):
     for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("gate", gate)):
-        if t is not None:
-            if t.dtype != torch.bfloat16 or tuple(t.shape) != (cols,):
-                raise ValueError(f"{who}: {name} must be bf16 [{cols}] (got {t.dtype} {tuple(t.shape)})")
-            t = _aligned(t.contiguous())
-        weights.append(t)
-    return dev, shape, rows, weights
+        if t is not None and (t.dtype is not torch.bfloat16 or t.shape != (cols,)):
+            raise ValueError(f"{who}: {name} must be bf16 [{cols}] (got {t.dtype} {tuple(t.shape)})")
+    return [t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0)
+            else t.contiguous().clone() for t in (post_weight, pre_weight, gate)]
 
 
 def rmsnorm_residual(h, residual, post_weight, pre_weight, eps, *, gate=None, residual_scale=1.0,
@@ -1508,17 +1490,24 @@ def rmsnorm_residual(h, residual, post_weight, pre_weight, eps, *, gate=None, re
     ``out = residual_scale * residual + gate * rmsnorm(h, post_weight)`` and
     ``y = rmsnorm(out, pre_weight)``; returns ``(out, y)``. ``gate``: bf16 [cols] or None (1)."""
     who = "rmsnorm_residual"
-    dev, shape, t, (post, pre, gate) = _residual_norm_args(
-        who, {"h": h, "residual": residual}, post_weight, pre_weight, gate)
-    h, residual = t["h"], t["residual"]
+    idx = _index_of(who, h, residual, post_weight, pre_weight, gate)
+    shape = h.shape
+    if residual.shape != shape:
+        raise ValueError(f"{who}: residual must be {tuple(shape)} (got {tuple(residual.shape)})")
+    post, pre, gate = _norm_weights(who, shape[-1], post_weight, pre_weight, gate)
+    h, residual = _rows_bf16(h), _rows_bf16(residual)
     rows, cols = h.shape
     out, y = torch.empty_like(h), torch.empty_like(h)
-    with _On(dev):
-        _lib.check(_lib.lib().bf8_rmsnorm_residual_bf16(
-            _ptr(h), _ptr(residual), rows, cols, _ptr(post), _ptr(pre), _ptr(gate),
-            float(residual_scale), float(eps), int(bool(zero_centered)), _ptr(out), _ptr(y),
-            _stream(dev)), "bf8_rmsnorm_residual_bf16")
-    return out.reshape(shape), y.reshape(shape)
+    if rows:
+        _call("bf8_rmsnorm_residual_bf16", idx, _lib.lib().bf8_rmsnorm_residual_bf16, h.data_ptr(),
+              residual.data_ptr(), rows, cols, post.data_ptr(), pre.data_ptr(), _ptr(gate),
+              residual_scale, eps, 1 if zero_centered else 0, out.data_ptr(), y.data_ptr())
+    return (out, y) if len(shape) == 2 else (out.view(shape), y.view(shape))
+
+
+@functools.lru_cache(maxsize=4096)
+def _residual_norm_ws_cached(rows, cols):
+    return int(_lib.lib().bf8_rmsnorm_residual_bwd_workspace(rows, cols))
 
 
 def rmsnorm_residual_backward(h, out, dout, dy, post_weight, pre_weight, eps, *, gate=None,
@@ -1530,26 +1519,32 @@ def rmsnorm_residual_backward(h, out, dout, dy, post_weight, pre_weight, eps, *,
     who = "rmsnorm_residual_backward"
     if dout is None and dy is None:
         raise ValueError(f"{who}: no gradient given")
-    dev, shape, t, (post, pre, gate) = _residual_norm_args(
-        who, {"h": h, "out": out, "dout": dout, "dy": dy}, post_weight, pre_weight, gate)
-    h, out, dout, dy = t["h"], t["out"], t["dout"], t["dy"]
+    idx = _index_of(who, h, out, dout, dy, post_weight, pre_weight, gate)
+    shape = h.shape
+    for name, t in (("out", out), ("dout", dout), ("dy", dy)):
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{who}: {name} must be {tuple(shape)} (got {tuple(t.shape)})")
+    post, pre, gate = _norm_weights(who, shape[-1], post_weight, pre_weight, gate)
+    h, out = _rows_bf16(h), _rows_bf16(out)
+    dout = dout if dout is None else _rows_bf16(dout)
+    dy = dy if dy is None else _rows_bf16(dy)
     rows, cols = h.shape
-    needs = tuple(needs[:4]) + (bool(needs[4]) and gate is not None,)
-    grads = [torch.empty_like(h) if n else None for n in needs[:2]]
-    grads += [torch.empty(cols, dtype=torch.bfloat16, device=dev) if n else None for n in needs[2:]]
-    if any(needs):
-        if rows == 0:
-            for g in grads[2:]:
-                if g is not None:
-                    g.zero_()
-        else:
-            L = _lib.lib()
-            nbytes = int(L.bf8_rmsnorm_residual_bwd_workspace(rows, cols)) if any(needs[2:]) else 0
-            ws, nbytes = _call_workspace(nbytes, dev)
-            with _On(dev):
-                _lib.check(L.bf8_rmsnorm_residual_bwd_bf16(
-                    _ptr(h), _ptr(out), _ptr(dout), _ptr(dy), rows, cols, _ptr(post), _ptr(pre),
-                    _ptr(gate), float(residual_scale), float(eps), int(bool(zero_centered)),
-                    *[_ptr(g) for g in grads], _ptr(ws), nbytes, _stream(dev)),
-                    "bf8_rmsnorm_residual_bwd_bf16")
-    return tuple(g.reshape(shape) if g is not None and i < 2 else g for i, g in enumerate(grads))
+    dh = torch.empty_like(h) if needs[0] else None
+    dres = torch.empty_like(h) if needs[1] else None
+    weights = [needs[2], needs[3], needs[4] and gate is not None]
+    dpost, dpre, dgate = [torch.empty_like(post) if n else None for n in weights]
+    if rows == 0:
+        for g in (dpost, dpre, dgate):
+            if g is not None:
+                g.zero_()
+    elif needs[0] or needs[1] or any(weights):
+        ws, nbytes = None, 0
+        if any(weights):
+            ws, nbytes = _call_workspace(_residual_norm_ws_cached(rows, cols), h)
+        _call("bf8_rmsnorm_residual_bwd_bf16", idx, _lib.lib().bf8_rmsnorm_residual_bwd_bf16,
+              h.data_ptr(), out.data_ptr(), _ptr(dout), _ptr(dy), rows, cols, post.data_ptr(),
+              pre.data_ptr(), _ptr(gate), residual_scale, eps, 1 if zero_centered else 0, _ptr(dh),
+              _ptr(dres), _ptr(dpost), _ptr(dpre), _ptr(dgate), _ptr(ws), nbytes)
+    if len(shape) != 2:
+        dh, dres = (g if g is None else g.view(shape) for g in (dh, dres))
+    return dh, dres, dpost, dpre, dgate
