@@ -21,30 +21,16 @@ __device__ __forceinline__ uint32_t mx4_exponent(uint32_t k) {
 }
 
 // 2^(e - 127) as the conversions take it: they read the exponent field alone, so that e = 0
-// stands for 2^-127 too.
+// stands for 2^-127 too (and 255 for a NaN, whatever the value).
 __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
-// Round-to-nearest-even onto the e2m1 grid, as the conversions do, for the blocks that hold inf or
-// NaN (a block with a NaN has no value: its codes are 0).
-__device__ __forceinline__ uint32_t mx4_code_slow(float x, uint32_t e) {
-  if (e == 0xFFu) return 0u;
-  const float p = x * (e == 0xFEu ? __uint_as_float(0x00400000u) : __uint_as_float((254u - e) << 23));
-  const float a = fabsf(p);
-  const uint32_t m = (uint32_t)(a > 0.25f) + (uint32_t)(a >= 0.75f) + (uint32_t)(a > 1.25f) +
-                     (uint32_t)(a >= 1.75f) + (uint32_t)(a > 2.5f) + (uint32_t)(a >= 3.5f) +
-                     (uint32_t)(a > 5.0f);
-  return m | ((__float_as_uint(p) >> 31) << 3);
-}
-
-// Byte B of c: the codes of a packed bf16 pair (low half in the low nibble).
+// Byte B of c: the codes of a packed bf16 pair (low half in the low nibble). The conversion rounds to
+// nearest even and takes an inf to 6; a block with a NaN (not FINITE alone) has no values, its codes are 0.
 template <int B, bool FINITE>
 __device__ __forceinline__ uint32_t mx4_pack2(uint32_t c, uint32_t pair, uint32_t e) {
-  if constexpr (FINITE)
-    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, pair),
-                                                     mx4_scale(e), B);
-  else
-    return c | ((mx4_code_slow(bf16_lo(pair), e) | (mx4_code_slow(bf16_hi(pair), e) << 4))
-                << (8 * B));
+  if (!FINITE && e == 0xFFu) pair = e = 0u;
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, __builtin_bit_cast(bf16x2_t, pair),
+                                                   mx4_scale(e), B);
 }
 
 // Where a quantizer writes: out [rows, cols / 2] with planes [(cols + 127) / 128][rows] (blocks
@@ -59,50 +45,89 @@ struct Mx4Out {
   uint32_t* planes_t;
 };
 
-// A tile of 32 W rows x 8 LPR columns, one wave per 32 rows: lane l holds columns 8 (l % LPR) ..
-// +7 of RL = LPR / 2 consecutive rows, RL (l / LPR) .. of its wave's 32 (v[k]: row k; zeros past
-// the tensor). A row block of 32 is four neighbouring lanes, a column block the lanes of one
-// column group, so both maxima are a few lane exchanges, and a lane's column codes are RL / 2
-// consecutive bytes of the columnwise copy. LPR = 32 and W = 8 write whole 128-byte lines of both
-// copies; a smaller tile gives a small tensor more waves.
-template <int LPR, int W>
-struct Mx4Tile {
-  static constexpr int kRows = 32 * W, kCols = 8 * LPR;
-  static constexpr int RL = LPR / 2;
-  static constexpr int kPitch = 16 * W + 4;  // bytes of a staged column (16 a wave)
-  struct Shared {
-    alignas(16) uint8_t rowsc[kRows][kCols / 32 < 4 ? 4 : kCols / 32];  // exponents by row block
-    alignas(16) uint8_t colsc[kCols][W < 4 ? 4 : W];                    // and by column block
-    alignas(16) uint8_t stage[kCols][kPitch];
-  };
+// A window of a tensor as a buffer: what lies past its `bytes` reads as zero and is not written, with no
+// branch around the access (each of which would wait for the load in it before the next is issued).
+constexpr uint32_t kPastEnd = 0x80000000u;  // an offset past the end of every window
+typedef __amdgpu_buffer_rsrc_t Window;
+__device__ __forceinline__ Window window(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ uint4 window_load(Window w, uint32_t off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)off, 0, 0));
+}
+
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// Per-half maxima of packed pairs over the lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them.
+__device__ __forceinline__ uint32_t mx4_groups_max(uint32_t m) {
+  u32x2_t s = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = pk_max_u16(s[0], s[1]);
+  s = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return pk_max_u16(s[0], s[1]);
+}
+
+// Transposes 4 x 4 dwords across the lane groups l / 16: register j of group g becomes what
+// register g of group j was.
+__device__ __forceinline__ void mx4_groups_transpose(uint32_t (&r)[4]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x2_t s = __builtin_amdgcn_permlane32_swap(r[i], r[i + 2], false, false);
+    r[i] = s[0];
+    r[i + 2] = s[1];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const u32x2_t s = __builtin_amdgcn_permlane16_swap(r[i], r[i + 1], false, false);
+    r[i] = s[0];
+    r[i + 1] = s[1];
+  }
+}
+
+// A wave's tile of 32 rows x 128 columns at (r0, c0): lane l holds columns 8 (l % 16) .. +7 of the
+// rows 8 (l / 16) .. +7 (v[k]: row k; zeros past the tensor). A row block of 32 is four
+// neighbouring lanes, a column block of 32 rows the four lanes of a column group, and a lane's column
+// codes are 4 consecutive bytes of the columnwise copy: a transpose of dwords across the lane groups
+// leaves every lane the 16 bytes of two whole column blocks. W waves of a block take tiles one below
+// the other (r0 is wave w's own). W = 1: those bytes go out as they are, no wave waits for another. W > 1:
+// they meet in LDS, and a column's leave as 16 W bytes side by side.
+constexpr int kMx4Rows = 32, kMx4Cols = 128;
+template <int W>
+struct Mx4Stage {
+  static constexpr int kPitch = W + 1;  // 16-byte chunks of a staged column
+  alignas(16) uint4 codes[W > 1 ? kMx4Cols * kPitch : 1];
+  alignas(4) uint8_t scales[W > 1 ? kMx4Cols : 1][W < 4 ? 4 : W];
 };
 
-template <int LPR, int W, bool FINITE>
-__device__ __forceinline__ void mx4_tile_body(const Mx4Out& p, int64_t r0, int64_t c0,
-                                              const uint4 (&v)[LPR / 2],
-                                              const uint32_t (&rk)[LPR / 2],
-                                              const uint32_t (&cm)[4],
-                                              typename Mx4Tile<LPR, W>::Shared& sh, int wid,
+template <int W, bool FINITE>
+__device__ __forceinline__ void mx4_wave_body(const Mx4Out& p, int64_t r0, int64_t c0,
+                                              const uint4 (&v)[8], const uint32_t (&rk)[8],
+                                              const uint32_t (&cm)[4], Mx4Stage<W>* sh, int wid,
                                               int lane) {
-  constexpr int RL = LPR / 2;
-  const int cl = lane % LPR, rg = lane / LPR;
-  const int64_t c = c0 + 8 * cl;
-  const int lrow = 32 * wid + RL * rg;  // the lane's first row in the tile
-  if (p.out) {
+  const int cl = lane & 15, g = lane >> 4;
+  const int64_t c = c0 + 8 * cl, r = r0 + 8 * g;
+  if (p.out && r0 < p.rows) {
+    // the tile's rows, cols / 2 bytes each
+    const uint32_t ld = (uint32_t)(p.cols >> 1), left = (uint32_t)min(p.rows - r0, (int64_t)kMx4Rows);
+    const Window w = window(p.out + r0 * (p.cols >> 1), left * ld);
+    const uint32_t o = c < p.cols ? 8 * g * ld + (uint32_t)(c >> 1) : kPastEnd;
+    uint32_t mine = 0;  // the scale dword of row r + cl, in the lanes cl < 8
 #pragma unroll
-    for (int k = 0; k < RL; ++k) {
-      const int64_t r = r0 + lrow + k;
-      const uint32_t e = FINITE ? mx4_exponent_finite(rk[k]) : mx4_exponent(rk[k]);
+    for (int k = 0; k < 8; ++k) {
+      uint32_t e = FINITE ? mx4_exponent_finite(rk[k]) : mx4_exponent(rk[k]);
       uint32_t q = 0;
       q = mx4_pack2<0, FINITE>(q, v[k].x, e);
       q = mx4_pack2<1, FINITE>(q, v[k].y, e);
       q = mx4_pack2<2, FINITE>(q, v[k].z, e);
       q = mx4_pack2<3, FINITE>(q, v[k].w, e);
-      if (r < p.rows && c < p.cols)
-        *reinterpret_cast<uint32_t*>(p.out + ((r * p.cols + c) >> 1)) = q;
-      if ((cl & 3) == 0)
-        sh.rowsc[lrow + k][cl >> 2] = c < p.cols ? (uint8_t)e : (uint8_t)kMxPadScale;
+      __builtin_amdgcn_raw_buffer_store_b32(q, w, (int)(o + k * ld), 0, 0);
+      if (c >= p.cols) e = kMxPadScale;  // blocks past the row pad its last dword of scales
+      // the row's four blocks, four lanes apart: rotations by 4 and by 8 within 16 lanes
+      e <<= 8 * (cl >> 2);
+      e |= (uint32_t)__builtin_amdgcn_mov_dpp((int)e, 0x124, 0xF, 0xF, true);
+      e |= (uint32_t)__builtin_amdgcn_mov_dpp((int)e, 0x128, 0xF, 0xF, true);
+      if (cl == k) mine = e;
     }
+    if (cl < 8 && r + cl < p.rows) p.planes[(c0 >> 7) * p.rows + r + cl] = mine;
   }
   if (!p.out_t) return;
   uint32_t e[8];
@@ -111,58 +136,57 @@ __device__ __forceinline__ void mx4_tile_body(const Mx4Out& p, int64_t r0, int64
     e[2 * i] = FINITE ? mx4_exponent_finite(cm[i] & 0xFFFFu) : mx4_exponent(cm[i] & 0xFFFFu);
     e[2 * i + 1] = FINITE ? mx4_exponent_finite(cm[i] >> 16) : mx4_exponent(cm[i] >> 16);
   }
+  const int64_t ldt = ((p.rows + 31) >> 5) * 16;
+  const int64_t blk = r0 >> 5, nblk = (p.rows + 31) >> 5;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {  // column pair 2 i, 2 i + 1
-    uint32_t lo[RL / 8 < 1 ? 1 : RL / 8] = {}, hi[RL / 8 < 1 ? 1 : RL / 8] = {};
+  for (int h = 0; h < 2; ++h) {  // columns 4 h .. 4 h + 3 of the lane's eight
+    uint32_t q[4];
 #pragma unroll
-    for (int k = 0; k < RL; k += 2) {
-      const uint32_t a = i == 0 ? v[k].x : i == 1 ? v[k].y : i == 2 ? v[k].z : v[k].w;
-      const uint32_t b = i == 0 ? v[k + 1].x : i == 1 ? v[k + 1].y : i == 2 ? v[k + 1].z : v[k + 1].w;
-      const uint32_t p0 = __byte_perm(a, b, 0x5410), p1 = __byte_perm(a, b, 0x7632);
-      uint32_t& x = lo[k / 8];
-      uint32_t& y = hi[k / 8];
-      switch ((k / 2) & 3) {
-        case 0: x = mx4_pack2<0, FINITE>(x, p0, e[2 * i]); y = mx4_pack2<0, FINITE>(y, p1, e[2 * i + 1]); break;
-        case 1: x = mx4_pack2<1, FINITE>(x, p0, e[2 * i]); y = mx4_pack2<1, FINITE>(y, p1, e[2 * i + 1]); break;
-        case 2: x = mx4_pack2<2, FINITE>(x, p0, e[2 * i]); y = mx4_pack2<2, FINITE>(y, p1, e[2 * i + 1]); break;
-        default: x = mx4_pack2<3, FINITE>(x, p0, e[2 * i]); y = mx4_pack2<3, FINITE>(y, p1, e[2 * i + 1]); break;
-      }
+    for (int i = 0; i < 2; ++i) {
+      uint32_t w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        w[k] = h == 0 ? (i == 0 ? v[k].x : v[k].y) : (i == 0 ? v[k].z : v[k].w);
+      const uint32_t ea = e[4 * h + 2 * i], eb = e[4 * h + 2 * i + 1];
+      uint32_t x = 0, y = 0;
+      x = mx4_pack2<0, FINITE>(x, __byte_perm(w[0], w[1], 0x5410), ea);
+      y = mx4_pack2<0, FINITE>(y, __byte_perm(w[0], w[1], 0x7632), eb);
+      x = mx4_pack2<1, FINITE>(x, __byte_perm(w[2], w[3], 0x5410), ea);
+      y = mx4_pack2<1, FINITE>(y, __byte_perm(w[2], w[3], 0x7632), eb);
+      x = mx4_pack2<2, FINITE>(x, __byte_perm(w[4], w[5], 0x5410), ea);
+      y = mx4_pack2<2, FINITE>(y, __byte_perm(w[4], w[5], 0x7632), eb);
+      x = mx4_pack2<3, FINITE>(x, __byte_perm(w[6], w[7], 0x5410), ea);
+      y = mx4_pack2<3, FINITE>(y, __byte_perm(w[6], w[7], 0x7632), eb);
+      q[2 * i] = x;
+      q[2 * i + 1] = y;
     }
-    uint8_t* s0 = &sh.stage[8 * cl + 2 * i][16 * wid + rg * (RL / 2)];
-    uint8_t* s1 = &sh.stage[8 * cl + 2 * i + 1][16 * wid + rg * (RL / 2)];
-    if constexpr (RL >= 8) {
-#pragma unroll
-      for (int j = 0; j < RL / 8; ++j) {
-        reinterpret_cast<uint32_t*>(s0)[j] = lo[j];
-        reinterpret_cast<uint32_t*>(s1)[j] = hi[j];
-      }
-    } else {
-      *reinterpret_cast<uint16_t*>(s0) = (uint16_t)lo[0];
-      *reinterpret_cast<uint16_t*>(s1) = (uint16_t)hi[0];
+    mx4_groups_transpose(q);
+    const int64_t col = c + 4 * h + g;  // the lane's own after the transpose
+    uint32_t es = (e[4 * h] | (e[4 * h + 1] << 8) | (e[4 * h + 2] << 16) | (e[4 * h + 3] << 24)) >> (8 * g);
+    if constexpr (W > 1) {
+      const int lc = 8 * cl + 4 * h + g;
+      sh->codes[lc * Mx4Stage<W>::kPitch + wid] = make_uint4(q[0], q[1], q[2], q[3]);
+      sh->scales[lc][wid] = r0 < p.rows ? (uint8_t)es : (uint8_t)kMxPadScale;
+    } else if (c < p.cols) {
+      *reinterpret_cast<uint4*>(p.out_t + col * ldt + 16 * blk) = make_uint4(q[0], q[1], q[2], q[3]);
+      uint8_t* d = reinterpret_cast<uint8_t*>(p.planes_t + (blk >> 2) * p.cols + col);
+      d[blk & 3] = (uint8_t)es;
+      if (blk == nblk - 1)  // a column's last block fills up its dword
+        for (int b = (int)(blk & 3) + 1; b < 4; ++b) d[b] = (uint8_t)kMxPadScale;
     }
-  }
-  if (rg == 0) {
-    const bool valid = r0 + 32 * wid < p.rows;
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      sh.colsc[8 * cl + j][wid] = valid ? (uint8_t)e[j] : (uint8_t)kMxPadScale;
   }
 }
 
-// The loaded tile at (r0, c0), by the W waves of a block (wid 0 .. W - 1), each of which calls it
-// alike. W < 4: planes_t's dword is written a byte at a time, and the wave of a tensor's last
-// block fills the absent ones of its dword.
-template <int LPR, int W>
-__device__ __forceinline__ void mx4_tile_finish(const Mx4Out& p, int64_t r0, int64_t c0,
-                                                const uint4 (&v)[LPR / 2],
-                                                typename Mx4Tile<LPR, W>::Shared& sh, int wid,
-                                                int lane) {
-  using T = Mx4Tile<LPR, W>;
-  constexpr int RL = LPR / 2;
-  uint32_t rk[RL], cm[4] = {};
+// The loaded tile. W > 1: every wave of the W calls it alike (wid: which), also one past the
+// tensor, with a stage of their own; before the stage's next use the caller waits for them.
+template <int W>
+__device__ __forceinline__ void mx4_wave_tile(const Mx4Out& p, int64_t r0, int64_t c0,
+                                              const uint4 (&v)[8], Mx4Stage<W>* sh, int wid,
+                                              int lane) {
+  uint32_t rk[8], cm[4] = {};
   uint32_t top = 0;
 #pragma unroll
-  for (int k = 0; k < RL; ++k) {
+  for (int k = 0; k < 8; ++k) {
     const uint32_t a[4] = {v[k].x & 0x7FFF7FFFu, v[k].y & 0x7FFF7FFFu, v[k].z & 0x7FFF7FFFu,
                            v[k].w & 0x7FFF7FFFu};
 #pragma unroll
@@ -175,76 +199,34 @@ __device__ __forceinline__ void mx4_tile_finish(const Mx4Out& p, int64_t r0, int
   }
   if (p.out_t) {
 #pragma unroll
-    for (int off = LPR; off < 64; off <<= 1)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        cm[i] = pk_max_u16(cm[i], (uint32_t)__shfl_xor((int)cm[i], off, 64));
+    for (int i = 0; i < 4; ++i) cm[i] = mx4_groups_max(cm[i]);
   }
   if (__builtin_expect(__any(top >= 0x7F80u), 0))
-    mx4_tile_body<LPR, W, false>(p, r0, c0, v, rk, cm, sh, wid, lane);
+    mx4_wave_body<W, false>(p, r0, c0, v, rk, cm, sh, wid, lane);
   else
-    mx4_tile_body<LPR, W, true>(p, r0, c0, v, rk, cm, sh, wid, lane);
-  __syncthreads();
-  const int tid = 64 * wid + lane;
-  if (p.out) {
-    // the rows' scale dwords: consecutive rows of a plane by consecutive lanes
-    constexpr int G = T::kCols / 128;  // planes a tile spans (0: part of one)
-    if constexpr (G > 0) {
-      for (int i = tid; i < T::kRows * G; i += 64 * W) {
-        const int row = i % T::kRows, g = i / T::kRows;
-        if (r0 + row < p.rows && c0 + 128 * g < p.cols)
-          p.planes[((c0 >> 7) + g) * p.rows + r0 + row] =
-              *reinterpret_cast<const uint32_t*>(&sh.rowsc[row][4 * g]);
-      }
-    } else {
-      constexpr int B = T::kCols / 32;
-      const int64_t nblk = p.cols >> 5;
-      for (int i = tid; i < T::kRows * B; i += 64 * W) {
-        const int row = i / B, b = i % B;
-        const int64_t blk = (c0 >> 5) + b;
-        if (r0 + row < p.rows && blk < nblk) {
-          uint8_t* d = reinterpret_cast<uint8_t*>(p.planes + (blk >> 2) * p.rows + r0 + row);
-          d[blk & 3] = sh.rowsc[row][b];
-          if (blk == nblk - 1)  // the row's last block fills up its dword
-            for (int64_t x = (blk & 3) + 1; x < 4; ++x) d[x] = (uint8_t)kMxPadScale;
-        }
-      }
+    mx4_wave_body<W, true>(p, r0, c0, v, rk, cm, sh, wid, lane);
+  if constexpr (W > 1) {
+    if (!p.out_t) return;
+    __syncthreads();
+    const int64_t rb = r0 - kMx4Rows * wid;  // the first wave's
+    const int64_t ldt = ((p.rows + 31) >> 5) * 16;
+    const int tid = 64 * wid + lane;
+    // chunk t % W of columns t / W, ..
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int col = tid / W + 64 * i, ch = tid % W;
+      if (c0 + col < p.cols && rb + kMx4Rows * ch < p.rows)
+        *reinterpret_cast<uint4*>(p.out_t + (c0 + col) * ldt + (rb >> 1) + 16 * ch) =
+            sh->codes[col * Mx4Stage<W>::kPitch + ch];
+    }
+    static_assert(W % 4 == 0, "whole dwords of scales");
+    if (tid < kMx4Cols * (W / 4)) {
+      const int col = tid % kMx4Cols, gr = tid / kMx4Cols;
+      if (c0 + col < p.cols && rb + 128 * gr < p.rows)
+        p.planes_t[((rb >> 7) + gr) * p.cols + c0 + col] =
+            *reinterpret_cast<const uint32_t*>(&sh->scales[col][4 * gr]);
     }
   }
-  if (p.out_t) {
-    const int64_t rowsp = (p.rows + 31) & ~31LL;
-    constexpr int CH = W;  // 16-byte chunks of a staged column
-    for (int i = tid; i < T::kCols * CH; i += 64 * W) {
-      const int col = i / CH, ch = i % CH;
-      if (c0 + col < p.cols && r0 + 32 * ch < p.rows) {
-        const uint32_t* s = reinterpret_cast<const uint32_t*>(&sh.stage[col][16 * ch]);
-        *reinterpret_cast<uint4*>(p.out_t + (c0 + col) * (rowsp >> 1) + (r0 >> 1) + 16 * ch) =
-            make_uint4(s[0], s[1], s[2], s[3]);
-      }
-    }
-    constexpr int G = W / 4;
-    if constexpr (G > 0) {
-      for (int i = tid; i < T::kCols * G; i += 64 * W) {
-        const int col = i % T::kCols, g = i / T::kCols;
-        if (c0 + col < p.cols && r0 + 128 * g < p.rows)
-          p.planes_t[((r0 >> 7) + g) * p.cols + c0 + col] =
-              *reinterpret_cast<const uint32_t*>(&sh.colsc[col][4 * g]);
-      }
-    } else {
-      const int64_t nblk = rowsp >> 5;
-      for (int i = tid; i < T::kCols * W; i += 64 * W) {
-        const int col = i % T::kCols, b = i / T::kCols;
-        const int64_t blk = (r0 >> 5) + b;
-        if (c0 + col < p.cols && blk < nblk) {
-          uint8_t* d = reinterpret_cast<uint8_t*>(p.planes_t + (blk >> 2) * p.cols + c0 + col);
-          d[blk & 3] = sh.colsc[col][b];
-          if (blk == nblk - 1)
-            for (int64_t x = (blk & 3) + 1; x < 4; ++x) d[x] = (uint8_t)kMxPadScale;
-        }
-      }
-    }
-  }
-  __syncthreads();
 }
 
 }  // namespace bf8

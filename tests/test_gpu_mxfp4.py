@@ -512,3 +512,35 @@ def test_gated_product_on_every_tile(gpu, monkeypatch, tile, M, K, I):
     want = ops.quantize_mxfp4(ops.geglu(GU)[0], colwise=True)
     assert torch.equal(hq.planes, want.planes) and torch.equal(hq.data, want.data)
     assert torch.equal(hq.planes_t, want.planes_t) and torch.equal(hq.data_t, want.data_t)
+
+
+@pytest.mark.parametrize("rows,cols", [(3300, 2560), (8193, 1096), (13000, 2592), (16416, 2080)])
+def test_quantize_both_copies_of_large_tensors(gpu, rows, cols):
+    """The block tilings of large tensors (past 8M and 32M elements): ragged rows and columns, special
+    blocks; the copies alone are the same."""
+    x = _special(rows, cols, 7)
+    rowwise = cols % 32 == 0
+    q = ops.quantize_mxfp4(x.to(gpu), rowwise=rowwise, colwise=True)
+    if rowwise:
+        codes, e = mx4.quantize(x)
+        assert torch.equal(q.planes.cpu(), mx4.planes(e)) and torch.equal(q.data.cpu(), codes)
+    codes, e = mx4.quantize(x, 0)
+    assert torch.equal(q.planes_t.cpu(), mx4.planes(e)) and torch.equal(q.data_t.cpu(), codes)
+    only = ops.quantize_mxfp4(x.to(gpu), rowwise=False, colwise=True)
+    assert torch.equal(only.data_t, q.data_t) and torch.equal(only.planes_t, q.planes_t)
+
+
+def test_gated_backward_takes_every_gate(gpu):
+    """Gates outside the gelu tables (zeros, tiny, 8 and above, inf, NaN) in some rows and all of them."""
+    g = torch.Generator().manual_seed(3)
+    for M, I in ((70, 256), (3300, 2560)):
+        GU = torch.randn(M, 2 * I, generator=g).to(torch.bfloat16)
+        GU[::7, :I] = 0.0
+        GU[3, :8] = torch.tensor([8.0, -8.0, 100.0, -100.0, float("inf"), -float("inf"), float("nan"), 1e-38])
+        GU[5, : I // 2] *= 1e-6
+        dH = (torch.randn(M, I, generator=g) * 1e-2).to(torch.bfloat16)
+        GU, dH = GU.to(gpu), dH.to(gpu)
+        want = ops.quantize_mxfp4(ops.geglu_bwd(dH, GU)[0], colwise=True)
+        q = ops.geglu_bwd_mxfp4(dH, GU, colwise=True)
+        assert torch.equal(q.data, want.data) and torch.equal(q.planes, want.planes)
+        assert torch.equal(q.data_t, want.data_t) and torch.equal(q.planes_t, want.planes_t)
