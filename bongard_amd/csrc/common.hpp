@@ -461,4 +461,19 @@ __device__ inline float delayed_scale_block(float* __restrict__ state, int len, 
   return s_scale;
 }
 
+// A window of a tensor as a buffer: what lies past its `bytes` reads as zero and is not written, with no
+// branch around the access (each of which would wait for the load in it before the next is issued).
+constexpr uint32_t kPastEnd = 0x80000000u;  // an offset past the end of every window
+typedef __amdgpu_buffer_rsrc_t Window;
+__device__ __forceinline__ Window window(const void* base, uint32_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ uint4 window_load(Window w, uint32_t off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)off, 0, 0));
+}
+__device__ __forceinline__ void window_store(Window w, uint32_t off, uint4 v) {
+  typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), w, (int)off, 0, 0);
+}
+
 }  // namespace bf8

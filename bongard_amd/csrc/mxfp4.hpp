@@ -45,17 +45,6 @@ struct Mx4Out {
   uint32_t* planes_t;
 };
 
-// A window of a tensor as a buffer: what lies past its `bytes` reads as zero and is not written, with no
-// branch around the access (each of which would wait for the load in it before the next is issued).
-constexpr uint32_t kPastEnd = 0x80000000u;  // an offset past the end of every window
-typedef __amdgpu_buffer_rsrc_t Window;
-__device__ __forceinline__ Window window(const void* base, uint32_t bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
-}
-__device__ __forceinline__ uint4 window_load(Window w, uint32_t off) {
-  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)off, 0, 0));
-}
-
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
 // Per-half maxima of packed pairs over the lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them.

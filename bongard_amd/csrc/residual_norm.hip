@@ -15,6 +15,16 @@
 //   dpre = bf16(P), P = sum over rows of dy n2;   dpost = bf16(g S), dgate = bf16((z + post) S),
 //   S = sum over rows of d n1
 // Sums over rows go through per-block partials added in a fixed order (deterministic).
+//
+// Both are bound by memory: 8 bytes an element forward and 12 backward, one read and one write of
+// each tensor. A row is held in registers across its two sums, up to 2,560 columns by one wave (no
+// barrier), wider ones by a block. Accesses go through a buffer descriptor of the row, which
+// drops what lies past its end without a branch: behind a branch each load was waited for before
+// the next. The backward also holds the column sums of its block (16 registers per 8 columns); with the
+// weights read from LDS where they are used and bf16 pairs unpacked anew in each pass it takes 251
+// registers at 2,560 columns, two waves a SIMD (held as floats: 471, one wave).
+// Measured, 18,494 x 2,560: forward 74 us, 5.1 TB/s; backward with the weights' gradients 122 us,
+// 4.7 TB/s (140 with the weights in registers). 3,001 x 2,560: 12.3 and 27 us (13.7 and 42).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -25,7 +35,11 @@ namespace bf8 {
 namespace {
 
 constexpr int kMaxCols = 16384;
-constexpr int64_t kMaxFwdBlocks = 2048, kMaxBwdBlocks = 512;
+constexpr int64_t kMaxFwdBlocks = 2048;
+// The backward's blocks: those resident at once (two a CU, or one of 16 waves), as each adds a
+// partial row to the weights' sums. 768 instead of 512: 135 us for 124 at 18,494 x 2,560; 256: 118 for
+// 122 there but 58 for 48 at 4,096 x 4,096. 512 instead of 256 of the wide ones: 120 us for 107 (4,096 x 8,192).
+constexpr int64_t max_bwd_blocks(int64_t cols) { return cols <= 4096 ? 512 : 256; }
 
 struct ResNorm {
   const uint16_t *h, *res, *post, *pre, *gate;  // backward: res is the forward's out
@@ -63,16 +77,22 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*red)[WPR]) {
   }
 }
 
+// Row `row` of a [rows, cols] tensor: past its end, and anywhere in one that is NULL, it reads as zeros.
+__device__ __forceinline__ Window row_of(const uint16_t* p, int64_t row, int cols) {
+  return window(p + row * cols, p ? 2u * cols : 0u);
+}
+
+// The thread's V pieces of a row lie 64 WPR pieces of 16 bytes apart.
 template <int V, int WPR>
-__device__ __forceinline__ void load_vecs(const uint16_t* __restrict__ p, int64_t row, int cols,
-                                          int t, uint4 (&v)[V]) {
-  const int nvec = cols >> 3;
-  const uint4* s = reinterpret_cast<const uint4*>(p + row * cols);
+__device__ __forceinline__ void load_row(Window w, int t, uint4 (&v)[V]) {
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int i = t + 64 * WPR * j;
-    v[j] = i < nvec ? s[i] : make_uint4(0u, 0u, 0u, 0u);
-  }
+  for (int j = 0; j < V; ++j) v[j] = window_load(w, 16u * (t + 64 * WPR * j));
+}
+
+// From here on the compiler knows nothing of v, so that it unpacks it again where it is used next
+// and does not hold two floats for each of its dwords.
+__device__ __forceinline__ void keep_packed(uint4& v) {
+  asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
 }
 
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
@@ -96,17 +116,19 @@ template <int V, int WPR>
 __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_kernel(ResNorm p) {
   __shared__ float red[2][1][WPR];
   const int t = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int nvec = p.cols >> 3;
-  const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * 4 + wid : blockIdx.x;
   const int64_t stride = WPR == 1 ? (int64_t)gridDim.x * 4 : gridDim.x;
+  const float one = p.gate ? 0.0f : 1.0f;  // the gate that is not there
   uint4 post[V], pre[V], gate[V];
-  load_vecs<V, WPR>(p.post, 0, p.cols, t, post);
-  load_vecs<V, WPR>(p.pre, 0, p.cols, t, pre);
-  if (p.gate) load_vecs<V, WPR>(p.gate, 0, p.cols, t, gate);
+  load_row<V, WPR>(row_of(p.post, 0, p.cols), t, post);
+  load_row<V, WPR>(row_of(p.pre, 0, p.cols), t, pre);
+  load_row<V, WPR>(row_of(p.gate, 0, p.cols), t, gate);
   for (int64_t row = first; row < p.rows; row += stride) {
     uint4 h[V], r[V];
-    load_vecs<V, WPR>(p.h, row, p.cols, t, h);
-    load_vecs<V, WPR>(p.res, row, p.cols, t, r);
+    load_row<V, WPR>(row_of(p.h, row, p.cols), t, h);
+    load_row<V, WPR>(row_of(p.res, row, p.cols), t, r);
+    const Window out = row_of(p.out, row, p.cols), y = row_of(p.y, row, p.cols);
     float ss[1] = {0.0f};
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -121,52 +143,76 @@ __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_kernel(ResNo
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float x[8], w[8], s[8], o[8], g[8];
+      keep_packed(h[j]);
+      keep_packed(post[j]);
+      keep_packed(gate[j]);
       unpack8(h[j], x);
       unpack8(post[j], w);
       unpack8(r[j], s);
-      if (p.gate) unpack8(gate[j], g);
+      unpack8(gate[j], g);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float n = (x[e] * r1) * (p.z + w[e]);
-        if (p.gate) n *= g[e];
-        o[e] = fmaf(p.scale, s[e], n);
-      }
+      for (int e = 0; e < 8; ++e)
+        o[e] = fmaf(p.scale, s[e], ((x[e] * r1) * (p.z + w[e])) * (one + g[e]));
       h[j] = pack8(o);
       unpack8(h[j], o);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss[0] = fmaf(o[e], o[e], ss[0]);
-      const int i = t + 64 * WPR * j;
-      if (i < nvec) reinterpret_cast<uint4*>(p.out + row * p.cols)[i] = h[j];
+      window_store(out, 16u * (t + 64 * WPR * j), h[j]);
     }
     row_sum<1, WPR>(ss, red[1]);
     const float r2 = rstd_of(ss[0], p.cols, p.eps);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       float o[8], w[8];
+      keep_packed(h[j]);
+      keep_packed(pre[j]);
       unpack8(h[j], o);
       unpack8(pre[j], w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = (o[e] * r2) * (p.z + w[e]);
-      const int i = t + 64 * WPR * j;
-      if (i < nvec) reinterpret_cast<uint4*>(p.y + row * p.cols)[i] = pack8(o);
+      window_store(y, 16u * (t + 64 * WPR * j), pack8(o));
     }
   }
+}
+
+// Whether the backward keeps the weights in LDS (6 bytes a column, 48 KB at most).
+constexpr bool weights_in_lds(int v, int wpr) { return v * wpr <= 16; }
+constexpr size_t bwd_lds(int v, int wpr, int64_t cols) {
+  const size_t w = weights_in_lds(v, wpr) ? (size_t)cols * 3 * sizeof(uint16_t) : 0;
+  const size_t sums = wpr == 1 ? (size_t)2 * v * 64 * 16 * sizeof(float) : 0;
+  return w > sums ? w : sums;
 }
 
 template <int V, int WPR>
 __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_bwd_kernel(ResNorm p) {
   __shared__ float red[2][3][WPR];
-  extern __shared__ float colsum[];  // [cols]
+  constexpr bool kLds = weights_in_lds(V, WPR);
+  extern __shared__ uint4 dyn[];  // (kLds) post, pre and gate; then (WPR 1) two waves' column sums
   const int t = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
-  const int wid = threadIdx.x >> 6;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nvec = p.cols >> 3;
   const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * 4 + wid : blockIdx.x;
   const int64_t stride = WPR == 1 ? (int64_t)gridDim.x * 4 : gridDim.x;
   const float inv = 1.0f / (float)p.cols;
-  uint4 post[V], pre[V], gate[V];
-  load_vecs<V, WPR>(p.post, 0, p.cols, t, post);
-  load_vecs<V, WPR>(p.pre, 0, p.cols, t, pre);
-  if (p.gate) load_vecs<V, WPR>(p.gate, 0, p.cols, t, gate);
+  const float one = p.gate ? 0.0f : 1.0f;  // the gate that is not there
+  const Window weights[3] = {row_of(p.post, 0, p.cols), row_of(p.pre, 0, p.cols),
+                             row_of(p.gate, 0, p.cols)};
+  if constexpr (kLds) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      for (int i = threadIdx.x; i < nvec; i += block_threads(WPR))
+        dyn[k * nvec + i] = window_load(weights[k], 16u * i);
+    __syncthreads();
+  }
+  // piece j of weight k, read where it is used: its floats, or all the pieces of a wide row, would
+  // not fit beside the sums
+  auto weight = [&](int k, int j, float (&f)[8]) __attribute__((always_inline)) {
+    const int i = t + 64 * WPR * j;
+    if constexpr (kLds)
+      unpack8(dyn[k * nvec + (i < nvec ? i : 0)], f);
+    else
+      unpack8(window_load(weights[k], 16u * i), f);
+  };
   float accp[V][8], accs[V][8];
 #pragma unroll
   for (int j = 0; j < V; ++j)
@@ -174,20 +220,20 @@ __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_bwd_kernel(R
     for (int e = 0; e < 8; ++e) accp[j][e] = accs[j][e] = 0.0f;
   for (int64_t row = first; row < p.rows; row += stride) {
     uint4 h[V], o[V], dy[V], dout[V];
-    load_vecs<V, WPR>(p.h, row, p.cols, t, h);
-    load_vecs<V, WPR>(p.res, row, p.cols, t, o);
-#pragma unroll
-    for (int j = 0; j < V; ++j) dy[j] = dout[j] = make_uint4(0u, 0u, 0u, 0u);
-    if (p.dy) load_vecs<V, WPR>(p.dy, row, p.cols, t, dy);
-    if (p.dout) load_vecs<V, WPR>(p.dout, row, p.cols, t, dout);
+    load_row<V, WPR>(row_of(p.h, row, p.cols), t, h);
+    load_row<V, WPR>(row_of(p.res, row, p.cols), t, o);
+    load_row<V, WPR>(row_of(p.dy, row, p.cols), t, dy);
+    load_row<V, WPR>(row_of(p.dout, row, p.cols), t, dout);
+    const Window dres = row_of(p.dres, row, p.cols), dh = row_of(p.dh, row, p.cols);
     float s[3] = {0.0f, 0.0f, 0.0f};  // sums of h^2, out^2, dy (z + pre) out
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      asm volatile("" ::: "memory");
       float x[8], n[8], g[8], w[8];
       unpack8(h[j], x);
       unpack8(o[j], n);
       unpack8(dy[j], g);
-      unpack8(pre[j], w);
+      weight(1, j, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         s[0] = fmaf(x[e], x[e], s[0]);
@@ -202,14 +248,18 @@ __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_bwd_kernel(R
     float dd[V][8];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
+      asm volatile("" ::: "memory");
+      keep_packed(h[j]);
+      keep_packed(o[j]);
+      keep_packed(dy[j]);
       float x[8], n[8], g[8], w[8], u[8], b[8], ga[8];
       unpack8(h[j], x);
       unpack8(o[j], n);
       unpack8(dy[j], g);
-      unpack8(pre[j], w);
       unpack8(dout[j], u);
-      unpack8(post[j], b);
-      if (p.gate) unpack8(gate[j], ga);
+      weight(0, j, b);
+      weight(1, j, w);
+      weight(2, j, ga);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float n2 = n[e] * r2;
@@ -217,61 +267,76 @@ __global__ __launch_bounds__(block_threads(WPR)) void residual_norm_bwd_kernel(R
         const float d = u[e] + r2 * (g[e] * (p.z + w[e]) - n2 * m2);
         accs[j][e] = fmaf(d, x[e] * r1, accs[j][e]);
         u[e] = p.scale * d;
-        dd[j][e] = d * (p.z + b[e]);
-        if (p.gate) dd[j][e] *= ga[e];
+        dd[j][e] = (d * (p.z + b[e])) * (one + ga[e]);
         q[0] = fmaf(dd[j][e], x[e], q[0]);
       }
-      const int i = t + 64 * WPR * j;
-      if (p.dres && i < nvec) reinterpret_cast<uint4*>(p.dres + row * p.cols)[i] = pack8(u);
+      window_store(dres, 16u * (t + 64 * WPR * j), pack8(u));
     }
     row_sum<1, WPR>(q, red[1]);
     const float m1 = q[0] * r1 * inv;  // mean(e n1)
-    if (p.dh) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float x[8];
-        unpack8(h[j], x);
+    for (int j = 0; j < V; ++j) {
+      keep_packed(h[j]);
+      float x[8];
+      unpack8(h[j], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = r1 * (dd[j][e] - (x[e] * r1) * m1);
-        const int i = t + 64 * WPR * j;
-        if (i < nvec) reinterpret_cast<uint4*>(p.dh + row * p.cols)[i] = pack8(x);
-      }
+      for (int e = 0; e < 8; ++e) x[e] = r1 * (dd[j][e] - (x[e] * r1) * m1);
+      window_store(dh, 16u * (t + 64 * WPR * j), pack8(x));
     }
   }
   if (!p.part) return;
-  float* dst = p.part + (int64_t)blockIdx.x * 2 * p.cols;
-  if constexpr (WPR > 1) {
+  auto write_sums = [&]() __attribute__((always_inline)) {
+    float* dst = p.part + (int64_t)blockIdx.x * 2 * p.cols;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int i = t + 64 * WPR * j;
       if (i >= nvec) continue;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        dst[8 * i + e] = accp[j][e];
-        dst[p.cols + 8 * i + e] = accs[j][e];
+      for (int h = 0; h < 4; ++h) {
+        const float(&a)[8] = h < 2 ? accp[j] : accs[j];
+        *reinterpret_cast<float4*>(dst + (h < 2 ? 0 : p.cols) + 8 * i + 4 * (h & 1)) =
+            make_float4(a[4 * (h & 1)], a[4 * (h & 1) + 1], a[4 * (h & 1) + 2], a[4 * (h & 1) + 3]);
       }
     }
+  };
+  if constexpr (WPR > 1) {
+    write_sums();
   } else {
-    // the block's four waves add their sums in order
+    // the block's four waves, done with the weights, add their sums: 2 to 0 and 3 to 1, then 1 to 0
+    float4* sums = reinterpret_cast<float4*>(dyn);
+    auto give = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      for (int w = 0; w < 4; ++w) {
-        if (wid == w) {
+      for (int j = 0; j < V; ++j)
 #pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const int i = t + 64 * j;
-            if (i >= nvec) continue;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float a = which == 0 ? accp[j][e] : accs[j][e];
-              colsum[8 * i + e] = w == 0 ? a : colsum[8 * i + e] + a;
-            }
-          }
+        for (int h = 0; h < 4; ++h) {
+          const float(&a)[8] = h < 2 ? accp[j] : accs[j];
+          sums[(to * 4 * V + 4 * j + h) * 64 + t] =
+              make_float4(a[4 * (h & 1)], a[4 * (h & 1) + 1], a[4 * (h & 1) + 2], a[4 * (h & 1) + 3]);
         }
-        __syncthreads();
-      }
-      for (int c = threadIdx.x; c < p.cols; c += block_threads(WPR)) dst[which * p.cols + c] = colsum[c];
-      __syncthreads();
+    };
+    auto take = [&](int from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          float(&a)[8] = h < 2 ? accp[j] : accs[j];
+          const float4 b = sums[(from * 4 * V + 4 * j + h) * 64 + t];
+          a[4 * (h & 1)] += b.x;
+          a[4 * (h & 1) + 1] += b.y;
+          a[4 * (h & 1) + 2] += b.z;
+          a[4 * (h & 1) + 3] += b.w;
+        }
+    };
+    __syncthreads();
+    if (wid >= 2) give(wid - 2);
+    __syncthreads();
+    if (wid < 2) take(wid);
+    __syncthreads();
+    if (wid == 1) give(0);
+    __syncthreads();
+    if (wid == 0) {
+      take(0);
+      write_sums();
     }
   }
 }
@@ -375,7 +440,7 @@ int bf8_rmsnorm_residual_bf16(const void* h, const void* residual, int64_t rows,
 
 size_t bf8_rmsnorm_residual_bwd_workspace(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
-  return (size_t)row_blocks(rows, (int)cols, kMaxBwdBlocks) * 2 * (size_t)cols * sizeof(float);
+  return (size_t)row_blocks(rows, (int)cols, max_bwd_blocks(cols)) * 2 * (size_t)cols * sizeof(float);
 }
 
 int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* dout, const void* dy,
@@ -394,9 +459,9 @@ int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* do
               (uintptr_t)pre | (uintptr_t)gate | (uintptr_t)dh | (uintptr_t)dresidual) & 15) == 0,
             "%s: every tensor must be 16-byte aligned", who);
   const bool wgrad = dpost || dpre || dgate;
-  BF8_CHECK(!wgrad || (ws && ((uintptr_t)ws & 3) == 0 &&
+  BF8_CHECK(!wgrad || (ws && ((uintptr_t)ws & 15) == 0 &&
                        ws_bytes >= bf8_rmsnorm_residual_bwd_workspace(rows, cols)),
-            "%s: workspace of %zu bytes, need %zu, 4-byte aligned", who, ws_bytes,
+            "%s: workspace of %zu bytes, need %zu, 16-byte aligned", who, ws_bytes,
             bf8_rmsnorm_residual_bwd_workspace(rows, cols));
   ResNorm p{};
   p.h = (const uint16_t*)h; p.res = (const uint16_t*)out;
@@ -406,11 +471,10 @@ int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* do
   p.scale = residual_scale; p.eps = eps; p.z = zero_centered ? 1.0f : 0.0f;
   p.dh = (uint16_t*)dh; p.dres = (uint16_t*)dresidual;
   p.part = wgrad ? (float*)ws : nullptr;
-  const int64_t nb = row_blocks(rows, (int)cols, kMaxBwdBlocks);
+  const int64_t nb = row_blocks(rows, (int)cols, max_bwd_blocks(cols));
   const dim3 grid((unsigned)nb);
-  const size_t lds = cols <= kWaveCols ? (size_t)cols * sizeof(float) : 0;
 #define BF8_RN_BWD(V, W)                                                                      \
-  hipLaunchKernelGGL((residual_norm_bwd_kernel<V, W>), grid, dim3(block_threads(W)), lds, \
+  hipLaunchKernelGGL((residual_norm_bwd_kernel<V, W>), grid, dim3(block_threads(W)), bwd_lds(V, W, cols), \
                      as_stream(stream), p)
   BF8_BY_WIDTH(BF8_RN_BWD)
 #undef BF8_RN_BWD

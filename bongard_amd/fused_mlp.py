@@ -87,7 +87,17 @@ class _ResidualNorm(torch.autograd.Function):
         return (*grads, None, None)
 
 
-@torch.compiler.disable
+def _residual_norm(h, residual, post_weight, pre_weight, eps, gate, residual_scale):
+    tensors = (h, residual, post_weight, pre_weight, gate)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return _ResidualNorm.apply(*tensors, eps, residual_scale)
+    return _ops.rmsnorm_residual(*tensors[:4], eps, gate=gate, residual_scale=residual_scale,
+                                 zero_centered=True)
+
+
+_residual_norm_uncompiled = torch.compiler.disable(_residual_norm)
+
+
 def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
                   residual_scale=1.0):
     """What a T5Gemma2 layer does between two blocks, in one kernel each way: the post-block norm
@@ -96,8 +106,9 @@ def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
     next block's input)``, differentiable in every tensor. ``gate`` (bf16 [hidden]) multiplies
     the normed h, ``residual_scale`` (a number) the old residual. The sum is formed in fp32 and
     rounded to bf16 once; the second norm is that of the rounded sum."""
-    return _ResidualNorm.apply(h, residual, post_weight, pre_weight, gate, float(eps),
-                               float(residual_scale))
+    # the wrapper that keeps a compiler out costs host time: it is for compiled callers only
+    call = _residual_norm_uncompiled if torch.compiler.is_compiling() else _residual_norm
+    return call(h, residual, post_weight, pre_weight, float(eps), gate, float(residual_scale))
 
 
 class FusedMLP(_ScalingExtraState, torch.nn.Module):

@@ -606,7 +606,7 @@ int bf8_rmsnorm_residual_bf16(const void* h, const void* residual, int64_t rows,
 /* Its backward from the forward's h and out: gradients dout and dy of out and y (either may be
  * NULL: zero). dh, dresidual [rows, cols], dpost, dpre, dgate [cols], each optional (at least
  * one); the last three need ws: bf8_rmsnorm_residual_bwd_workspace(rows, cols) bytes of block
- * partials, added in a fixed order. rows > 0. */
+ * partials, 16-byte aligned, added in a fixed order. rows > 0. */
 size_t bf8_rmsnorm_residual_bwd_workspace(int64_t rows, int64_t cols);
 int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* dout, const void* dy,
                                   int64_t rows, int64_t cols, const void* post, const void* pre,

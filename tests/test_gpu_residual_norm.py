@@ -206,3 +206,28 @@ def test_refusals(gpu):
         ops.rmsnorm_residual(z, z, z[0], z[0], EPS)
     with pytest.raises(ValueError, match="no gradient"):
         ops.rmsnorm_residual_backward(t["h"], t["res"], None, None, t["post"], t["pre"], EPS)
+
+
+@pytest.mark.parametrize("mode", ["no_grad", "nothing_trained", "compiled"])
+def test_every_way_of_calling_gives_the_same(gpu, mode):
+    """residual_norm without gradients, and from code under torch.compile (which leaves it out of its
+    graphs), against a recorded call."""
+    t = {k: v.to(gpu) for k, v in _inputs(9, 264, 5, True).items()}
+
+    def call(h, res, post, pre, gate):
+        out, y = fused_mlp.residual_norm(h, res, post, pre, EPS, gate=gate, residual_scale=0.5)
+        return out + 0.0, y + 0.0
+
+    args = [t[k].clone().requires_grad_(True) for k in ("h", "res", "post", "pre", "gate")]
+    want = call(*args)
+    if mode == "compiled":
+        got = torch.compile(call, backend="eager")(*args)
+        grads = [torch.autograd.grad(r, args, (t["dout"], t["dy"])) for r in (got, want)]
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+    elif mode == "no_grad":
+        with torch.no_grad():
+            got = call(*args)
+    else:
+        got = call(*(a.detach() for a in args))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(a.requires_grad == (mode == "compiled") for a in got)
