@@ -19,7 +19,6 @@
 namespace bf8 {
 namespace {
 
-constexpr int kNumCus = 256;  // MI355X: 8 XCDs x 32 CUs
 constexpr int kStepBytes = 128;
 constexpr int kMaxSplits = 8;
 constexpr int kMinStepsPerSplit = 4;

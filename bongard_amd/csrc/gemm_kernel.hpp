@@ -83,6 +83,8 @@ __host__ __device__ inline void walk_tile(int tiles_m, int tiles_n, int id, int&
   tn = in_g / gm;
 }
 
+constexpr int kNumCus = 256;  // MI355X: 8 XCDs x 32 CUs
+
 // A workgroup is KG groups of NW = WM x WN wave64s (four, or eight: two per SIMD); the
 // waves of a group are arranged WM x WN and each owns FM x FN MFMA tiles of 32 x 32
 // outputs, so the block tile is (WM*FM*32) x (WN*FN*32). Each group has its own NS LDS

@@ -556,7 +556,7 @@ gemm_kernel(GemmParams p) {
   constexpr int BM = T::BM, BN = T::BN, FM = T::FM, FN = T::FN, WM = T::WM, NS = T::NS;
   constexpr int KG = T::KG, XB = T::XB, NW = T::NW;
   constexpr int NSB = NS + XB;  // B slots: the NS stages' B parts, then XB B-only slots
-  static_assert(KG == 1 || (EPI == EPI_LINEAR && !MX), "K groups: linear epilogues only");
+  static_assert(KG == 1 || (EPI == EPI_LINEAR && (!MX || FA == kFmtFp4)), "K groups: linear epilogues only");
   constexpr int kA = BM * kBK;               // A tile bytes per stage
   // MX: each stage also holds the E8M0 block scales of its K step: one dword (4 blocks of
   // 32) per tile row, A rows at kData + 4 r, B rows at kData + 1024 + 4 r (r < 256).
@@ -1440,6 +1440,14 @@ struct FitTile {
 template <class T>
 int launch_f4(const GemmParams& p, int out_dtype, hipStream_t s) {
   const dim3 grid(grid_blocks(p)), block(tile_threads<T>());
+  if constexpr (T::OCC == 2 && T::NS == 3) {
+    // One workgroup a CU at most: two K groups in it, taking alternate steps, share what a step waits for
+    // (128x64, 200 x 2560 x 10240: 23.8 -> 20.7 us, 512 x 2560 x 10240: 26.2 -> 24.2, 512 x 2048 x 2560:
+    // 8.9 -> 8.5). Below eight steps their longer fill and the exchange cost more (64 x 512 x 1280: 6.1
+    // -> 6.5 us). A step takes 0.4-0.5 us however many stages are in flight (six instead of three: 1-2%).
+    if (grid.x <= kNumCus && p.splits == 1 && p.K >= 8 * kBK)
+      return launch_f4<GemmTile<T::WM, T::WN, T::FM, T::FN, 3, 1, 2>>(p, out_dtype, s);
+  }
   if (out_dtype == BF8_OUT_BF16)
     hipLaunchKernelGGL((gemm_kernel<T, kFmtFp4, kFmtFp4, EPI_LINEAR, BF8_OUT_BF16, true>), grid,
                        block, 0, s, p);

@@ -482,6 +482,20 @@ def test_product_on_every_tile(gpu, monkeypatch, tile, M, N, K):
         _check_product(y, ref, mag, K, dtype)
 
 
+@pytest.mark.parametrize("tile", ["128x64", "64x128"])
+@pytest.mark.parametrize("M,N,K", [(1040, 2056, 2208), (70, 136, 2080), (130, 72, 1792), (33, 520, 2048)])
+def test_product_of_few_and_many_small_tiles(gpu, monkeypatch, tile, M, N, K):
+    """The small tiles with more of them than CUs, and with fewer on either side of the eight K steps from
+    which two groups of waves share a tile's steps (even and odd numbers of them)."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    a, ra = _operand(M, K, M + K, gpu)
+    b, rb = _operand(N, K, N + K, gpu, spread=False)
+    ref, mag = mx4.mm(ra, rb)
+    for dtype in (torch.float32, torch.bfloat16):
+        y = ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=dtype)
+        _check_product(y, ref, mag, K, dtype)
+
+
 def test_tail_split(gpu, monkeypatch):
     """Whole tiles in full rounds, the last round's tiles in K pieces."""
     monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", "256x256w8:t")
