@@ -260,6 +260,47 @@ double geglu_cost(const Plan& p) {
   return eff_rounds * (p.kps + 2) * step_ns / 1e3;
 }
 
+// The MXFP4 gated-GELU plans: rounds as in linear_cost, the gelu and H's quantization in f. Its MFMAs
+// take half the time of FP8's and the epilogue the same, which geglu_cost cannot say: with it the
+// picks lost 5.3% on average and up to twofold (190 rows, I 10240, K 352: 192x256 18.2 us,
+// 64x128 8.8). Least squares over the measured times of 5,000 shapes (M 1 .. 8192, I 128 ..
+// 10240, K 32 .. 5120; with and without H's columnwise copy and GU, their geometric mean): picks on as
+// many others lose 0.15% on average, 6% in one of a hundred, 10% at worst. 192x256 and 128x128,
+// the best of one or two shapes in a hundred, are left out: with them the picks lose 0.38%.
+constexpr RoundCost kGeglu4_256x256w8 = {0.987, 1.656, 15.708, 1.633};
+constexpr RoundCost kGeglu4_160x256 = {1.096, 1.12, 15.387, 1.463};
+constexpr RoundCost kGeglu4_64x128 = {0.459, 0.574, 7.024, 0.0, 1.062, 0.713, 6.043, 0.0};
+constexpr double kGeglu4LaterSaves[2] = {0.2, 0.3};
+
+const RoundCost* geglu4_rounds(int tile) {
+  return tile == TILE_256x256w8 ? &kGeglu4_256x256w8
+         : tile == TILE_160x256 ? &kGeglu4_160x256
+         : tile == TILE_64x128  ? &kGeglu4_64x128
+                                : nullptr;
+}
+
+double geglu4_cost(const Plan& p, int64_t M, int64_t N) {
+  const TileInfo& ti = kTiles[p.tile];
+  const RoundCost& rc = *geglu4_rounds(p.tile);
+  const double loaded =
+      (double)(std::min<int64_t>(M, ti.bm) + std::min<int64_t>(N, ti.bn)) / (ti.bm + ti.bn);
+  const double steps = p.kps * (1 - kEmptySaves * (1 - loaded));
+  auto round = [&](int64_t ctas, bool first) {
+    const double x = (double)std::min<int64_t>(ctas, kNumCus) / kNumCus;
+    const double y = (double)(ctas - kNumCus) / kNumCus;
+    const bool two = ctas > kNumCus;  // occ 2
+    const double fixed = two ? rc.f2 + rc.g2 * y : rc.f1 + rc.g1 * x;
+    return steps * (two ? rc.s2 + (rc.s3 - rc.s2) * y : rc.s0 + (rc.s1 - rc.s0) * x) +
+           fixed * (first ? 1.0 : 1.0 - kGeglu4LaterSaves[ti.occ - 1]);
+  };
+  const int64_t slots = (int64_t)kNumCus * ti.occ, ctas = (int64_t)p.tiles_m * p.tiles_n;
+  const int64_t whole = ctas / slots, rest = ctas % slots;
+  double t = 0;
+  if (whole > 0) t = round(slots, true) + (whole - 1) * round(slots, false);
+  if (rest > 0) t += round(rest, whole == 0);
+  return t;
+}
+
 // Tuning override, read on every call: BONGARD_FP8_GEMM_TILE=<bm>x<bn>[:<splits>|:t]
 // (e.g. "256x160:4"; ":t" the tail split, when the shape has one). Unknown values are
 // ignored.
@@ -281,9 +322,10 @@ bool env_override(int& tile, int& splits) {
 }
 
 // Chooses the tile and K split for C[M, N] = A[M, K] . B[N, K]^T. GEGLU plans never split
-// and depend on (M, N) only, so the per-tile amax partial count is known without K.
+// and, but for MXFP4's (f4), depend on (M, N) only, so the per-tile amax partial count is known
+// without K.
 Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, bool mx = false,
-                 int kmajor = 0) {
+                 int kmajor = 0, bool f4 = false) {
   const int64_t ksteps = std::max<int64_t>(cdiv(K, kStepBytes), 1);
   int otile, osplits;
   if (env_override(otile, osplits) && (!geglu || geglu_tile_ok(otile, N, mx)) &&
@@ -304,6 +346,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
   for (int tile = 0; tile < NUM_TILES; ++tile) {
     if (!kTiles[tile].planned || (geglu && !geglu_tile_ok(tile, N, mx)) || (mx && !kTiles[tile].mx))
       continue;
+    if (geglu && f4 && !geglu4_rounds(tile)) continue;
     // K-major operands: the eight-wave 256x256 tiles only
     if (kmajor && tile != TILE_256x256w8) continue;
     // The two-stage tiles run unsplit: in K pieces the modelled time is up to 13% short (M = 1024,
@@ -314,15 +357,17 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
     const bool two_stage = tile == TILE_192x128o2 || tile == TILE_128x128o2;
     const bool two_groups = tile == TILE_128x64k2 || tile == TILE_64x128k2;
     for (int s = 1; s <= (geglu || two_stage || two_groups ? 1 : kMaxSplits); ++s) {
-      const Plan p = make_plan(tile, M, N, geglu ? kGegluNominalSteps : ksteps, s);
+      const Plan p = make_plan(tile, M, N, geglu && !f4 ? kGegluNominalSteps : ksteps, s);
       if (p.splits != s || (s > 1 && p.kps < kMinStepsPerSplit) || p.ws_bytes > ws_avail)
         continue;
       if (two_groups && (int64_t)p.tiles_m * p.tiles_n > kNumCus) continue;
-      const double c = geglu ? geglu_cost(p) : linear_cost(p, M, N, ksteps, mx, kmajor);
+      const double c = geglu && f4 ? geglu4_cost(p, M, N)
+                       : geglu     ? geglu_cost(p)
+                                   : linear_cost(p, M, N, ksteps, mx, kmajor);
       // Ties go to the earlier (larger, unsplit) plan. geglu_cost is the coarser model: within 3%
       // the earlier tile was the faster on every shape that differed (M = 4457, I = 2560, K = 10240
       // on 192x256 200.9 us, on 256x256w8 223.5; M = 8340, I = 2048, K = 2560 117.7 and 122.5).
-      if (!have || c < best_cost * (geglu ? 0.97 : 0.99)) {
+      if (!have || c < best_cost * (geglu && !f4 ? 0.97 : 0.99)) {
         best = p;
         best_cost = c;
         have = true;
@@ -1014,7 +1059,9 @@ static int check_mx4_operand(const char* who, const char* what, const uint8_t* q
 }
 
 size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
-  return bf8_gemm_mx_workspace(M, N, K / 2);  // plans are made on K bytes
+  // plans are made on K bytes, with MXFP8's costs: over 3,900 shapes the picks lose 0.9% on average
+  // against the best measured plan, 3% in one of ten (costs fitted to FP4 itself: 0.8% and 3%)
+  return bf8_gemm_mx_workspace(M, N, K / 2);
 }
 
 int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
@@ -1063,7 +1110,7 @@ static int geglu_mx_launch(const uint8_t* X, int64_t ldx, MxScales x_sc, const u
   p.C = H; p.ldc = ldh; p.GU = (uint16_t*)GU; p.partials = nullptr;
   p.h8 = H8; p.h8_sc = h8_sc;
   p.h8t = H8t; p.h8t_sc = h8t_sc;
-  Plan pl = choose_plan(M, 2 * I, K, true, 0, true);
+  Plan pl = choose_plan(M, 2 * I, K, true, 0, true, 0, fmt == kFmtFp4);
   return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, fmt, fmt, nullptr, as_stream(stream), true);
 }
 
