@@ -25,6 +25,7 @@ weight gradient of the HF formula's autograd, fp32 math) is a kernel as well
 from collections import Counter
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import linear as _linear
 from . import ops as _ops
@@ -76,6 +77,7 @@ class _ResidualNorm(torch.autograd.Function):
         return out, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout, dy):
         h, out, post_weight, pre_weight, gate = ctx.saved_tensors
         if dout is None and dy is None:

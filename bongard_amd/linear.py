@@ -26,6 +26,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from . import scaling as _scaling
@@ -536,6 +537,7 @@ class Mxfp4LinearFunction(_Fp8Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x4t, xpt, w4t, wpt = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
@@ -577,6 +579,7 @@ class Mxfp4GegluMlpFunction(_Fp8Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         GU, x4t, xpt, h4t, hpt, gu4t, gupt, d4t, dpt = ctx.saved_tensors
         need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]

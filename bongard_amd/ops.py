@@ -1472,9 +1472,6 @@ def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
 
 
 # ---- the norms on either side of a residual connection ---------------------------------------
-RESIDUAL_NORM_MAX_COLS = 16384
-
-
 def _norm_weights(who, cols, post_weight, pre_weight, gate):
     for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("gate", gate)):
         if t is not None and (t.dtype is not torch.bfloat16 or t.shape != (cols,)):

@@ -409,6 +409,66 @@ def test_layer_together_in_a_graph(gpu):
                 assert torch.equal(a, b), f"replay {rep}"
 
 
+def test_two_graphs_at_once(gpu):
+    """Calls with a workspace (a product in K pieces, the norm's backward) captured into two graphs,
+    replayed side by side on two streams: neither touches the other's."""
+    M, N, K = 96, 256, 16384
+    assert ops._gemm_mxfp4_ws_cached(M, N, K, "") > 0
+    post, pre = _x(1, 512, 3).to(gpu)[0], _x(1, 512, 4).to(gpu)[0]
+
+    def work(a, b, h, dy):
+        y = ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=torch.float32)
+        out, _ = ops.rmsnorm_residual(h, dy, post, pre, 1e-6)
+        return [y, *ops.rmsnorm_residual_backward(h, out, dy, dy, post, pre, 1e-6)[:4]]
+
+    sides, ins = [], []
+    for k in range(2):
+        ins.append((ops.quantize_mxfp4(_x(M, K, 10 + k).to(gpu)), ops.quantize_mxfp4(_x(N, K, 20 + k).to(gpu)),
+                    _x(700, 512, 30 + k).to(gpu), _x(700, 512, 40 + k).to(gpu)))
+    want = [[t.clone() for t in work(*i)] for i in ins]
+    torch.cuda.synchronize()
+    for i in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = work(*i)
+        sides.append((torch.cuda.Stream(), graph, outs))
+    for rep in range(5):
+        for _, _, outs in sides:
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        for stream, graph, _ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outs), w in zip(sides, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, w)), f"replay {rep}"
+
+
+def test_one_tensor_as_both_operands(gpu):
+    """A Gram matrix: symmetric to the bit, and the product of two equal tensors."""
+    q = ops.quantize_mxfp4(_x(300, 2080, 9).to(gpu))
+    y = ops.gemm_mxfp4(q.data, q.planes, q.data[:296], q.planes[:, :296].contiguous(),
+                       out_dtype=torch.float32)
+    z = ops.gemm_mxfp4(q.data, q.planes, q.data.clone()[:296], q.planes[:, :296].contiguous(),
+                       out_dtype=torch.float32)
+    assert torch.equal(y, z)
+
+
+def test_second_derivatives_are_refused(gpu):
+    x = _x(40, 64, 1).to(gpu).requires_grad_()
+    w = _x(32, 64, 2).to(gpu).requires_grad_()
+    n = _x(1, 64, 3).to(gpu)[0].requires_grad_()
+    results = [linear.Mxfp4LinearFunction.apply(x, w, None), fused_mlp.residual_norm(x, x, n, n)[1],
+               linear.Mxfp4GegluMlpFunction.apply(x, _x(256, 64, 4).to(gpu).requires_grad_(),
+                                                  _x(64, 128, 5).to(gpu), None, None, 128)]
+    for y in results:
+        for dy, told in ((torch.ones_like(y), "does not require grad"), (2 * y, "once_differentiable")):
+            (g,) = torch.autograd.grad(y, x, dy, create_graph=True)
+            with pytest.raises(RuntimeError, match=told):
+                g.float().square().sum().backward()
+
+
 def test_another_stream(gpu):
     x, w = _x(300, 512, 1).to(gpu), _x(256, 512, 2).to(gpu)
     def f():
