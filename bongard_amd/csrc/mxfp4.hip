@@ -2,11 +2,12 @@
 // two (OCP Microscaling Formats v1.0, section 5) and their exact read-back. The products are
 // gemm.hip's.
 //
-// The scale of a block is the smallest power of two 2^k with max |x| <= 6 * 2^k (e = k + 127), so no
-// value is clipped: the specification's own floor(log2(max)) - 2 would clip the magnitudes between
-// 6 and 8 steps of the grid, a bias that the gradients of a training step carry on. It is the rule of the MXFP8 quantizer (mx.hip) for a
-// largest value of 6. Codes round to nearest, ties to the even code; x ~ e2m1(q) * 2^(e - 127), which
-// bf16 holds exactly (but for what overflows in a block that holds inf: bf16 rounds it to inf).
+// The scale of a block is the smallest power of two 2^k with max |x| <= 6 * 2^k (e = k + 127), so
+// no value is clipped: the specification's own floor(log2(max)) - 2 would clip the magnitudes
+// between 6 and 8 steps of the grid, a bias that the gradients of a training step carry on. It is
+// the rule of the MXFP8 quantizer (mx.hip) for a largest value of 6. Codes round to nearest, ties
+// to the even code; x ~ e2m1(q) * 2^(e - 127), which bf16 holds exactly (but for what overflows in
+// a block that holds inf: bf16 rounds it to inf).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -17,14 +18,15 @@
 namespace bf8 {
 namespace {
 
-// A block of W waves takes W tiles one below the other. Memory-bound: 2 B read, 17 / 32 B written an
-// element and copy; one pass for both copies. Inputs rotated past the MALL, W = 1 / 4 / 8, us (a copy
-// of as many bytes at the 5.1 TB/s of large ones): along rows [512, 10240] 5.4 / 5.5 / 5.4 (2.6), [4096, 10240]
-// 24.6 / 24.7 / 24.8 (20.8), [4096, 20480] 45.7 / 46.1 / 47.0 (41.6); both copies [500, 2048] 3.8 / 4.2 / 5.2,
-// [2001, 4096] 8.9 / 9.1 / 9.1 (4.9), [4096, 2560] 12.1 / 10.7 / 11.8 (6.3), [2560, 10240] 23.0 / 21.5 / 22.6
-// (15.7), [4096, 10240] 35.6 / 31.4 / 30.1 (25.2), [20480, 2560] 48.9 / 40.7 / 38.3 (31.5): columnwise
-// codes in pieces of 16 bytes cost the large tensors a quarter, waiting for the block's other waves the
-// small ones as much. Loads behind a branch each (a wait each) took 24% more at [4096, 2560].
+// A block of W waves takes W tiles one below the other. Memory-bound: 2 B read, 17 / 32 B written
+// an element and copy; one pass for both copies. Inputs rotated past the MALL, W = 1 / 4 / 8, us (a
+// copy of as many bytes at the 5.1 TB/s of large ones): along rows [512, 10240] 5.4 / 5.5 / 5.4
+// (2.6), [4096, 10240] 24.6 / 24.7 / 24.8 (20.8), [4096, 20480] 45.7 / 46.1 / 47.0 (41.6); both
+// copies [500, 2048] 3.8 / 4.2 / 5.2, [2001, 4096] 8.9 / 9.1 / 9.1 (4.9), [4096, 2560] 12.1 / 10.7
+// / 11.8 (6.3), [2560, 10240] 23.0 / 21.5 / 22.6 (15.7), [4096, 10240] 35.6 / 31.4 / 30.1 (25.2),
+// [20480, 2560] 48.9 / 40.7 / 38.3 (31.5): columnwise codes in pieces of 16 bytes cost the large
+// tensors a quarter, waiting for the block's other waves the small ones as much. Loads behind a
+// branch each (a wait each) took 24% more at [4096, 2560].
 template <int W>
 __global__ __launch_bounds__(64 * W) void mx4_kernel(const uint16_t* __restrict__ x, Mx4Out p) {
   const int lane = threadIdx.x & 63;
@@ -113,13 +115,14 @@ __device__ __forceinline__ void geglu_bwd_rows(Window wd, Window wg, uint32_t od
   }
 }
 
-// The gated-GELU backward and the quantization of its dGU [M, 2I] (p: rows M, cols 2I) from
-// dH [M, I] and GU [M, 2I], I % 128 == 0: dGU goes from registers to its copies. A block takes W / 2
-// tiles of H one below the other, of each the d_g tile by one wave and the d_u tile by another.
-// 6 B read, 17 / 16 B a copy written per element of H; the lookups and conversions, 22 instructions
-// an element of dGU, take about as long as the bytes and overlap them by half. Both copies, W = 2 / 8, us (a copy of as many
-// bytes): [64, 10240] 9.0 / 17.4, [512, 10240] 20.3 / 23.8 (8.4), [2001, 10240] 63.8 / 58.1 (32.6),
-// [4096, 10240] 115 / 104 (66.8), [8192, 10240] 236 / 200 (134); in two passes 73 + 66 at [4096, 10240].
+// The gated-GELU backward and the quantization of its dGU [M, 2I] (p: rows M, cols 2I) from dH [M,
+// I] and GU [M, 2I], I % 128 == 0: dGU goes from registers to its copies. A block takes W / 2 tiles
+// of H one below the other, of each the d_g tile by one wave and the d_u tile by another. 6 B read,
+// 17 / 16 B a copy written per element of H; the lookups and conversions, 22 instructions an
+// element of dGU, take about as long as the bytes and overlap them by half. Both copies, W = 2 / 8,
+// us (a copy of as many bytes): [64, 10240] 9.0 / 17.4, [512, 10240] 20.3 / 23.8 (8.4), [2001,
+// 10240] 63.8 / 58.1 (32.6), [4096, 10240] 115 / 104 (66.8), [8192, 10240] 236 / 200 (134); in two
+// passes 73 + 66 at [4096, 10240].
 template <int W>
 __global__ __launch_bounds__(64 * W, 4) void geglu_bwd_mx4_kernel(const uint16_t* __restrict__ dH,
                                                                const uint16_t* __restrict__ GU,
@@ -175,8 +178,9 @@ __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint8_t* __restr
 
 // Elements up to which a tensor's columnwise codes leave each wave by themselves, and in 64-byte pieces
 // (mx4_kernel's figures).
-constexpr int64_t kBwdTwo = 8 << 20;  // elements of H
 constexpr int64_t kMx4Alone = 8 << 20, kMx4Four = 32 << 20;
+// Elements of H up to which the gated backward's blocks are of two waves (its kernel's figures).
+constexpr int64_t kBwdTwo = 8 << 20;
 
 template <int W>
 int mx4_launch(const uint16_t* x, const Mx4Out& p, hipStream_t s) {

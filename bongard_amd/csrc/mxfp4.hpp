@@ -7,9 +7,10 @@
 
 namespace bf8 {
 
-// Biased exponent e of a block whose max |x| is the bf16 key k (the bits without the sign): 2^(e - 127) is the
-// smallest power of two with max |x| <= 6 * 2^(e - 127), 2^-127 at least. 6 = 1.5 * 2^2, so it is
-// E - 2, one more where the mantissa passes 1.5 (64 / 128 above 1): ((k + 63) >> 7) - 2.
+// Biased exponent e of a block whose max |x| is the bf16 key k (the bits without the sign): 2^(e -
+// 127) is the smallest power of two with max |x| <= 6 * 2^(e - 127), 2^-127 at least. 6 = 1.5 *
+// 2^2, so it is E - 2, one more where the mantissa passes 1.5 (64 / 128 above 1): ((k + 63) >> 7) -
+// 2.
 __device__ __forceinline__ uint32_t mx4_exponent_finite(uint32_t k) {
   const uint32_t t = (k + 63u) >> 7;
   return t > 2u ? t - 2u : 0u;

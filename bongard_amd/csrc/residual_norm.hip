@@ -35,10 +35,11 @@ namespace bf8 {
 namespace {
 
 constexpr int kMaxCols = 16384;
-constexpr int64_t kMaxFwdBlocks = 2048;
+constexpr int64_t kMaxFwdBlocks = 2048;  // (1,024 blocks are level with them)
 // The backward's blocks: those resident at once (two a CU, or one of 16 waves), as each adds a
-// partial row to the weights' sums. 768 instead of 512: 135 us for 124 at 18,494 x 2,560; 256: 118 for
-// 122 there but 58 for 48 at 4,096 x 4,096. 512 instead of 256 of the wide ones: 120 us for 107 (4,096 x 8,192).
+// partial row to the weights' sums. 768 instead of 512: 135 us for 124 at 18,494 x 2,560; 256: 118
+// for 122 there but 58 for 48 at 4,096 x 4,096. 512 instead of 256 of the wide ones: 120 us for 107
+// (4,096 x 8,192).
 constexpr int64_t max_bwd_blocks(int64_t cols) { return cols <= 4096 ? 512 : 256; }
 
 struct ResNorm {
