@@ -279,6 +279,11 @@ const RoundCost* geglu4_rounds(int tile) {
                                 : nullptr;
 }
 
+// Whether MXFP4 has a linear or gated-GELU variant of `tile`: of those that its plans can take.
+bool f4_tile_ok(int tile, bool geglu) {
+  return geglu ? geglu4_rounds(tile) != nullptr : kTiles[tile].planned && kTiles[tile].mx;
+}
+
 double geglu4_cost(const Plan& p, int64_t M, int64_t N) {
   const TileInfo& ti = kTiles[p.tile];
   const RoundCost& rc = *geglu4_rounds(p.tile);
@@ -329,7 +334,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
   const int64_t ksteps = std::max<int64_t>(cdiv(K, kStepBytes), 1);
   int otile, osplits;
   if (env_override(otile, osplits) && (!geglu || geglu_tile_ok(otile, N, mx)) &&
-      (!mx || kTiles[otile].mx) &&
+      (!mx || kTiles[otile].mx) && (!f4 || f4_tile_ok(otile, geglu)) &&
       (!kmajor || otile == TILE_256x256w8 || otile == TILE_256x256w8x)) {
     Plan p;
     if (!geglu && osplits == kTailSplitOverride) {
@@ -346,7 +351,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
   for (int tile = 0; tile < NUM_TILES; ++tile) {
     if (!kTiles[tile].planned || (geglu && !geglu_tile_ok(tile, N, mx)) || (mx && !kTiles[tile].mx))
       continue;
-    if (geglu && f4 && !geglu4_rounds(tile)) continue;
+    if (f4 && !f4_tile_ok(tile, geglu)) continue;
     // K-major operands: the eight-wave 256x256 tiles only
     if (kmajor && tile != TILE_256x256w8) continue;
     // The two-stage tiles run unsplit: in K pieces the modelled time is up to 13% short (M = 1024,
@@ -1012,7 +1017,7 @@ static int gemm_mx_launch(const uint8_t* A, int64_t lda, MxScales a_sc, const ui
   p.n_seg = 1;
   for (int s = 0; s < 4; ++s) p.seg_end[s] = (int)N;
   p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
-  const Plan pl = choose_plan(M, N, K, false, ws ? ws_bytes : 0, true);
+  const Plan pl = choose_plan(M, N, K, false, ws ? ws_bytes : 0, true, 0, fmt == kFmtFp4);
   return launch_plan(pl, p, EPI_LINEAR, out_dtype, fmt, fmt, ws, as_stream(stream), true);
 }
 
@@ -1061,7 +1066,8 @@ static int check_mx4_operand(const char* who, const char* what, const uint8_t* q
 size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
   // plans are made on K bytes, with MXFP8's costs: over 3,900 shapes the picks lose 0.9% on average
   // against the best measured plan, 3% in one of ten (costs fitted to FP4 itself: 0.8% and 3%)
-  return bf8_gemm_mx_workspace(M, N, K / 2);
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return choose_plan(M, N, K / 2, false, (size_t)-1, true, 0, true).ws_bytes;
 }
 
 int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,

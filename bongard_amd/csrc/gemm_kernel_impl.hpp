@@ -1439,6 +1439,19 @@ struct FitTile {
   static_assert(bytes(type::NS, type::XB) <= kLimit, "stages do not fit the LDS");
 };
 
+// The tiles that MXFP4 plans take (gemm.hip's f4_tile_ok).
+template <class T>
+constexpr bool f4_tile(int epi) {
+  if (epi == EPI_GEGLU)
+    return std::is_same<T, Tile256x256w8>::value || std::is_same<T, Tile160x256>::value ||
+           std::is_same<T, Tile64x128>::value;
+  return !std::is_same<T, Tile256x256>::value && !std::is_same<T, Tile256x128>::value;
+}
+inline int no_f4_tile(int bm, int bn) {
+  set_error("gemm: tile %dx%d has no such MXFP4 variant", bm, bn);
+  return BF8_EINVAL;
+}
+
 // The linear MXFP4 GEMM on tile T.
 template <class T>
 int launch_f4(const GemmParams& p, int out_dtype, hipStream_t s) {
@@ -1512,10 +1525,13 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
       if (mx) {
         if constexpr (T::NW == 4 || (T::BM == 256 && T::BN == 256)) {
           if (fmt_a == kFmtFp4) {
-            using TF = typename FitTile<T, EPI_GEGLU, true, true>::type;
-            hipLaunchKernelGGL((gemm_kernel<TF, kFmtFp4, kFmtFp4, EPI_GEGLU, BF8_OUT_BF16, true>),
-                               grid, block, 0, stream, p);
-            return launch_status("gemm_kernel(geglu, mxfp4)");
+            if constexpr (f4_tile<T>(EPI_GEGLU)) {
+              using TF = typename FitTile<T, EPI_GEGLU, true, true>::type;
+              hipLaunchKernelGGL((gemm_kernel<TF, kFmtFp4, kFmtFp4, EPI_GEGLU, BF8_OUT_BF16, true>),
+                                 grid, block, 0, stream, p);
+              return launch_status("gemm_kernel(geglu, mxfp4)");
+            }
+            return no_f4_tile(T::BM, T::BN);
           }
           using TG = typename FitTile<T, EPI_GEGLU, true>::type;
           hipLaunchKernelGGL((gemm_kernel<TG, 0, 0, EPI_GEGLU, BF8_OUT_BF16, true>), grid, block,
@@ -1557,8 +1573,11 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
   }
   if (mx) {
     if constexpr (T::NW == 4 || (T::BM == 256 && T::BN == 256)) {
-      if (fmt_a == kFmtFp4)
-        return launch_f4<typename FitTile<T, EPI_LINEAR, true, true>::type>(p, out_dtype, stream);
+      if (fmt_a == kFmtFp4) {
+        if constexpr (f4_tile<T>(EPI_LINEAR))
+          return launch_f4<typename FitTile<T, EPI_LINEAR, true, true>::type>(p, out_dtype, stream);
+        return no_f4_tile(T::BM, T::BN);
+      }
       // MX block scales (e4m3 operands) beside the stages
       using TM = typename FitTile<T, EPI_LINEAR, true>::type;
       if (out_dtype == BF8_OUT_BF16)

@@ -409,6 +409,33 @@ def test_layer_together_in_a_graph(gpu):
                 assert torch.equal(a, b), f"replay {rep}"
 
 
+def test_products_past_32_bit_offsets(gpu):
+    """Results of more than 4 GiB: the rows at the end are those of a call on them alone, which differ in no
+    sum (the same plan's K order), and so are the gated product's and its backward's."""
+    M, N, K, tail = 70016, 32768, 64, 512
+    a, b = _x(tail, K, 1, spread=False).to(gpu), ops.quantize_mxfp4(_x(N, K, 2, spread=False).to(gpu))
+    big = torch.zeros(M, K, dtype=torch.bfloat16, device=gpu)
+    big[-tail:] = a
+    q, small = ops.quantize_mxfp4(big), ops.quantize_mxfp4(a)
+    y = ops.gemm_mxfp4(q.data, q.planes, b.data, b.planes)
+    assert y.numel() * 2 > 1 << 32
+    assert torch.equal(y[-tail:], ops.gemm_mxfp4(small.data, small.planes, b.data, b.planes))
+    assert not bool(y[:-tail].any())
+    del y
+    hq, GU = ops.gemm_geglu_mxfp4(q.data, q.planes, b.data, b.planes, N // 2, colwise=True, keep_gu=True)
+    h2, GU2 = ops.gemm_geglu_mxfp4(small.data, small.planes, b.data, b.planes, N // 2, colwise=True,
+                                   keep_gu=True)
+    assert torch.equal(GU[-tail:], GU2) and torch.equal(hq.data[-tail:], h2.data)
+    assert torch.equal(hq.data_t[:, -tail // 2:], h2.data_t)
+    assert torch.equal(hq.planes[:, -tail:], h2.planes) and torch.equal(hq.planes_t[-4:], h2.planes_t)
+    dH = torch.zeros(M, N // 2, dtype=torch.bfloat16, device=gpu)
+    dH[-tail:] = _x(tail, N // 2, 3, spread=False).to(gpu)
+    d = ops.geglu_bwd_mxfp4(dH, GU, colwise=True)
+    d2 = ops.geglu_bwd_mxfp4(dH[-tail:], GU2, colwise=True)
+    assert torch.equal(d.data[-tail:], d2.data) and torch.equal(d.planes[:, -tail:], d2.planes)
+    assert torch.equal(d.data_t[:, -tail // 2:], d2.data_t) and torch.equal(d.planes_t[-4:], d2.planes_t)
+
+
 def test_two_graphs_at_once(gpu):
     """Calls with a workspace (a product in K pieces, the norm's backward) captured into two graphs,
     replayed side by side on two streams: neither touches the other's."""
@@ -524,8 +551,8 @@ def test_refusals(gpu):
                                                         requires_grad=True), None)
 
 
-TILES = ["256x256", "256x160", "160x256", "128x128", "192x256", "128x64", "64x128", "256x128",
-         "256x256w8", "128x128o2", "128x64:3", "256x256w8:2"]
+TILES = ["256x160", "160x256", "128x128", "192x256", "128x64", "64x128", "256x256w8", "128x128o2",
+         "128x64:3", "256x256w8:2", "256x128"]  # (the last has no FP4 variant: the plan's own)
 
 
 @pytest.mark.parametrize("tile", TILES)
@@ -569,7 +596,7 @@ def test_tail_split(gpu, monkeypatch):
     _check_product(y[rows.to(gpu)], ref, mag, K, torch.float32)
 
 
-@pytest.mark.parametrize("tile", ["256x256w8", "256x256", "160x256", "192x256", "128x128", "64x128", "256x128"])
+@pytest.mark.parametrize("tile", ["256x256w8", "160x256", "64x128", "192x256"])
 @pytest.mark.parametrize("M,K,I", [(1, 32, 128), (45, 288, 256), (290, 544, 640)])
 def test_gated_product_on_every_tile(gpu, monkeypatch, tile, M, K, I):
     """The gated-GELU epilogue of every tile: H's copies from its own GU, one K step and several, ragged

@@ -160,6 +160,23 @@ def test_autograd_and_differences(gpu):
         assert abs(diff - told) <= 0.05 * abs(told), (n, diff.item(), told.item())
 
 
+def test_rows_past_32_bit_offsets(gpu):
+    """Tensors of more than 4 GiB: every row's results are those of a call on a few rows."""
+    cols, few = 2560, 64
+    t = {k: v.to(gpu) for k, v in _inputs(few, cols, 7, True).items()}
+    rows = few * 13200
+    many = {k: (v.repeat(rows // few, 1) if v.dim() == 2 else v) for k, v in t.items()}
+    assert many["h"].numel() * 2 > 1 << 32
+    kw = dict(gate=t["gate"], residual_scale=0.5)
+    out, y = ops.rmsnorm_residual(many["h"], many["res"], t["post"], t["pre"], EPS, **kw)
+    want = ops.rmsnorm_residual(t["h"], t["res"], t["post"], t["pre"], EPS, **kw)
+    grads = ops.rmsnorm_residual_backward(many["h"], out, many["dout"], many["dy"], t["post"], t["pre"],
+                                          EPS, **kw, needs=(True, True, False, False, False))
+    told = ops.rmsnorm_residual_backward(t["h"], want[0], t["dout"], t["dy"], t["post"], t["pre"], EPS, **kw)
+    for a, b in zip((out, y, *grads[:2]), (*want, *told[:2])):
+        assert bool((a.view(-1, few, cols) == b).all())
+
+
 def test_rows_as_they_come(gpu):
     """Strided and misaligned inputs, no rows, and NaN or inf rows that leave the others alone."""
     t = {k: v.to(gpu) for k, v in _inputs(64, 256, 5, False).items() if v is not None}
