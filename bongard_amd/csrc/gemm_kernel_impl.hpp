@@ -572,7 +572,13 @@ gemm_kernel(GemmParams p) {
   constexpr int kStage = kData + (MX ? mx_stage_bytes(BM, BN, F4) : 0);  // [A tile | B tile | scales]
   constexpr int DA = BM / (8 * NW), DB = BN / (8 * NW);  // 1 KB DMA blocks per wave per stage
   static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole 1 KB blocks per wave");
-  constexpr int NSC = MX ? (MX8 ? 1 : 2) * (F4 ? 2 : 1) : 0;  // of scales
+  // Each wave loads 64 scale dwords of A or of B a plane where the tile has no more such pieces than
+  // waves, else of both. The loads issued, not their bytes, are what a small tile's step waits for: with
+  // four of scales a wave instead of two 64 x 2048 x 2560 took 8.2 us (now 7.9), 512 x 2560 x 10240 24.2
+  // (21.8), 2001 x 2560 x 10240 42.6 (41.2).
+  constexpr int kScPieces = (RA + RB) / 64;
+  constexpr bool kScOne = MX8 || (F4 && kScPieces <= NW);
+  constexpr int NSC = MX ? (kScOne ? 1 : 2) * (F4 ? 2 : 1) : 0;
   constexpr int ND = DA + DB + NSC;  // loads per wave per stage
   constexpr int NM = FM * FN;                // MFMAs per sub-step
   constexpr int NH = 2 * (FM + FN);          // 16-byte fragment halves per sub-step
@@ -697,11 +703,12 @@ gemm_kernel(GemmParams p) {
   // read as zero.
   i32x4 srd_sa = {0, 0, 0, 0}, srd_sb = {0, 0, 0, 0};
   uint32_t sa_off = kOob, sb_off = kOob, sa_gs = 0, sb_gs = 0;
-  // FP4: the waves past an operand's last 64 rows load its first ones again, so that every wave
-  // issues the same number of loads
-  const int sc_wave = MX8 ? wid & 3 : wid;
-  const int sa_wave = F4 ? sc_wave % (RA / 64) : sc_wave;
-  const int sb_wave = F4 ? sc_wave % (RB / 64) : sc_wave;
+  // Waves past the last piece load an earlier one again, so that every wave issues the same number
+  // of loads.
+  const int sc_piece = __builtin_amdgcn_readfirstlane(kScOne ? wid % kScPieces : wid);
+  const bool sc_b = kScOne && sc_piece >= RA / 64;
+  const int sa_wave = kScOne ? sc_piece - (sc_b ? RA / 64 : 0) : F4 ? sc_piece % (RA / 64) : sc_piece;
+  const int sb_wave = kScOne ? sa_wave : F4 ? sc_piece % (RB / 64) : sc_piece;
   const int ngroups = F4 ? (p.K + 63) / 64 : ksteps;  // groups of 128 K-values
   if constexpr (MX) {
     auto sc_srd = [&](const MxScales& m, int rows) {
@@ -725,11 +732,10 @@ gemm_kernel(GemmParams p) {
       }
       if (bvalid) ob = (uint32_t)((int64_t)bn * p.b_sc.rs);
     }
-    const bool second = MX8 && __builtin_amdgcn_readfirstlane(wid) >= 4;
-    srd_sa = second ? sc_srd(p.b_sc, p.N) : sc_srd(p.a_sc, p.M);
-    sa_off = second ? ob : oa;
-    sa_gs = (uint32_t)(second ? p.b_sc.gs : p.a_sc.gs);
-    if constexpr (!MX8) {
+    srd_sa = sc_b ? sc_srd(p.b_sc, p.N) : sc_srd(p.a_sc, p.M);
+    sa_off = sc_b ? ob : oa;
+    sa_gs = (uint32_t)(sc_b ? p.b_sc.gs : p.a_sc.gs);
+    if constexpr (!kScOne) {
       srd_sb = sc_srd(p.b_sc, p.N);
       sb_off = ob;
       sb_gs = (uint32_t)p.b_sc.gs;
@@ -759,13 +765,13 @@ gemm_kernel(GemmParams p) {
       dma16(rb, lds_addr(bdst) + (j * NW + wid) * 1024, off, BKM ? k0 * (uint32_t)p.ldb : k0);
     }
     else if constexpr (F4) {
-      // eight waves: plane x (of A, or of B in the upper four); four: A and B of plane 0, of plane 1
-      const int pl = MX8 ? x - (DA + DB) : (x - (DA + DB)) >> 1;
-      const bool b = MX8 ? false : ((x - (DA + DB)) & 1) != 0;
+      // the wave's piece of plane 0, of plane 1; or A and B of plane 0, of plane 1
+      const int pl = kScOne ? x - (DA + DB) : (x - (DA + DB)) >> 1;
+      const bool b = kScOne ? false : ((x - (DA + DB)) & 1) != 0;
       const int group = (int)(k0 / (kBK / 2)) + pl;
       const bool dead = kill_sc || group >= ngroups;
       const uint32_t lds = base + kData + pl * 4 * (RA + RB) +
-                           ((MX8 ? wid >= 4 : b) ? 4 * RA + 256 * sb_wave : 256 * sa_wave);
+                           ((kScOne ? sc_b : b) ? 4 * RA + 256 * sb_wave : 256 * sa_wave);
       dma4(b ? srd_sb : srd_sa, lds, dead ? kOob : b ? sb_off : sa_off,
            dead ? 0u : (uint32_t)group * (b ? sb_gs : sa_gs));
     } else if (x == DA + DB)
@@ -1457,10 +1463,11 @@ template <class T>
 int launch_f4(const GemmParams& p, int out_dtype, hipStream_t s) {
   const dim3 grid(grid_blocks(p)), block(tile_threads<T>());
   if constexpr (T::OCC == 2 && T::NS == 3) {
-    // One workgroup a CU at most: two K groups in it, taking alternate steps, share what a step waits for
-    // (128x64, 200 x 2560 x 10240: 23.8 -> 20.7 us, 512 x 2560 x 10240: 26.2 -> 24.2, 512 x 2048 x 2560:
-    // 8.9 -> 8.5). Below eight steps their longer fill and the exchange cost more (64 x 512 x 1280: 6.1
-    // -> 6.5 us). A step takes 0.4-0.5 us however many stages are in flight (six instead of three: 1-2%).
+    // One workgroup a CU at most: two K groups in it, taking alternate steps, share what a step waits
+    // for (128x64, 200 x 2560 x 10240: 22.3 -> 19.6 us, 512 x 2560 x 10240: 23.6 -> 21.9, 512 x 2048 x
+    // 2560: 8.4 -> 8.0). Below eight steps their longer fill and the exchange cost more (64 x 512 x
+    // 1280: 6.1 -> 6.5 us). More stages in flight instead (six for three) gain 1-2%: what a step of
+    // 0.4-0.5 us is short of is room in the CU's load path, about 28 cycles a 1 KB load.
     if (grid.x <= kNumCus && p.splits == 1 && p.K >= 8 * kBK)
       return launch_f4<GemmTile<T::WM, T::WN, T::FM, T::FN, 3, 1, 2>>(p, out_dtype, s);
   }
