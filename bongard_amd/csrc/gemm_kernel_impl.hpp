@@ -912,12 +912,21 @@ gemm_kernel(GemmParams p) {
           dma16(rt, tab + (wid + NW * c) * 1024, lane * 16, (wid + NW * c) * 1024);
     }
   };
+  // FP4 with three stages or more: a step's second half issues the first D1 loads of stage ls + NS,
+  // the next step's first half the others, so that the CU's load path has work through the whole step (a
+  // small tile's loads, all in one half, took longer than it: 512 x 2560 x 10240 on 128x64 22.1 us, now
+  // 19.2; 64 x 2048 x 2560 7.8, now 7.5). With two stages they would land too late.
+  constexpr int D1 = F4 && NS >= 3 ? ND / 2 : ND;
+  auto late_load = [&](int ls, int d) __attribute__((always_inline)) {
+    dma_load(d, stage_ptr(ls), (uint32_t)gstep(ls) * kBK, stage_kill(ls), kstep(ls) >= nsteps,
+             b_ptr(ls));
+  };
   // a resident table goes ahead of the stage loads, so the prologue's wait for stage 0 covers it
   if constexpr (EPI == EPI_GEGLU && !kLateTab) load_table();
 #pragma unroll
   for (int ls = 0; ls < NS; ++ls) {
 #pragma unroll
-    for (int x = 0; x < ND; ++x)
+    for (int x = 0; x < (ls < NS - 1 ? ND : D1); ++x)
       dma_load(x, stage_ptr(ls), (uint32_t)gstep(ls) * kBK, stage_kill(ls),
                kstep(ls) >= nsteps, b_ptr(ls));
   }
@@ -931,7 +940,7 @@ gemm_kernel(GemmParams p) {
   }
   // stage 0 landed: the NS-1 later stages (ND loads each) and the XB B tiles may still be
   // in flight
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ND * (NS - 1) + DB * XB) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(ND * (NS - 2) + D1 + DB * XB) : "memory");
   __syncthreads();
   Frags<NH> f0, f1;
   // same read order as the loop's second half, so that the wait counts at the loop header
@@ -966,6 +975,11 @@ gemm_kernel(GemmParams p) {
 #pragma unroll
       for (int h = x * NH / NR; h < (x + 1) * NH / NR && h < NH; ++h)
         read_one(f1, cur, curb, 1, h);
+      if constexpr (kDma) {
+#pragma unroll
+        for (int d = D1 + x * (ND - D1) / NM; d < D1 + (x + 1) * (ND - D1) / NM; ++d)
+          late_load(ls - 1 + NS, d);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     // stage ls+1 landed (stages ls+2 .. ls+NS-1 may still be in flight; with XB, each
@@ -1000,7 +1014,7 @@ gemm_kernel(GemmParams p) {
       for (int h = x * NH / NM; h < (x + 1) * NH / NM; ++h) read_one(f0, nxt, nxtb, 0, h);
       if constexpr (kDma) {
 #pragma unroll
-        for (int d = x * ND / NM; d < (x + 1) * ND / NM; ++d) {
+        for (int d = x * D1 / NM; d < (x + 1) * D1 / NM; ++d) {
           if (XB == 0 || d < DA)
             dma_load(d, cur, kn, killn, killn_sc, curb);
           else
@@ -1019,6 +1033,8 @@ gemm_kernel(GemmParams p) {
   int ls = 0;
   const std::integral_constant<int, EXTRA_NONE> none{};
   for (; ls < niters - NS; ++ls) step(std::true_type{}, none, ls);
+#pragma unroll
+  for (int d = D1; d < ND; ++d) late_load(ls - 1 + NS, d);
   if constexpr (kLateTab) {
     if (niters >= 2)
       step(std::false_type{}, std::integral_constant<int, EXTRA_TABLE>{}, ls++);
@@ -1464,8 +1480,8 @@ int launch_f4(const GemmParams& p, int out_dtype, hipStream_t s) {
   const dim3 grid(grid_blocks(p)), block(tile_threads<T>());
   if constexpr (T::OCC == 2 && T::NS == 3) {
     // One workgroup a CU at most: two K groups in it, taking alternate steps, share what a step waits
-    // for (128x64, 200 x 2560 x 10240: 22.3 -> 19.6 us, 512 x 2560 x 10240: 23.6 -> 21.9, 512 x 2048 x
-    // 2560: 8.4 -> 8.0). Below eight steps their longer fill and the exchange cost more (64 x 512 x
+    // for (128x64, before the loads were spread: 200 x 2560 x 10240 22.3 -> 19.6 us, 512 x 2560 x 10240
+    // 23.6 -> 21.9, 512 x 2048 x 2560 8.4 -> 8.0). Below eight steps their longer fill and the exchange cost more (64 x 512 x
     // 1280: 6.1 -> 6.5 us). More stages in flight instead (six for three) gain 1-2%: what a step of
     // 0.4-0.5 us is short of is room in the CU's load path, about 28 cycles a 1 KB load.
     if (grid.x <= kNumCus && p.splits == 1 && p.K >= 8 * kBK)
