@@ -398,6 +398,27 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
   return best;
 }
 
+// The plan of an MXFP4 product (K in bytes). Choosing takes 1-2 us of a call's nine on the host, so a
+// thread keeps its last choices by shape; not while one is forced or printed.
+Plan f4_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail) {
+  struct Choice {
+    int64_t M, N, K;
+    size_t ws_avail;
+    bool geglu;
+    Plan plan;
+  };
+  thread_local Choice kept[64] = {};  // (M = 0 holds none)
+  const char* forced = std::getenv("BONGARD_FP8_GEMM_TILE");
+  const char* debug = std::getenv("BONGARD_FP8_GEMM_DEBUG");
+  if ((forced && *forced) || (debug && *debug))
+    return choose_plan(M, N, K, geglu, ws_avail, true, 0, true);
+  const uint64_t h = ((uint64_t)M * 0x9E3779B97F4A7C15u ^ (uint64_t)N) * 0x9E3779B97F4A7C15u ^ (uint64_t)K;
+  Choice& c = kept[(h * 0x9E3779B97F4A7C15u + ws_avail) >> 58];
+  if (c.M != M || c.N != N || c.K != K || c.ws_avail != ws_avail || c.geglu != geglu)
+    c = {M, N, K, ws_avail, geglu, choose_plan(M, N, K, geglu, ws_avail, true, 0, true)};
+  return c.plan;
+}
+
 // ---- K-major operands on small shapes ------------------------------------------------
 // The K-major GEMM runs on the eight-wave 256x256 tiles only, which leave most CUs idle when
 // the output is small (M = 512, N = 2560, K = 2048: 20 tiles; measured 30 us against 12 us
@@ -1017,7 +1038,9 @@ static int gemm_mx_launch(const uint8_t* A, int64_t lda, MxScales a_sc, const ui
   p.n_seg = 1;
   for (int s = 0; s < 4; ++s) p.seg_end[s] = (int)N;
   p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
-  const Plan pl = choose_plan(M, N, K, false, ws ? ws_bytes : 0, true, 0, fmt == kFmtFp4);
+  const size_t ws_avail = ws ? ws_bytes : 0;
+  const Plan pl = fmt == kFmtFp4 ? f4_plan(M, N, K, false, ws_avail)
+                                 : choose_plan(M, N, K, false, ws_avail, true);
   return launch_plan(pl, p, EPI_LINEAR, out_dtype, fmt, fmt, ws, as_stream(stream), true);
 }
 
@@ -1067,7 +1090,7 @@ size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
   // plans are made on K bytes, with MXFP8's costs: over 3,900 shapes the picks lose 0.9% on average
   // against the best measured plan, 3% in one of ten (costs fitted to FP4 itself: 0.8% and 3%)
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return choose_plan(M, N, K / 2, false, (size_t)-1, true, 0, true).ws_bytes;
+  return f4_plan(M, N, K / 2, false, (size_t)-1).ws_bytes;
 }
 
 int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
@@ -1116,7 +1139,8 @@ static int geglu_mx_launch(const uint8_t* X, int64_t ldx, MxScales x_sc, const u
   p.C = H; p.ldc = ldh; p.GU = (uint16_t*)GU; p.partials = nullptr;
   p.h8 = H8; p.h8_sc = h8_sc;
   p.h8t = H8t; p.h8t_sc = h8t_sc;
-  Plan pl = choose_plan(M, 2 * I, K, true, 0, true, 0, fmt == kFmtFp4);
+  const Plan pl = fmt == kFmtFp4 ? f4_plan(M, 2 * I, K, true, 0)
+                                 : choose_plan(M, 2 * I, K, true, 0, true);
   return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, fmt, fmt, nullptr, as_stream(stream), true);
 }
 

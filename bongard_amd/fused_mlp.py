@@ -90,11 +90,12 @@ class _ResidualNorm(torch.autograd.Function):
 
 
 def _residual_norm(h, residual, post_weight, pre_weight, eps, gate, residual_scale):
-    tensors = (h, residual, post_weight, pre_weight, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return _ResidualNorm.apply(*tensors, eps, residual_scale)
-    return _ops.rmsnorm_residual(*tensors[:4], eps, gate=gate, residual_scale=residual_scale,
-                                 zero_centered=True)
+    if torch.is_grad_enabled() and (
+            h.requires_grad or residual.requires_grad or post_weight.requires_grad
+            or pre_weight.requires_grad or (gate is not None and gate.requires_grad)):
+        return _ResidualNorm.apply(h, residual, post_weight, pre_weight, gate, eps, residual_scale)
+    return _ops.rmsnorm_residual(h, residual, post_weight, pre_weight, eps, gate=gate,
+                                 residual_scale=residual_scale, zero_centered=True)
 
 
 _residual_norm_uncompiled = torch.compiler.disable(_residual_norm)

@@ -1387,11 +1387,6 @@ def dequant_mxfp4(q, *, transpose=False):
     return out[:, :q.rows] if transpose and q.rows != cols else out
 
 
-@functools.lru_cache(maxsize=4096)
-def _gemm_mxfp4_ws_cached(M, N, K, override):
-    return int(_lib.lib().bf8_gemm_mxfp4_workspace(M, N, K))
-
-
 def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16, out=None):
     """``C = A @ B.T (+ bias)`` of MXFP4 operands A [M, K] and B [N, K] (codes and scale planes as
     :func:`quantize_mxfp4` writes them) on the block-scaled FP4 MFMA, sums in fp32."""
@@ -1416,11 +1411,11 @@ def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16,
             bias = bias.clone()
     if K == 0:  # an empty sum
         return out.zero_() if bias is None else out.copy_(bias.reshape(1, N).expand(M, N))
-    ws = None
-    ws_bytes = _gemm_mxfp4_ws_cached(M, N, K, _tile_override())
+    L, ws = _lib.lib(), None
+    ws_bytes = L.bf8_gemm_mxfp4_workspace(M, N, K)
     if ws_bytes:
         ws, ws_bytes = _call_workspace(ws_bytes, a)
-    _call("bf8_gemm_mxfp4", idx, _lib.lib().bf8_gemm_mxfp4, a.data_ptr(), a.stride(0),
+    _call("bf8_gemm_mxfp4", idx, L.bf8_gemm_mxfp4, a.data_ptr(), a.stride(0),
           a_planes.data_ptr(), b.data_ptr(), b.stride(0), b_planes.data_ptr(), M, N, K, _ptr(bias),
           out.data_ptr(), OUT_BF16 if out_dtype is torch.bfloat16 else OUT_F32, ldc, _ptr(ws), ws_bytes)
     return out
@@ -1472,12 +1467,16 @@ def geglu_bwd_mxfp4(dH, GU, *, rowwise=True, colwise=False):
 
 
 # ---- the norms on either side of a residual connection ---------------------------------------
+def _norm_weight(who, name, t, cols):
+    if t.dtype is not torch.bfloat16 or t.shape != (cols,):
+        raise ValueError(f"{who}: {name} must be bf16 [{cols}] (got {t.dtype} {tuple(t.shape)})")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone()
+
+
 def _norm_weights(who, cols, post_weight, pre_weight, gate):
-    for name, t in (("post_weight", post_weight), ("pre_weight", pre_weight), ("gate", gate)):
-        if t is not None and (t.dtype is not torch.bfloat16 or t.shape != (cols,)):
-            raise ValueError(f"{who}: {name} must be bf16 [{cols}] (got {t.dtype} {tuple(t.shape)})")
-    return [t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0)
-            else t.contiguous().clone() for t in (post_weight, pre_weight, gate)]
+    return (_norm_weight(who, "post_weight", post_weight, cols),
+            _norm_weight(who, "pre_weight", pre_weight, cols),
+            None if gate is None else _norm_weight(who, "gate", gate, cols))
 
 
 def rmsnorm_residual(h, residual, post_weight, pre_weight, eps, *, gate=None, residual_scale=1.0,

@@ -15,7 +15,7 @@ import pytest
 import torch
 from torch import nn
 
-from bongard_amd import fused_mlp, linear, ops, te_linear
+from bongard_amd import _lib, fused_mlp, linear, ops, te_linear
 from oracle import fp8_oracle as orc
 from oracle import mxfp4_oracle as mx4
 
@@ -440,7 +440,7 @@ def test_two_graphs_at_once(gpu):
     """Calls with a workspace (a product in K pieces, the norm's backward) captured into two graphs,
     replayed side by side on two streams: neither touches the other's."""
     M, N, K = 96, 256, 16384
-    assert ops._gemm_mxfp4_ws_cached(M, N, K, "") > 0
+    assert _lib.lib().bf8_gemm_mxfp4_workspace(M, N, K) > 0
     post, pre = _x(1, 512, 3).to(gpu)[0], _x(1, 512, 4).to(gpu)[0]
 
     def work(a, b, h, dy):
