@@ -577,7 +577,7 @@ gemm_kernel(GemmParams p) {
   // four of scales a wave instead of two 64 x 2048 x 2560 took 8.2 us (now 7.9), 512 x 2560 x 10240 24.2
   // (21.8), 2001 x 2560 x 10240 42.6 (41.2).
   constexpr int kScPieces = (RA + RB) / 64;
-  constexpr bool kScOne = MX8 || (F4 && kScPieces <= NW);
+  constexpr bool kScOne = F4 ? kScPieces <= NW : MX8;
   constexpr int NSC = MX ? (kScOne ? 1 : 2) * (F4 ? 2 : 1) : 0;
   constexpr int ND = DA + DB + NSC;  // loads per wave per stage
   constexpr int NM = FM * FN;                // MFMAs per sub-step
@@ -703,12 +703,13 @@ gemm_kernel(GemmParams p) {
   // read as zero.
   i32x4 srd_sa = {0, 0, 0, 0}, srd_sb = {0, 0, 0, 0};
   uint32_t sa_off = kOob, sb_off = kOob, sa_gs = 0, sb_gs = 0;
-  // Waves past the last piece load an earlier one again, so that every wave issues the same number
-  // of loads.
-  const int sc_piece = __builtin_amdgcn_readfirstlane(kScOne ? wid % kScPieces : wid);
-  const bool sc_b = kScOne && sc_piece >= RA / 64;
-  const int sa_wave = kScOne ? sc_piece - (sc_b ? RA / 64 : 0) : F4 ? sc_piece % (RA / 64) : sc_piece;
-  const int sb_wave = kScOne ? sa_wave : F4 ? sc_piece % (RB / 64) : sc_piece;
+  // FP4: waves past the last piece load an earlier one again, so that every wave issues the same
+  // number of loads.
+  const int sc_piece = F4 ? __builtin_amdgcn_readfirstlane(kScOne ? wid % kScPieces : wid)
+                          : MX8 ? wid & 3 : wid;
+  const bool sc_b = kScOne && (F4 ? sc_piece >= RA / 64 : __builtin_amdgcn_readfirstlane(wid) >= 4);
+  const int sa_wave = !F4 ? sc_piece : kScOne ? sc_piece - (sc_b ? RA / 64 : 0) : sc_piece % (RA / 64);
+  const int sb_wave = !F4 || kScOne ? sa_wave : sc_piece % (RB / 64);
   const int ngroups = F4 ? (p.K + 63) / 64 : ksteps;  // groups of 128 K-values
   if constexpr (MX) {
     auto sc_srd = [&](const MxScales& m, int rows) {
