@@ -25,6 +25,7 @@ weight gradient of the HF formula's autograd, fp32 math) is a kernel as well
 from collections import Counter
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import linear as _linear
@@ -89,10 +90,19 @@ class _ResidualNorm(torch.autograd.Function):
         return (*grads, None, None)
 
 
+def _has_tangent(*tensors):
+    """Whether one of the tensors (None is skipped) is a forward-mode dual: that is no requires_grad,
+    and grad mode does not switch it off."""
+    return _forward_ad._current_level >= 0 and any(
+        t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _residual_norm(h, residual, post_weight, pre_weight, eps, gate, residual_scale):
-    if torch.is_grad_enabled() and (
+    # a recorded call, and one with a tangent (which the function refuses: it has no forward-mode rule)
+    if (torch.is_grad_enabled() and (
             h.requires_grad or residual.requires_grad or post_weight.requires_grad
-            or pre_weight.requires_grad or (gate is not None and gate.requires_grad)):
+            or pre_weight.requires_grad or (gate is not None and gate.requires_grad))
+            or _has_tangent(h, residual, post_weight, pre_weight, gate)):
         return _ResidualNorm.apply(h, residual, post_weight, pre_weight, gate, eps, residual_scale)
     return _ops.rmsnorm_residual(h, residual, post_weight, pre_weight, eps, gate=gate,
                                  residual_scale=residual_scale, zero_centered=True)
@@ -108,7 +118,8 @@ def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
     (``pre_weight``) of the sum. bf16 [..., hidden] tensors; returns ``(the new residual, the
     next block's input)``, differentiable in every tensor. ``gate`` (bf16 [hidden]) multiplies
     the normed h, ``residual_scale`` (a number) the old residual. The sum is formed in fp32 and
-    rounded to bf16 once; the second norm is that of the rounded sum."""
+    rounded to bf16 once; the second norm is that of the rounded sum. Second derivatives and
+    forward-mode tangents raise."""
     # the wrapper that keeps a compiler out costs host time: it is for compiled callers only
     call = _residual_norm_uncompiled if torch.compiler.is_compiling() else _residual_norm
     return call(h, residual, post_weight, pre_weight, float(eps), gate, float(residual_scale))

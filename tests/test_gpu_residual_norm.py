@@ -11,8 +11,9 @@ by one more rounding per row. y is compared with the norm of the kernel's own ro
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from bongard_amd import fused_mlp, ops
+from bongard_amd import fused_mlp, linear, ops
 from oracle import mxfp4_oracle as mx4
 
 pytestmark = pytest.mark.gpu
@@ -248,3 +249,27 @@ def test_every_way_of_calling_gives_the_same(gpu, mode):
         got = call(*(a.detach() for a in args))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert all(a.requires_grad == (mode == "compiled") for a in got)
+
+
+def test_forward_mode(gpu):
+    """A dual tensor is refused by residual_norm and by the layers around it, in and out of no_grad, and no
+    call returns results without its tangent; calls that hold none are as ever, beside it and after."""
+    t = {k: v.to(gpu) for k, v in _inputs(9, 256, 5, True).items()}
+    names = ("h", "res", "post", "pre")
+    want = fused_mlp.residual_norm(*[t[n] for n in names], EPS, gate=t["gate"])
+    w = torch.zeros(256, 256, dtype=torch.bfloat16, device=gpu)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            got = fused_mlp.residual_norm(*[t[n] for n in names], EPS, gate=t["gate"])
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            for name in (*names, "gate"):
+                d = {**t, name: forward_ad.make_dual(t[name], torch.ones_like(t[name]))}
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    fused_mlp.residual_norm(*[d[n] for n in names], EPS, gate=d["gate"])
+            d = forward_ad.make_dual(t["h"], t["h"])
+            with pytest.raises(NotImplementedError, match="jvp"):
+                linear.Mxfp4LinearFunction.apply(d, w, None)
+            with pytest.raises(NotImplementedError, match="jvp"):
+                linear.Mxfp4GegluMlpFunction.apply(d, w, w[:, :128].contiguous(), None, None, 128)
+    got = fused_mlp.residual_norm(*[t[n] for n in names], EPS, gate=t["gate"])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

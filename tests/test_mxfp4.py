@@ -5,8 +5,9 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from bongard_amd import _lib, linear, te_linear
+from bongard_amd import _lib, fused_mlp, linear, ops, te_linear
 from oracle import fp8_oracle as orc
 from oracle import mxfp4_oracle as mx4
 
@@ -138,3 +139,23 @@ def test_sizes_of_nothing():
     assert L.bf8_gemm_mxfp4_workspace(0, 8, 64) == 0
     assert L.bf8_rmsnorm_residual_bwd_workspace(0, 64) == 0
     assert L.bf8_rmsnorm_residual_bwd_workspace(3, 64) >= 2 * 64 * 4
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", ["h", "residual", "post_weight", "pre_weight", "gate"])
+def test_residual_norm_refuses_forward_mode_tangents(monkeypatch, name, grad):
+    """No tangent is dropped: a dual argument is refused, whether gradients are recorded or not, while
+    a call that holds none goes through, also beside a level of forward mode."""
+    monkeypatch.setattr(ops, "rmsnorm_residual",
+                        lambda h, residual, *a, **k: (torch.zeros_like(h), torch.zeros_like(h)))
+    args = dict(h=torch.ones(4, 16), residual=torch.ones(4, 16), post_weight=torch.ones(16),
+                pre_weight=torch.ones(16), gate=torch.ones(16))
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        out, y = fused_mlp.residual_norm(**args)
+        assert out.shape == y.shape == (4, 16)
+        dual = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            fused_mlp.residual_norm(**{**args, name: dual})
+    x = args["h"]
+    told = torch.func.jvp(lambda t: t + fused_mlp.residual_norm(**args)[0], (x,), (x,))
+    assert torch.equal(told[1], x)  # what the transform does not touch is called as ever
