@@ -117,9 +117,13 @@ def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
     of ``h`` (zero-centred ``post_weight``), its addition to ``residual`` and the pre-block norm
     (``pre_weight``) of the sum. bf16 [..., hidden] tensors; returns ``(the new residual, the
     next block's input)``, differentiable in every tensor. ``gate`` (bf16 [hidden]) multiplies
-    the normed h, ``residual_scale`` (a number) the old residual. The sum is formed in fp32 and
-    rounded to bf16 once; the second norm is that of the rounded sum. Second derivatives and
-    forward-mode tangents raise."""
+    the normed h, ``residual_scale`` (a number: it has no gradient) the old residual. The sum is
+    formed in fp32 and rounded to bf16 once; the second norm is that of the rounded sum. Second
+    derivatives and forward-mode tangents raise."""
+    if isinstance(residual_scale, torch.Tensor) and (
+            (torch.is_grad_enabled() and residual_scale.requires_grad) or _has_tangent(residual_scale)):
+        raise ValueError("residual_norm: residual_scale is a number, no gradient of it is computed "
+                         "(got a tensor that asks for one; detach it to pass its value)")
     # the wrapper that keeps a compiler out costs host time: it is for compiled callers only
     call = _residual_norm_uncompiled if torch.compiler.is_compiling() else _residual_norm
     return call(h, residual, post_weight, pre_weight, float(eps), gate, float(residual_scale))

@@ -159,3 +159,26 @@ def test_residual_norm_refuses_forward_mode_tangents(monkeypatch, name, grad):
     x = args["h"]
     told = torch.func.jvp(lambda t: t + fused_mlp.residual_norm(**args)[0], (x,), (x,))
     assert torch.equal(told[1], x)  # what the transform does not touch is called as ever
+
+
+def test_residual_norm_refuses_a_scale_that_wants_a_gradient(monkeypatch):
+    """The residual's scale is a number, for which no gradient is computed: a tensor that asks for one (or
+    holds a tangent) is refused, one that does not is taken as the number it holds."""
+    seen = []
+
+    def record(h, residual, *a, residual_scale, **k):
+        seen.append(residual_scale)
+        return torch.zeros_like(h), torch.zeros_like(h)
+
+    monkeypatch.setattr(ops, "rmsnorm_residual", record)
+    h, w = torch.ones(4, 16), torch.ones(16)
+    scale = torch.tensor(0.5, requires_grad=True)
+    with pytest.raises(ValueError, match="residual_scale"):
+        fused_mlp.residual_norm(h, h, w, w, residual_scale=scale)
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="residual_scale"):
+        dual = forward_ad.make_dual(torch.tensor(0.5), torch.tensor(1.0))
+        fused_mlp.residual_norm(h, h, w, w, residual_scale=dual)
+    fused_mlp.residual_norm(h, h, w, w, residual_scale=scale.detach())
+    with torch.no_grad():
+        fused_mlp.residual_norm(h, h, w, w, residual_scale=scale)
+    assert seen == [0.5, 0.5]
