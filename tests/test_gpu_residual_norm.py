@@ -273,3 +273,25 @@ def test_forward_mode(gpu):
                 linear.Mxfp4GegluMlpFunction.apply(d, w, w[:, :128].contiguous(), None, None, 128)
     got = fused_mlp.residual_norm(*[t[n] for n in names], EPS, gate=t["gate"])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("rows,cols", [(2100, 2568), (2100, 4104), (2100, 8200)])
+def test_blocks_that_take_several_wide_rows(gpu, rows, cols):
+    """Rows of a block each (past 2560 columns, every width's kernel), more of them than the forward's and the
+    backward's blocks: a block's next row, its sums over rows, and the partials of the whole grid."""
+    t = _inputs(rows, cols, rows + cols, True)
+    dev = {k: v.to(gpu) for k, v in t.items()}
+    kw = dict(gate=dev["gate"], residual_scale=0.5)
+
+    def call():
+        out, y = ops.rmsnorm_residual(dev["h"], dev["res"], dev["post"], dev["pre"], EPS, **kw)
+        return dict(zip(("out", "y", "dh", "dres", "dpost", "dpre", "dgate"),
+                        (out, y, *ops.rmsnorm_residual_backward(dev["h"], out, dev["dout"], dev["dy"],
+                                                                dev["post"], dev["pre"], EPS, **kw))))
+
+    got, again = call(), call()
+    ref, tol = _formulas(t, 0.5, 1.0, got["out"].cpu().double())
+    for name, v in got.items():
+        worst = ((v.cpu().double() - ref[name]).abs() / tol[name].clamp(min=1e-300)).max().item()
+        assert worst <= 1.0, f"{name}: {worst:.3g} of the bound"
+        assert torch.equal(v, again[name]), name
