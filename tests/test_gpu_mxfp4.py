@@ -645,3 +645,15 @@ def test_gated_backward_takes_every_gate(gpu):
         q = ops.geglu_bwd_mxfp4(dH, GU, colwise=True)
         assert torch.equal(q.data, want.data) and torch.equal(q.planes, want.planes)
         assert torch.equal(q.data_t, want.data_t) and torch.equal(q.planes_t, want.planes_t)
+
+
+def test_gram_matrix_is_symmetric(gpu):
+    """One tensor as both operands: y is the oracle's product, and y[i, j] and y[j, i], sums of the same
+    terms, differ by no more than two sums of them may."""
+    K, n = 2080, 296
+    a, ra = _operand(n, K, 9, gpu)
+    y = ops.gemm_mxfp4(a.data, a.planes, a.data, a.planes, out_dtype=torch.float32)
+    ref, mag = mx4.mm(ra, ra)
+    _check_product(y, ref, mag, K, torch.float32)
+    y = y.cpu().double()
+    assert bool(((y - y.t()).abs() <= 2 * K * 2.0 ** -23 * mag).all())
