@@ -657,3 +657,23 @@ def test_gram_matrix_is_symmetric(gpu):
     _check_product(y, ref, mag, K, torch.float32)
     y = y.cpu().double()
     assert bool(((y - y.t()).abs() <= 2 * K * 2.0 ** -23 * mag).all())
+
+
+@pytest.mark.parametrize("tile,has", [("256x256w8", True), ("160x256", True), ("64x128", True),
+                                      ("192x256", False)])
+def test_gated_product_runs_the_tile_that_is_named(gpu, monkeypatch, capfd, tile, has):
+    """A named tile is the one that runs where it has a gated FP4 variant (192x256 has none: the plan's own
+    choice, which is printed where it is made), and gives the product and its copies."""
+    M, K, I = 290, 544, 640
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    monkeypatch.setenv("BONGARD_FP8_GEMM_DEBUG", "1")
+    x, w, _, _ = _mlp_inputs(M, K, I, 7, gpu)
+    xq, wq = ops.quantize_mxfp4(x), ops.quantize_mxfp4(w)
+    capfd.readouterr()
+    hq, GU = ops.gemm_geglu_mxfp4(xq.data, xq.planes, wq.data, wq.planes, I, colwise=True, keep_gu=True)
+    assert ("bf8 plan geglu mx" in capfd.readouterr().err) == (not has)
+    ref, mag = mx4.mm(mx4.quantize(x.cpu()), mx4.quantize(w.cpu()))
+    _check_product(GU, ref, mag, K, torch.bfloat16)
+    want = ops.quantize_mxfp4(ops.geglu(GU)[0], colwise=True)
+    assert torch.equal(hq.planes, want.planes) and torch.equal(hq.data, want.data)
+    assert torch.equal(hq.planes_t, want.planes_t) and torch.equal(hq.data_t, want.data_t)

@@ -182,3 +182,21 @@ def test_residual_norm_refuses_a_scale_that_wants_a_gradient(monkeypatch):
     with torch.no_grad():
         fused_mlp.residual_norm(h, h, w, w, residual_scale=scale)
     assert seen == [0.5, 0.5]
+
+
+@pytest.mark.parametrize("tile", ["256x160", "160x256", "128x128", "192x256", "128x64", "64x128", "256x256w8",
+                                  "128x128o2", "128x64:3", "256x256w8:2"])
+def test_a_named_tile_is_the_plan(monkeypatch, capfd, tile):
+    """Every tile of the linear FP4 product can be named (a plan of the planner's own is printed), in as many
+    pieces; 256x128 and 256x256 have no such variant."""
+    L = _lib.lib()
+    M, N, K = 517, 1040, 8224
+    monkeypatch.setenv("BONGARD_FP8_GEMM_DEBUG", "1")
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    pieces = int(tile.partition(":")[2] or 1)
+    assert L.bf8_gemm_mxfp4_workspace(M, N, K) == (4 * pieces * M * N if pieces > 1 else 0)
+    assert "bf8 plan" not in capfd.readouterr().err
+    for none in ("256x128", "256x256"):
+        monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", none)
+        L.bf8_gemm_mxfp4_workspace(M, N, K)
+        assert "bf8 plan gemm mx" in capfd.readouterr().err
