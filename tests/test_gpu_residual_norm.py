@@ -295,3 +295,20 @@ def test_blocks_that_take_several_wide_rows(gpu, rows, cols):
         worst = ((v.cpu().double() - ref[name]).abs() / tol[name].clamp(min=1e-300)).max().item()
         assert worst <= 1.0, f"{name}: {worst:.3g} of the bound"
         assert torch.equal(v, again[name]), name
+
+
+@pytest.mark.parametrize("rows,cols,gate,scale,z", [(65, 2560, True, 0.5, 1.0), (33, 4096, False, -1.25, 0.0)])
+def test_forward_against_the_oracle(gpu, rows, cols, gate, scale, z):
+    """out, and y as the norm of that out (a normed h of zeros added to it)."""
+    t = _inputs(rows, cols, 13, gate)
+    dev = {k: None if v is None else v.to(gpu) for k, v in t.items()}
+    out, y = (v.cpu().double() for v in ops.rmsnorm_residual(
+        dev["h"], dev["res"], dev["post"], dev["pre"], EPS, gate=dev["gate"], residual_scale=scale,
+        zero_centered=bool(z)))
+    d = {k: None if v is None else v.double() for k, v in t.items()}
+    ref, _ = mx4.residual_norm(d["h"], d["res"], d["post"], d["pre"], EPS, d["gate"], scale, z)
+    n = (ref - scale * d["res"]).abs()
+    tol = B16 * ref.abs() + (cols + 16) * U * n + 4 * U * (scale * d["res"]).abs()
+    assert bool(((out - ref).abs() <= tol).all())
+    _, ref = mx4.residual_norm(0 * d["h"], out, d["post"], d["pre"], EPS, d["gate"], 1.0, z)
+    assert bool(((y - ref).abs() <= (B16 + (cols + 16) * U) * ref.abs()).all())

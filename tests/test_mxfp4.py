@@ -200,3 +200,24 @@ def test_a_named_tile_is_the_plan(monkeypatch, capfd, tile):
         monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", none)
         L.bf8_gemm_mxfp4_workspace(M, N, K)
         assert "bf8 plan gemm mx" in capfd.readouterr().err
+
+
+def test_oracle_residual_norm_of_hand_worked_rows():
+    """Rows whose root mean squares are whole: |h| = 2 and |h| = 3, sums of |4| and |2|; a row of zeros."""
+    h = torch.tensor([[2., -2., 2., 2.], [3., 3., -3., 3.], [0., 0., 0., 0.]], dtype=torch.float64)
+    post = torch.tensor([0.5, 0.0, 1.0, -0.5], dtype=torch.float64)
+    gate = torch.tensor([2.0, 1.0, -1.0, 4.0], dtype=torch.float64)
+    pre = torch.tensor([0.0, 1.0, -0.5, -1.0], dtype=torch.float64)
+    # normed h times 1 + post and the gate: [3, -1, -2, 2], [3, 1, 2, 2], zeros
+    res = torch.tensor([[2., 10., -4., 4.], [-2., -6., -8., 0.], [4., 4., -4., 4.]], dtype=torch.float64)
+    out, y = mx4.residual_norm(h, res, post, pre, 1e-300, gate=gate, scale=0.5)
+    assert out.tolist() == [[4., 4., -4., 4.], [2., -2., -2., 2.], [2., 2., -2., 2.]]
+    assert y.tolist() == [[1., 2., -0.5, 0.]] + [[1., -2., -0.5, 0.], [1., 2., -0.5, 0.]]
+    out, y = mx4.residual_norm(h[:2], res[:2], post, pre, 0.0, scale=1.0, z=0.0)
+    assert out.tolist() == [[2.5, 10., -3., 3.5], [-1.5, -6., -9., -0.5]]
+    r = (out.square().sum(-1, keepdim=True) / 4).sqrt()
+    assert torch.allclose(y, out / r * pre, rtol=1e-15, atol=0)
+    # eps counts in the mean of squares: a row of ones under eps 3 is halved
+    one = torch.ones(1, 4, dtype=torch.float64)
+    out, _ = mx4.residual_norm(one, 0 * one, 0 * post, pre, 3.0)
+    assert out.tolist() == [[0.5] * 4]
