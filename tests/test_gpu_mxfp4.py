@@ -677,3 +677,34 @@ def test_gated_product_runs_the_tile_that_is_named(gpu, monkeypatch, capfd, tile
     want = ops.quantize_mxfp4(ops.geglu(GU)[0], colwise=True)
     assert torch.equal(hq.planes, want.planes) and torch.equal(hq.data, want.data)
     assert torch.equal(hq.planes_t, want.planes_t) and torch.equal(hq.data_t, want.data_t)
+
+
+def test_product_with_every_workspace(gpu):
+    """The C entry with its workspace, with less and with none: other plans, each within the product's bound,
+    what lies behind the bytes it was given left alone, and the same bits whenever the bytes are the same."""
+    M, N, K = 96, 256, 16384
+    L = _lib.lib()
+    need = L.bf8_gemm_mxfp4_workspace(M, N, K)
+    assert need > 512
+    a, ra = _operand(M, K, 1, gpu)
+    b, rb = _operand(N, K, 2, gpu, spread=False)
+    ref, mag = mx4.mm(ra, rb)
+    stream = torch.cuda.current_stream(gpu).cuda_stream
+
+    def call(given):
+        ws = torch.full((need,), 0x5A, dtype=torch.uint8, device=gpu)
+        y = torch.full((M, N), 7.0, device=gpu)
+        rc = L.bf8_gemm_mxfp4(a.data.data_ptr(), K // 2, a.planes.data_ptr(), b.data.data_ptr(), K // 2,
+                              b.planes.data_ptr(), M, N, K, None, y.data_ptr(), ops.OUT_F32, N,
+                              ws.data_ptr() if given else None, given, stream)
+        assert rc == 0, L.bf8_last_error()
+        torch.cuda.synchronize()
+        assert bool((ws[given:] == 0x5A).all())
+        _check_product(y, ref, mag, K, torch.float32)
+        return y
+
+    sizes = (0, 256, need // 2 // 256 * 256, need - 256, need)
+    first = [call(s) for s in sizes]
+    for s, y in zip(sizes[::-1], first[::-1]):
+        assert torch.equal(call(s), y), s
+    assert torch.equal(ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=torch.float32), first[-1])
