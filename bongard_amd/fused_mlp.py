@@ -93,16 +93,16 @@ class _ResidualNorm(torch.autograd.Function):
 def _has_tangent(*tensors):
     """Whether one of the tensors (None is skipped) is a forward-mode dual: that is no requires_grad,
     and grad mode does not switch it off."""
-    return _forward_ad._current_level >= 0 and any(
-        t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    return any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _residual_norm(h, residual, post_weight, pre_weight, eps, gate, residual_scale):
-    # a recorded call, and one with a tangent (which the function refuses: it has no forward-mode rule)
+    # a recorded call, and one with a tangent (which the function refuses: it has no forward-mode rule;
+    # looked for inside a forward-mode level only, the one place that has them)
     if (torch.is_grad_enabled() and (
             h.requires_grad or residual.requires_grad or post_weight.requires_grad
             or pre_weight.requires_grad or (gate is not None and gate.requires_grad))
-            or _has_tangent(h, residual, post_weight, pre_weight, gate)):
+            or _forward_ad._current_level >= 0 and _has_tangent(h, residual, post_weight, pre_weight, gate)):
         return _ResidualNorm.apply(h, residual, post_weight, pre_weight, gate, eps, residual_scale)
     return _ops.rmsnorm_residual(h, residual, post_weight, pre_weight, eps, gate=gate,
                                  residual_scale=residual_scale, zero_centered=True)
