@@ -193,10 +193,11 @@ __device__ __forceinline__ v16f mfma_mx(v8i a, v8i b, v16f c, uint32_t sa, uint3
 }
 
 // The FP4 form: 16 bytes a lane, the 32 K-values of block lane >> 5 of 64. At twice the FP8
-// rate, so the two of a 64-byte sub-step take an FP8 MFMA's time. Power bounds the large products: fed
-// from registers with codes of normal numbers the MFMA runs at 6.0-6.5 PFLOP/s (9.6 on zeros); 16384^3
-// reaches 4.8, 8192^3 4.0-4.3. The eight-wave tile's K step of 256 takes 1.0 us on four CUs, 1.6-2.0 on all
-// of them, 1.3-1.5 there with the loads and LDS reads left out.
+// rate, so the two of a 64-byte sub-step take an FP8 MFMA's time. Power seems to bound the large products
+// (from times alone, no clock was read): fed from registers with codes of normal numbers the MFMA runs at
+// 6.0-6.5 PFLOP/s (9.6 on zeros); 16384^3 reaches 4.6-4.8, 8192^3 4.2-4.5. The eight-wave tile's K step of
+// 256 takes 1.0 us on four CUs, 1.6-2.0 on all of them, 1.3-1.5 there with the loads and LDS reads left
+// out. Its FP4 kernels keep 20-32 bytes a lane in scratch (4-7 registers), as its MXFP8 ones do (20-36).
 template <int OPSEL>
 __device__ __forceinline__ v16f mfma_f4(v4u a, v4u b, v16f c, uint32_t sa, uint32_t sb) {
   const v8i av = __builtin_bit_cast(v8i, __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1));

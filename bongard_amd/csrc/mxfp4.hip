@@ -117,9 +117,10 @@ __device__ __forceinline__ void geglu_bwd_rows(Window wd, Window wg, uint32_t od
 
 // The gated-GELU backward and the quantization of its dGU [M, 2I] (p: rows M, cols 2I) from dH [M,
 // I] and GU [M, 2I], I % 128 == 0: dGU goes from registers to its copies. A block takes W / 2 tiles
-// of H one below the other, of each the d_g tile by one wave and the d_u tile by another. 6 B read,
-// 17 / 16 B a copy written per element of H; the lookups and conversions, 22 instructions an
-// element of dGU, take about as long as the bytes and overlap them by half. Both copies, W = 2 / 8,
+// of H one below the other, of each the d_g tile by one wave and the d_u tile by another. 6 B read (10 B
+// of loads: dH and the gate by both waves), 17 / 16 B a copy written per element of H; the lookups and conversions, 22 instructions an
+// element of dGU, take about as long as the bytes and overlap them by half. W = 8 keeps 64 bytes a lane
+// in scratch (13 registers), to fit four waves a SIMD. Both copies, W = 2 / 8,
 // us (a copy of as many bytes): [64, 10240] 9.0 / 17.4, [512, 10240] 20.3 / 23.8 (8.4), [2001,
 // 10240] 63.8 / 58.1 (32.6), [4096, 10240] 115 / 104 (66.8), [8192, 10240] 236 / 200 (134); in two
 // passes 73 + 66 at [4096, 10240].

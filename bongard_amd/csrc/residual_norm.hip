@@ -22,7 +22,8 @@
 // drops what lies past its end without a branch: behind a branch each load was waited for before
 // the next. The backward also holds the column sums of its block (16 registers per 8 columns); with the
 // weights read from LDS where they are used and bf16 pairs unpacked anew in each pass it takes 251
-// registers at 2,560 columns, two waves a SIMD (held as floats: 471, one wave).
+// registers at 2,560 columns, two waves a SIMD (held as floats: 471, one wave). Rows past 8,192 columns
+// spill: the backward's block of 16 waves has 128 registers a lane and keeps 35 more in scratch.
 // Measured, 18,494 x 2,560: forward 74 us, 5.1 TB/s; backward with the weights' gradients 122 us,
 // 4.7 TB/s (140 with the weights in registers). 3,001 x 2,560: 12.3 and 27 us (13.7 and 42).
 #include <hip/hip_runtime.h>

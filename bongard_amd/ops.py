@@ -1484,7 +1484,8 @@ def rmsnorm_residual(h, residual, post_weight, pre_weight, eps, *, gate=None, re
     """The norm of a block's output ``h``, its addition to the residual stream and the norm of the
     sum for the next block, in one kernel (bf16 tensors [..., cols], fp32 arithmetic):
     ``out = residual_scale * residual + gate * rmsnorm(h, post_weight)`` and
-    ``y = rmsnorm(out, pre_weight)``; returns ``(out, y)``. ``gate``: bf16 [cols] or None (1)."""
+    ``y = rmsnorm(out, pre_weight)``; returns ``(out, y)``. ``gate``: bf16 [cols] or None (1). cols: a
+    multiple of 8, 16384 at most. No gradients (:func:`bongard_amd.fused_mlp.residual_norm` has them)."""
     who = "rmsnorm_residual"
     idx = _index_of(who, h, residual, post_weight, pre_weight, gate)
     shape = h.shape

@@ -554,7 +554,7 @@ int bf8_gemm_geglu_mx_planes(const uint8_t* X, int64_t ldx, const uint32_t* X_pl
 /* x: bf16 [rows, cols], cols % 8 == 0. out [rows, cols / 2] with out_planes: blocks along rows,
  * cols % 32 == 0. out_t [cols, R / 2] with out_t_planes [(rows + 127) / 128][cols]: blocks
  * along columns, stored transposed, R = rows rounded up to 32 and the codes past rows 0. Either
- * pair may be NULL (not both). x and out_t 16-byte, the others 4-byte aligned. */
+ * pair may be NULL (not both). cols < 2^24. x and out_t 16-byte, the others 4-byte aligned. */
 int bf8_quantize_mxfp4_bf16(const void* x, int64_t rows, int64_t cols, uint8_t* out,
                             uint32_t* out_planes, uint8_t* out_t, uint32_t* out_t_planes,
                             void* stream);
@@ -565,8 +565,9 @@ int bf8_dequant_mxfp4(const uint8_t* codes, const uint32_t* planes, int64_t rows
                       void* out, void* stream);
 
 /* C [M, N] = A . B^T (+ bias[n]) on MXFP4 operands A [M, K], B [N, K] (row strides lda, ldb in
- * bytes, multiples of 16), sums in fp32; K % 32 == 0, N % 8 == 0, ldc % 4 == 0. ws:
- * bf8_gemm_mxfp4_workspace(M, N, K) bytes, 256-byte aligned, or fewer (a slower plan). */
+ * bytes, multiples of 16; each operand below 2 GiB), sums in fp32; K % 32 == 0, N % 8 == 0,
+ * ldc % 4 == 0. ws: bf8_gemm_mxfp4_workspace(M, N, K) bytes, 256-byte aligned, or fewer (a slower
+ * plan). */
 size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
 int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
                    int64_t ldb, const uint32_t* B_planes, int64_t M, int64_t N, int64_t K,
@@ -577,7 +578,7 @@ int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, cons
  * gated GELU and the quantization of H [M, I] in its epilogue (bongard/te_linear.py:98-103's
  * chain): g, u rounded to bf16, H = bf16(bf16(gelu_tanh(g)) * u), H4 [M, I / 2] with H4_planes and
  * optionally H4t [I, R / 2] with H4t_planes, the bytes bf8_quantize_mxfp4_bf16 gives for that H
- * (which is not written). GU: bf16 [M, 2 I] pre-activations or NULL. I % 128 == 0. */
+ * (which is not written). GU: bf16 [M, 2 I] pre-activations or NULL. I % 128 == 0, M I < 2^31. */
 int bf8_gemm_geglu_mxfp4(const uint8_t* X, int64_t ldx, const uint32_t* X_planes, const uint8_t* W,
                          int64_t ldw, const uint32_t* W_planes, int64_t M, int64_t I, int64_t K,
                          uint8_t* H4, uint32_t* H4_planes, uint8_t* H4t, uint32_t* H4t_planes,
