@@ -1402,7 +1402,7 @@ def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16,
         out, ldc = torch.empty((M, N), dtype=out_dtype, device=a.device), N
     else:
         _out_matrix(who, out, (M, N), out_dtype)
-        ldc = out.stride(0)
+        ldc = out.stride(0) if M > 1 else N
     if bias is not None:
         if bias.dtype != torch.bfloat16 or bias.numel() != N:
             raise ValueError(f"{who}: bias must be bfloat16 [{N}] (got {bias.dtype} {tuple(bias.shape)})")
@@ -1415,7 +1415,8 @@ def gemm_mxfp4(a, a_planes, b, b_planes, *, bias=None, out_dtype=torch.bfloat16,
     ws_bytes = L.bf8_gemm_mxfp4_workspace(M, N, K)
     if ws_bytes:
         ws, ws_bytes = _call_workspace(ws_bytes, a)
-    _call("bf8_gemm_mxfp4", idx, L.bf8_gemm_mxfp4, a.data_ptr(), a.stride(0),
+    # (a single row's stride(0) may be anything)
+    _call("bf8_gemm_mxfp4", idx, L.bf8_gemm_mxfp4, a.data_ptr(), a.stride(0) if M > 1 else K // 2,
           a_planes.data_ptr(), b.data_ptr(), b.stride(0), b_planes.data_ptr(), M, N, K, _ptr(bias),
           out.data_ptr(), OUT_BF16 if out_dtype is torch.bfloat16 else OUT_F32, ldc, _ptr(ws), ws_bytes)
     return out
@@ -1441,7 +1442,8 @@ def gemm_geglu_mxfp4(x, x_planes, w, w_planes, intermediate, *, colwise=False, k
     hq = _new_mxfp4(M, I, True, colwise, x.device)
     GU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=x.device) if keep_gu else None
     if M and I:
-        _call("bf8_gemm_geglu_mxfp4", idx, _lib.lib().bf8_gemm_geglu_mxfp4, x.data_ptr(), x.stride(0),
+        _call("bf8_gemm_geglu_mxfp4", idx, _lib.lib().bf8_gemm_geglu_mxfp4, x.data_ptr(),
+              x.stride(0) if M > 1 else K // 2,
               x_planes.data_ptr(), w.data_ptr(), w.stride(0), w_planes.data_ptr(), M, I, K,
               hq.data.data_ptr(), hq.planes.data_ptr(), _ptr(hq.data_t), _ptr(hq.planes_t), _ptr(GU))
     return hq, GU

@@ -708,3 +708,16 @@ def test_product_with_every_workspace(gpu):
     for s, y in zip(sizes[::-1], first[::-1]):
         assert torch.equal(call(s), y), s
     assert torch.equal(ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=torch.float32), first[-1])
+
+
+def test_one_row_of_any_stride(gpu):
+    """A single row is contiguous whatever its row stride says: operands and results of one row."""
+    x, b = ops.quantize_mxfp4(_x(1, 64, 1).to(gpu)), ops.quantize_mxfp4(_x(256, 64, 2).to(gpu))
+    row = x.data.reshape(-1, 1).t()
+    assert row.stride() == (1, 1) and row.is_contiguous()
+    want = ops.gemm_mxfp4(x.data, x.planes, b.data, b.planes)
+    out = torch.empty(256, 1, dtype=torch.bfloat16, device=gpu).t()
+    assert torch.equal(ops.gemm_mxfp4(row, x.planes, b.data, b.planes, out=out), want)
+    h, gu = ops.gemm_geglu_mxfp4(row, x.planes, b.data, b.planes, 128, keep_gu=True)
+    h2, gu2 = ops.gemm_geglu_mxfp4(x.data, x.planes, b.data, b.planes, 128, keep_gu=True)
+    assert torch.equal(gu, gu2) and torch.equal(h.data, h2.data) and torch.equal(h.planes, h2.planes)
