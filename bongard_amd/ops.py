@@ -945,6 +945,8 @@ def rmsnorm_backward(x, dy, weight, eps, *, zero_centered=True, need_dx=True, ne
     L = _lib.lib()
     dx = torch.empty_like(x) if need_dx else None
     dw = torch.empty(cols, dtype=torch.bfloat16, device=x.device) if need_dw else None
+    if rows == 0:  # a sum over no rows
+        return dx, dw if dw is None else dw.zero_()
     ws, nbytes = None, 0
     if need_dw:
         nbytes = int(L.bf8_rmsnorm_bwd_workspace(rows, cols))

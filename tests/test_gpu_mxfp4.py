@@ -721,3 +721,19 @@ def test_one_row_of_any_stride(gpu):
     h, gu = ops.gemm_geglu_mxfp4(row, x.planes, b.data, b.planes, 128, keep_gu=True)
     h2, gu2 = ops.gemm_geglu_mxfp4(x.data, x.planes, b.data, b.planes, 128, keep_gu=True)
     assert torch.equal(gu, gu2) and torch.equal(h.data, h2.data) and torch.equal(h.planes, h2.planes)
+
+
+def test_modules_train_on_no_rows(gpu):
+    """A step on an empty batch: empty results, gradients of zeros."""
+    H, I = 128, 256
+    torch.manual_seed(0)
+    norm = nn.Module()
+    norm.weight, norm.eps = nn.Parameter(torch.randn(H).to(torch.bfloat16) * 0.1), 1e-6
+    for mod in (te_linear.TELinear([nn.Linear(H, H, bias=False)], "mxfp4"),
+                te_linear.TEMLP(_Mlp(H, I), "mxfp4"), fused_mlp.FusedMLP(_Mlp(H, I), norm, "mxfp4")):
+        mod = mod.to(gpu).train()
+        x = torch.empty(0, H, dtype=torch.bfloat16, device=gpu, requires_grad=True)
+        y = mod(x)
+        y.sum().backward()
+        assert y.shape == x.grad.shape == (0, H)
+        assert all(bool((p.grad == 0).all()) for p in mod.parameters())
