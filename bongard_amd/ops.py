@@ -949,9 +949,7 @@ def rmsnorm_backward(x, dy, weight, eps, *, zero_centered=True, need_dx=True, ne
         return dx, dw if dw is None else dw.zero_()
     ws, nbytes = None, 0
     if need_dw:
-        nbytes = int(L.bf8_rmsnorm_bwd_workspace(rows, cols))
-        ws = gemm_workspace(nbytes, x.device)
-        nbytes = ws.numel()
+        ws, nbytes = _call_workspace(int(L.bf8_rmsnorm_bwd_workspace(rows, cols)), x)
     _lib.check(L.bf8_rmsnorm_bwd_bf16(_ptr(x), _ptr(dy), rows, cols, _ptr(weight), float(eps),
                                       int(bool(zero_centered)), _ptr(dx), _ptr(dw), _ptr(ws),
                                       nbytes, _stream(x.device)), "bf8_rmsnorm_bwd_bf16")

@@ -123,3 +123,29 @@ def test_rmsnorm_backward_matches_autograd(gpu, rows, cols):
     dx_only, none = ops.rmsnorm_backward(x.to(gpu), dy.to(gpu), w.to(gpu), 1e-6, need_dw=False)
     torch.cuda.synchronize()
     assert none is None and torch.equal(dx_only.cpu(), dx.cpu())
+
+
+def test_backwards_of_two_graphs_at_once(gpu):
+    """The weight gradient's partials belong to a graph: two captured backwards replayed side by side on two
+    streams give the eager results each time."""
+    w = _inputs(1, 512, 3)[1].to(gpu)
+    ins = [(_inputs(700, 512, 5 + k)[0].to(gpu), _inputs(700, 512, 15 + k)[0].to(gpu)) for k in range(2)]
+    want = [[t.clone() for t in ops.rmsnorm_backward(*i, w, 1e-6)] for i in ins]
+    torch.cuda.synchronize()
+    sides = []
+    for i in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = ops.rmsnorm_backward(*i, w, 1e-6)
+        sides.append((torch.cuda.Stream(), graph, outs))
+    for rep in range(5):
+        for _, _, outs in sides:
+            for t in outs:
+                t.zero_()
+        torch.cuda.synchronize()
+        for stream, graph, _ in sides:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, _, outs), told in zip(sides, want):
+            assert all(torch.equal(a, b) for a, b in zip(outs, told)), f"replay {rep}"
