@@ -1291,13 +1291,10 @@ def _stream_of(idx):
 
 
 def _call_workspace(nbytes, like):
-    """``(workspace, its bytes)`` of a call: the stream's shared one, or while a graph is captured
-    one of the graph's own (two graphs captured on a stream may replay side by side)."""
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
-    else:
-        ws = gemm_workspace(nbytes, like.device)
-    return ws, ws.numel()
+    """``(workspace, its bytes)`` of a call, its own: two threads may launch on one stream by turns, and
+    two graphs captured on one may replay side by side. It is free for the stream's next call where this one
+    returns. (0.2-0.3 us of host time over a workspace that the stream's calls share, 12-16 us a call.)"""
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes
 
 
 def _rows_bf16(t):

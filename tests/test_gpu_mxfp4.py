@@ -9,6 +9,7 @@
     bit, and on inputs the format holds exactly the gradients are the differences.
 """
 
+import threading
 import types
 
 import pytest
@@ -737,3 +738,37 @@ def test_modules_train_on_no_rows(gpu):
         y.sum().backward()
         assert y.shape == x.grad.shape == (0, H)
         assert all(bool((p.grad == 0).all()) for p in mod.parameters())
+
+
+def test_two_threads_on_one_stream(gpu):
+    """Calls of several launches with a workspace between them (a product in K pieces, the norms' backwards),
+    issued by two threads on one stream: each gets its own results."""
+    M, N, K = 96, 256, 16384
+    w = _x(1, 512, 3).to(gpu)[0]
+
+    def work(a, b, h, dy):
+        y = ops.gemm_mxfp4(a.data, a.planes, b.data, b.planes, out_dtype=torch.float32)
+        out, _ = ops.rmsnorm_residual(h, dy, w, w, 1e-6)
+        return [y, *ops.rmsnorm_residual_backward(h, out, dy, dy, w, w, 1e-6)[:4],
+                *ops.rmsnorm_backward(h, dy, w, 1e-6)]
+
+    ins = [(ops.quantize_mxfp4(_x(M, K, 10 + k).to(gpu)), ops.quantize_mxfp4(_x(N, K, 20 + k).to(gpu)),
+            _x(700, 512, 30 + k).to(gpu), _x(700, 512, 40 + k).to(gpu)) for k in range(2)]
+    want = [work(*i) for i in ins]
+    torch.cuda.synchronize()
+    got, start = [[], []], threading.Barrier(2)
+
+    def run(k):
+        start.wait(30)
+        for _ in range(40):
+            got[k].append(work(*ins[k]))
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        assert len(got[k]) == 40
+        assert all(torch.equal(a, b) for outs in got[k] for a, b in zip(outs, want[k]))

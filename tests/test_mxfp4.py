@@ -221,3 +221,11 @@ def test_oracle_residual_norm_of_hand_worked_rows():
     one = torch.ones(1, 4, dtype=torch.float64)
     out, _ = mx4.residual_norm(one, 0 * one, 0 * post, pre, 3.0)
     assert out.tolist() == [[0.5] * 4]
+
+
+def test_a_call_has_its_workspace_to_itself():
+    """Two calls at once (of two threads on one stream, of two graphs) never share one."""
+    like = torch.empty(0)
+    a, b = ops._call_workspace(1 << 16, like), ops._call_workspace(1 << 16, like)
+    assert a[1] == b[1] == a[0].numel() == 1 << 16
+    assert a[0].data_ptr() != b[0].data_ptr() and a[0].device == like.device
