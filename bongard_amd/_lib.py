@@ -9,7 +9,7 @@ from ctypes import c_float, c_int, c_int64, c_size_t, c_uint32, c_void_p, POINTE
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("libbongard_fp8.so")
-ABI_VERSION = 23
+ABI_VERSION = 24
 
 # name -> (restype, argtypes); mirrors include/bongard_fp8.h one to one.
 SIGNATURES = {
@@ -149,6 +149,30 @@ SIGNATURES = {
     "bf8_rmsnorm_bwd_workspace": (c_size_t, [c_int64, c_int64]),
     "bf8_rmsnorm_bwd_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_float,
                                      c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "bf8_quantize_int8_workspace": (c_size_t, [c_int64, c_int64]),
+    "bf8_quantize_int8_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_size_t, c_void_p]),
+    "bf8_dequant_int8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "bf8_gemm_int8_workspace": (c_size_t, [c_int64, c_int64, c_int64]),
+    "bf8_gemm_int8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                              c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_void_p,
+                              c_size_t, c_void_p]),
+    "bf8_gemm_geglu_int8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                    c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "bf8_column_sums_workspace": (c_size_t, [c_int64, c_int64]),
+    "bf8_column_sums_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_size_t,
+                                     c_void_p]),
+    "bf8_quantize_mxint8_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "bf8_dequant_mxint8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "bf8_geglu_mxint8": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "bf8_geglu_bwd_mxint8": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                     c_void_p]),
+    "bf8_layernorm_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "bf8_layernorm_bwd_workspace": (c_size_t, [c_int64, c_int64]),
+    "bf8_layernorm_bwd_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
 }
 
 _lib = None

@@ -284,6 +284,13 @@ bool f4_tile_ok(int tile, bool geglu) {
   return geglu ? geglu4_rounds(tile) != nullptr : kTiles[tile].planned && kTiles[tile].mx;
 }
 
+// Whether int8 has a linear or gated-GELU variant of `tile` (as gemm_kernel_impl.hpp's i8_tile): its
+// checkpoint blocks of 32 columns do not fit the 256x160 tile's halves of 80.
+bool i8_tile_ok(int tile, bool geglu) {
+  if (geglu) return kTiles[tile].planned && kTiles[tile].geglu_rate > 0 && kTiles[tile].bn % 64 == 0;
+  return kTiles[tile].planned || tile == TILE_256x256w8x;
+}
+
 double geglu4_cost(const Plan& p, int64_t M, int64_t N) {
   const TileInfo& ti = kTiles[p.tile];
   const RoundCost& rc = *geglu4_rounds(p.tile);
@@ -330,11 +337,12 @@ bool env_override(int& tile, int& splits) {
 // and, but for MXFP4's (f4), depend on (M, N) only, so the per-tile amax partial count is known
 // without K.
 Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, bool mx = false,
-                 int kmajor = 0, bool f4 = false) {
+                 int kmajor = 0, bool f4 = false, bool i8 = false) {
   const int64_t ksteps = std::max<int64_t>(cdiv(K, kStepBytes), 1);
   int otile, osplits;
   if (env_override(otile, osplits) && (!geglu || geglu_tile_ok(otile, N, mx)) &&
       (!mx || kTiles[otile].mx) && (!f4 || f4_tile_ok(otile, geglu)) &&
+      (!i8 || i8_tile_ok(otile, geglu)) &&
       (!kmajor || otile == TILE_256x256w8 || otile == TILE_256x256w8x)) {
     Plan p;
     if (!geglu && osplits == kTailSplitOverride) {
@@ -352,6 +360,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
     if (!kTiles[tile].planned || (geglu && !geglu_tile_ok(tile, N, mx)) || (mx && !kTiles[tile].mx))
       continue;
     if (f4 && !f4_tile_ok(tile, geglu)) continue;
+    if (i8 && !i8_tile_ok(tile, geglu)) continue;
     // K-major operands: the eight-wave 256x256 tiles only
     if (kmajor && tile != TILE_256x256w8) continue;
     // The two-stage tiles run unsplit: in K pieces the modelled time is up to 13% short (M = 1024,
@@ -398,24 +407,25 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
   return best;
 }
 
-// The plan of an MXFP4 product (K in bytes). Choosing takes 1-2 us of a call's nine on the host, so a
-// thread keeps its last choices by shape; not while one is forced or printed.
-Plan f4_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail) {
+// The plan of an MXFP4 (fmt kFmtFp4) or int8 product, K in bytes. Choosing takes 1-2 us of a call's nine on
+// the host, so a thread keeps its last choices by shape; not while one is forced or printed.
+Plan kept_plan(int fmt, int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail) {
+  const bool f4 = fmt == kFmtFp4;
   struct Choice {
     int64_t M, N, K;
     size_t ws_avail;
-    bool geglu;
+    bool geglu, f4;
     Plan plan;
   };
   thread_local Choice kept[64] = {};  // (M = 0 holds none)
   const char* forced = std::getenv("BONGARD_FP8_GEMM_TILE");
   const char* debug = std::getenv("BONGARD_FP8_GEMM_DEBUG");
   if ((forced && *forced) || (debug && *debug))
-    return choose_plan(M, N, K, geglu, ws_avail, true, 0, true);
+    return choose_plan(M, N, K, geglu, ws_avail, f4, 0, f4, !f4);
   const uint64_t h = ((uint64_t)M * 0x9E3779B97F4A7C15u ^ (uint64_t)N) * 0x9E3779B97F4A7C15u ^ (uint64_t)K;
   Choice& c = kept[(h * 0x9E3779B97F4A7C15u + ws_avail) >> 58];
-  if (c.M != M || c.N != N || c.K != K || c.ws_avail != ws_avail || c.geglu != geglu)
-    c = {M, N, K, ws_avail, geglu, choose_plan(M, N, K, geglu, ws_avail, true, 0, true)};
+  if (c.M != M || c.N != N || c.K != K || c.ws_avail != ws_avail || c.geglu != geglu || c.f4 != f4)
+    c = {M, N, K, ws_avail, geglu, f4, choose_plan(M, N, K, geglu, ws_avail, f4, 0, f4, !f4)};
   return c.plan;
 }
 
@@ -605,34 +615,39 @@ __device__ __forceinline__ void reduce_store(const ReduceOut& o, float (&v)[8], 
   }
 }
 
-// v = P[0] + P[1] + ... + P[count-1] (8 fp32 at src + s * stride), summed in index order.
-// count <= kMaxSplits. Every load is issued before the first add, so the partials come in
+// v = P[0] + P[1] + ... + P[count-1] (8 fp32 at src + s * stride), summed in index order; SUM int: the
+// int32 sums of an int8 product, exact. count <= kMaxSplits. Every load is issued before the first add, so the partials come in
 // one memory latency instead of one per piece.
+template <class SUM>
 __device__ __forceinline__ void sum_pieces(const float* src, int64_t stride, int count,
                                            float (&v)[8]) {
-  float4 lo[kMaxSplits], hi[kMaxSplits];
+  typedef SUM S4 __attribute__((ext_vector_type(4)));
+  S4 lo[kMaxSplits], hi[kMaxSplits];
 #pragma unroll
   for (int s = 0; s < kMaxSplits; ++s) {
     if (s < count) {
-      lo[s] = *reinterpret_cast<const float4*>(src + s * stride);
-      hi[s] = *reinterpret_cast<const float4*>(src + s * stride + 4);
+      lo[s] = *reinterpret_cast<const S4*>(src + s * stride);
+      hi[s] = *reinterpret_cast<const S4*>(src + s * stride + 4);
     }
   }
-  v[0] = lo[0].x; v[1] = lo[0].y; v[2] = lo[0].z; v[3] = lo[0].w;
-  v[4] = hi[0].x; v[5] = hi[0].y; v[6] = hi[0].z; v[7] = hi[0].w;
 #pragma unroll
   for (int s = 1; s < kMaxSplits; ++s) {
     if (s < count) {
-      v[0] += lo[s].x; v[1] += lo[s].y; v[2] += lo[s].z; v[3] += lo[s].w;
-      v[4] += hi[s].x; v[5] += hi[s].y; v[6] += hi[s].z; v[7] += hi[s].w;
+      lo[0] += lo[s];
+      hi[0] += hi[s];
     }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = (float)lo[0][e];
+    v[4 + e] = (float)hi[0][e];
   }
 }
 
 // C = alpha(n) * sum_s P[s] + bias(n) for the split-K partials P [splits][M][N] (fp32),
 // summed in split order, so the result does not depend on which split finished first.
 // Each thread does 8 columns.
-template <int OUT>
+template <int OUT, class SUM>
 __global__ __launch_bounds__(256) void split_reduce_kernel(const float* __restrict__ P, int splits,
                                                            int64_t stride, int M, int N,
                                                            ReduceOut o) {
@@ -643,7 +658,7 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const float* __restri
     const int m = (int)(g / n8), n = (int)(g % n8) * 8;
     const float* src = P + (int64_t)m * N + n;
     float v[8];
-    sum_pieces(src, stride, splits, v);
+    sum_pieces<SUM>(src, stride, splits, v);
     reduce_store<OUT>(o, v, m, n);
   }
 }
@@ -651,7 +666,7 @@ __global__ __launch_bounds__(256) void split_reduce_kernel(const float* __restri
 // The tail tiles of a tail-split schedule: tile t (walk position full_tiles + t) is the sum
 // of its pieces P[t * pieces + s] ([BM][BN] fp32 each), taken in piece order. A block covers
 // 2048 outputs of one tile, 8 columns a thread.
-template <int OUT>
+template <int OUT, class SUM>
 __global__ __launch_bounds__(256) void tail_reduce_kernel(const float* __restrict__ P, int pieces,
                                                           int bm, int bn, int full_tiles,
                                                           int tiles_m, int tiles_n, int M, int N,
@@ -666,7 +681,7 @@ __global__ __launch_bounds__(256) void tail_reduce_kernel(const float* __restric
   if (m >= M || n >= N) return;  // N % 8 == 0: eight columns are all in or all out
   const float* src = P + (int64_t)t * pieces * bm * bn + row * bn + col;
   float v[8];
-  sum_pieces(src, (int64_t)bm * bn, pieces, v);
+  sum_pieces<SUM>(src, (int64_t)bm * bn, pieces, v);
   reduce_store<OUT>(o, v, m, n);
 }
 
@@ -682,6 +697,7 @@ int launch_plan(const Plan& pl, GemmParams p, int epi, int out_dtype, int fa, in
   o.bias = p.bias; o.C = p.C; o.ldc = p.ldc; o.a_vec = p.a_vec; o.b_vec = p.b_vec;
   o.add = p.add;
   o.unit = mx ? 1 : 0;
+  const bool bf16 = out_dtype == BF8_OUT_BF16;
   if (pl.tail_pieces > 0) {
     // whole tiles write C; the tail tiles' pieces write raw partials, reduced after
     p.full_tiles = pl.full_tiles;
@@ -692,14 +708,11 @@ int launch_plan(const Plan& pl, GemmParams p, int epi, int out_dtype, int fa, in
     const TileInfo& ti = kTiles[pl.tile];
     const int tails = pl.tiles_m * pl.tiles_n - pl.full_tiles;
     const unsigned blocks = (unsigned)(tails * (ti.bm * ti.bn / 2048));
-    if (out_dtype == BF8_OUT_BF16)
-      hipLaunchKernelGGL(tail_reduce_kernel<BF8_OUT_BF16>, dim3(blocks), dim3(256), 0, s,
-                         (const float*)ws, pl.tail_pieces, ti.bm, ti.bn, pl.full_tiles,
-                         pl.tiles_m, pl.tiles_n, p.M, p.N, o);
-    else
-      hipLaunchKernelGGL(tail_reduce_kernel<BF8_OUT_F32>, dim3(blocks), dim3(256), 0, s,
-                         (const float*)ws, pl.tail_pieces, ti.bm, ti.bn, pl.full_tiles,
-                         pl.tiles_m, pl.tiles_n, p.M, p.N, o);
+    const auto reduce = fa == kFmtInt8
+                            ? (bf16 ? tail_reduce_kernel<BF8_OUT_BF16, int> : tail_reduce_kernel<BF8_OUT_F32, int>)
+                            : (bf16 ? tail_reduce_kernel<BF8_OUT_BF16, float> : tail_reduce_kernel<BF8_OUT_F32, float>);
+    hipLaunchKernelGGL(reduce, dim3(blocks), dim3(256), 0, s, (const float*)ws, pl.tail_pieces, ti.bm,
+                       ti.bn, pl.full_tiles, pl.tiles_m, pl.tiles_n, p.M, p.N, o);
     return launch_status("tail_reduce_kernel");
   }
   if (pl.splits == 1) return launch_tile(pl, p, epi, out_dtype, fa, fb, s, mx);
@@ -713,12 +726,11 @@ int launch_plan(const Plan& pl, GemmParams p, int epi, int out_dtype, int fa, in
   if (rc != BF8_OK) return rc;
   const int64_t items = (int64_t)p.M * (p.N / 8);
   const unsigned blocks = (unsigned)std::min<int64_t>(cdiv(items, 256), 4096);
-  if (out_dtype == BF8_OUT_BF16)
-    hipLaunchKernelGGL(split_reduce_kernel<BF8_OUT_BF16>, dim3(blocks), dim3(256), 0, s,
-                       (const float*)ws, pl.splits, q.split_stride, p.M, p.N, o);
-  else
-    hipLaunchKernelGGL(split_reduce_kernel<BF8_OUT_F32>, dim3(blocks), dim3(256), 0, s,
-                       (const float*)ws, pl.splits, q.split_stride, p.M, p.N, o);
+  const auto reduce = fa == kFmtInt8
+                          ? (bf16 ? split_reduce_kernel<BF8_OUT_BF16, int> : split_reduce_kernel<BF8_OUT_F32, int>)
+                          : (bf16 ? split_reduce_kernel<BF8_OUT_BF16, float> : split_reduce_kernel<BF8_OUT_F32, float>);
+  hipLaunchKernelGGL(reduce, dim3(blocks), dim3(256), 0, s, (const float*)ws, pl.splits, q.split_stride,
+                     p.M, p.N, o);
   return launch_status("split_reduce_kernel");
 }
 
@@ -1039,7 +1051,7 @@ static int gemm_mx_launch(const uint8_t* A, int64_t lda, MxScales a_sc, const ui
   for (int s = 0; s < 4; ++s) p.seg_end[s] = (int)N;
   p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
   const size_t ws_avail = ws ? ws_bytes : 0;
-  const Plan pl = fmt == kFmtFp4 ? f4_plan(M, N, K, false, ws_avail)
+  const Plan pl = fmt == kFmtFp4 ? kept_plan(fmt, M, N, K, false, ws_avail)
                                  : choose_plan(M, N, K, false, ws_avail, true);
   return launch_plan(pl, p, EPI_LINEAR, out_dtype, fmt, fmt, ws, as_stream(stream), true);
 }
@@ -1090,7 +1102,7 @@ size_t bf8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
   // plans are made on K bytes, with MXFP8's costs: over 3,900 shapes the picks lose 0.9% on average
   // against the best measured plan, 3% in one of ten (costs fitted to FP4 itself: 0.8% and 3%)
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return f4_plan(M, N, K / 2, false, (size_t)-1).ws_bytes;
+  return kept_plan(kFmtFp4, M, N, K / 2, false, (size_t)-1).ws_bytes;
 }
 
 int bf8_gemm_mxfp4(const uint8_t* A, int64_t lda, const uint32_t* A_planes, const uint8_t* B,
@@ -1139,7 +1151,7 @@ static int geglu_mx_launch(const uint8_t* X, int64_t ldx, MxScales x_sc, const u
   p.C = H; p.ldc = ldh; p.GU = (uint16_t*)GU; p.partials = nullptr;
   p.h8 = H8; p.h8_sc = h8_sc;
   p.h8t = H8t; p.h8t_sc = h8t_sc;
-  const Plan pl = fmt == kFmtFp4 ? f4_plan(M, 2 * I, K, true, 0)
+  const Plan pl = fmt == kFmtFp4 ? kept_plan(fmt, M, 2 * I, K, true, 0)
                                  : choose_plan(M, 2 * I, K, true, 0, true);
   return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, fmt, fmt, nullptr, as_stream(stream), true);
 }
@@ -1229,6 +1241,84 @@ int bf8_gemm_geglu_mxfp4(const uint8_t* X, int64_t ldx, const uint32_t* X_planes
   return geglu_mx_launch(X, ldx, plane_scales(X_planes, M), W, ldw, plane_scales(W_planes, 2 * I),
                          M, I, K / 2, nullptr, I, H4, plane_scales(H4_planes, M), H4t,
                          plane_scales(H4t_planes, I), GU, stream, kFmtFp4);
+}
+
+// ---- int8 ------------------------------------------------------------------------------
+static int check_i8_operand(const char* who, const char* what, const int8_t* q, int64_t ld,
+                            const float* scale, int64_t rows, int64_t K) {
+  BF8_CHECK(q && scale, "%s: %s or its scales are NULL", who, what);
+  BF8_CHECK(ld % 16 == 0 && ld >= K && ((uintptr_t)q & 15) == 0 && ((uintptr_t)scale & 15) == 0,
+            "%s: %s and its scales need 16-byte aligned bases, %s a row stride >= K in multiples of 16",
+            who, what, what);
+  BF8_CHECK(rows * ld < (1LL << 31), "%s: %s larger than 2 GiB", who, what);
+  return BF8_OK;
+}
+
+// An int8 product's operands as the GEMM takes them: a factor for each row of either.
+static GemmParams i8_params(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B,
+                            int64_t ldb, const float* b_scale, int64_t M, int64_t N, int64_t K) {
+  GemmParams p{};
+  p.A = (const uint8_t*)A; p.B = (const uint8_t*)B; p.lda = lda; p.ldb = ldb;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  p.a_sinv = a_scale; p.b_sinv = b_scale;
+  p.a_vec = p.b_vec = 1;
+  p.n_seg = 1;
+  for (int s = 0; s < 4; ++s) p.seg_end[s] = (int)N;
+  return p;
+}
+
+size_t bf8_gemm_int8_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return kept_plan(kFmtInt8, M, N, K, false, (size_t)-1).ws_bytes;
+}
+
+int bf8_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
+                  const float* b_scale, int64_t M, int64_t N, int64_t K, const void* bias, void* C,
+                  int out_dtype, int64_t ldc, void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "bf8_gemm_int8";
+  BF8_CHECK(out_dtype == BF8_OUT_BF16 || out_dtype == BF8_OUT_F32, "%s: bad out_dtype", who);
+  BF8_CHECK(M >= 0 && N >= 0 && K >= 0, "%s: negative shape", who);
+  BF8_CHECK(K % 16 == 0 && K <= kInt8MaxK, "%s: need K %% 16 == 0 and K <= %lld (got %lld)", who,
+            (long long)kInt8MaxK, (long long)K);
+  BF8_CHECK(N % 8 == 0 && ldc >= N && ldc % 4 == 0, "%s: need N %% 8 == 0, ldc >= N, ldc %% 4 == 0",
+            who);
+  BF8_CHECK(((uintptr_t)C & 15) == 0 && ((uintptr_t)bias & 7) == 0,
+            "%s: C must be 16-byte, bias 8-byte aligned", who);
+  BF8_CHECK(ws_bytes == 0 || (ws && ((uintptr_t)ws & 255) == 0),
+            "%s: workspace must be 256-byte aligned", who);
+  if (M == 0 || N == 0) return BF8_OK;
+  BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
+  BF8_CHECK(C != nullptr, "%s: C is NULL", who);
+  if (const int rc = check_i8_operand(who, "A", A, lda, a_scale, M, K)) return rc;
+  if (const int rc = check_i8_operand(who, "B", B, ldb, b_scale, N, K)) return rc;
+  GemmParams p = i8_params(A, lda, a_scale, B, ldb, b_scale, M, N, K);
+  p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
+  const Plan pl = kept_plan(kFmtInt8, M, N, K, false, ws ? ws_bytes : 0);
+  return launch_plan(pl, p, EPI_LINEAR, out_dtype, kFmtInt8, kFmtInt8, ws, as_stream(stream));
+}
+
+int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
+                        const float* w_scale, int64_t M, int64_t I, int64_t K, void* H, int8_t* GU8,
+                        uint8_t* GU8_exp, void* stream) {
+  const char* who = "bf8_gemm_geglu_int8";
+  BF8_CHECK(M >= 0 && I >= 0 && K >= 0, "%s: negative shape", who);
+  BF8_CHECK(I % 128 == 0, "%s: I must be a multiple of 128 (got %lld)", who, (long long)I);
+  BF8_CHECK(K % 16 == 0 && K <= kInt8MaxK, "%s: need K %% 16 == 0 and K <= %lld (got %lld)", who,
+            (long long)kInt8MaxK, (long long)K);
+  BF8_CHECK((GU8 == nullptr) == (GU8_exp == nullptr), "%s: GU8 needs its block exponents", who);
+  BF8_CHECK(((uintptr_t)H & 15) == 0 && ((uintptr_t)GU8 & 7) == 0,
+            "%s: H must be 16-byte, GU8 8-byte aligned", who);
+  if (M == 0 || I == 0) return BF8_OK;
+  BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
+  BF8_CHECK(H != nullptr, "%s: H is NULL", who);
+  if (const int rc = check_i8_operand(who, "X", X, ldx, x_scale, M, K)) return rc;
+  if (const int rc = check_i8_operand(who, "W", W, ldw, w_scale, 2 * I, K)) return rc;
+  GemmParams p = i8_params(X, ldx, x_scale, W, ldw, w_scale, M, 2 * I, K);
+  p.I = (int)I;
+  p.C = H; p.ldc = I;
+  p.gu8 = GU8; p.gu8_e = GU8_exp;
+  const Plan pl = kept_plan(kFmtInt8, M, 2 * I, K, true, 0);
+  return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, kFmtInt8, kFmtInt8, nullptr, as_stream(stream));
 }
 
 }  // extern "C"

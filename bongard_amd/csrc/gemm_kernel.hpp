@@ -12,6 +12,10 @@ enum GemmEpi { EPI_LINEAR = 0, EPI_GEGLU = 1 };
 // Operand format of a bf16 GEMM (both operands bf16: 64 K-values per 128-byte step, so K,
 // lda and ldb are passed in bytes); the FP8 formats are BF8_E4M3 (0) and BF8_E5M2 (1).
 constexpr int kFmtBf16 = 2;
+// Signed 8-bit integers (both), summed in int32 (exactly, for K up to kInt8MaxK); scales a row and a
+// column as a_vec and b_vec.
+constexpr int kFmtInt8 = 3;
+constexpr int64_t kInt8MaxK = 133120;  // * 127^2 < 2^31
 // MXFP4 operands (both; the code the FP4 MFMA names them by): 256 K-values per 128-byte step, K, lda and ldb
 // in bytes, block scales in planes.
 constexpr int kFmtFp4 = 4;
@@ -44,6 +48,8 @@ struct GemmParams {
   void* C;
   int64_t ldc;
   uint16_t* GU;
+  int8_t* gu8;     // int8 GEGLU: the pre-activations as blocks of 32 codes (int8.hpp) [M, 2I] instead of
+  uint8_t* gu8_e;  // GU, with their bytes [M, 2I / 32]
   uint32_t* partials;     // GEGLU: one amax key of |H| per tile
   // GEGLU with H quantized in the epilogue (C, the bf16 H, may then be NULL). h8: e4m3
   // [M, I]; h8t (optional, needs M % 32 == 0): e4m3 H^T [I, M]. MX: E8M0 block scales

@@ -26,6 +26,7 @@
 
 #include "gelu.hpp"
 #include "gemm_kernel.hpp"
+#include "int8.hpp"
 #include "mxfp4.hpp"
 
 namespace bf8 {
@@ -33,6 +34,7 @@ namespace {
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef int v16i __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -181,6 +183,17 @@ __device__ __forceinline__ v16f mfma(v8i a, v8i b, v16f c) {
     // scale operands 0: plain (unscaled) f8f6f4 MFMA; FA/FB select e4m3 (0) / e5m2 (1).
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, 0, 0, 0, 0);
   }
+}
+
+// The int8 form: the 64 bytes of a sub-step are two 32x32x32 MFMAs, one for each 16-byte half of the
+// fragments (as for bf16; together they take an FP8 MFMA's time). Sums are exact.
+template <int FA, int FB>
+__device__ __forceinline__ v16i mfma(v8i a, v8i b, v16i c) {
+  static_assert(FA == kFmtInt8 && FB == kFmtInt8, "int8 GEMMs take two int8 operands");
+  const i32x4 a0 = __builtin_shufflevector(a, a, 0, 1, 2, 3), a1 = __builtin_shufflevector(a, a, 4, 5, 6, 7);
+  const i32x4 b0 = __builtin_shufflevector(b, b, 0, 1, 2, 3), b1 = __builtin_shufflevector(b, b, 4, 5, 6, 7);
+  c = __builtin_amdgcn_mfma_i32_32x32x32_i8(a0, b0, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_i32_32x32x32_i8(a1, b1, c, 0, 0, 0);
 }
 
 // Block-scaled (MX) form: each lane supplies the E8M0 scale of the 32 K-values it holds
@@ -520,6 +533,29 @@ __device__ __forceinline__ void scaled_h_epilogue(const GemmParams& p, const uin
   }
 }
 
+// int8 gated-GELU epilogue: the wave's staged pre-activations (ROWS rows x CH*8 bf16 columns, first row
+// gm0, first column n0 of [M, 2I]) as checkpoint blocks of 32 along the rows (int8.hpp), a group of four
+// lanes a block.
+template <int ROWS, int CH>
+__device__ __forceinline__ void mxi8_gu_epilogue(const GemmParams& p, const uint8_t* wbuf, int lane,
+                                                 int gm0, int n0) {
+  static_assert(CH % 4 == 0, "whole blocks of 32 columns a wave");
+  const int64_t ld = 2 * (int64_t)p.I;
+#pragma unroll 4
+  for (int it = 0; it < ROWS * CH / 64; ++it) {
+    const int idx = it * 64 + lane;
+    const int row = idx / CH, c = idx % CH;
+    const uint4 d = stage_get<CH>(wbuf, row, c);
+    const uint32_t e = mxi8_exponent(quad_max(absmax16(d)));
+    const int gm = gm0 + row;
+    if (gm < p.M) {
+      const int n = n0 + c * 8;
+      *reinterpret_cast<uint2*>(p.gu8 + gm * ld + n) = mxi8_codes8(d, e);
+      if ((c & 3) == 0) p.gu8_e[gm * (ld >> 5) + (n >> 5)] = (uint8_t)e;
+    }
+  }
+}
+
 // The operand fragments of one MFMA sub-step as 16-byte halves, in the order the MFMAs
 // of the sub-step consume them: b0, a0 .. a(FM-1), b1 .. b(FN-1).
 template <int NH>
@@ -829,13 +865,15 @@ gemm_kernel(GemmParams p) {
     }
   };
 
-  v16f acc[FN][FM];
+  constexpr bool I8 = FA == kFmtInt8;
+  using Sum = std::conditional_t<I8, int, float>;
+  std::conditional_t<I8, v16i, v16f> acc[FN][FM];
 #pragma unroll
   for (int i = 0; i < FN; ++i)
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
   // MFMA x of a sub-step: n-subtile x / FM, m-subtile x % FM.
   // MX scales of the current stage (per fragment: the row's four block scales, shifted
@@ -1066,7 +1104,7 @@ gemm_kernel(GemmParams p) {
     // then leaves; group 0 adds them and runs the epilogue alone
     constexpr int kAccBytes = FN * FM * 16 * 64 * 4;  // one wave's accumulators
     static_assert(4 * kAccBytes <= KG * NS * kStage, "accumulator exchange fits the ring");
-    float* xbuf = reinterpret_cast<float*>(smem + wid * kAccBytes);
+    Sum* xbuf = reinterpret_cast<Sum*>(smem + wid * kAccBytes);
     if (kg == 1) {
 #pragma unroll
       for (int i = 0; i < FN; ++i)
@@ -1089,6 +1127,15 @@ gemm_kernel(GemmParams p) {
   }
 
   // ---- epilogue --------------------------------------------------------------------
+  // quad q of sub-tile (i, j) as it is summed up: the bits of its fp32 or int32 sums
+  auto raw4 = [&](int i, int j, int q) __attribute__((always_inline)) {
+    if constexpr (I8)
+      return make_float4(__int_as_float(acc[i][j][4 * q]), __int_as_float(acc[i][j][4 * q + 1]),
+                         __int_as_float(acc[i][j][4 * q + 2]), __int_as_float(acc[i][j][4 * q + 3]));
+    else
+      return make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                         acc[i][j][4 * q + 3]);
+  };
   if constexpr (EPI == EPI_LINEAR) {
     if (tail_slot >= 0) {
       // a K piece of a tail-split tile: raw fp32 sums of the whole BM x BN tile (rows and
@@ -1102,9 +1149,7 @@ gemm_kernel(GemmParams p) {
           for (int j = 0; j < FM; ++j) {
             const int m = wave_m0 + j * 32 + (lane & 31);
             const int n = wn * FN * 32 + i * 32 + 8 * q + (lane >> 5) * 4;
-            *reinterpret_cast<float4*>(base + m * BN + n) =
-                make_float4(acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
-                            acc[i][j][4 * q + 3]);
+            *reinterpret_cast<float4*>(base + m * BN + n) = raw4(i, j, q);
           }
       return;
     }
@@ -1125,7 +1170,7 @@ gemm_kernel(GemmParams p) {
 #pragma unroll
   for (int j = 0; j < FM; ++j) {
     const int m = m0 + wave_m0 + j * 32 + lrow_m;
-    rsa[j] = (vec && p.a_vec) ? p.a_sinv[m < p.M ? m : p.M - 1] : sa;
+    rsa[j] = (vec && p.a_vec) || (I8 && EPI == EPI_GEGLU) ? p.a_sinv[m < p.M ? m : p.M - 1] : sa;
   }
   auto col_factors = [&](int n, float alpha, float* cf) __attribute__((always_inline)) {
     if (vec && p.b_vec && n < p.N) {
@@ -1163,10 +1208,10 @@ gemm_kernel(GemmParams p) {
 #pragma unroll
           for (int j = 0; j < FM; ++j) {
             uint2 w;
-            w.x = pack_bf16x2(__builtin_fmaf(acc[i][j][4 * q + 0], rsa[j] * cf[0], bias[0]),
-                              __builtin_fmaf(acc[i][j][4 * q + 1], rsa[j] * cf[1], bias[1]));
-            w.y = pack_bf16x2(__builtin_fmaf(acc[i][j][4 * q + 2], rsa[j] * cf[2], bias[2]),
-                              __builtin_fmaf(acc[i][j][4 * q + 3], rsa[j] * cf[3], bias[3]));
+            w.x = pack_bf16x2(__builtin_fmaf((float)acc[i][j][4 * q + 0], rsa[j] * cf[0], bias[0]),
+                              __builtin_fmaf((float)acc[i][j][4 * q + 1], rsa[j] * cf[1], bias[1]));
+            w.y = pack_bf16x2(__builtin_fmaf((float)acc[i][j][4 * q + 2], rsa[j] * cf[2], bias[2]),
+                              __builtin_fmaf((float)acc[i][j][4 * q + 3], rsa[j] * cf[3], bias[3]));
             stage_put<CH>(wbuf, j * 32 + lrow_m, col, w);
           }
           continue;
@@ -1174,10 +1219,10 @@ gemm_kernel(GemmParams p) {
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
           uint2 w;
-          w.x = pack_bf16x2(__builtin_fmaf(acc[i][j][4 * q + 0], alpha, bias[0]),
-                            __builtin_fmaf(acc[i][j][4 * q + 1], alpha, bias[1]));
-          w.y = pack_bf16x2(__builtin_fmaf(acc[i][j][4 * q + 2], alpha, bias[2]),
-                            __builtin_fmaf(acc[i][j][4 * q + 3], alpha, bias[3]));
+          w.x = pack_bf16x2(__builtin_fmaf((float)acc[i][j][4 * q + 0], alpha, bias[0]),
+                            __builtin_fmaf((float)acc[i][j][4 * q + 1], alpha, bias[1]));
+          w.y = pack_bf16x2(__builtin_fmaf((float)acc[i][j][4 * q + 2], alpha, bias[2]),
+                            __builtin_fmaf((float)acc[i][j][4 * q + 3], alpha, bias[3]));
           stage_put<CH>(wbuf, j * 32 + lrow_m, col, w);
         }
       }
@@ -1230,10 +1275,10 @@ gemm_kernel(GemmParams p) {
             if (m >= p.M) continue;
             float* c = cbase + (int64_t)m * p.ldc + n;
             *reinterpret_cast<float4*>(c) = make_float4(
-                __builtin_fmaf(acc[i][j][4 * q + 0], rsa[j] * cf[0], bias[0]),
-                __builtin_fmaf(acc[i][j][4 * q + 1], rsa[j] * cf[1], bias[1]),
-                __builtin_fmaf(acc[i][j][4 * q + 2], rsa[j] * cf[2], bias[2]),
-                __builtin_fmaf(acc[i][j][4 * q + 3], rsa[j] * cf[3], bias[3]));
+                __builtin_fmaf((float)acc[i][j][4 * q + 0], rsa[j] * cf[0], bias[0]),
+                __builtin_fmaf((float)acc[i][j][4 * q + 1], rsa[j] * cf[1], bias[1]),
+                __builtin_fmaf((float)acc[i][j][4 * q + 2], rsa[j] * cf[2], bias[2]),
+                __builtin_fmaf((float)acc[i][j][4 * q + 3], rsa[j] * cf[3], bias[3]));
           }
           continue;
         }
@@ -1242,11 +1287,15 @@ gemm_kernel(GemmParams p) {
           const int m = m0 + wave_m0 + j * 32 + lrow_m;
           if (m >= p.M) continue;
           float* c = cbase + (int64_t)m * p.ldc + n;
+          if constexpr (I8) {  // (scaled sums took the branch before)
+            *reinterpret_cast<float4*>(c) = raw4(i, j, q);
+            continue;
+          }
           *reinterpret_cast<float4*>(c) =
-              make_float4(__builtin_fmaf(acc[i][j][4 * q + 0], alpha, bias[0]),
-                          __builtin_fmaf(acc[i][j][4 * q + 1], alpha, bias[1]),
-                          __builtin_fmaf(acc[i][j][4 * q + 2], alpha, bias[2]),
-                          __builtin_fmaf(acc[i][j][4 * q + 3], alpha, bias[3]));
+              make_float4(__builtin_fmaf((float)acc[i][j][4 * q + 0], alpha, bias[0]),
+                          __builtin_fmaf((float)acc[i][j][4 * q + 1], alpha, bias[1]),
+                          __builtin_fmaf((float)acc[i][j][4 * q + 2], alpha, bias[2]),
+                          __builtin_fmaf((float)acc[i][j][4 * q + 3], alpha, bias[3]));
         }
       }
     }
@@ -1271,6 +1320,26 @@ gemm_kernel(GemmParams p) {
         constexpr int gs = Runs::gate_s(k), gq = Runs::gate_q(k);
         constexpr int us = Runs::up_s(k), uq = Runs::up_q(k);
         const int col = 8 * k + lcol;
+        // bf16 pairs of the run's gates (or ups): columns 2 x and 2 x + 1 of row j
+        float fg[4] = {ag, ag, ag, ag}, fu[4] = {au, au, au, au};
+        if constexpr (I8) {  // a scale a column (and a row, below)
+          if (pass != 2) {
+            const float4 f = *reinterpret_cast<const float4*>(p.b_sinv + wave_h0 + col);
+            fg[0] = f.x; fg[1] = f.y; fg[2] = f.z; fg[3] = f.w;
+          }
+          if (pass != 1) {
+            const float4 f = *reinterpret_cast<const float4*>(p.b_sinv + p.I + wave_h0 + col);
+            fu[0] = f.x; fu[1] = f.y; fu[2] = f.z; fu[3] = f.w;
+          }
+        }
+        auto scaled = [&](int s, int q, int j, int x, const float (&f)[4])
+                          __attribute__((always_inline)) {
+          if constexpr (I8)
+            return pack_bf16x2((float)acc[s][j][4 * q + 2 * x] * (rsa[j] * f[2 * x]),
+                               (float)acc[s][j][4 * q + 2 * x + 1] * (rsa[j] * f[2 * x + 1]));
+          else
+            return pack_bf16x2(acc[s][j][4 * q + 2 * x] * f[0], acc[s][j][4 * q + 2 * x + 1] * f[0]);
+        };
         if constexpr (pass == 0) {
           // H of the run's FM rows: bf16 g, u pairs first, then all 4 FM gelu table reads
           // (independent LDS reads in flight together), then the products. Gates outside
@@ -1280,10 +1349,10 @@ gemm_kernel(GemmParams p) {
           uint32_t outside = 0;
 #pragma unroll
           for (int j = 0; j < FM; ++j) {
-            gw[2 * j] = pack_bf16x2(acc[gs][j][4 * gq] * ag, acc[gs][j][4 * gq + 1] * ag);
-            gw[2 * j + 1] = pack_bf16x2(acc[gs][j][4 * gq + 2] * ag, acc[gs][j][4 * gq + 3] * ag);
-            uw[2 * j] = pack_bf16x2(acc[us][j][4 * uq] * au, acc[us][j][4 * uq + 1] * au);
-            uw[2 * j + 1] = pack_bf16x2(acc[us][j][4 * uq + 2] * au, acc[us][j][4 * uq + 3] * au);
+            gw[2 * j] = scaled(gs, gq, j, 0, fg);
+            gw[2 * j + 1] = scaled(gs, gq, j, 1, fg);
+            uw[2 * j] = scaled(us, uq, j, 0, fu);
+            uw[2 * j + 1] = scaled(us, uq, j, 1, fu);
           }
           // gelu(g) as fp32 from the table at LDS offset 0 (byte offsets in packed halves)
 #pragma unroll
@@ -1320,18 +1389,22 @@ gemm_kernel(GemmParams p) {
           for (int j = 0; j < FM; ++j) {
             uint32_t w0, w1;  // packed bf16 pairs (columns 0-1, 2-3 of the run)
             if constexpr (pass == 1) {
-              w0 = pack_bf16x2(acc[gs][j][4 * gq] * ag, acc[gs][j][4 * gq + 1] * ag);
-              w1 = pack_bf16x2(acc[gs][j][4 * gq + 2] * ag, acc[gs][j][4 * gq + 3] * ag);
+              w0 = scaled(gs, gq, j, 0, fg);
+              w1 = scaled(gs, gq, j, 1, fg);
             } else {
-              w0 = pack_bf16x2(acc[us][j][4 * uq] * au, acc[us][j][4 * uq + 1] * au);
-              w1 = pack_bf16x2(acc[us][j][4 * uq + 2] * au, acc[us][j][4 * uq + 3] * au);
+              w0 = scaled(us, uq, j, 0, fu);
+              w1 = scaled(us, uq, j, 1, fu);
             }
             stage_put<CH>(wbuf, j * 32 + lrow_m, col, make_uint2(w0, w1));
           }
         }
       });
       if constexpr (pass == 0) hmax = max(hkeys << 16, hkeys & 0xFFFF0000u);
-      if constexpr (pass == 0) {
+      if constexpr (I8 && pass != 0) {
+        mxi8_gu_epilogue<ROWS, CH>(p, wbuf, lane, m0 + wave_m0, (pass == 2 ? p.I : 0) + wave_h0);
+        return;
+      }
+      if constexpr (pass == 0 && !I8) {
         if (p.h8) {
           // every value this wave quantizes is one it staged: with none of them inf or NaN
           // (and a finite scale) no product can be NaN, so the NaN patch is skipped
@@ -1371,15 +1444,16 @@ gemm_kernel(GemmParams p) {
     // stores drain while the wave computes and stages H (c5's gate/up kernel with GU:
     // 408 -> 397 us alone). Tiles with 256 accumulators a lane keep H first: the other
     // order spills 60 more bytes per lane there.
+    const bool keep_gu = I8 ? p.gu8 != nullptr : p.GU != nullptr;
     if constexpr (NW == 8) {
-      if (p.GU) {
+      if (keep_gu) {
         run_pass(std::integral_constant<int, 1>{});
         run_pass(std::integral_constant<int, 2>{});
       }
       run_pass(std::integral_constant<int, 0>{});
     } else {
       run_pass(std::integral_constant<int, 0>{});
-      if (p.GU) {
+      if (keep_gu) {
         run_pass(std::integral_constant<int, 1>{});
         run_pass(std::integral_constant<int, 2>{});
       }
@@ -1395,6 +1469,19 @@ inline unsigned grid_blocks(const GemmParams& p) {
   const int ntiles = p.tiles_m * p.tiles_n;
   if (p.tail_pieces > 0) return (unsigned)(p.full_tiles + (ntiles - p.full_tiles) * p.tail_pieces);
   return (unsigned)(ntiles * p.splits);
+}
+
+// The tiles that int8 plans take (gemm.hip's i8_tile_ok).
+template <class T>
+constexpr bool i8_tile(int epi) {
+  if (std::is_same<T, Tile256x256>::value || std::is_same<T, Tile256x128>::value ||
+      std::is_same<T, Tile128x128k2>::value)
+    return false;
+  return epi == EPI_LINEAR || T::FN % 2 == 0;
+}
+inline int no_i8_tile(int bm, int bn) {
+  set_error("gemm: tile %dx%d has no such int8 variant", bm, bn);
+  return BF8_EINVAL;
 }
 
 template <class T, int EPI, int OUT>
@@ -1425,6 +1512,13 @@ int launch_typed(const GemmParams& p, int fa, int fb, hipStream_t s) {
     }
     set_error("gemm: bf16 operands need a bf16 partner and a linear epilogue");
     return BF8_EINVAL;
+  }
+  if (fa == kFmtInt8) {
+    if constexpr (EPI == EPI_LINEAR && i8_tile<T>(EPI_LINEAR)) {
+      hipLaunchKernelGGL((gemm_kernel<T, kFmtInt8, kFmtInt8, EPI, OUT>), grid, block, 0, s, p);
+      return launch_status("gemm_kernel(int8)");
+    }
+    return no_i8_tile(T::BM, T::BN);
   }
   if (fa == BF8_E4M3 && fb == BF8_E4M3)
     hipLaunchKernelGGL((gemm_kernel<T, 0, 0, EPI, OUT>), grid, block, 0, s, p);
@@ -1568,6 +1662,14 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
         }
       }
       using TG = typename FitTile<T, EPI_GEGLU, false>::type;
+      if (fmt_a == kFmtInt8) {
+        if constexpr (i8_tile<T>(EPI_GEGLU)) {
+          hipLaunchKernelGGL((gemm_kernel<TG, kFmtInt8, kFmtInt8, EPI_GEGLU, BF8_OUT_BF16>), grid, block,
+                             0, stream, p);
+          return launch_status("gemm_kernel(geglu, int8)");
+        }
+        return no_i8_tile(T::BM, T::BN);
+      }
       if (fmt_a == kFmtBf16 && fmt_b == kFmtBf16) {
         // bf16 operands (NVFP4's exactly dequantized ones): the same epilogue on the sums
         hipLaunchKernelGGL((gemm_kernel<TG, kFmtBf16, kFmtBf16, EPI_GEGLU, BF8_OUT_BF16>), grid,
@@ -1584,6 +1686,7 @@ int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int
         return BF8_EINVAL;
       }
       using TG = typename FitTile<T, EPI_GEGLU, false>::type;
+      if (fmt_a == kFmtInt8) return no_i8_tile(T::BM, T::BN);  // (blocks of 32 columns, as under MX)
       if (fmt_a == kFmtBf16 && fmt_b == kFmtBf16) {
         hipLaunchKernelGGL((gemm_kernel<TG, kFmtBf16, kFmtBf16, EPI_GEGLU, BF8_OUT_BF16>), grid,
                            block, 0, stream, p);

@@ -16,6 +16,7 @@
 
 #include "common.hpp"
 #include "gelu.hpp"
+#include "int8.hpp"
 
 namespace bf8 {
 namespace {
@@ -81,6 +82,67 @@ __global__ __launch_bounds__(kNT) void geglu_fwd_kernel(const uint16_t* __restri
   }
   m = block_max_u32<kNT>(m);
   if (threadIdx.x == 0) partials[blockIdx.x] = m;
+}
+
+// The same, and GU's checkpoint: blocks of 32 codes along its rows (gu8 [M, 2I], gu8_e [M, 2I / 32],
+// I % 32 == 0), a group of four lanes a block of gates and one of ups.
+__global__ __launch_bounds__(kNT) void geglu_fwd_mxi8_kernel(const uint16_t* __restrict__ GU, int64_t M,
+                                                             int64_t I, uint16_t* __restrict__ H,
+                                                             int8_t* __restrict__ gu8,
+                                                             uint8_t* __restrict__ gu8_e) {
+  __shared__ __attribute__((aligned(16))) uint16_t ta[kGeluABytes / 2];
+  load_gelu_tables<kNT>(ta, nullptr);
+  __syncthreads();
+  const int64_t per_row = I / 8;
+  const int64_t nvec = M * per_row;
+  const int64_t stride = (int64_t)gridDim.x * kNT;
+  for (int64_t v = (int64_t)blockIdx.x * kNT + threadIdx.x; v < nvec; v += stride) {
+    const int64_t row = v / per_row;
+    const int64_t col = (v - row * per_row) * 8;
+    const int64_t at = row * 2 * I + col;
+    const uint4 g = *reinterpret_cast<const uint4*>(GU + at);
+    const uint4 u = *reinterpret_cast<const uint4*>(GU + at + I);
+    *reinterpret_cast<uint4*>(H + row * I + col) = geglu_fwd8(g, u, ta);
+    const uint32_t eg = mxi8_exponent(quad_max(absmax16(g)));
+    const uint32_t eu = mxi8_exponent(quad_max(absmax16(u)));
+    *reinterpret_cast<uint2*>(gu8 + at) = mxi8_codes8(g, eg);
+    *reinterpret_cast<uint2*>(gu8 + at + I) = mxi8_codes8(u, eu);
+    if ((v & 3) == 0) {
+      gu8_e[at >> 5] = (uint8_t)eg;
+      gu8_e[(at + I) >> 5] = (uint8_t)eu;
+    }
+  }
+}
+
+// geglu_bwd_kernel from the checkpoint: the same chain on the bf16 values that it holds.
+__global__ __launch_bounds__(kNT) void geglu_bwd_mxi8_kernel(const uint16_t* __restrict__ dH,
+                                                             const int8_t* __restrict__ gu8,
+                                                             const uint8_t* __restrict__ gu8_e,
+                                                             int64_t M, int64_t I,
+                                                             uint16_t* __restrict__ dGU) {
+  __shared__ __attribute__((aligned(16))) uint16_t ta[kGeluABytes / 2];
+  __shared__ __attribute__((aligned(16))) uint32_t tf[kGeluFBytes / 4];
+  load_gelu_tables<kNT>(ta, tf);
+  __syncthreads();
+  const int64_t per_row = I / 8;
+  const int64_t nvec = M * per_row;
+  const int64_t stride = (int64_t)gridDim.x * kNT;
+  for (int64_t v = (int64_t)blockIdx.x * kNT + threadIdx.x; v < nvec; v += stride) {
+    const int64_t row = v / per_row;
+    const int64_t col = (v - row * per_row) * 8;
+    const int64_t at = row * 2 * I + col;
+    const uint4 dh = *reinterpret_cast<const uint4*>(dH + row * I + col);
+    const uint4 g = mxi8_values8(*reinterpret_cast<const uint2*>(gu8 + at), mxi8_step(gu8_e[at >> 5]));
+    const uint4 u = mxi8_values8(*reinterpret_cast<const uint2*>(gu8 + at + I),
+                                 mxi8_step(gu8_e[(at + I) >> 5]));
+    const uint32_t dhw[4] = {dh.x, dh.y, dh.z, dh.w};
+    const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
+    const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
+    uint32_t dg[4], du[4], m = 0;
+    geglu_bwd8(dhw, gw, uw, ta, tf, dg, du, m);
+    *reinterpret_cast<uint4*>(dGU + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
+    *reinterpret_cast<uint4*>(dGU + at + I) = make_uint4(du[0], du[1], du[2], du[3]);
+  }
 }
 
 __global__ __launch_bounds__(kNT) void geglu_bwd_kernel(const uint16_t* __restrict__ dH,
@@ -346,6 +408,35 @@ int bf8_geglu_bwd_delayed(const void* dH, const void* GU, int64_t M, int64_t I, 
                        dh, gu, M, I, state, len, pos, prev_partials, n_prev, meta_out, out, out_t,
                        partials_out);
   return launch_status("geglu_bwd_delayed_kernel");
+}
+
+static int check_geglu_mxi8(const char* who, const void* in, const void* out, const void* gu8,
+                            const void* gu8_e, int64_t M, int64_t I) {
+  BF8_CHECK(M >= 0 && I >= 0 && I % 32 == 0, "%s: need I %% 32 == 0 (M=%lld, I=%lld)", who, (long long)M,
+            (long long)I);
+  if (M == 0 || I == 0) return BF8_OK;
+  BF8_CHECK(in && out && gu8 && gu8_e, "%s: NULL pointer", who);
+  BF8_CHECK((((uintptr_t)in | (uintptr_t)out) & 15) == 0 && ((uintptr_t)gu8 & 7) == 0,
+            "%s: bf16 tensors must be 16-byte, GU8 8-byte aligned", who);
+  return BF8_OK;
+}
+
+int bf8_geglu_mxint8(const void* GU, int64_t M, int64_t I, void* H, int8_t* GU8, uint8_t* GU8_exp,
+                     void* stream) {
+  if (const int rc = check_geglu_mxi8("bf8_geglu_mxint8", GU, H, GU8, GU8_exp, M, I)) return rc;
+  if (M == 0 || I == 0) return BF8_OK;
+  hipLaunchKernelGGL(geglu_fwd_mxi8_kernel, dim3((unsigned)bwd_blocks(M, I)), dim3(kNT), 0,
+                     as_stream(stream), (const uint16_t*)GU, M, I, (uint16_t*)H, GU8, GU8_exp);
+  return launch_status("geglu_fwd_mxi8_kernel");
+}
+
+int bf8_geglu_bwd_mxint8(const void* dH, const int8_t* GU8, const uint8_t* GU8_exp, int64_t M, int64_t I,
+                         void* dGU, void* stream) {
+  if (const int rc = check_geglu_mxi8("bf8_geglu_bwd_mxint8", dH, dGU, GU8, GU8_exp, M, I)) return rc;
+  if (M == 0 || I == 0) return BF8_OK;
+  hipLaunchKernelGGL(geglu_bwd_mxi8_kernel, dim3((unsigned)bwd_blocks(M, I)), dim3(kNT), 0,
+                     as_stream(stream), (const uint16_t*)dH, GU8, GU8_exp, M, I, (uint16_t*)dGU);
+  return launch_status("geglu_bwd_mxi8_kernel");
 }
 
 }  // extern "C"

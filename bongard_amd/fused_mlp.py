@@ -31,10 +31,11 @@ from torch.autograd.function import once_differentiable
 from . import linear as _linear
 from . import ops as _ops
 from . import scaling as _scaling
-from .te_linear import (RECIPES, _is_blocked, _is_mx, _is_mxfp4, _is_nvfp4, _make_recipe,
+from .te_linear import (RECIPES, _is_blocked, _is_int8, _is_mx, _is_mxfp4, _is_nvfp4, _make_recipe,
                         _new_scaling, _pad_rows, _ScalingExtraState, present)
 
-__all__ = ["RECIPES", "FusedMLP", "enable_fused_mlp", "hf_state_dict", "residual_norm"]
+__all__ = ["RECIPES", "FusedMLP", "enable_fused_mlp", "gated_gelu", "hf_state_dict", "layer_norm",
+           "residual_norm"]
 
 
 def _rms_norm(x, weight, eps):
@@ -129,6 +130,69 @@ def residual_norm(h, residual, post_weight, pre_weight, eps=1e-6, *, gate=None,
     return call(h, residual, post_weight, pre_weight, float(eps), gate, float(residual_scale))
 
 
+class _LayerNorm(torch.autograd.Function):
+    """The kernels behind :func:`layer_norm`."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        y, mean, rstd, q = _ops.layernorm(x, weight, bias, eps, want_stats=True, checkpoint=checkpoint)
+        ctx.save_for_backward(*((q.data, q.exps) if checkpoint else (x, None)), weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, exps, weight, mean, rstd = ctx.saved_tensors
+        grads = _ops.layernorm_backward(x if exps is None else _ops.MxInt8Tensor(x, exps), dy, weight, mean,
+                                        rstd, needs=ctx.needs_input_grad[:3])
+        return (*grads, None, None)
+
+
+def _layer_norm(x, weight, bias, eps, checkpoint):
+    # a recorded call, and one with a tangent (as in _residual_norm)
+    if (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad
+                                     or (bias is not None and bias.requires_grad))
+            or _forward_ad._current_level >= 0 and _has_tangent(x, weight, bias)):
+        return _LayerNorm.apply(x, weight, bias, eps, checkpoint)
+    return _ops.layernorm(x, weight, bias, eps)[0]
+
+
+_layer_norm_uncompiled = torch.compiler.disable(_layer_norm)
+
+
+def layer_norm(x, weight, bias=None, eps=1e-6, *, checkpoint=False):
+    """Layer norm of the rows of a bf16 tensor [..., cols] as one kernel each way: ``(x - mean) /
+    sqrt(var + eps) * weight + bias`` in fp32, rounded once; ``weight`` and ``bias`` (or None) bf16
+    [cols], cols a multiple of 8 up to 16384. Differentiable in every tensor; the backward reads x, or
+    with ``checkpoint`` an 8-bit copy of it that the forward writes (blocks of 32 along a row under a power
+    of two, half the bytes; the gradients are those of its values with the mean and variance of x itself).
+    Second derivatives and forward-mode tangents raise."""
+    call = _layer_norm_uncompiled if torch.compiler.is_compiling() else _layer_norm
+    return call(x, weight, bias, float(eps), bool(checkpoint))
+
+
+def _gated_gelu(gu, checkpoint):
+    flat = gu.reshape(-1, gu.shape[-1])
+    if checkpoint:
+        h = _linear.GegluCheckpointFunction.apply(flat)
+    else:
+        h, _ = _linear.GegluFunction.apply(_linear.dense_rows(flat))
+    return h.reshape(*gu.shape[:-1], h.shape[-1])
+
+
+_gated_gelu_uncompiled = torch.compiler.disable(_gated_gelu)
+
+
+def gated_gelu(gu, *, checkpoint=False):
+    """``gelu_tanh(gate) * up`` of bf16 pre-activations [..., 2I] (gate | up), bit for bit the bf16 chain of
+    the gated MLP (bongard/te_linear.py:103), with its backward. ``checkpoint``: the pre-activations are
+    kept for the backward in 8 bits (blocks of 32 along a row under a power of two, half the
+    bytes; I a multiple of 32), and the gradient is the chain's at the values so kept; second derivatives
+    and forward-mode tangents then raise."""
+    call = _gated_gelu_uncompiled if torch.compiler.is_compiling() else _gated_gelu
+    return call(gu, bool(checkpoint))
+
+
 class FusedMLP(_ScalingExtraState, torch.nn.Module):
     """RMSNorm -> fc1 = [gate; up] -> gelu_tanh(gate) * up -> fc2, in FP8 while training."""
 
@@ -208,9 +272,12 @@ class FusedMLP(_ScalingExtraState, torch.nn.Module):
         mx = _is_mx(self.recipe)
         if _is_nvfp4(self.recipe):
             return self._nvfp4_forward(x, flat, length, first)
-        mxfp4 = _is_mxfp4(self.recipe)
+        mxfp4, int8 = _is_mxfp4(self.recipe), _is_int8(self.recipe)
         if first:
-            if mxfp4:
+            if int8:
+                self._fp8_weights = (_linear.quantize_weight_int8(self.fc1_weight),
+                                     _linear.quantize_weight_int8(self.fc2_weight))
+            elif mxfp4:
                 self._fp8_weights = (_linear.quantize_weight_mxfp4(self.fc1_weight),
                                      _linear.quantize_weight_mxfp4(self.fc2_weight))
             elif mx:
@@ -229,15 +296,16 @@ class FusedMLP(_ScalingExtraState, torch.nn.Module):
                     _linear.quantize_weight(self.fc2_weight))
         gu_q, down_q = self._fp8_weights
         flat = _linear.dense_rows(flat.to(torch.bfloat16))
-        if mx or mxfp4:
-            # block scales need no tensor-wide amax: the norm's partials go unused
+        if mx or mxfp4 or int8:
+            # block and row scales need no tensor-wide amax: the norm's partials go unused
             if _ops.rmsnorm_supported(flat.shape[1]):
                 parts = torch.empty(_ops.rmsnorm_partials_count(flat.shape[0]),
                                     dtype=torch.int32, device=flat.device)
                 normed = _FusedRMSNorm.apply(flat, self.layer_norm_weight, self.eps, parts)
             else:
                 normed = _rms_norm(flat, self.layer_norm_weight, self.eps)
-            mlp = _linear.Mxfp4GegluMlpFunction if mxfp4 else _linear.Fp8GegluMlpMxFunction
+            mlp = (_linear.Int8GegluMlpFunction if int8 else _linear.Mxfp4GegluMlpFunction if mxfp4
+                   else _linear.Fp8GegluMlpMxFunction)
             out = mlp.apply(normed, self.fc1_weight, self.fc2_weight, gu_q, down_q,
                             self.intermediate_size)
             # sliced only if padded: a slice's backward fills and copies the whole gradient

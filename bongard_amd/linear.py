@@ -597,6 +597,129 @@ class Mxfp4GegluMlpFunction(_Fp8Function):
         return dx, dgu, dd, None, None, None
 
 
+def quantize_weight_int8(weight, *, transpose=True):
+    """int8 copy of a weight [N, K]: one scale for each row (forward), and with ``transpose`` the
+    columnwise copy with one for each column (the input-gradient GEMM's operand)."""
+    return ops.quantize_int8(dense_rows(weight.detach()), rowwise=True, colwise=transpose)
+
+
+def _check_int8(who, *dims):
+    bad = [d for d in dims if d % 16]
+    if bad:
+        raise ValueError(f"{who}: int8 products need feature sizes that are multiples of 16 "
+                         f"(got {list(dims)})")
+
+
+class Int8LinearFunction(_Fp8Function):
+    """y = x @ W^T (+ b) with every tensor in 8-bit integers, one scale for each token or channel
+    (gradients included; round to nearest even), sums exact in int32; x: bf16 [M, K], any M; W [N, K],
+    K a multiple of 16, N of 8 (of 16 for gradients). ``wq``: a cached int8 weight
+    (:func:`quantize_weight_int8`) or None.
+
+      forward  y  = X8 . W8^T           scales by token and by output channel
+      dgrad    dX = dY8 . (W^T)8^T      dY by token, W by input channel
+      wgrad    dW = (dY^T)8 . (X^T)8^T  dY by output channel, X by input channel (M filled up with
+                                        zeros to whole 16)
+
+    Beside the per-row recipes of bongard/float8_training.py:9 ('rowwise': FP8 with the same
+    granularity); the reference has no counterpart."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, wq):
+        need_dx, need_dw = _forward_needs(ctx, 2)
+        _check_int8("int8 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
+        xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dw)
+        if wq is None or (need_dx and wq.data_t is None):
+            wq = quantize_weight_int8(weight, transpose=need_dx)
+        y = ops.gemm_int8(xq.data, xq.row_scale, wq.data, wq.row_scale, bias=bias)
+        ctx.save_for_backward(xq.data_t, xq.col_scale, wq.data_t if need_dx else None,
+                              wq.col_scale if need_dx else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x8t, xs, w8t, ws = ctx.saved_tensors
+        need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
+        dy = dense_rows(dy)
+        dx = dw = None
+        if need_dx or need_dw:
+            dyq = ops.quantize_int8(dy, rowwise=need_dx, colwise=need_dw)
+        if need_dx:
+            dx = ops.gemm_int8(dyq.data, dyq.row_scale, w8t, ws)
+        if need_dw:
+            dw = ops.gemm_int8(dyq.data_t, dyq.col_scale, x8t, xs)
+        return dx, dw, ops.column_sums(dy) if need_db else None, None
+
+
+class Int8GegluMlpFunction(_Fp8Function):
+    """The gated MLP of :class:`Fp8GegluMlpFunction` with every product in 8-bit integers
+    (:class:`Int8LinearFunction`'s granularity) and the pre-activations kept for the backward as an
+    8-bit checkpoint, half the bytes of bf16: the gate/up product with the gated GELU and the checkpoint
+    in its epilogue, the down product; backward through dH, the gelu chain on the checkpoint's values and
+    the dgrad/wgrad products. x: bf16 [M, K], any M; w_gu [2I, K], w_down [K_out, I], K and K_out
+    multiples of 16, I of 128. ``gu_q`` / ``down_q``: optional cached int8 weights. TEMLP / FusedMLP under
+    'int8' (bongard/te_linear.py:98-103, bongard/fused_mlp.py:25-33 for the chain)."""
+
+    @staticmethod
+    def forward(ctx, x, w_gu, w_down, gu_q, down_q, intermediate):
+        I = int(intermediate)
+        need_dx, need_dgu, need_dd = _forward_needs(ctx, 3)
+        keep = need_dx or need_dgu
+        _check_int8("int8 gated MLP", x.shape[-1], *([w_down.shape[0]] if keep or need_dd else []))
+        xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dgu)
+        if gu_q is None or (need_dx and gu_q.data_t is None):
+            gu_q = quantize_weight_int8(w_gu, transpose=need_dx)
+        H, gu = ops.gemm_geglu_int8(xq.data, xq.row_scale, gu_q.data, gu_q.row_scale, I, keep_gu=keep)
+        if down_q is None or (keep and down_q.data_t is None):
+            down_q = quantize_weight_int8(w_down, transpose=keep)
+        hq = ops.quantize_int8(H, rowwise=True, colwise=need_dd)
+        y = ops.gemm_int8(hq.data, hq.row_scale, down_q.data, down_q.row_scale)
+        ctx.save_for_backward(*((gu.data, gu.exps) if keep else (None, None)), xq.data_t, xq.col_scale,
+                              hq.data_t, hq.col_scale, gu_q.data_t if need_dx else None,
+                              gu_q.col_scale if need_dx else None, down_q.data_t if keep else None,
+                              down_q.col_scale if keep else None)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        gu8, gu_exps, x8t, xs, h8t, hs, gu8t, gus, d8t, ds = ctx.saved_tensors
+        need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]
+        dyq = ops.quantize_int8(dense_rows(dy), rowwise=need_dx or need_dgu, colwise=need_dd)
+        dx = dgu = dd = None
+        if need_dd:
+            dd = ops.gemm_int8(dyq.data_t, dyq.col_scale, h8t, hs)
+        if need_dx or need_dgu:
+            dH = ops.gemm_int8(dyq.data, dyq.row_scale, d8t, ds)
+            dGU = ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(gu8, gu_exps))
+            dq = ops.quantize_int8(dGU, rowwise=need_dx, colwise=need_dgu)
+            if need_dx:
+                dx = ops.gemm_int8(dq.data, dq.row_scale, gu8t, gus)
+            if need_dgu:
+                dgu = ops.gemm_int8(dq.data_t, dq.col_scale, x8t, xs)
+        return dx, dgu, dd, None, None, None
+
+
+class GegluCheckpointFunction(_Fp8Function):
+    """:class:`GegluFunction` that keeps its pre-activations GU [M, 2I] for the backward as an 8-bit
+    checkpoint (I a multiple of 32): H = bf16(bf16(gelu_tanh(gate)) * up), and the gradient of the same
+    bf16 chain (bongard/te_linear.py:103) at the checkpoint's values."""
+
+    @staticmethod
+    def forward(ctx, GU):
+        if not _forward_needs(ctx, 1)[0]:
+            return ops.geglu(GU)[0]
+        H, gu = ops.geglu_mxint8(GU)
+        ctx.save_for_backward(gu.data, gu.exps)
+        return H
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dH):
+        return ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(*ctx.saved_tensors))
+
+
 def mlp_forward(x, w_gu, w_down, gu_q, down_q, intermediate, split_scales, scaling, x_amax,
                 needs):
     """Forward of the FP8 gated MLP (see Fp8GegluMlpFunction): ``(y, saved)`` with saved =

@@ -1544,3 +1544,356 @@ def rmsnorm_residual_backward(h, out, dout, dy, post_weight, pre_weight, eps, *,
     if len(shape) != 2:
         dh, dres = (g if g is None else g.view(shape) for g in (dh, dres))
     return dh, dres, dpost, dpre, dgate
+
+
+# ---- int8: codes under one scale for each row, checkpoints in blocks of 32 ----------------------
+@dataclass
+class Int8Tensor:
+    """An int8 tensor of x [rows, cols]: ``data`` [rows, cols] with ``row_scale`` fp32 [rows] (x ~
+    data * row_scale[:, None]), and/or ``data_t`` [cols, R], one scale for each column of x in
+    ``col_scale`` fp32 [cols] (R is ``rows`` rounded up to 16, the codes past ``rows`` 0)."""
+
+    data: Optional[torch.Tensor]
+    row_scale: Optional[torch.Tensor]
+    data_t: Optional[torch.Tensor]
+    col_scale: Optional[torch.Tensor]
+    rows: int
+    cols: int
+
+
+@functools.lru_cache(maxsize=4096)
+def _quantize_int8_ws_cached(rows, cols):
+    return int(_lib.lib().bf8_quantize_int8_workspace(rows, cols))
+
+
+def quantize_int8(x, *, rowwise=True, colwise=False):
+    """int8 quantization of a bf16 tensor (flattened to [rows, cols]) as an :class:`Int8Tensor`: of each
+    row the scale a / 127, a = max(max|x|, 2^-40), and the codes 127 x / a to nearest (ties to even);
+    ``colwise``: of each column likewise, stored transposed. A row (column) that holds inf or NaN has the
+    scale NaN and codes 0. cols: a multiple of 8 (16 for a product), 32768 at most."""
+    who = "quantize_int8"
+    idx = _index_of(who, x)
+    x = _rows_bf16(x)
+    rows, cols = x.shape
+    if not (rowwise or colwise):
+        raise ValueError(f"{who}: nothing requested")
+    dev = x.device
+    out = scale = out_t = scale_t = ws = None
+    nbytes = 0
+    if rowwise:
+        out = torch.empty((rows, cols), dtype=torch.int8, device=dev)
+        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    if colwise:
+        out_t = torch.empty((cols, (rows + 15) // 16 * 16), dtype=torch.int8, device=dev)
+        scale_t = torch.empty(cols, dtype=torch.float32, device=dev)
+        if rows and cols:
+            ws, nbytes = _call_workspace(_quantize_int8_ws_cached(rows, cols), x)
+    if rows and cols:
+        _call("bf8_quantize_int8_bf16", idx, _lib.lib().bf8_quantize_int8_bf16, x.data_ptr(), rows, cols,
+              _ptr(out), _ptr(scale), _ptr(out_t), _ptr(scale_t), _ptr(ws), nbytes)
+    elif colwise:
+        scale_t.fill_(2.0 ** -40 / 127)
+    if rowwise and not cols:
+        scale.fill_(2.0 ** -40 / 127)
+    return Int8Tensor(out, scale, out_t, scale_t, rows, cols)
+
+
+def _int8_matrix(who, **tensors):
+    for name, t in tensors.items():
+        if t.dtype is not torch.int8:
+            raise TypeError(f"{who}: {name} must be int8 codes (got {t.dtype})")
+        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+            _byte_matrix(who, **{name: t})
+
+
+def _int8_scale(who, name, t, rows):
+    """The scales of an operand of ``rows`` rows as the kernels read them."""
+    if t.dtype is not torch.float32 or t.shape != (rows,):
+        raise ValueError(f"{who}: {name} must be float32 [{rows}] (got {t.dtype} {tuple(t.shape)})")
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.contiguous().clone()
+
+
+def dequant_int8(q, *, transpose=False):
+    """The values of an :class:`Int8Tensor` as bf16 [rows, cols] (code times scale, rounded once), or with
+    ``transpose`` those of its columnwise copy, [cols, rows] (a view of rows padded to 16 where rows
+    is not a multiple)."""
+    who = "dequant_int8"
+    codes, scale = (q.data_t, q.col_scale) if transpose else (q.data, q.row_scale)
+    if codes is None:
+        raise ValueError(f"{who}: the tensor has no {'columnwise' if transpose else 'rowwise'} copy")
+    idx = _index_of(who, codes, scale)
+    _int8_matrix(who, codes=codes)
+    codes = codes.contiguous()
+    rows, cols = codes.shape
+    scale = _int8_scale(who, "scale", scale, rows)
+    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=codes.device)
+    if rows and cols:
+        _call("bf8_dequant_int8", idx, _lib.lib().bf8_dequant_int8, codes.data_ptr(), scale.data_ptr(),
+              rows, cols, out.data_ptr())
+    return out[:, :q.rows] if transpose and q.rows != cols else out
+
+
+def _linear_bias(who, bias, N):
+    if bias.dtype is not torch.bfloat16 or bias.numel() != N:
+        raise ValueError(f"{who}: bias must be bfloat16 [{N}] (got {bias.dtype} {tuple(bias.shape)})")
+    bias = bias.contiguous()
+    return bias if bias.data_ptr() % 8 == 0 else bias.clone()
+
+
+def gemm_int8(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat16, out=None):
+    """``C = a_scale[:, None] * b_scale * (A @ B.T) (+ bias)`` of int8 codes A [M, K] and B [N, K] with
+    fp32 scales [M] and [N] (as :func:`quantize_int8` writes them) on the int8 MFMA; the sums are exact in
+    int32. K a multiple of 16, 133120 at most, N of 8; C bf16 or fp32."""
+    who = "gemm_int8"
+    idx = _index_of(who, a, a_scale, b, b_scale, bias, out)
+    _int8_matrix(who, a=a, b=b)
+    M, K = a.shape
+    N, Kb = b.shape
+    if K != Kb:
+        raise ValueError(f"{who}: inner dims differ ({K} vs {Kb})")
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise TypeError(f"{who}: out_dtype must be bfloat16 or float32")
+    a_scale, b_scale = _int8_scale(who, "a_scale", a_scale, M), _int8_scale(who, "b_scale", b_scale, N)
+    if out is None:
+        out, ldc = torch.empty((M, N), dtype=out_dtype, device=a.device), N
+    else:
+        _out_matrix(who, out, (M, N), out_dtype)
+        ldc = out.stride(0) if M > 1 else N
+    if bias is not None:
+        bias = _linear_bias(who, bias, N)
+    if K == 0:  # an empty sum
+        return out.zero_() if bias is None else out.copy_(bias.reshape(1, N).expand(M, N))
+    L, ws = _lib.lib(), None
+    ws_bytes = L.bf8_gemm_int8_workspace(M, N, K)
+    if ws_bytes:
+        ws, ws_bytes = _call_workspace(ws_bytes, a)
+    # (a single row's stride(0) may be anything)
+    _call("bf8_gemm_int8", idx, L.bf8_gemm_int8, a.data_ptr(), a.stride(0) if M > 1 else K,
+          a_scale.data_ptr(), b.data_ptr(), b.stride(0) if N > 1 else K, b_scale.data_ptr(), M, N, K,
+          _ptr(bias), out.data_ptr(), OUT_BF16 if out_dtype is torch.bfloat16 else OUT_F32, ldc, _ptr(ws),
+          ws_bytes)
+    return out
+
+
+def linear_int8(x, w, w_scale, *, bias=None, out_dtype=torch.bfloat16):
+    """A linear layer of int8 weights in serving: ``y = x @ W.T (+ bias)`` with bf16 x [..., K]
+    quantized by token in the call and W as codes [N, K] under ``w_scale`` [N]. No gradients
+    (:class:`bongard_amd.linear.Int8LinearFunction` has them)."""
+    shape = x.shape
+    q = quantize_int8(x)
+    y = gemm_int8(q.data, q.row_scale, w, w_scale, bias=bias, out_dtype=out_dtype)
+    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[-1])
+
+
+@dataclass
+class MxInt8Tensor:
+    """An 8-bit checkpoint of a bf16 tensor [rows, cols]: ``data`` int8 [rows, cols] and ``exps`` uint8
+    [rows, ceil(cols / 32)], one for each block of 32 along a row; the values are
+    data * 2^(exps - 133) (255: NaN), which bf16 holds exactly."""
+
+    data: torch.Tensor
+    exps: torch.Tensor
+
+
+def _new_mxint8(rows, cols, device):
+    return MxInt8Tensor(torch.empty((rows, cols), dtype=torch.int8, device=device),
+                        torch.empty((rows, (cols + 31) // 32), dtype=torch.uint8, device=device))
+
+
+def _mxint8_of(who, q, rows, cols):
+    if (q.data.dtype is not torch.int8 or q.exps.dtype is not torch.uint8 or q.data.shape != (rows, cols)
+            or q.exps.shape != (rows, (cols + 31) // 32)):
+        raise ValueError(f"{who}: the checkpoint must be int8 [{rows}, {cols}] with uint8 exponents "
+                         f"[{rows}, {(cols + 31) // 32}] (got {q.data.dtype} {tuple(q.data.shape)}, "
+                         f"{q.exps.dtype} {tuple(q.exps.shape)})")
+    data = q.data.contiguous()
+    return data if data.data_ptr() % 8 == 0 else data.clone(), q.exps.contiguous()
+
+
+def quantize_mxint8(x):
+    """The 8-bit checkpoint of a bf16 tensor (flattened to [rows, cols], cols a multiple of 8) as a
+    :class:`MxInt8Tensor`: of each block of 32 along a row the least power of two at which its largest
+    value is within 127 steps, and the values to the nearest step (ties to even); a block that
+    holds inf or NaN reads back as NaN."""
+    idx = _index_of("quantize_mxint8", x)
+    x = _rows_bf16(x)
+    rows, cols = x.shape
+    q = _new_mxint8(rows, cols, x.device)
+    if rows and cols:
+        _call("bf8_quantize_mxint8_bf16", idx, _lib.lib().bf8_quantize_mxint8_bf16, x.data_ptr(), rows,
+              cols, q.data.data_ptr(), q.exps.data_ptr())
+    return q
+
+
+def dequant_mxint8(q):
+    """The values of a :class:`MxInt8Tensor` as bf16 [rows, cols]."""
+    who = "dequant_mxint8"
+    idx = _index_of(who, q.data, q.exps)
+    rows, cols = q.data.shape
+    data, exps = _mxint8_of(who, q, rows, cols)
+    out = torch.empty((rows, cols), dtype=torch.bfloat16, device=data.device)
+    if rows and cols:
+        _call("bf8_dequant_mxint8", idx, _lib.lib().bf8_dequant_mxint8, data.data_ptr(), exps.data_ptr(),
+              rows, cols, out.data_ptr())
+    return out
+
+
+def gemm_geglu_int8(x, x_scale, w, w_scale, intermediate, *, keep_gu=False):
+    """Gate/up product of int8 operands X [M, K] and W [2I, K] (gate rows then up rows) with the gated
+    GELU: ``(H, checkpoint or None)``, H bf16 [M, I] = gelu_tanh(gate) * up (gate, up, the activation
+    and H rounded to bf16, as :func:`geglu` does) and, with ``keep_gu``, the :class:`MxInt8Tensor` of the
+    bf16 pre-activations. I must be a multiple of 128."""
+    who = "gemm_geglu_int8"
+    idx = _index_of(who, x, x_scale, w, w_scale)
+    _int8_matrix(who, x=x, w=w)
+    I = int(intermediate)
+    M, K = x.shape
+    N, Kw = w.shape
+    if N != 2 * I or K != Kw:
+        raise ValueError(f"{who}: w must have {2 * I} rows of {K} values (got {N} of {Kw})")
+    if I % 128:
+        raise ValueError(f"{who}: the intermediate size must be a multiple of 128 (got {I})")
+    if K == 0:
+        raise ValueError(f"{who}: K must not be 0")
+    x_scale, w_scale = _int8_scale(who, "x_scale", x_scale, M), _int8_scale(who, "w_scale", w_scale, N)
+    H = torch.empty((M, I), dtype=torch.bfloat16, device=x.device)
+    gu = _new_mxint8(M, N, x.device) if keep_gu else None
+    if M and I:
+        _call("bf8_gemm_geglu_int8", idx, _lib.lib().bf8_gemm_geglu_int8, x.data_ptr(),
+              x.stride(0) if M > 1 else K, x_scale.data_ptr(), w.data_ptr(), w.stride(0),
+              w_scale.data_ptr(), M, I, K, H.data_ptr(), gu.data.data_ptr() if keep_gu else None,
+              gu.exps.data_ptr() if keep_gu else None)
+    return H, gu
+
+
+def geglu_mlp_int8(x, w_gu, w_gu_scale, w_down, w_down_scale):
+    """The gated MLP of int8 weights in serving: bf16 x [..., K], W_gu as codes [2I, K] (gate rows then
+    up rows) and W_down [N, I], each with its scales; x and the activation are quantized by token in the
+    call. No gradients (:class:`bongard_amd.linear.Int8GegluMlpFunction` has them)."""
+    shape = x.shape
+    q = quantize_int8(x)
+    H, _ = gemm_geglu_int8(q.data, q.row_scale, w_gu, w_gu_scale, w_gu.shape[0] // 2)
+    y = linear_int8(H, w_down, w_down_scale)
+    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[-1])
+
+
+def geglu_mxint8(GU):
+    """:func:`geglu` whose pre-activations are kept for the backward in 8 bits: ``(H bf16 [M, I], the
+    MxInt8Tensor of GU [M, 2I])`` from bf16 GU in one pass. I must be a multiple of 32."""
+    who = "geglu_mxint8"
+    idx = _index_of(who, GU)
+    if GU.dtype is not torch.bfloat16 or GU.dim() != 2 or GU.shape[1] % 64:
+        raise ValueError(f"{who}: GU must be bf16 [M, 2I], I a multiple of 32 (got {GU.dtype} "
+                         f"{tuple(GU.shape)})")
+    GU = _rows_bf16(GU)
+    M, I = GU.shape[0], GU.shape[1] // 2
+    H, q = torch.empty((M, I), dtype=torch.bfloat16, device=GU.device), _new_mxint8(M, 2 * I, GU.device)
+    if M and I:
+        _call("bf8_geglu_mxint8", idx, _lib.lib().bf8_geglu_mxint8, GU.data_ptr(), M, I, H.data_ptr(),
+              q.data.data_ptr(), q.exps.data_ptr())
+    return H, q
+
+
+def geglu_bwd_mxint8(dH, gu):
+    """:func:`geglu_bwd` on the values of GU's checkpoint: dGU bf16 [M, 2I]."""
+    who = "geglu_bwd_mxint8"
+    idx = _index_of(who, dH, gu.data, gu.exps)
+    dH = _rows_bf16(dH)
+    M, I = dH.shape
+    if I % 32:
+        raise ValueError(f"{who}: the intermediate size must be a multiple of 32 (got {I})")
+    data, exps = _mxint8_of(who, gu, M, 2 * I)
+    dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
+    if M and I:
+        _call("bf8_geglu_bwd_mxint8", idx, _lib.lib().bf8_geglu_bwd_mxint8, dH.data_ptr(),
+              data.data_ptr(), exps.data_ptr(), M, I, dGU.data_ptr())
+    return dGU
+
+
+def column_sums(x):
+    """bf16 [cols] sums over the rows of a bf16 tensor (flattened to [rows, cols], cols a multiple of 8),
+    in fp32 and a fixed order: the gradient of a bias."""
+    idx = _index_of("column_sums", x)
+    x = _rows_bf16(x)
+    rows, cols = x.shape
+    if not rows:
+        return x.new_zeros(cols)
+    out = torch.empty(cols, dtype=torch.bfloat16, device=x.device)
+    if cols:
+        L = _lib.lib()
+        ws, nbytes = _call_workspace(L.bf8_column_sums_workspace(rows, cols), x)
+        _call("bf8_column_sums_bf16", idx, L.bf8_column_sums_bf16, x.data_ptr(), rows, cols,
+              out.data_ptr(), ws.data_ptr(), nbytes)
+    return out
+
+
+# ---- layer norm ------------------------------------------------------------------------------
+def layernorm(x, weight, bias, eps, *, want_stats=False, checkpoint=False):
+    """Layer norm of the rows of a bf16 tensor [..., cols] (fp32 arithmetic): ``(y, mean, rstd,
+    checkpoint)``. ``bias``: bf16 [cols] or None. ``want_stats``: the rows' fp32 mean and 1 / sqrt(var +
+    eps) (else None); ``checkpoint``: the :class:`MxInt8Tensor` of x, written in the same pass (else
+    None). cols: a multiple of 8, 16384 at most. No gradients
+    (:func:`bongard_amd.fused_mlp.layer_norm` has them)."""
+    who = "layernorm"
+    idx = _index_of(who, x, weight, bias)
+    shape = x.shape
+    weight = _norm_weight(who, "weight", weight, shape[-1])
+    bias = None if bias is None else _norm_weight(who, "bias", bias, shape[-1])
+    x = _rows_bf16(x)
+    rows, cols = x.shape
+    y = torch.empty_like(x)
+    mean = rstd = q = None
+    if want_stats:
+        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+    if checkpoint:
+        q = _new_mxint8(rows, cols, x.device)
+    if rows:
+        _call("bf8_layernorm_bf16", idx, _lib.lib().bf8_layernorm_bf16, x.data_ptr(), rows, cols,
+              weight.data_ptr(), _ptr(bias), eps, y.data_ptr(), _ptr(mean), _ptr(rstd),
+              q.data.data_ptr() if checkpoint else None, q.exps.data_ptr() if checkpoint else None)
+    return y if len(shape) == 2 else y.view(shape), mean, rstd, q
+
+
+@functools.lru_cache(maxsize=4096)
+def _layernorm_ws_cached(rows, cols):
+    return int(_lib.lib().bf8_layernorm_bwd_workspace(rows, cols))
+
+
+def layernorm_backward(x, dy, weight, mean, rstd, *, needs=(True, True, True)):
+    """Gradients ``(dx, dweight, dbias)`` of :func:`layernorm` for ``dy``, from the forward's ``mean`` and
+    ``rstd`` and its input ``x`` or that input's checkpoint (an :class:`MxInt8Tensor`). ``needs``: which
+    to compute (the others are None)."""
+    who = "layernorm_backward"
+    q = x if isinstance(x, MxInt8Tensor) else None
+    idx = _index_of(who, dy, q.data if q else x, q.exps if q else None, weight, mean, rstd)
+    shape = dy.shape
+    weight = _norm_weight(who, "weight", weight, shape[-1])
+    dy = _rows_bf16(dy)
+    rows, cols = dy.shape
+    if q is not None:
+        data, exps = _mxint8_of(who, q, rows, cols)
+    elif x.shape != shape:
+        raise ValueError(f"{who}: x must be {tuple(shape)} (got {tuple(x.shape)})")
+    else:
+        x = _rows_bf16(x)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype is not torch.float32 or t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous float32 [{rows}] (got {t.dtype} "
+                             f"{tuple(t.shape)})")
+    dx = torch.empty_like(dy) if needs[0] else None
+    dw, db = (torch.empty_like(weight) if n else None for n in needs[1:])
+    if rows == 0:
+        for g in (dw, db):
+            if g is not None:
+                g.zero_()
+    elif any(needs):
+        ws, nbytes = None, 0
+        if needs[1] or needs[2]:
+            ws, nbytes = _call_workspace(_layernorm_ws_cached(rows, cols), dy)
+        _call("bf8_layernorm_bwd_bf16", idx, _lib.lib().bf8_layernorm_bwd_bf16,
+              None if q else x.data_ptr(), data.data_ptr() if q else None, exps.data_ptr() if q else None,
+              dy.data_ptr(), rows, cols, weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(dx),
+              _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+    if dx is not None and len(shape) != 2:
+        dx = dx.view(shape)
+    return dx, dw, db

@@ -31,7 +31,10 @@ gate_up GEMM's epilogue (GegluGateUpNvfp4Function; the split projections use the
 GegluFunction); stateless, like 'mxfp8'. 'mxfp4' (an addition to the reference's names) is the
 4-bit format that gfx950 multiplies itself: every tensor in e2m1 blocks of 32 under a power of
 two, round to nearest even (bongard_amd.linear.Mxfp4LinearFunction / Mxfp4GegluMlpFunction), any
-number of rows unpadded; stateless.
+number of rows unpadded; stateless. 'int8' (an addition as well) holds every tensor in 8-bit
+integers with one scale for each token or channel (bongard_amd.linear.Int8LinearFunction /
+Int8GegluMlpFunction, which also keeps the MLP's pre-activations for the backward in 8 bits), any number of
+rows unpadded; stateless.
 """
 
 import os
@@ -45,7 +48,7 @@ from . import linear as _linear
 from . import scaling as _scaling
 from .scaling import LinearScaling
 
-RECIPES = ('nvfp4', 'mxfp8', 'fp8', 'fp8_delayed', 'mxfp4')
+RECIPES = ('nvfp4', 'mxfp8', 'fp8', 'fp8_delayed', 'mxfp4', 'int8')
 ATTENTION_PROJECTIONS = ('q_proj', 'k_proj', 'v_proj', 'o_proj')
 
 
@@ -92,6 +95,15 @@ class MXFP4BlockScaling:
     block_size: int = 32
 
 
+@dataclass(frozen=True)
+class Int8Scaling:
+    """8-bit integers under one fp32 scale for each token or channel, for every tensor (round to nearest
+    even); the gated MLP's pre-activations are kept for the backward in blocks of 8-bit codes."""
+
+    granularity: str = "row"
+    checkpoint_block: int = 32
+
+
 def _make_recipe(name):
     if name == 'fp8':
         return Float8CurrentScaling()
@@ -103,6 +115,8 @@ def _make_recipe(name):
         return NVFP4BlockScaling()
     if name == 'mxfp4':
         return MXFP4BlockScaling()
+    if name == 'int8':
+        return Int8Scaling()
     raise ValueError(f'TE recipe must be one of {RECIPES}')
 
 
@@ -116,6 +130,10 @@ def _is_nvfp4(recipe):
 
 def _is_mxfp4(recipe):
     return isinstance(recipe, MXFP4BlockScaling)
+
+
+def _is_int8(recipe):
+    return isinstance(recipe, Int8Scaling)
 
 
 def _is_blocked(recipe):
@@ -224,6 +242,8 @@ class TELinear(_ScalingExtraState, torch.nn.Module):
                                                   cache_dequant=is_first_microbatch is not None)
             elif _is_mxfp4(self.recipe):
                 q = _linear.quantize_weight_mxfp4(self.weight, transpose=True)
+            elif _is_int8(self.recipe):
+                q = _linear.quantize_weight_int8(self.weight, transpose=True)
             else:
                 q = _linear.quantize_weight(self.weight,
                                             scaler=self.scaling and self.scaling.weight)
@@ -281,6 +301,9 @@ class TELinear(_ScalingExtraState, torch.nn.Module):
         elif _is_mxfp4(self.recipe):
             out = _linear.Mxfp4LinearFunction.apply(flat, self.weight,
                                                     self.fp8_weight(first_microbatch))
+        elif _is_int8(self.recipe):
+            out = _linear.Int8LinearFunction.apply(flat, self.weight, None,
+                                                   self.fp8_weight(first_microbatch))
         else:
             out = _linear.Fp8LinearFunction.apply(flat, self.weight, None,
                                                   self.fp8_weight(first_microbatch), self.scaling)
@@ -351,7 +374,7 @@ class TEMLP(torch.nn.Module):
                                          first or self.gate_up._fp8_weight is None,
                                          down_first or self.down._fp8_weight is None)
         down_q = self.down.fp8_weight(down_first)
-        if _is_mx(self.down.recipe) or _is_mxfp4(self.down.recipe):
+        if _is_mx(self.down.recipe) or _is_mxfp4(self.down.recipe) or _is_int8(self.down.recipe):
             return self._mx_forward(x, flat, length, aligned, down_q)
         if self.fused_gate_up:
             first = self.gate_up._note_microbatch()
@@ -405,15 +428,20 @@ class TEMLP(torch.nn.Module):
         return out.reshape(*x.shape[:-1], out.shape[-1])
 
     def _mx_forward(self, x, flat, length, aligned, down_q):
-        """MXFP8 and MXFP4: blocks along K never straddle gate and up rows, so the stacked
-        weight's copy is the two projections' copies side by side (fused or split alike)."""
+        """MXFP8, MXFP4 and int8: scales along K never straddle gate and up rows, so the stacked weight's
+        rowwise copy is the two projections' copies side by side (fused or split alike)."""
         I = self.intermediate_size
-        mxfp4 = _is_mxfp4(self.down.recipe)
+        recipe = self.down.recipe
+        if _is_int8(recipe):
+            quantize, mlp = _linear.quantize_weight_int8, _linear.Int8GegluMlpFunction
+        elif _is_mxfp4(recipe):
+            quantize, mlp = _linear.quantize_weight_mxfp4, _linear.Mxfp4GegluMlpFunction
+        else:
+            quantize, mlp = _linear.quantize_weight_mx, _linear.Fp8GegluMlpMxFunction
         if self.fused_gate_up:
             first = self.gate_up._note_microbatch()
             if first or self.gate_up._fp8_weight is None:
-                self.gate_up._fp8_weight = (_linear.quantize_weight_mxfp4 if mxfp4 else
-                                            _linear.quantize_weight_mx)(self.gate_up.weight)
+                self.gate_up._fp8_weight = quantize(self.gate_up.weight)
             gu_q = self.gate_up._fp8_weight
             w_gu = self.gate_up.weight
         else:
@@ -421,11 +449,10 @@ class TEMLP(torch.nn.Module):
             first_u = self.up_proj._note_microbatch()
             if first_g or first_u or self._split_cache is None:
                 stacked = torch.cat([self.gate_proj.weight, self.up_proj.weight], 0)
-                self._split_cache = (_linear.quantize_weight_mxfp4(stacked) if mxfp4 else
-                                     _linear.quantize_weight_mx(stacked, scale_rows=False))
+                self._split_cache = (quantize(stacked, scale_rows=False) if _is_mx(recipe)
+                                     else quantize(stacked))
             gu_q = self._split_cache
             w_gu = _SplitGateUp.apply(self.gate_proj.weight, self.up_proj.weight)
-        mlp = _linear.Mxfp4GegluMlpFunction if mxfp4 else _linear.Fp8GegluMlpMxFunction
         out = mlp.apply(flat, w_gu, self.down.weight, gu_q, down_q, I)
         if aligned != length:
             out = out[:length]

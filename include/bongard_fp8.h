@@ -616,6 +616,92 @@ int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* do
                                   void* dpre, void* dgate, void* ws, size_t ws_bytes,
                                   void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * 8-bit integers with one scale for each row (token, output channel) of either operand, the
+ * 'int8' recipe of bongard_amd (beside the reference's recipes, bongard/te_linear.py:17; no
+ * counterpart there). Per row: a = max(max |x|, 2^-40), scale = fp32(a / 127), code = 127 x / a
+ * rounded to nearest, ties to even; x ~ code * scale. A row that holds inf or NaN: scale NaN,
+ * codes 0 (its products are NaN).
+ * out: [rows, cols] with row_scale [rows]; out_t: the columns' copy [cols, R], R = rows rounded up
+ * to 16 (zeros past the rows), with col_scale [cols]; each optional (at least one). cols % 8 == 0 and
+ * <= 32768. out_t needs ws: bf8_quantize_int8_workspace(rows, cols) bytes, 256-byte aligned. x
+ * and out_t 16-byte, out 8-byte aligned.
+ * ------------------------------------------------------------------------------- */
+size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols);
+int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* out, float* row_scale,
+                           int8_t* out_t, float* col_scale, void* ws, size_t ws_bytes,
+                           void* stream);
+
+/* out bf16 [rows, cols] = codes * scale[row] (rounded once). cols % 8 == 0; out 16-byte, codes
+ * 8-byte aligned. */
+int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int64_t cols, void* out,
+                     void* stream);
+
+/* C[m, n] = a_scale[m] * b_scale[n] * sum_k A[m, k] B[n, k] (+ bias[n]), the sum exact in int32: A
+ * [M, K] and B [N, K] row-major, K and row strides multiples of 16, K <= 133120, N % 8 == 0; bias
+ * bf16 [N] or NULL; C bf16 or fp32. Operands and scales 16-byte aligned. ws:
+ * bf8_gemm_int8_workspace(M, N, K) bytes, 256-byte aligned (less, or none, runs a plan that needs
+ * less). */
+size_t bf8_gemm_int8_workspace(int64_t M, int64_t N, int64_t K);
+int bf8_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8_t* B, int64_t ldb,
+                  const float* b_scale, int64_t M, int64_t N, int64_t K, const void* bias, void* C,
+                  int out_dtype, int64_t ldc, void* ws, size_t ws_bytes, void* stream);
+
+/* The gate/up product of int8 operands X [M, K] and W [2 I, K] (gate rows then up rows) with the
+ * gated GELU (TEMLP's chain, bongard/te_linear.py:98-103): H bf16 [M, I], and where GU8 is given
+ * the checkpoint of the bf16 pre-activations [M, 2 I] as bf8_quantize_mxint8_bf16 writes it.
+ * I % 128 == 0, K as bf8_gemm_int8. */
+int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W,
+                        int64_t ldw, const float* w_scale, int64_t M, int64_t I, int64_t K, void* H,
+                        int8_t* GU8, uint8_t* GU8_exp, void* stream);
+
+/* out bf16 [cols] = the sum over rows of x [rows, cols], in fp32 and a fixed order (the gradient of
+ * a bias). cols % 8 == 0, x 16-byte aligned; ws: bf8_column_sums_workspace(rows, cols) bytes, 16-byte
+ * aligned. rows > 0. */
+size_t bf8_column_sums_workspace(int64_t rows, int64_t cols);
+int bf8_column_sums_bf16(const void* x, int64_t rows, int64_t cols, void* out, void* ws,
+                         size_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * 8-bit activation checkpoints (OCP MXINT8: blocks of 32 along a row under a power of two): codes
+ * [rows, cols], exponent bytes [rows, ceil(cols / 32)], x ~ code * 2^(E - 133). E is the least with
+ * max |x| <= 127 * 2^(E - 133), 7 at least; codes -127 .. 127 to nearest, ties to even (the largest
+ * finite values are held as 127). A block that holds inf or NaN: E = 255, it reads back as NaN. A
+ * read-back is exact in bf16. cols % 8 == 0; bf16 tensors 16-byte, codes 8-byte aligned.
+ * ------------------------------------------------------------------------------- */
+int bf8_quantize_mxint8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* codes,
+                             uint8_t* exponents, void* stream);
+int bf8_dequant_mxint8(const int8_t* codes, const uint8_t* exponents, int64_t rows, int64_t cols,
+                       void* out, void* stream);
+
+/* bf8_geglu_bf16 (H from GU [M, 2 I]; no amax partials) that writes GU's checkpoint in the same
+ * pass, and bf8_geglu_bwd (dGU; no amax partials) on the values of the checkpoint. I % 32 == 0. */
+int bf8_geglu_mxint8(const void* GU, int64_t M, int64_t I, void* H, int8_t* GU8, uint8_t* GU8_exp,
+                     void* stream);
+int bf8_geglu_bwd_mxint8(const void* dH, const int8_t* GU8, const uint8_t* GU8_exp, int64_t M,
+                         int64_t I, void* dGU, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Layer norm of rows (beside the RMSNorm of bongard/fused_mlp.py:25-30; torch's layer_norm), in fp32:
+ *   y = bf16((x - mean) * rstd * weight + bias),  rstd = 1 / sqrt(mean((x - mean)^2) + eps)
+ * x, y bf16 [rows, cols], weight bf16 [cols], bias bf16 [cols] or NULL; mean, rstd fp32 [rows] or
+ * NULL (both); x8, x8_exp: x's checkpoint as bf8_quantize_mxint8_bf16 writes it, or NULL (both).
+ * cols % 8 == 0 and <= 16384; bf16 tensors 16-byte, x8 8-byte aligned.
+ * ------------------------------------------------------------------------------- */
+int bf8_layernorm_bf16(const void* x, int64_t rows, int64_t cols, const void* weight, const void* bias,
+                       float eps, void* y, float* mean, float* rstd, int8_t* x8, uint8_t* x8_exp,
+                       void* stream);
+
+/* Its backward of dy from the forward's mean and rstd and either x or x's checkpoint (the other
+ * NULL): dx [rows, cols], dweight, dbias bf16 [cols], each optional (at least one); the last two need
+ * ws: bf8_layernorm_bwd_workspace(rows, cols) bytes of block partials, 16-byte aligned, added in a
+ * fixed order. rows > 0. */
+size_t bf8_layernorm_bwd_workspace(int64_t rows, int64_t cols);
+int bf8_layernorm_bwd_bf16(const void* x, const int8_t* x8, const uint8_t* x8_exp, const void* dy,
+                           int64_t rows, int64_t cols, const void* weight, const float* mean,
+                           const float* rstd, void* dx, void* dweight, void* dbias, void* ws,
+                           size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,239 @@
+"""CPU tests of the int8 and layer-norm oracle (against values worked out by hand) and of the refusals of
+the int8, checkpoint and layer-norm entries, before any launch."""
+
+import ctypes
+from fractions import Fraction
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from bongard_amd import _lib, fused_mlp, linear, ops, te_linear
+from oracle import int8_oracle as i8
+
+
+def test_codes_and_scales_of_hand_worked_rows():
+    x = torch.tensor([[127.0, 63.5, 0.5, 1.5, -2.5, -127.0, 0.25, 64.0],   # steps of 1: ties to even
+                      [254.0, 1.0, 3.0, 5.0, -7.0, 127.0, 0.0, 2.0],       # steps of 2
+                      [1.0, 0.5, -0.5, 0.0, -1.0, 0.25, 0.0078125, 0.00390625],
+                      [0.0] * 8]).to(torch.bfloat16)
+    codes, scale = i8.quantize(x)
+    assert codes[0].tolist() == [127, 64, 0, 2, -2, -127, 0, 64]
+    assert codes[1].tolist() == [127, 0, 2, 2, -4, 64, 0, 1]
+    # 127 x: 63.5 is a tie, to 64; 31.75; 0.9921875; 0.49609375
+    assert codes[2].tolist() == [127, 64, -64, 0, -127, 32, 1, 0]
+    assert codes[3].tolist() == [0] * 8
+    assert scale.tolist()[:2] == [1.0, 2.0]
+    assert scale[2].item() == torch.tensor(1 / 127, dtype=torch.float64).float().item()
+    assert scale[3].item() == torch.tensor(2.0 ** -40 / 127, dtype=torch.float64).float().item()
+    x[0, 3] = float("inf")
+    x[2, 0] = float("nan")
+    codes, scale = i8.quantize(x)
+    assert torch.isnan(scale).tolist() == [True, False, True, False]
+    assert not codes[0].any() and not codes[2].any()
+
+
+def test_codes_are_the_nearest_of_the_exact_quotient():
+    """Against rational arithmetic, rows of every seventh mantissa of their largest value."""
+    g = torch.Generator().manual_seed(0)
+    for m in range(128, 256, 7):
+        x = torch.randint(-m, m + 1, (1, 24), generator=g).float() * 2.0 ** torch.randint(-9, 1, (1, 24), generator=g)
+        x[0, 0], x[0, 1] = m, m / 2
+        x = x.to(torch.bfloat16)
+        codes, _ = i8.quantize(x)
+        for c, v in zip(codes[0].tolist(), x[0].tolist()):
+            q = Fraction(v) * 127 / Fraction(x.double().abs().max().item())
+            assert c == round(q), (m, v)  # Python's round: ties to even
+
+
+def test_columns_are_the_rows_of_the_transpose():
+    x = torch.randn(21, 24).to(torch.bfloat16)
+    codes, scale = i8.quantize(x, 0)
+    want, ws = i8.quantize(x.t().contiguous())
+    assert codes.shape == (24, 32) and torch.equal(codes[:, :21], want) and not codes[:, 21:].any()
+    assert torch.equal(scale, ws)
+
+
+@pytest.mark.parametrize("amax,e", [(127.0, 133), (127.5, 134), (64.0, 133), (63.5, 132), (1.0, 127),
+                                    (1.984375, 127), (1.9921875, 128), (2.0 ** -126, 7), (2.0 ** -133, 7),
+                                    (0.0, 7), (3.3895e38, 254), (float("inf"), 255), (float("nan"), 255)])
+def test_checkpoint_exponents(amax, e):
+    x = torch.zeros(1, 40)
+    x[0, 3], x[0, 5] = amax, -amax / 2 if amax == amax else 0.0
+    codes, exps = i8.checkpoint(x.to(torch.bfloat16))
+    assert exps.tolist() == [[e, 7]]
+    if amax == 3.3895e38:
+        assert codes[0, 3] == 127  # 127.5 steps of the last power of two
+    elif 7 < e < 255:
+        assert codes.abs().max() >= 64 and i8.restored(codes, exps)[0, 3] == pytest.approx(amax, rel=1 / 128)
+
+
+def test_checkpoint_codes_are_the_nearest_and_bf16_holds_the_values():
+    x = torch.randn(9, 72).to(torch.bfloat16)
+    codes, e = i8.checkpoint(x)
+    v = i8.restored(codes, e)
+    step = torch.ldexp(torch.ones(()), e.int() - 133).double().repeat_interleave(32, 1)[:, :72]
+    assert bool(((v - x.double()).abs() <= step / 2).all())
+    assert torch.equal(v.to(torch.bfloat16).double(), v)
+    x = torch.zeros(1, 32)
+    x[0, :5] = torch.tensor([64.0, 0.5, 1.5, -2.5, 63.5])
+    assert i8.checkpoint(x.to(torch.bfloat16))[0][0, :5].tolist() == [64, 0, 2, -2, 64]
+
+
+def test_layer_norm_of_hand_worked_rows():
+    x = torch.tensor([[1.0, 3.0, 1.0, 3.0], [5.0, 5.0, 5.0, 5.0], [0.0, 0.0, 0.0, 8.0]])
+    w, b = torch.tensor([1.0, 2.0, 3.0, 4.0]), torch.tensor([0.0, 1.0, 0.0, -1.0])
+    y, n, mean, sd = i8.layer_norm(x, w, b, 0.0)
+    assert mean.flatten().tolist() == [2, 5, 2] and sd[0].item() == 1 and sd[2].item() == 12 ** 0.5
+    assert y[0].tolist() == [-1, 3, -3, 3]
+    y, _, _, sd = i8.layer_norm(x, w, b, 9.0)
+    assert sd[1].item() == 3 and y[1].tolist() == b.tolist()
+    # the gradients are autograd's of the formula
+    x = torch.randn(5, 8, dtype=torch.float64, requires_grad=True)
+    w, b, dy = (torch.randn(s, dtype=torch.float64) for s in ((8,), (8,), (5, 8)))
+    w.requires_grad_(), b.requires_grad_()
+    want = torch.autograd.grad(torch.nn.functional.layer_norm(x, (8,), w, b, 1e-5), [x, w, b], dy)
+    _, n, _, sd = i8.layer_norm(x.detach(), w.detach(), b.detach(), 1e-5)
+    for a, v in zip(i8.layer_norm_backward(n, sd, dy, w.detach()), want):
+        assert torch.allclose(a, v, rtol=1e-12, atol=1e-13)
+
+
+def test_recipe_is_offered():
+    assert "int8" in te_linear.RECIPES
+    t = te_linear.TELinear([torch.nn.Linear(64, 32, bias=False)], "int8")
+    assert t.get_extra_state().numel() == 0 and t.recipe.checkpoint_block == 32
+    with pytest.raises(ValueError, match="multiples of 16"):
+        linear._check_int8("layer", 64, 40)
+
+
+def _calls(L):
+    null = ctypes.c_void_p(0)
+    p, odd = ctypes.c_void_p(4096), ctypes.c_void_p(4100)
+    q, d, g, h = L.bf8_quantize_int8_bf16, L.bf8_dequant_int8, L.bf8_gemm_int8, L.bf8_gemm_geglu_int8
+    m, dm, cs = L.bf8_quantize_mxint8_bf16, L.bf8_dequant_mxint8, L.bf8_column_sums_bf16
+    f, b = L.bf8_geglu_mxint8, L.bf8_geglu_bwd_mxint8
+    n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
+    return [
+        (q, (p, 4, 12, p, p, null, null, null, 0, null), "cols % 8"),
+        (q, (p, 4, 32776, p, p, null, null, null, 0, null), "32768"),
+        (q, (p, -1, 16, p, p, null, null, null, 0, null), "bad shape"),
+        (q, (p, 4, 16, null, null, null, null, null, 0, null), "give out"),
+        (q, (p, 4, 16, p, null, null, null, null, 0, null), "give out"),
+        (q, (p, 4, 16, null, null, p, null, p, 1 << 20, null), "give out"),
+        (q, (null, 4, 16, p, p, null, null, null, 0, null), "x is NULL"),
+        (q, (odd, 4, 16, p, p, null, null, null, 0, null), "16-byte"),
+        (q, (p, 4, 16, odd, p, null, null, null, 0, null), "8-byte"),
+        (q, (p, 4, 16, null, null, p, p, null, 0, null), "workspace needs"),
+        (q, (p, 4, 16, null, null, p, p, p, 8, null), "workspace needs"),
+        (d, (p, p, 4, 12, p, null), "cols % 8"),
+        (d, (p, null, 4, 16, p, null), "NULL"),
+        (d, (p, p, 4, 16, odd, null), "16-byte"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 24, null, p, 0, 8, null, 0, null), "K % 16"),
+        (g, (p, 133136, p, p, 133136, p, 4, 8, 133136, null, p, 0, 8, null, 0, null), "133120"),
+        (g, (p, 32, p, p, 32, p, 4, 9, 32, null, p, 0, 12, null, 0, null), "N % 8"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 32, null, p, 0, 4, null, 0, null), "ldc"),
+        (g, (p, 16, p, p, 32, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "row stride"),
+        (g, (p, 40, p, p, 32, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "row stride"),
+        (g, (p, 32, odd, p, 32, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "16-byte"),
+        (g, (p, 32, p, p, 32, null, 4, 8, 32, null, p, 0, 8, null, 0, null), "B or its scales"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 32, null, p, 2, 8, null, 0, null), "out_dtype"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 32, odd, p, 0, 8, null, 0, null), "bias"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 32, null, null, 0, 8, null, 0, null), "C is NULL"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 32, null, p, 0, 8, odd, 64, null), "workspace"),
+        (g, (p, 32, p, p, 32, p, 4, 8, 0, null, p, 0, 8, null, 0, null), "K == 0"),
+        (g, (p, 1 << 20, p, p, 32, p, 1 << 11, 8, 32, null, p, 0, 8, null, 0, null), "2 GiB"),
+        (h, (p, 32, p, p, 32, p, 4, 96, 32, p, null, null, null), "multiple of 128"),
+        (h, (p, 32, p, p, 32, p, 4, 128, 40, p, null, null, null), "K % 16"),
+        (h, (p, 32, p, p, 32, p, 4, 128, 0, p, null, null, null), "K == 0"),
+        (h, (p, 32, p, p, 32, p, 4, 128, 32, null, null, null, null), "H is NULL"),
+        (h, (p, 32, p, p, 32, p, 4, 128, 32, p, p, null, null), "exponents"),
+        (h, (p, 32, p, p, 32, p, 4, 128, 32, p, odd, p, null), "8-byte"),
+        (h, (p, 32, null, p, 32, p, 4, 128, 32, p, null, null, null), "X or its scales"),
+        (m, (p, 4, 12, p, p, null), "cols % 8"),
+        (m, (p, 4, 16, p, null, null), "NULL"),
+        (m, (odd, 4, 16, p, p, null), "16-byte"),
+        (dm, (odd, p, 4, 16, p, null), "8-byte"),
+        (dm, (p, p, 4, 16, null, null), "NULL"),
+        (f, (p, 4, 40, p, p, p, null), "I % 32"),
+        (f, (p, 4, 64, p, p, null, null), "NULL"),
+        (f, (odd, 4, 64, p, p, p, null), "16-byte"),
+        (b, (p, p, p, 4, 24, p, null), "I % 32"),
+        (b, (p, null, p, 4, 32, p, null), "NULL"),
+        (b, (p, odd, p, 4, 32, p, null), "8-byte"),
+        (cs, (p, 0, 16, p, p, 1 << 20, null), "rows > 0"),
+        (cs, (p, 4, 12, p, p, 1 << 20, null), "cols % 8"),
+        (cs, (p, 4, 16, null, p, 1 << 20, null), "must be given"),
+        (cs, (p, 4, 16, p, p, 8, null), "workspace of 8 bytes"),
+        (n, (p, 4, 12, p, null, 1e-6, p, null, null, null, null, null), "cols % 8"),
+        (n, (p, 4, 16392, p, null, 1e-6, p, null, null, null, null, null), "16384"),
+        (n, (p, 4, 16, null, null, 1e-6, p, null, null, null, null, null), "NULL"),
+        (n, (p, 4, 16, p, odd, 1e-6, p, null, null, null, null, null), "16-byte"),
+        (n, (p, 4, 16, p, p, 1e-6, p, p, null, null, null, null), "mean and rstd"),
+        (n, (p, 4, 16, p, p, 1e-6, p, p, p, p, null, null), "go together"),
+        (nb, (p, null, null, p, 0, 16, p, p, p, p, null, null, null, 0, null), "no rows"),
+        (nb, (p, p, p, p, 4, 16, p, p, p, p, null, null, null, 0, null), "give x or"),
+        (nb, (null, null, null, p, 4, 16, p, p, p, p, null, null, null, 0, null), "give x or"),
+        (nb, (p, null, null, p, 4, 16, p, p, null, p, null, null, null, 0, null), "NULL"),
+        (nb, (p, null, null, p, 4, 16, p, p, p, null, null, null, null, 0, null), "nothing"),
+        (nb, (p, null, null, p, 4, 16, p, p, p, p, p, null, p, 8, null), "workspace of 8 bytes"),
+        (nb, (p, null, null, odd, 4, 16, p, p, p, p, null, null, null, 0, null), "16-byte"),
+    ]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are no memory: the host checks alone")
+def test_entries_refuse_before_any_launch():
+    L = _lib.lib()
+    for fn, args, message in _calls(L):
+        assert fn(*args) == 1, (fn.__name__, args)
+        told = L.bf8_last_error().decode()
+        assert told.startswith(fn.__name__ + ":") and message in told, (message, told)
+
+
+def test_sizes_of_nothing():
+    """Empty calls return without a launch or a pointer; the workspaces of nothing are empty."""
+    L = _lib.lib()
+    null, p = ctypes.c_void_p(0), ctypes.c_void_p(4096)
+    assert L.bf8_quantize_int8_bf16(null, 0, 64, p, p, null, null, null, 0, null) == 0
+    assert L.bf8_dequant_int8(null, null, 0, 64, null, null) == 0
+    assert L.bf8_gemm_int8(null, 64, null, null, 64, null, 0, 8, 64, null, null, 0, 8, null, 0, null) == 0
+    assert L.bf8_gemm_geglu_int8(null, 64, null, null, 64, null, 0, 128, 64, null, null, null, null) == 0
+    assert L.bf8_quantize_mxint8_bf16(null, 0, 64, null, null, null) == 0
+    assert L.bf8_dequant_mxint8(null, null, 3, 0, null, null) == 0
+    assert L.bf8_geglu_mxint8(null, 0, 32, null, null, null, null) == 0
+    assert L.bf8_geglu_bwd_mxint8(null, null, null, 0, 32, null, null) == 0
+    assert L.bf8_layernorm_bf16(null, 0, 64, null, null, 1e-6, null, null, null, null, null, null) == 0
+    for ws in (L.bf8_quantize_int8_workspace, L.bf8_column_sums_workspace, L.bf8_layernorm_bwd_workspace):
+        assert ws(0, 64) == 0 and ws(3, 64) >= 64 * 4
+    assert L.bf8_gemm_int8_workspace(0, 8, 64) == 0
+
+
+@pytest.mark.parametrize("tile", ["256x160", "160x256", "128x128", "192x256", "128x64", "64x128", "256x256w8",
+                                  "256x256w8x", "192x128o2", "128x128o2", "128x64k2", "64x128k2", "128x64:3",
+                                  "256x256w8:2"])
+def test_a_named_tile_is_the_plan(monkeypatch, capfd, tile):
+    """Every tile of the int8 product can be named, in as many pieces; 256x128, 256x256 and 128x128k2 have
+    no such variant (a plan of the planner's own is printed)."""
+    L = _lib.lib()
+    M, N, K = 517, 1040, 8224
+    monkeypatch.setenv("BONGARD_FP8_GEMM_DEBUG", "1")
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    pieces = int(tile.partition(":")[2] or 1)
+    assert L.bf8_gemm_int8_workspace(M, N, K) == (4 * pieces * M * N if pieces > 1 else 0)
+    assert "bf8 plan" not in capfd.readouterr().err
+    for none in ("256x128", "256x256", "128x128k2"):
+        monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", none)
+        L.bf8_gemm_int8_workspace(M, N, K)
+        assert "bf8 plan gemm" in capfd.readouterr().err
+
+
+def test_layer_norm_refuses_forward_mode_tangents(monkeypatch):
+    """No tangent is dropped, whether gradients are recorded or not."""
+    monkeypatch.setattr(ops, "layernorm", lambda x, *a, **k: (torch.zeros_like(x), None, None, None))
+    args = dict(x=torch.ones(4, 16), weight=torch.ones(16), bias=torch.ones(16))
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), forward_ad.dual_level():
+            assert fused_mlp.layer_norm(**args).shape == (4, 16)
+            for name in args:
+                dual = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
+                with pytest.raises(NotImplementedError, match="jvp"):
+                    fused_mlp.layer_norm(**{**args, name: dual})
