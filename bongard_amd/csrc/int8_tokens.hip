@@ -1,0 +1,242 @@
+// A linear layer of int8 weights on a few tokens (decoding), for gfx950: each token's quantization and the
+// product as one kernel where the tokens' codes fit the LDS, else the quantizer and the GEMM.
+//
+//   s_t = max(max |x_t|, 2^-40) / 127, q_t the codes of x_t (int8.hpp)
+//   y[t, n] = s_t w_scale[n] sum_k q_t[k] W[n, k] + bias[n],  the sum exact in int32
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "gemm_kernel.hpp"
+#include "int8.hpp"
+
+namespace bf8 {
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+constexpr int kWaves = 8, kNT = 64 * kWaves;
+constexpr int kStep = 64;        // K bytes of an MFMA
+constexpr int kAhead = 8;        // steps of weights a wave has in flight
+constexpr int kMaxTokens = 32;
+constexpr int64_t kMaxCodes = 57344;  // LDS bytes of the tokens' codes (two workgroups a CU)
+constexpr int64_t kMaxBlocks = 2 * kNumCus;
+
+struct Tokens {
+  const uint16_t* x;  // [M, K]
+  const int8_t* W;
+  int64_t ldw;
+  const float* w_scale;
+  int M, N, K, steps;
+  int split;   // waves that share a group of 16 output channels, each a range of K
+  int groups;
+  const uint16_t* bias;
+  void* C;
+  int64_t ldc;
+};
+
+// Bound by the weights' bytes; for few of them by latency. A wave takes 16 output channels (rows of W) and a
+// range of K: its lanes load W in the MFMA's operand layout straight from memory (lane l: row l mod 16,
+// bytes 16 (l / 16) .. +15 of each 64), kAhead steps in flight, the first of them before the tokens are
+// quantized. The codes lie in LDS as [step][quarter of 64 bytes][token][16 bytes], so that the 64 lanes of
+// an operand read 1 KB side by side (lanes of absent tokens read the last one's, and are not stored).
+// Bytes past K of a row are whatever follows it: the codes there are zeros.
+template <int TG, bool F32>
+__global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
+  extern __shared__ uint8_t codes[];
+  __shared__ float scales[kMaxTokens];
+  __shared__ uint32_t top[kWaves];
+  __shared__ v4i parts[kWaves][TG][64];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per_block = kWaves / p.split, sub = wid & (p.split - 1), slot = wid / p.split;
+  const int s0 = p.steps * sub / p.split, s1 = p.steps * (sub + 1) / p.split;
+
+  auto load = [&](int group, int step, v4i (&w)[kAhead]) __attribute__((always_inline)) {
+    const int r0 = group * 16;
+    const int rows = min(16, p.N - r0);  // (a group past the last: no bytes)
+    const Window win = window(p.W + (int64_t)r0 * p.ldw,
+                              rows > 0 ? (uint32_t)((rows - 1) * p.ldw + p.K) : 0u);
+    const uint32_t o = (uint32_t)((lane & 15) * p.ldw) + 16 * (lane >> 4);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      w[i] = __builtin_bit_cast(v4i, window_load(win, step + i < s1 ? o + kStep * (step + i) : kPastEnd));
+  };
+  v4i w[kAhead];
+  int base = blockIdx.x * per_block;
+  load(base + slot, s0, w);
+
+  // the tokens' codes: `share` waves a token, the row's 16-byte vectors spread over their lanes
+  const int share = p.M >= 5 ? 1 : p.M >= 3 ? 2 : p.M == 2 ? 4 : 8;
+  const int nvec = p.K >> 3;
+  for (int t0 = 0; t0 < p.M; t0 += kWaves / share) {
+    const int t = t0 + wid / share;
+    const bool in = t < p.M;
+    const uint4* xr = reinterpret_cast<const uint4*>(p.x + (int64_t)(in ? t : 0) * p.K);
+    const int first = 64 * (wid & (share - 1)) + lane;
+    uint32_t m = 0;
+    constexpr int kHold = 5;
+    uint4 held[kHold];
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      const int v = first + 64 * share * j;
+      held[j] = in && v < nvec ? xr[v] : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) m = max(m, absmax16(held[j]));
+    for (int v = first + 64 * share * kHold; in && v < nvec; v += 64 * share) m = max(m, absmax16(xr[v]));
+    m = wave_max_u32(m);
+    if (share > 1) {
+      if (lane == 0) top[wid] = m;
+      __syncthreads();
+      for (int i = 0; i < share; ++i) m = max(m, top[wid / share * share + i]);
+      __syncthreads();
+    }
+    if (!in) continue;
+    const Int8Scale s = int8_scale(m << 16);
+    if (first == 0) scales[t] = s.scale;
+    auto put = [&](int v, uint4 x) __attribute__((always_inline)) {
+      *reinterpret_cast<uint2*>(codes + ((v >> 1) * p.M + t) * 16 + 8 * (v & 1)) = int8_codes8(x, s.mult);
+    };
+#pragma unroll
+    for (int j = 0; j < kHold; ++j) {
+      const int v = first + 64 * share * j;
+      if (v < nvec) put(v, held[j]);
+    }
+    for (int v = first + 64 * share * kHold; v < nvec; v += 64 * share) put(v, xr[v]);
+  }
+  // the last step's chunks past K
+  for (int i = threadIdx.x; i < (p.steps * 4 - p.K / 16) * p.M; i += kNT)
+    reinterpret_cast<uint4*>(codes)[p.K / 16 * p.M + i] = make_uint4(0u, 0u, 0u, 0u);
+  __syncthreads();
+
+  const int tok = lane & 15;
+  uint32_t at[TG];
+#pragma unroll
+  for (int g = 0; g < TG; ++g) at[g] = 16 * ((lane >> 4) * p.M + min(16 * g + tok, p.M - 1));
+  const uint32_t per_step = 64 * p.M;
+  for (; base < p.groups; base += gridDim.x * per_block) {
+    v4i acc[TG];
+#pragma unroll
+    for (int g = 0; g < TG; ++g) acc[g] = v4i{0, 0, 0, 0};
+    for (int step = s0; step < s1; step += kAhead) {
+      v4i next[kAhead];
+      if (step + kAhead < s1)
+        load(base + slot, step + kAhead, next);
+      else
+        load(base + gridDim.x * per_block + slot, s0, next);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int st = min(step + i, p.steps - 1);  // (steps past the range: weights of zeros)
+#pragma unroll
+        for (int g = 0; g < TG; ++g) {
+          const v4i b = *reinterpret_cast<const v4i*>(codes + st * per_step + at[g]);
+          acc[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], b, acc[g], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) w[i] = next[i];
+    }
+    if (p.split > 1) {
+      __syncthreads();  // the group before has been read
+#pragma unroll
+      for (int g = 0; g < TG; ++g) parts[wid][g][lane] = acc[g];
+      __syncthreads();
+      if (sub != 0) continue;
+      for (int i = 1; i < p.split; ++i)
+#pragma unroll
+        for (int g = 0; g < TG; ++g) acc[g] += parts[wid + i][g][lane];
+    }
+    // acc[g][r]: token 16 g + lane mod 16, channel 4 (lane / 16) + r of the group
+    const int n = (base + slot) * 16 + 4 * (lane >> 4);
+    if (n >= p.N) continue;
+    const float4 ws = *reinterpret_cast<const float4*>(p.w_scale + n);
+    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias) {
+      const uint2 v = *reinterpret_cast<const uint2*>(p.bias + n);
+      b[0] = bf16_lo(v.x); b[1] = bf16_hi(v.x); b[2] = bf16_lo(v.y); b[3] = bf16_hi(v.y);
+    }
+#pragma unroll
+    for (int g = 0; g < TG; ++g) {
+      const int t = 16 * g + tok;
+      if (t >= p.M) continue;
+      const float s = scales[t];
+      const float y0 = __builtin_fmaf((float)acc[g][0], s * ws.x, b[0]);
+      const float y1 = __builtin_fmaf((float)acc[g][1], s * ws.y, b[1]);
+      const float y2 = __builtin_fmaf((float)acc[g][2], s * ws.z, b[2]);
+      const float y3 = __builtin_fmaf((float)acc[g][3], s * ws.w, b[3]);
+      if constexpr (F32)
+        *reinterpret_cast<float4*>((float*)p.C + t * p.ldc + n) = make_float4(y0, y1, y2, y3);
+      else
+        *reinterpret_cast<uint2*>((uint16_t*)p.C + t * p.ldc + n) =
+            make_uint2(pack_bf16x2(y0, y1), pack_bf16x2(y2, y3));
+    }
+  }
+}
+
+int64_t token_steps(int64_t K) { return (K + kStep - 1) / kStep; }
+bool one_kernel(int64_t M, int64_t K) {
+  return M <= kMaxTokens && M * token_steps(K) * kStep <= kMaxCodes;
+}
+size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+
+}  // namespace
+}  // namespace bf8
+
+using namespace bf8;
+
+extern "C" {
+
+size_t bf8_linear_int8_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || one_kernel(M, K)) return 0;
+  return align256((size_t)M * K) + align256((size_t)M * 4) + bf8_gemm_int8_workspace(M, N, K);
+}
+
+int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_scale, int64_t M,
+                    int64_t N, int64_t K, const void* bias, void* C, int out_dtype, int64_t ldc,
+                    void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "bf8_linear_int8";
+  BF8_CHECK(out_dtype == BF8_OUT_BF16 || out_dtype == BF8_OUT_F32, "%s: bad out_dtype", who);
+  BF8_CHECK(M >= 0 && N >= 0 && K >= 0, "%s: negative shape", who);
+  BF8_CHECK(K % 16 == 0 && K <= 32768, "%s: need K %% 16 == 0 and K <= 32768 (got %lld)", who,
+            (long long)K);
+  BF8_CHECK(N % 8 == 0 && ldc >= N && ldc % 4 == 0, "%s: need N %% 8 == 0, ldc >= N, ldc %% 4 == 0",
+            who);
+  BF8_CHECK((((uintptr_t)x | (uintptr_t)W | (uintptr_t)w_scale | (uintptr_t)C) & 15) == 0 &&
+                ((uintptr_t)bias & 7) == 0,
+            "%s: x, W, w_scale and C must be 16-byte, bias 8-byte aligned", who);
+  BF8_CHECK(ldw % 16 == 0 && ldw >= K && N * ldw < (1LL << 31) && M * K < (1LL << 31),
+            "%s: need a row stride >= K in multiples of 16, operands below 2 GiB", who);
+  if (M == 0 || N == 0) return BF8_OK;
+  BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
+  BF8_CHECK(x && W && w_scale && C, "%s: NULL pointer", who);
+  if (!one_kernel(M, K)) {
+    const size_t head = align256((size_t)M * K) + align256((size_t)M * 4);
+    BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= head,
+              "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who,
+              bf8_linear_int8_workspace(M, N, K), ws_bytes);
+    int8_t* q = (int8_t*)ws;
+    float* s = (float*)(q + align256((size_t)M * K));
+    const int rc = bf8_quantize_int8_bf16(x, M, K, q, s, nullptr, nullptr, nullptr, 0, stream);
+    if (rc != BF8_OK) return rc;
+    return bf8_gemm_int8(q, K, s, W, ldw, w_scale, M, N, K, bias, C, out_dtype, ldc,
+                         ws_bytes > head ? q + head : nullptr, ws_bytes - head, stream);
+  }
+  Tokens p{};
+  p.x = (const uint16_t*)x; p.W = W; p.ldw = ldw; p.w_scale = w_scale;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.steps = (int)token_steps(K);
+  p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
+  p.groups = (int)((N + 15) / 16);
+  p.split = 1;
+  while (p.split < kWaves && p.groups * p.split < 8 * kNumCus && p.split < p.steps) p.split *= 2;
+  const int64_t per_block = kWaves / p.split;
+  const dim3 grid((unsigned)std::min<int64_t>((p.groups + per_block - 1) / per_block, kMaxBlocks));
+  const size_t lds = (size_t)p.M * p.steps * kStep;
+  const bool f32 = out_dtype == BF8_OUT_F32;
+  const auto kernel = M <= 16 ? (f32 ? int8_tokens_kernel<1, true> : int8_tokens_kernel<1, false>)
+                              : (f32 ? int8_tokens_kernel<2, true> : int8_tokens_kernel<2, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kNT), lds, as_stream(stream), p);
+  return launch_status("int8_tokens_kernel");
+}
+
+}  // extern "C"

@@ -1679,10 +1679,32 @@ def linear_int8(x, w, w_scale, *, bias=None, out_dtype=torch.bfloat16):
     """A linear layer of int8 weights in serving: ``y = x @ W.T (+ bias)`` with bf16 x [..., K]
     quantized by token in the call and W as codes [N, K] under ``w_scale`` [N]. No gradients
     (:class:`bongard_amd.linear.Int8LinearFunction` has them)."""
+    who = "linear_int8"
+    idx = _index_of(who, x, w, w_scale, bias)
+    _int8_matrix(who, w=w)
     shape = x.shape
-    q = quantize_int8(x)
-    y = gemm_int8(q.data, q.row_scale, w, w_scale, bias=bias, out_dtype=out_dtype)
-    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[-1])
+    N, K = w.shape
+    if shape[-1] != K:
+        raise ValueError(f"{who}: inner dims differ ({shape[-1]} vs {K})")
+    if out_dtype is not torch.bfloat16 and out_dtype is not torch.float32:
+        raise TypeError(f"{who}: out_dtype must be bfloat16 or float32")
+    w_scale = _int8_scale(who, "w_scale", w_scale, N)
+    if bias is not None:
+        bias = _linear_bias(who, bias, N)
+    x = _rows_bf16(x)
+    M = x.shape[0]
+    out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+    if K == 0:  # an empty sum
+        out = out.zero_() if bias is None else out.copy_(bias.reshape(1, N).expand(M, N))
+    elif M:
+        L, ws = _lib.lib(), None
+        ws_bytes = L.bf8_linear_int8_workspace(M, N, K)
+        if ws_bytes:
+            ws, ws_bytes = _call_workspace(ws_bytes, x)
+        _call("bf8_linear_int8", idx, L.bf8_linear_int8, x.data_ptr(), w.data_ptr(),
+              w.stride(0) if N > 1 else K, w_scale.data_ptr(), M, N, K, _ptr(bias), out.data_ptr(),
+              OUT_BF16 if out_dtype is torch.bfloat16 else OUT_F32, N, _ptr(ws), ws_bytes)
+    return out if len(shape) == 2 else out.view(*shape[:-1], N)
 
 
 @dataclass

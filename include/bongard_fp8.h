@@ -647,6 +647,14 @@ int bf8_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8
                   const float* b_scale, int64_t M, int64_t N, int64_t K, const void* bias, void* C,
                   int out_dtype, int64_t ldc, void* ws, size_t ws_bytes, void* stream);
 
+/* A linear layer of int8 weights W [N, K] on bf16 x [M, K] (contiguous): x quantized by row as
+ * bf8_quantize_int8_bf16 does, then bf8_gemm_int8 (the same product; few rows take one kernel). K a
+ * multiple of 16, 32768 at most. ws: bf8_linear_int8_workspace(M, N, K) bytes, 256-byte aligned. */
+size_t bf8_linear_int8_workspace(int64_t M, int64_t N, int64_t K);
+int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_scale, int64_t M,
+                    int64_t N, int64_t K, const void* bias, void* C, int out_dtype, int64_t ldc,
+                    void* ws, size_t ws_bytes, void* stream);
+
 /* The gate/up product of int8 operands X [M, K] and W [2 I, K] (gate rows then up rows) with the
  * gated GELU (TEMLP's chain, bongard/te_linear.py:98-103): H bf16 [M, I], and where GU8 is given
  * the checkpoint of the bf16 pre-activations [M, 2 I] as bf8_quantize_mxint8_bf16 writes it.

@@ -112,6 +112,7 @@ def _calls(L):
     q, d, g, h = L.bf8_quantize_int8_bf16, L.bf8_dequant_int8, L.bf8_gemm_int8, L.bf8_gemm_geglu_int8
     m, dm, cs = L.bf8_quantize_mxint8_bf16, L.bf8_dequant_mxint8, L.bf8_column_sums_bf16
     f, b = L.bf8_geglu_mxint8, L.bf8_geglu_bwd_mxint8
+    t = L.bf8_linear_int8
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
     return [
         (q, (p, 4, 12, p, p, null, null, null, 0, null), "cols % 8"),
@@ -142,6 +143,16 @@ def _calls(L):
         (g, (p, 32, p, p, 32, p, 4, 8, 32, null, p, 0, 8, odd, 64, null), "workspace"),
         (g, (p, 32, p, p, 32, p, 4, 8, 0, null, p, 0, 8, null, 0, null), "K == 0"),
         (g, (p, 1 << 20, p, p, 32, p, 1 << 11, 8, 32, null, p, 0, 8, null, 0, null), "2 GiB"),
+        (t, (p, p, 32, p, 4, 8, 24, null, p, 0, 8, null, 0, null), "K % 16"),
+        (t, (p, p, 32784, p, 4, 8, 32784, null, p, 0, 8, null, 0, null), "32768"),
+        (t, (p, p, 32, p, 4, 12, 32, null, p, 0, 12, null, 0, null), "N % 8"),
+        (t, (p, p, 16, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "row stride"),
+        (t, (odd, p, 32, p, 4, 8, 32, null, p, 0, 8, null, 0, null), "16-byte"),
+        (t, (p, p, 32, p, 4, 8, 32, odd, p, 0, 8, null, 0, null), "8-byte"),
+        (t, (p, p, 32, null, 4, 8, 32, null, p, 0, 8, null, 0, null), "NULL"),
+        (t, (p, p, 32, p, 4, 8, 32, null, p, 3, 8, null, 0, null), "out_dtype"),
+        (t, (p, p, 32, p, 4, 8, 0, null, p, 0, 8, null, 0, null), "K == 0"),
+        (t, (p, p, 32, p, 400, 8, 32, null, p, 0, 8, null, 0, null), "workspace needs"),
         (h, (p, 32, p, p, 32, p, 4, 96, 32, p, null, null, null), "multiple of 128"),
         (h, (p, 32, p, p, 32, p, 4, 128, 40, p, null, null, null), "K % 16"),
         (h, (p, 32, p, p, 32, p, 4, 128, 0, p, null, null, null), "K == 0"),
