@@ -17,7 +17,7 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 8, kNT = 64 * kWaves;
 constexpr int kStep = 64;        // K bytes of an MFMA
-constexpr int kAhead = 8;        // steps of weights a wave has in flight
+constexpr int kAhead = 5;        // steps of weights a wave has in flight
 constexpr int kMaxTokens = 32;
 constexpr int64_t kMaxCodes = 57344;  // LDS bytes of the tokens' codes (two workgroups a CU)
 constexpr int64_t kMaxBlocks = 2 * kNumCus;
@@ -28,7 +28,7 @@ struct Tokens {
   int64_t ldw;
   const float* w_scale;
   int M, N, K, steps;
-  int split;   // waves that share a group of 16 output channels, each a range of K
+  int split;   // waves that share a group of 16 output channels, each a range of K (a power of two)
   int groups;
   const uint16_t* bias;
   void* C;
@@ -37,7 +37,7 @@ struct Tokens {
 
 // Bound by the weights' bytes; for few of them by latency. A wave takes 16 output channels (rows of W) and a
 // range of K: its lanes load W in the MFMA's operand layout straight from memory (lane l: row l mod 16,
-// bytes 16 (l / 16) .. +15 of each 64), kAhead steps in flight, the first of them before the tokens are
+// bytes 16 (l / 16) .. +15 of each 64), kAhead steps in flight, the first of them while the tokens are
 // quantized. The codes lie in LDS as [step][quarter of 64 bytes][token][16 bytes], so that the 64 lanes of
 // an operand read 1 KB side by side (lanes of absent tokens read the last one's, and are not stored).
 // Bytes past K of a row are whatever follows it: the codes there are zeros.
@@ -62,29 +62,47 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
     for (int i = 0; i < kAhead; ++i)
       w[i] = __builtin_bit_cast(v4i, window_load(win, step + i < s1 ? o + kStep * (step + i) : kPastEnd));
   };
+  // the group's output channels of this lane: 4 (lane / 16) .. +3; their scales and biases come with the
+  // group's first weights
+  const int stride = gridDim.x * per_block;
+  float4 ws = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  uint2 wb = make_uint2(0u, 0u);
+  auto load_channels = [&](int group) __attribute__((always_inline)) {
+    const int n = group * 16 + 4 * (lane >> 4);
+    if (sub != 0 || n >= p.N) return;
+    ws = *reinterpret_cast<const float4*>(p.w_scale + n);
+    if (p.bias) wb = *reinterpret_cast<const uint2*>(p.bias + n);
+  };
+  // the tokens' codes: `share` waves a token, the row's 16-byte vectors spread over their lanes; the next
+  // token's first kHold of a lane are loaded before this one's maximum is known
+  const int share = p.M >= 5 ? 1 : p.M >= 3 ? 2 : p.M == 2 ? 4 : 8;
+  const int nvec = p.K >> 3, first = 64 * (wid & (share - 1)) + lane;
+  constexpr int kHold = 5;
+  auto row = [&](int t) __attribute__((always_inline)) {
+    return window(p.x + (int64_t)t * p.K, t < p.M ? 2u * p.K : 0u);
+  };
+  uint4 next_x[kHold];
+#pragma unroll
+  for (int j = 0; j < kHold; ++j) next_x[j] = window_load(row(wid / share), 16u * (first + 64 * share * j));
   v4i w[kAhead];
   int base = blockIdx.x * per_block;
   load(base + slot, s0, w);
-
-  // the tokens' codes: `share` waves a token, the row's 16-byte vectors spread over their lanes
-  const int share = p.M >= 5 ? 1 : p.M >= 3 ? 2 : p.M == 2 ? 4 : 8;
-  const int nvec = p.K >> 3;
+  load_channels(base + slot);
   for (int t0 = 0; t0 < p.M; t0 += kWaves / share) {
     const int t = t0 + wid / share;
-    const bool in = t < p.M;
-    const uint4* xr = reinterpret_cast<const uint4*>(p.x + (int64_t)(in ? t : 0) * p.K);
-    const int first = 64 * (wid & (share - 1)) + lane;
-    uint32_t m = 0;
-    constexpr int kHold = 5;
+    const Window xr = row(t);
     uint4 held[kHold];
+    uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < kHold; ++j) {
-      const int v = first + 64 * share * j;
-      held[j] = in && v < nvec ? xr[v] : make_uint4(0u, 0u, 0u, 0u);
+      held[j] = next_x[j];
+      if (t0 + kWaves / share < p.M)
+        next_x[j] = window_load(row(t + kWaves / share), 16u * (first + 64 * share * j));
     }
 #pragma unroll
     for (int j = 0; j < kHold; ++j) m = max(m, absmax16(held[j]));
-    for (int v = first + 64 * share * kHold; in && v < nvec; v += 64 * share) m = max(m, absmax16(xr[v]));
+    for (int v = first + 64 * share * kHold; v < nvec; v += 64 * share)
+      m = max(m, absmax16(window_load(xr, 16u * v)));
     m = wave_max_u32(m);
     if (share > 1) {
       if (lane == 0) top[wid] = m;
@@ -92,7 +110,7 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
       for (int i = 0; i < share; ++i) m = max(m, top[wid / share * share + i]);
       __syncthreads();
     }
-    if (!in) continue;
+    if (t >= p.M) continue;
     const Int8Scale s = int8_scale(m << 16);
     if (first == 0) scales[t] = s.scale;
     auto put = [&](int v, uint4 x) __attribute__((always_inline)) {
@@ -103,7 +121,7 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
       const int v = first + 64 * share * j;
       if (v < nvec) put(v, held[j]);
     }
-    for (int v = first + 64 * share * kHold; v < nvec; v += 64 * share) put(v, xr[v]);
+    for (int v = first + 64 * share * kHold; v < nvec; v += 64 * share) put(v, window_load(xr, 16u * v));
   }
   // the last step's chunks past K
   for (int i = threadIdx.x; i < (p.steps * 4 - p.K / 16) * p.M; i += kNT)
@@ -115,7 +133,7 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
 #pragma unroll
   for (int g = 0; g < TG; ++g) at[g] = 16 * ((lane >> 4) * p.M + min(16 * g + tok, p.M - 1));
   const uint32_t per_step = 64 * p.M;
-  for (; base < p.groups; base += gridDim.x * per_block) {
+  for (; base < p.groups; base += stride) {
     v4i acc[TG];
 #pragma unroll
     for (int g = 0; g < TG; ++g) acc[g] = v4i{0, 0, 0, 0};
@@ -124,7 +142,7 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
       if (step + kAhead < s1)
         load(base + slot, step + kAhead, next);
       else
-        load(base + gridDim.x * per_block + slot, s0, next);
+        load(base + stride + slot, s0, next);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
         const int st = min(step + i, p.steps - 1);  // (steps past the range: weights of zeros)
@@ -137,6 +155,9 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) w[i] = next[i];
     }
+    const float4 f = ws;
+    const uint2 bb = wb;
+    load_channels(base + stride + slot);
     if (p.split > 1) {
       __syncthreads();  // the group before has been read
 #pragma unroll
@@ -150,21 +171,16 @@ __global__ __launch_bounds__(kNT) void int8_tokens_kernel(Tokens p) {
     // acc[g][r]: token 16 g + lane mod 16, channel 4 (lane / 16) + r of the group
     const int n = (base + slot) * 16 + 4 * (lane >> 4);
     if (n >= p.N) continue;
-    const float4 ws = *reinterpret_cast<const float4*>(p.w_scale + n);
-    float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (p.bias) {
-      const uint2 v = *reinterpret_cast<const uint2*>(p.bias + n);
-      b[0] = bf16_lo(v.x); b[1] = bf16_hi(v.x); b[2] = bf16_lo(v.y); b[3] = bf16_hi(v.y);
-    }
+    const float b[4] = {bf16_lo(bb.x), bf16_hi(bb.x), bf16_lo(bb.y), bf16_hi(bb.y)};
 #pragma unroll
     for (int g = 0; g < TG; ++g) {
       const int t = 16 * g + tok;
       if (t >= p.M) continue;
       const float s = scales[t];
-      const float y0 = __builtin_fmaf((float)acc[g][0], s * ws.x, b[0]);
-      const float y1 = __builtin_fmaf((float)acc[g][1], s * ws.y, b[1]);
-      const float y2 = __builtin_fmaf((float)acc[g][2], s * ws.z, b[2]);
-      const float y3 = __builtin_fmaf((float)acc[g][3], s * ws.w, b[3]);
+      const float y0 = __builtin_fmaf((float)acc[g][0], s * f.x, b[0]);
+      const float y1 = __builtin_fmaf((float)acc[g][1], s * f.y, b[1]);
+      const float y2 = __builtin_fmaf((float)acc[g][2], s * f.z, b[2]);
+      const float y3 = __builtin_fmaf((float)acc[g][3], s * f.w, b[3]);
       if constexpr (F32)
         *reinterpret_cast<float4*>((float*)p.C + t * p.ldc + n) = make_float4(y0, y1, y2, y3);
       else
@@ -228,7 +244,7 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
   p.bias = (const uint16_t*)bias; p.C = C; p.ldc = ldc;
   p.groups = (int)((N + 15) / 16);
   p.split = 1;
-  while (p.split < kWaves && p.groups * p.split < 8 * kNumCus && p.split < p.steps) p.split *= 2;
+  while (p.split < kWaves && 2 * p.split <= p.steps) p.split *= 2;
   const int64_t per_block = kWaves / p.split;
   const dim3 grid((unsigned)std::min<int64_t>((p.groups + per_block - 1) / per_block, kMaxBlocks));
   const size_t lds = (size_t)p.M * p.steps * kStep;
