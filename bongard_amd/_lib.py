@@ -149,7 +149,7 @@ SIGNATURES = {
     "bf8_rmsnorm_bwd_workspace": (c_size_t, [c_int64, c_int64]),
     "bf8_rmsnorm_bwd_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_float,
                                      c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "bf8_quantize_int8_workspace": (c_size_t, [c_int64, c_int64]),
+    "bf8_quantize_int8_workspace": (c_size_t, [c_int64, c_int64, c_int]),
     "bf8_quantize_int8_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_size_t, c_void_p]),
     "bf8_dequant_int8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),

@@ -6,10 +6,13 @@
 // to even (int8.hpp); x ~ code * scale. The columnwise copy is stored transposed, [cols, R] with R the
 // rows rounded up to 16 and zeros past the rows, so that any number of rows is an operand.
 //
-// Kernels (x is read at most twice):
-//   int8_row_kernel        one pass: each row's maximum, scale and codes; per-block column maxima
-//   int8_col_scale_kernel  the blocks' column maxima -> scale and multiplier of each column
-//   int8_col_kernel        second pass: the columns' codes, turned in LDS
+// Kernels (x is read once for rows alone, else twice):
+//   int8_row_kernel     rows alone: each row's maximum, scale and codes in one pass
+//   int8_maxima_kernel  else one pass for the maxima: of each row in tiles of 512 columns, of each column in
+//                       strips of rows (the gated-GELU backward writes its output's itself, mlp.hip)
+//   int8_tile_kernel    and one for the codes: a tile's scales from those maxima, either copy or both
+//   int8_pair_kernel    both copies of few rows in one launch: some blocks take rows, the others all rows of
+//                       32 columns
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -19,15 +22,13 @@
 namespace bf8 {
 namespace {
 
-constexpr int kNT = 512;                 // threads of the row kernel (8 waves)
-constexpr int64_t kMaxCols = 32768;      // widest row that the row kernel holds in registers
-constexpr int64_t kBlocksColumns = 512;  // row-kernel blocks where it writes column maxima
-constexpr int64_t kBlocksRows = 2048;    // ... where it does not
-constexpr int kScaleNT = 1024;
-constexpr int kColNT = 256;
-constexpr int kTile = 128;               // column kernel's tile (rows x cols)
-constexpr int kPitch = kTile / 4 + 1;    // dwords per staged row (odd)
-constexpr int64_t kMaxColBlocks = 2048;
+constexpr int kNT = 512;               // threads of the row kernel (8 waves)
+constexpr int64_t kMaxCols = 32768;    // widest row that the row kernel holds in registers
+constexpr int64_t kRowBlocks = 2048;   // its most blocks
+constexpr int kTileNT = 256;
+constexpr int kTile = 128;             // the tile kernel's tile (rows x cols)
+constexpr int kPitch = kTile / 4 + 1;  // dwords per staged row (odd)
+constexpr int64_t kTileBlocks = 1024;
 
 // Max of m over the TPR threads of a row; every thread of the block must call it (TPR > 64: through LDS).
 template <int TPR>
@@ -52,20 +53,15 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 // Rows [blockIdx.x * strip, + strip) of x, one row per TPR threads at a time (strip is a multiple of the
 // kNT / TPR rows taken at once, so every group runs the same number of steps). Thread tl of a group holds
 // the row's 16-byte vectors tl, tl + TPR, ... (V of them); the next row's are loaded before this
-// row's maximum is known. out / row_scale, colpart ([gridDim.x][cols] bf16 keys): each may be NULL.
+// row's maximum is known.
 template <int TPR, int V>
 __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restrict__ x, int64_t rows,
                                                        int cols, int64_t strip,
                                                        int8_t* __restrict__ out,
-                                                       float* __restrict__ row_scale,
-                                                       uint16_t* __restrict__ colpart) {
+                                                       float* __restrict__ row_scale) {
   constexpr int G = kNT / TPR;
-  extern __shared__ uint4 cbuf[];  // [G - 1][cols / 8] column keys of groups 1.. (colpart)
   const int g = threadIdx.x / TPR, tl = threadIdx.x % TPR;
   const int nvec = cols >> 3;
-  uint4 ck[V];
-#pragma unroll
-  for (int j = 0; j < V; ++j) ck[j] = make_uint4(0u, 0u, 0u, 0u);
   const int64_t r0 = blockIdx.x * strip;
   constexpr bool kAhead = V < 8;  // (eight vectors of two rows leave too few waves)
   uint4 next[V];
@@ -87,15 +83,7 @@ __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restric
     if (kAhead && rr + G < strip) load(r + G);
     uint32_t m = 0;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      m = max(m, absmax16(xv[j]));
-      if (colpart)
-        ck[j] = make_uint4(pk_max_u16(ck[j].x, xv[j].x & 0x7FFF7FFFu),
-                           pk_max_u16(ck[j].y, xv[j].y & 0x7FFF7FFFu),
-                           pk_max_u16(ck[j].z, xv[j].z & 0x7FFF7FFFu),
-                           pk_max_u16(ck[j].w, xv[j].w & 0x7FFF7FFFu));
-    }
-    if (!out) continue;
+    for (int j = 0; j < V; ++j) m = max(m, absmax16(xv[j]));
     m = group_max<TPR>(m);
     if (r >= rows) continue;
     const Int8Scale s = int8_scale(m << 16);
@@ -107,112 +95,102 @@ __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restric
       if (v < nvec) orow[v] = int8_codes8(xv[j], s.mult);
     }
   }
-  if (!colpart) return;
-  uint4* dst = reinterpret_cast<uint4*>(colpart + (int64_t)blockIdx.x * cols);
-  if constexpr (G == 1) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int v = tl + TPR * j;
-      if (v < nvec) dst[v] = ck[j];
-    }
-  } else {
-    // groups 1.. hand their keys to group 0, whose threads hold the same columns
-    if (g > 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int v = tl + TPR * j;
-        if (v < nvec) cbuf[(g - 1) * nvec + v] = ck[j];
-      }
-    }
-    __syncthreads();
-    if (g == 0) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int v = tl + TPR * j;
-        if (v >= nvec) continue;
-        uint4 k = ck[j];
-#pragma unroll
-        for (int gg = 1; gg < G; ++gg) {
-          const uint4 o = cbuf[(gg - 1) * nvec + v];
-          k = make_uint4(pk_max_u16(k.x, o.x), pk_max_u16(k.y, o.y), pk_max_u16(k.z, o.z),
-                         pk_max_u16(k.w, o.w));
-        }
-        dst[v] = k;
-      }
-    }
-  }
 }
 
-// Scale and multiplier of each column from the row kernel's maxima [nblk][cols]: a block takes 64 columns
-// (8 threads of 8) and spreads the nblk rows over 128 thread rows.
-__global__ __launch_bounds__(kScaleNT) void int8_col_scale_kernel(
-    const uint16_t* __restrict__ colpart, int nblk, int cols, float* __restrict__ col_mult,
-    float* __restrict__ col_scale) {
-  constexpr int kTR = kScaleNT / 8, kW = kScaleNT / 64;
-  __shared__ uint4 red[kW][8];
-  const int cg = threadIdx.x & 7, rg = threadIdx.x >> 3;
-  const int nvec = cols >> 3;
-  const int v = blockIdx.x * 8 + cg;
-  uint32_t k[4] = {0u, 0u, 0u, 0u};
-  if (v < nvec) {
-    const uint4* src = reinterpret_cast<const uint4*>(colpart);
-#pragma unroll 4
-    for (int b = rg; b < nblk; b += kTR) {
-      const uint4 o = src[(int64_t)b * nvec + v];
-      k[0] = pk_max_u16(k[0], o.x);
-      k[1] = pk_max_u16(k[1], o.y);
-      k[2] = pk_max_u16(k[2], o.z);
-      k[3] = pk_max_u16(k[3], o.w);
-    }
-  }
-#pragma unroll
-  for (int off = 8; off < 64; off <<= 1) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) k[i] = pk_max_u16(k[i], (uint32_t)__shfl_xor((int)k[i], off, 64));
-  }
-  if ((threadIdx.x & 63) < 8) red[threadIdx.x >> 6][cg] = make_uint4(k[0], k[1], k[2], k[3]);
-  __syncthreads();
-  const int c = blockIdx.x * 64 + threadIdx.x;
-  if (threadIdx.x >= 64 || c >= cols) return;
-  uint32_t m = 0;
-#pragma unroll
-  for (int w = 0; w < kW; ++w)
-    m = max(m, (uint32_t)reinterpret_cast<const uint16_t*>(red[w])[threadIdx.x]);
-  const Int8Scale s = int8_scale(m << 16);
-  col_mult[c] = s.mult;
-  col_scale[c] = s.scale;
-}
-
-// out_t [cols, ld] = the columns' codes. A block takes 128 x 128 tiles, each wave 32 rows of all 128
-// columns: lane l holds columns 8 (l & 15) .. +7 of the rows 4 k + l / 16, k < 8; the codes meet in LDS and
-// each wave turns 32 columns of all 128 rows, so that every store instruction writes whole 128-byte
-// lines. Rows past the tensor's are zeros.
-__global__ __launch_bounds__(kColNT) void int8_col_kernel(const uint16_t* __restrict__ x,
-                                                          int64_t rows, int64_t cols, int64_t ld,
-                                                          const float* __restrict__ col_mult,
-                                                          int8_t* __restrict__ out_t) {
-  __shared__ uint32_t stage[kTile * kPitch];
+// The maxima of strips of `strip` rows (a multiple of 32) by 512 columns, a block each: lane l of a wave holds
+// columns 8 l .. +7 of the tile, the waves take eight rows at a time by turns.
+__global__ __launch_bounds__(kTileNT) void int8_maxima_kernel(const uint16_t* __restrict__ x,
+                                                              Int8Maxima p, int strip) {
+  __shared__ uint4 red[kTileNT / 64][64];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int tiles_c = (int)int8_col_tiles(p.cols);
+  const int tc = blockIdx.x % tiles_c;
+  const int64_t ts = blockIdx.x / tiles_c;
+  const int64_t r0 = ts * strip, c = 512 * tc + 8 * lane;
+  const int64_t left = min((int64_t)strip, p.rows - r0);
+  uint4 k = make_uint4(0u, 0u, 0u, 0u);
+  for (int r = 8 * wid; r < left; r += 8 * (kTileNT / 64)) {
+    const Window w = window(x + (r0 + r) * p.cols, (uint32_t)(min((int64_t)8, left - r) * p.cols * 2));
+    uint4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = window_load(w, c < p.cols ? 2u * (uint32_t)(i * p.cols + c) : kPastEnd);
+    int8_strip_maxima(p, v, k, r0 + r, tc, lane);
+  }
+  int8_column_maxima<kTileNT / 64>(p, red, k, ts, c, wid, lane);
+}
+
+// The codes of 128 x 128 tiles. The tile's row and column maxima first: 16 threads hold 128 of either, 16 groups
+// of them take the tiles (strips) by turns. Each wave casts 32 rows of all 128 columns: lane l holds columns
+// 8 (l & 15) .. +7 of the rows 4 k + l / 16, k < 8; the columnwise codes meet in LDS and each wave turns 32
+// columns of all 128 rows, so that every store instruction writes whole 128-byte lines. Rows past the
+// tensor's are zeros in out_t [cols, ld].
+template <bool ROWS, bool COLS>
+__global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* __restrict__ x, Int8Maxima p,
+                                                            int strips, int64_t ld,
+                                                            int8_t* __restrict__ out,
+                                                            float* __restrict__ row_scale,
+                                                            int8_t* __restrict__ out_t,
+                                                            float* __restrict__ col_scale) {
+  __shared__ uint32_t stage[kTile * kPitch];
+  __shared__ float mults[2][kTile];
+  uint4(*red)[2][16] = reinterpret_cast<uint4(*)[2][16]>(stage);  // [group][rows, columns][8 each]
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  const int64_t rows = p.rows, cols = p.cols;
+  const int tiles_k = (int)int8_col_tiles(cols);
   const int64_t tiles_c = (cols + kTile - 1) / kTile;
   const int64_t ntiles = tiles_c * ((rows + kTile - 1) / kTile);
   const int cl = lane & 15, lr = lane >> 4;
   for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x) {
     const int64_t r0 = (t / tiles_c) * kTile, c0 = (t % tiles_c) * kTile;
     const int64_t c = c0 + 8 * cl;
+    const int left = (int)min((int64_t)kTile, rows - r0);
+    const Window w = window(x + r0 * cols, (uint32_t)(left * cols * 2));
     uint4 v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int64_t r = r0 + 32 * wid + 4 * k + lr;
-      v[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < rows && c < cols) v[k] = *reinterpret_cast<const uint4*>(x + r * cols + c);
+    for (int k = 0; k < 8; ++k)
+      v[k] = window_load(w, c < cols ? 2u * (uint32_t)((32 * wid + 4 * k + lr) * cols + c) : kPastEnd);
+    {
+      const int g = threadIdx.x >> 4, e = 8 * (threadIdx.x & 15);
+      auto more = [](uint4 a, uint4 b) __attribute__((always_inline)) {
+        return make_uint4(pk_max_u16(a.x, b.x), pk_max_u16(a.y, b.y), pk_max_u16(a.z, b.z),
+                          pk_max_u16(a.w, b.w));
+      };
+      uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+      if (ROWS && e < left)
+#pragma unroll 4
+        for (int i = g; i < tiles_k; i += 16)
+          a = more(a, *reinterpret_cast<const uint4*>(p.rowpart + i * int8_row_pad(rows) + r0 + e));
+      if (COLS && c0 + e < cols)
+#pragma unroll 4
+        for (int i = g; i < strips; i += 16)
+          b = more(b, *reinterpret_cast<const uint4*>(p.colpart + (int64_t)i * cols + c0 + e));
+      if (ROWS) red[g][0][threadIdx.x & 15] = a;
+      if (COLS) red[g][1][threadIdx.x & 15] = b;
+      __syncthreads();
+      const int which = threadIdx.x >> 7, i = threadIdx.x & 127;  // threads 0 .. 127: rows, the others: columns
+      if (which ? COLS : ROWS) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int gg = 0; gg < 16; ++gg) m = max(m, (uint32_t)reinterpret_cast<const uint16_t*>(red[gg][which])[i]);
+        const Int8Scale s = int8_scale(m << 16);
+        mults[which][i] = s.mult;
+        if (!which && c0 == 0 && i < left) row_scale[r0 + i] = s.scale;
+        if (which && r0 == 0 && c0 + i < cols) col_scale[c0 + i] = s.scale;
+      }
+      __syncthreads();
     }
-    float m[8] = {};
-    if (c < cols) {
-      const float4 s0 = reinterpret_cast<const float4*>(col_mult + c)[0];
-      const float4 s1 = reinterpret_cast<const float4*>(col_mult + c)[1];
-      m[0] = s0.x; m[1] = s0.y; m[2] = s0.z; m[3] = s0.w;
-      m[4] = s1.x; m[5] = s1.y; m[6] = s1.z; m[7] = s1.w;
+    if constexpr (ROWS) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int r = 32 * wid + 4 * k + lr;
+        if (r < left && c < cols)
+          *reinterpret_cast<uint2*>(out + (r0 + r) * cols + c) = int8_codes8(v[k], mults[0][r]);
+      }
     }
+    if constexpr (!COLS) continue;
+    float m[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m[e] = mults[1][8 * cl + e];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint2 q = int8_codes8(v[k], m);
@@ -228,7 +206,7 @@ __global__ __launch_bounds__(kColNT) void int8_col_kernel(const uint16_t* __rest
     for (int i = 0; i < 16; ++i) d[i] = stage[(rg + i) * kPitch + cg];
     uint4 tq[4];
     transpose_4x16(d, tq);
-    if (r0 + rg < rows) {  // ld holds whole pieces of 16 rows
+    if (rg < left) {  // ld holds whole pieces of 16 rows
 #pragma unroll
       for (int cc = 0; cc < 4; ++cc) {
         const int64_t tr = c0 + 4 * cg + cc;  // row of out_t (a column of x)
@@ -236,6 +214,104 @@ __global__ __launch_bounds__(kColNT) void int8_col_kernel(const uint16_t* __rest
       }
     }
     __syncthreads();
+  }
+}
+
+// Both copies of up to 128 R rows. Blocks [0, row_blocks) are int8_row_kernel's of eight rows each (TPR 64, V
+// vectors a lane). Of the others each takes 32 columns of all rows: four lanes a row (8 columns each), 128 rows
+// a step, R steps held in registers; the columns' maxima by packed 16-bit maxima over lanes and waves, the
+// codes turned in LDS, 1,024 rows at a time.
+constexpr int kPairCols = 32, kPairPitch = kPairCols / 4 + 1, kPairStage = 8;  // stage: steps of 128 rows
+template <int V, int R>
+__global__ __launch_bounds__(kNT) void int8_pair_kernel(const uint16_t* __restrict__ x, int rows, int cols,
+                                                        int row_blocks, int8_t* __restrict__ out,
+                                                        float* __restrict__ row_scale,
+                                                        int8_t* __restrict__ out_t,
+                                                        float* __restrict__ col_scale) {
+  __shared__ uint32_t stage[(R < kPairStage ? R : kPairStage) * 128 * kPairPitch];
+  __shared__ uint4 top[kNT / 64][4];
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
+  if ((int)blockIdx.x < row_blocks) {
+    const int r = blockIdx.x * 8 + wid, nvec = cols >> 3;
+    if (r >= rows) return;
+    const Window w = window(x + (int64_t)r * cols, 2u * cols);
+    uint4 v[V];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = window_load(w, 16u * (lane + 64 * j));
+#pragma unroll
+    for (int j = 0; j < V; ++j) m = max(m, absmax16(v[j]));
+    const Int8Scale s = int8_scale(wave_max_u32(m) << 16);
+    if (lane == 0) row_scale[r] = s.scale;
+    uint2* orow = reinterpret_cast<uint2*>(out + (int64_t)r * cols);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+      if (lane + 64 * j < nvec) orow[lane + 64 * j] = int8_codes8(v[j], s.mult);
+    return;
+  }
+  const int c0 = (blockIdx.x - row_blocks) * kPairCols, cg = threadIdx.x & 3, rl = threadIdx.x >> 2;
+  const int c = c0 + 8 * cg, ld = (rows + 15) / 16 * 16;
+  const Window w = window(x, (uint32_t)(2 * rows * cols));
+  uint4 v[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    v[i] = window_load(w, c < cols && 128 * i + rl < rows ? 2u * ((128 * i + rl) * cols + c) : kPastEnd);
+  uint4 k = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+    k = make_uint4(pk_max_u16(k.x, v[i].x & 0x7FFF7FFFu), pk_max_u16(k.y, v[i].y & 0x7FFF7FFFu),
+                   pk_max_u16(k.z, v[i].z & 0x7FFF7FFFu), pk_max_u16(k.w, v[i].w & 0x7FFF7FFFu));
+#pragma unroll
+  for (int off = 4; off < 64; off <<= 1)
+    k = make_uint4(pk_max_u16(k.x, (uint32_t)__shfl_xor((int)k.x, off, 64)),
+                   pk_max_u16(k.y, (uint32_t)__shfl_xor((int)k.y, off, 64)),
+                   pk_max_u16(k.z, (uint32_t)__shfl_xor((int)k.z, off, 64)),
+                   pk_max_u16(k.w, (uint32_t)__shfl_xor((int)k.w, off, 64)));
+  if (lane < 4) top[wid][lane] = k;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kNT / 64; ++i) {
+    const uint4 o = top[i][cg];
+    k = make_uint4(pk_max_u16(k.x, o.x), pk_max_u16(k.y, o.y), pk_max_u16(k.z, o.z), pk_max_u16(k.w, o.w));
+  }
+  float mult[8], scale[8];
+  const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const Int8Scale s = int8_scale(e & 1 ? kw[e >> 1] & 0xFFFF0000u : kw[e >> 1] << 16);
+    mult[e] = s.mult;
+    scale[e] = s.scale;
+  }
+  if (rl == 0 && c < cols) {
+    reinterpret_cast<float4*>(col_scale + c)[0] = make_float4(scale[0], scale[1], scale[2], scale[3]);
+    reinterpret_cast<float4*>(col_scale + c)[1] = make_float4(scale[4], scale[5], scale[6], scale[7]);
+  }
+#pragma unroll
+  for (int i0 = 0; i0 < R; i0 += kPairStage) {
+    if (i0) __syncthreads();
+#pragma unroll
+    for (int i = i0; i < R && i < i0 + kPairStage; ++i) {
+      const uint2 q = int8_codes8(v[i], mult);
+      uint32_t* d = stage + (128 * (i - i0) + rl) * kPairPitch + 2 * cg;
+      d[0] = q.x;
+      d[1] = q.y;
+    }
+    __syncthreads();
+    // a thread turns 16 rows of 4 columns: 8 pieces of rows a step of 128, 8 groups of columns
+    constexpr int kSteps = R < kPairStage ? R : kPairStage;
+    for (int it = threadIdx.x; it < kSteps * 64; it += kNT) {
+      const int rg = (it & (8 * kSteps - 1)) * 16, g = it / (8 * kSteps);
+      const int r = 128 * i0 + rg;
+      if (r >= rows || c0 + 4 * g >= cols) continue;
+      uint32_t d[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) d[i] = stage[(rg + i) * kPairPitch + g];
+      uint4 tq[4];
+      transpose_4x16(d, tq);
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc)
+        *reinterpret_cast<uint4*>(out_t + (int64_t)(c0 + 4 * g + cc) * ld + r) = tq[cc];
+    }
   }
 }
 
@@ -330,33 +406,18 @@ __global__ __launch_bounds__(256) void column_finish_kernel(const float* __restr
   out[col] = (uint16_t)f32_to_bf16_bits(s);
 }
 
-struct RowPlan {
-  int tpr, v;
-  int64_t strip, blocks;
-  size_t part_bytes;  // column maxima, 256-byte aligned
-};
-
-RowPlan row_plan(int64_t rows, int64_t cols, bool colwise) {
-  RowPlan p{};
-  p.tpr = cols <= 4096 ? 64 : cols <= 16384 ? 256 : 512;
-  p.v = (int)((cols / 8 + p.tpr - 1) / p.tpr);  // <= 8
-  const int64_t groups = kNT / p.tpr, cap = colwise ? kBlocksColumns : kBlocksRows;
-  p.strip = ((rows + cap - 1) / cap + groups - 1) / groups * groups;
-  p.blocks = (rows + p.strip - 1) / p.strip;
-  p.part_bytes = colwise ? ((size_t)p.blocks * (size_t)cols * 2 + 255) / 256 * 256 : 0;
-  return p;
-}
-
 template <int TPR>
-void launch_rows(const RowPlan& p, const uint16_t* x, int64_t rows, int cols, int8_t* out,
-                 float* row_scale, uint16_t* colpart, hipStream_t s) {
-  const size_t lds = colpart ? (size_t)(kNT / TPR - 1) * cols * 2 : 0;
-#define BF8_INT8_ROW(VV)                                                                        \
-  case VV:                                                                                      \
-    hipLaunchKernelGGL((int8_row_kernel<TPR, VV>), dim3((unsigned)p.blocks), dim3(kNT), lds, s, \
-                       x, rows, cols, p.strip, out, row_scale, colpart);                        \
+void launch_rows(const uint16_t* x, int64_t rows, int cols, int8_t* out, float* row_scale,
+                 hipStream_t s) {
+  const int64_t groups = kNT / TPR;
+  const int64_t strip = ((rows + kRowBlocks - 1) / kRowBlocks + groups - 1) / groups * groups;
+  const dim3 grid((unsigned)((rows + strip - 1) / strip));
+#define BF8_INT8_ROW(VV)                                                                          \
+  case VV:                                                                                        \
+    hipLaunchKernelGGL((int8_row_kernel<TPR, VV>), grid, dim3(kNT), 0, s, x, rows, cols, strip,   \
+                       out, row_scale);                                                           \
     break
-  switch (p.v) {
+  switch ((cols / 8 + TPR - 1) / TPR) {
     BF8_INT8_ROW(1);
     BF8_INT8_ROW(2);
     BF8_INT8_ROW(3);
@@ -369,6 +430,48 @@ void launch_rows(const RowPlan& p, const uint16_t* x, int64_t rows, int cols, in
 #undef BF8_INT8_ROW
 }
 
+// Tensors whose both copies int8_pair_kernel makes.
+bool pair_fits(int64_t rows, int64_t cols) { return rows <= 1024 && cols <= 4096; }
+
+int launch_tiles(const uint16_t* x, const Int8Maxima& p, int8_t* out, float* row_scale, int8_t* out_t,
+                 float* col_scale, hipStream_t s) {
+  const int64_t strip = int8_strip(p.rows, p.cols);
+  const int64_t tiles = ((p.rows + kTile - 1) / kTile) * ((p.cols + kTile - 1) / kTile);
+  const auto kernel = !out_t ? int8_tile_kernel<true, false>
+                      : out  ? int8_tile_kernel<true, true>
+                             : int8_tile_kernel<false, true>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(tiles, kTileBlocks)), dim3(kTileNT), 0, s, x, p,
+                     (int)((p.rows + strip - 1) / strip), (p.rows + 15) / 16 * 16, out, row_scale, out_t,
+                     col_scale);
+  return launch_status("int8_tile_kernel");
+}
+
+int launch_pair(const uint16_t* x, int rows, int cols, int8_t* out, float* row_scale, int8_t* out_t,
+                float* col_scale, hipStream_t s) {
+  const int row_blocks = (rows + 7) / 8, v = (cols / 8 + 63) / 64;
+  const dim3 grid((unsigned)(row_blocks + (cols + kPairCols - 1) / kPairCols));
+  const auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kNT), 0, s, x, rows, cols, row_blocks, out, row_scale, out_t,
+                       col_scale);
+  };
+#define BF8_INT8_PAIR(R)                                             \
+  if (v <= 2)                                                        \
+    run(int8_pair_kernel<2, R>);                                     \
+  else if (v <= 5)                                                   \
+    run(int8_pair_kernel<5, R>);                                     \
+  else                                                               \
+    run(int8_pair_kernel<8, R>)
+  if (rows <= 128) {
+    BF8_INT8_PAIR(1);
+  } else if (rows <= 512) {
+    BF8_INT8_PAIR(4);
+  } else {
+    BF8_INT8_PAIR(8);
+  }
+#undef BF8_INT8_PAIR
+  return launch_status("int8_pair_kernel");
+}
+
 }  // namespace
 }  // namespace bf8
 
@@ -376,9 +479,9 @@ using namespace bf8;
 
 extern "C" {
 
-size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols) {
-  if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
-  return row_plan(rows, cols, true).part_bytes + (size_t)cols * 4;
+size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols, int both) {
+  if (rows <= 0 || cols <= 0 || cols > kMaxCols || (both && pair_fits(rows, cols))) return 0;
+  return int8_maxima_bytes(rows, cols);
 }
 
 int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* out, float* row_scale,
@@ -395,30 +498,30 @@ int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* ou
   BF8_CHECK(x != nullptr, "%s: x is NULL", who);
   BF8_CHECK((((uintptr_t)x | (uintptr_t)out_t) & 15) == 0 && ((uintptr_t)out & 7) == 0,
             "%s: x and out_t must be 16-byte, out 8-byte aligned", who);
-  if (out_t)
-    BF8_CHECK(ws && ws_bytes >= bf8_quantize_int8_workspace(rows, cols) && ((uintptr_t)ws & 255) == 0,
-              "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who,
-              bf8_quantize_int8_workspace(rows, cols), ws_bytes);
-  const auto* xs = (const uint16_t*)x;
+  BF8_CHECK(!out_t || ((uintptr_t)col_scale & 15) == 0, "%s: col_scale must be 16-byte aligned", who);
   hipStream_t s = as_stream(stream);
-  const RowPlan p = row_plan(rows, cols, out_t != nullptr);
-  uint16_t* colpart = out_t ? (uint16_t*)ws : nullptr;
-  if (p.tpr == 64)
-    launch_rows<64>(p, xs, rows, (int)cols, out, row_scale, colpart, s);
-  else if (p.tpr == 256)
-    launch_rows<256>(p, xs, rows, (int)cols, out, row_scale, colpart, s);
-  else
-    launch_rows<512>(p, xs, rows, (int)cols, out, row_scale, colpart, s);
-  int rc = launch_status("int8_row_kernel");
-  if (rc != BF8_OK || !out_t) return rc;
-  float* col_mult = (float*)((uint8_t*)ws + p.part_bytes);
-  hipLaunchKernelGGL(int8_col_scale_kernel, dim3((unsigned)((cols / 8 + 7) / 8)), dim3(kScaleNT), 0, s,
-                     colpart, (int)p.blocks, (int)cols, col_mult, col_scale);
-  if ((rc = launch_status("int8_col_scale_kernel")) != BF8_OK) return rc;
-  const int64_t tiles = ((rows + kTile - 1) / kTile) * ((cols + kTile - 1) / kTile);
-  hipLaunchKernelGGL(int8_col_kernel, dim3((unsigned)std::min(tiles, kMaxColBlocks)), dim3(kColNT), 0, s,
-                     xs, rows, cols, (rows + 15) / 16 * 16, col_mult, out_t);
-  return launch_status("int8_col_kernel");
+  const auto* xs = (const uint16_t*)x;
+  if (out && out_t && pair_fits(rows, cols))
+    return launch_pair(xs, (int)rows, (int)cols, out, row_scale, out_t, col_scale, s);
+  if (out_t)
+    BF8_CHECK(ws && ws_bytes >= bf8_quantize_int8_workspace(rows, cols, 0) && ((uintptr_t)ws & 255) == 0,
+              "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who,
+              bf8_quantize_int8_workspace(rows, cols, 0), ws_bytes);
+  if (!out_t) {
+    if (cols <= 4096)
+      launch_rows<64>(xs, rows, (int)cols, out, row_scale, s);
+    else if (cols <= 16384)
+      launch_rows<256>(xs, rows, (int)cols, out, row_scale, s);
+    else
+      launch_rows<512>(xs, rows, (int)cols, out, row_scale, s);
+    return launch_status("int8_row_kernel");
+  }
+  const Int8Maxima p = int8_maxima(ws, rows, cols);
+  const int64_t strip = int8_strip(rows, cols), strips = (rows + strip - 1) / strip;
+  hipLaunchKernelGGL(int8_maxima_kernel, dim3((unsigned)(strips * int8_col_tiles(cols))), dim3(kTileNT), 0,
+                     s, xs, p, (int)strip);
+  if (const int rc = launch_status("int8_maxima_kernel")) return rc;
+  return launch_tiles(xs, p, out, row_scale, out_t, col_scale, s);
 }
 
 int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int64_t cols, void* out,

@@ -1562,8 +1562,8 @@ class Int8Tensor:
 
 
 @functools.lru_cache(maxsize=4096)
-def _quantize_int8_ws_cached(rows, cols):
-    return int(_lib.lib().bf8_quantize_int8_workspace(rows, cols))
+def _quantize_int8_ws_cached(rows, cols, both):
+    return int(_lib.lib().bf8_quantize_int8_workspace(rows, cols, both))
 
 
 def quantize_int8(x, *, rowwise=True, colwise=False):
@@ -1586,8 +1586,9 @@ def quantize_int8(x, *, rowwise=True, colwise=False):
     if colwise:
         out_t = torch.empty((cols, (rows + 15) // 16 * 16), dtype=torch.int8, device=dev)
         scale_t = torch.empty(cols, dtype=torch.float32, device=dev)
-        if rows and cols:
-            ws, nbytes = _call_workspace(_quantize_int8_ws_cached(rows, cols), x)
+        nbytes = _quantize_int8_ws_cached(rows, cols, 1 if rowwise else 0)
+        if nbytes:
+            ws, nbytes = _call_workspace(nbytes, x)
     if rows and cols:
         _call("bf8_quantize_int8_bf16", idx, _lib.lib().bf8_quantize_int8_bf16, x.data_ptr(), rows, cols,
               _ptr(out), _ptr(scale), _ptr(out_t), _ptr(scale_t), _ptr(ws), nbytes)

@@ -627,7 +627,7 @@ int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* do
  * <= 32768. out_t needs ws: bf8_quantize_int8_workspace(rows, cols) bytes, 256-byte aligned. x
  * and out_t 16-byte, out 8-byte aligned.
  * ------------------------------------------------------------------------------- */
-size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols);
+size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols, int both);
 int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* out, float* row_scale,
                            int8_t* out_t, float* col_scale, void* ws, size_t ws_bytes,
                            void* stream);

@@ -213,7 +213,9 @@ def test_sizes_of_nothing():
     assert L.bf8_geglu_mxint8(null, 0, 32, null, null, null, null) == 0
     assert L.bf8_geglu_bwd_mxint8(null, null, null, 0, 32, null, null) == 0
     assert L.bf8_layernorm_bf16(null, 0, 64, null, null, 1e-6, null, null, null, null, null, null) == 0
-    for ws in (L.bf8_quantize_int8_workspace, L.bf8_column_sums_workspace, L.bf8_layernorm_bwd_workspace):
+    assert L.bf8_quantize_int8_workspace(0, 64, 0) == 0 and L.bf8_quantize_int8_workspace(3, 64, 0) >= 64 * 6
+    assert L.bf8_quantize_int8_workspace(3, 64, 1) == 0 and L.bf8_quantize_int8_workspace(5000, 64, 1) >= 64 * 6
+    for ws in (L.bf8_column_sums_workspace, L.bf8_layernorm_bwd_workspace):
         assert ws(0, 64) == 0 and ws(3, 64) >= 64 * 4
     assert L.bf8_gemm_int8_workspace(0, 8, 64) == 0
 
