@@ -122,10 +122,18 @@ __device__ __forceinline__ void load_gelu_tables(uint16_t* tab_a, uint32_t* tab_
   }
 }
 
+// A packed bf16 pair's halves that are not +-0, as 1 each.
+__device__ __forceinline__ uint32_t nonzero2(uint32_t g2) {
+  const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, g2 & 0x7FFF7FFFu), u16x2{1, 1});
+  return __builtin_bit_cast(uint32_t, m);
+}
+
 // The backward chain for 8 elements (4 packed bf16 pairs of dh, g, u): d_g, d_u as packed bf16
 // pairs (NaNs 0xFFFF) and the running amax key of |d_g|, |d_u|. ta / tf: the LDS copies
 // of the gelu tables; all 16 table reads are issued before any is used, gates outside the
-// tables take a wave-uniform slow path.
+// tables take a wave-uniform slow path. ZEROS: gates are read from codes, where one in a hundred
+// is 0 (and none -0), which then is a value of its own and not the slow path: activation 0, factor 1/2.
+template <bool ZEROS = false>
 __device__ __forceinline__ void geglu_bwd8(const uint32_t (&dhw)[4], const uint32_t (&gw)[4],
                                            const uint32_t (&uw)[4], const uint16_t* ta,
                                            const uint32_t* tf, uint32_t (&dg)[4],
@@ -133,8 +141,14 @@ __device__ __forceinline__ void geglu_bwd8(const uint32_t (&dhw)[4], const uint3
   uint32_t outside = 0, ia[4], jf[4], va[8], vf[8];
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
-    ia[w] = gelu_index2(gw[w], outside);
-    jf[w] = gelu_factor_index2(gw[w], outside);
+    uint32_t out = 0;
+    ia[w] = gelu_index2(gw[w], out);
+    jf[w] = gelu_factor_index2(gw[w], out);
+    if constexpr (ZEROS)
+      outside |= __builtin_bit_cast(uint32_t, __builtin_bit_cast(u16x2, out) *
+                                                  __builtin_bit_cast(u16x2, nonzero2(gw[w])));
+    else
+      outside |= out;
   }
 #pragma unroll
   for (int w = 0; w < 4; ++w) {
@@ -150,6 +164,16 @@ __device__ __forceinline__ void geglu_bwd8(const uint32_t (&dhw)[4], const uint3
       va[2 * w + 1] = gelu_finish(gw[w] >> 16, va[2 * w + 1]);
       vf[2 * w] = gelu_factor_finish(gw[w], vf[2 * w]);
       vf[2 * w + 1] = gelu_factor_finish(gw[w] >> 16, vf[2 * w + 1]);
+    }
+  }
+  if constexpr (ZEROS) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const bool lo = (gw[w] & 0xFFFFu) != 0, hi = (gw[w] >> 16) != 0;
+      va[2 * w] = lo ? va[2 * w] : 0u;
+      va[2 * w + 1] = hi ? va[2 * w + 1] : 0u;
+      vf[2 * w] = lo ? vf[2 * w] : 0x3F000000u;
+      vf[2 * w + 1] = hi ? vf[2 * w + 1] : 0x3F000000u;
     }
   }
 #pragma unroll

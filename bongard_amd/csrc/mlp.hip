@@ -139,7 +139,7 @@ __global__ __launch_bounds__(kNT) void geglu_bwd_mxi8_kernel(const uint16_t* __r
     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
     const uint32_t uw[4] = {u.x, u.y, u.z, u.w};
     uint32_t dg[4], du[4], m = 0;
-    geglu_bwd8(dhw, gw, uw, ta, tf, dg, du, m);
+    geglu_bwd8<true>(dhw, gw, uw, ta, tf, dg, du, m);
     *reinterpret_cast<uint4*>(dGU + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
     *reinterpret_cast<uint4*>(dGU + at + I) = make_uint4(du[0], du[1], du[2], du[3]);
   }
