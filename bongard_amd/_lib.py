@@ -168,8 +168,11 @@ SIGNATURES = {
     "bf8_quantize_mxint8_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "bf8_dequant_mxint8": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "bf8_geglu_mxint8": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "bf8_geglu_bwd_mxint8_maxima": (c_size_t, [c_int64, c_int64]),
     "bf8_geglu_bwd_mxint8": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
-                                     c_void_p]),
+                                     c_void_p, c_size_t, c_void_p]),
+    "bf8_quantize_int8_maxima_bf16": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                              c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "bf8_layernorm_bf16": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_float, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "bf8_layernorm_bwd_workspace": (c_size_t, [c_int64, c_int64]),

@@ -471,6 +471,12 @@ __device__ __forceinline__ Window window(const void* base, uint32_t bytes) {
 __device__ __forceinline__ uint4 window_load(Window w, uint32_t off) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(w, (int)off, 0, 0));
 }
+__device__ __forceinline__ uint2 window_load8(Window w, uint32_t off) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(w, (int)off, 0, 0));
+}
+__device__ __forceinline__ uint32_t window_load1(Window w, uint32_t off) {
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(w, (int)off, 0, 0);
+}
 __device__ __forceinline__ void window_store(Window w, uint32_t off, uint4 v) {
   typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
   __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), w, (int)off, 0, 0);

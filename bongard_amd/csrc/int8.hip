@@ -97,24 +97,26 @@ __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restric
   }
 }
 
-// The maxima of strips of `strip` rows (a multiple of 32) by 512 columns, a block each: lane l of a wave holds
+// The maxima of strips of rows (a multiple of 32) by 512 columns, a block each: lane l of a wave holds
 // columns 8 l .. +7 of the tile, the waves take eight rows at a time by turns.
 __global__ __launch_bounds__(kTileNT) void int8_maxima_kernel(const uint16_t* __restrict__ x,
-                                                              Int8Maxima p, int strip) {
+                                                              Int8Maxima p) {
   __shared__ uint4 red[kTileNT / 64][64];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int tiles_c = (int)int8_col_tiles(p.cols);
-  const int tc = blockIdx.x % tiles_c;
-  const int64_t ts = blockIdx.x / tiles_c;
-  const int64_t r0 = ts * strip, c = 512 * tc + 8 * lane;
-  const int64_t left = min((int64_t)strip, p.rows - r0);
+  const int tc = blockIdx.x % p.row_tiles;
+  const int64_t ts = blockIdx.x / p.row_tiles;
+  const int64_t r0 = ts * p.strip, c = 512 * tc + 8 * lane;
+  const int64_t left = min((int64_t)p.strip, p.rows - r0);
   uint4 k = make_uint4(0u, 0u, 0u, 0u);
   for (int r = 8 * wid; r < left; r += 8 * (kTileNT / 64)) {
     const Window w = window(x + (r0 + r) * p.cols, (uint32_t)(min((int64_t)8, left - r) * p.cols * 2));
     uint4 v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = window_load(w, c < p.cols ? 2u * (uint32_t)(i * p.cols + c) : kPastEnd);
-    int8_strip_maxima(p, v, k, r0 + r, tc, lane);
+    Int8Rows m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m.add(i, v[i], k);
+    m.store(p, r0 + r, tc, lane);
   }
   int8_column_maxima<kTileNT / 64>(p, red, k, ts, c, wid, lane);
 }
@@ -126,7 +128,7 @@ __global__ __launch_bounds__(kTileNT) void int8_maxima_kernel(const uint16_t* __
 // tensor's are zeros in out_t [cols, ld].
 template <bool ROWS, bool COLS>
 __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* __restrict__ x, Int8Maxima p,
-                                                            int strips, int64_t ld,
+                                                            int64_t ld,
                                                             int8_t* __restrict__ out,
                                                             float* __restrict__ row_scale,
                                                             int8_t* __restrict__ out_t,
@@ -136,7 +138,6 @@ __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* _
   uint4(*red)[2][16] = reinterpret_cast<uint4(*)[2][16]>(stage);  // [group][rows, columns][8 each]
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   const int64_t rows = p.rows, cols = p.cols;
-  const int tiles_k = (int)int8_col_tiles(cols);
   const int64_t tiles_c = (cols + kTile - 1) / kTile;
   const int64_t ntiles = tiles_c * ((rows + kTile - 1) / kTile);
   const int cl = lane & 15, lr = lane >> 4;
@@ -158,11 +159,11 @@ __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* _
       uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
       if (ROWS && e < left)
 #pragma unroll 4
-        for (int i = g; i < tiles_k; i += 16)
+        for (int i = g; i < p.row_tiles; i += 16)
           a = more(a, *reinterpret_cast<const uint4*>(p.rowpart + i * int8_row_pad(rows) + r0 + e));
       if (COLS && c0 + e < cols)
 #pragma unroll 4
-        for (int i = g; i < strips; i += 16)
+        for (int i = g; i < p.strips; i += 16)
           b = more(b, *reinterpret_cast<const uint4*>(p.colpart + (int64_t)i * cols + c0 + e));
       if (ROWS) red[g][0][threadIdx.x & 15] = a;
       if (COLS) red[g][1][threadIdx.x & 15] = b;
@@ -435,14 +436,12 @@ bool pair_fits(int64_t rows, int64_t cols) { return rows <= 1024 && cols <= 4096
 
 int launch_tiles(const uint16_t* x, const Int8Maxima& p, int8_t* out, float* row_scale, int8_t* out_t,
                  float* col_scale, hipStream_t s) {
-  const int64_t strip = int8_strip(p.rows, p.cols);
   const int64_t tiles = ((p.rows + kTile - 1) / kTile) * ((p.cols + kTile - 1) / kTile);
   const auto kernel = !out_t ? int8_tile_kernel<true, false>
                       : out  ? int8_tile_kernel<true, true>
                              : int8_tile_kernel<false, true>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(tiles, kTileBlocks)), dim3(kTileNT), 0, s, x, p,
-                     (int)((p.rows + strip - 1) / strip), (p.rows + 15) / 16 * 16, out, row_scale, out_t,
-                     col_scale);
+                     (p.rows + 15) / 16 * 16, out, row_scale, out_t, col_scale);
   return launch_status("int8_tile_kernel");
 }
 
@@ -517,11 +516,30 @@ int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* ou
     return launch_status("int8_row_kernel");
   }
   const Int8Maxima p = int8_maxima(ws, rows, cols);
-  const int64_t strip = int8_strip(rows, cols), strips = (rows + strip - 1) / strip;
-  hipLaunchKernelGGL(int8_maxima_kernel, dim3((unsigned)(strips * int8_col_tiles(cols))), dim3(kTileNT), 0,
-                     s, xs, p, (int)strip);
+  hipLaunchKernelGGL(int8_maxima_kernel, dim3((unsigned)p.strips * p.row_tiles), dim3(kTileNT), 0, s, xs, p);
   if (const int rc = launch_status("int8_maxima_kernel")) return rc;
   return launch_tiles(xs, p, out, row_scale, out_t, col_scale, s);
+}
+
+int bf8_quantize_int8_maxima_bf16(const void* x, int64_t rows, int64_t cols, int halves, int8_t* out,
+                                  float* row_scale, int8_t* out_t, float* col_scale, const void* maxima,
+                                  size_t maxima_bytes, void* stream) {
+  const char* who = "bf8_quantize_int8_maxima_bf16";
+  BF8_CHECK(rows >= 0 && cols >= 0 && rows < (1LL << 31) && cols < (1 << 24), "%s: bad shape", who);
+  BF8_CHECK((halves == 1 || halves == 2) && cols % (8 * halves) == 0,
+            "%s: need cols %% 8 == 0 of each of 1 or 2 parts (got %lld of %d)", who, (long long)cols, halves);
+  BF8_CHECK((out == nullptr) == (row_scale == nullptr) && (out_t == nullptr) == (col_scale == nullptr) &&
+                (out || out_t),
+            "%s: give out with row_scale and / or out_t with col_scale", who);
+  if (rows == 0 || cols == 0) return BF8_OK;
+  BF8_CHECK((((uintptr_t)x | (uintptr_t)out_t | (uintptr_t)col_scale) & 15) == 0 && ((uintptr_t)out & 7) == 0,
+            "%s: x, out_t and col_scale must be 16-byte, out 8-byte aligned", who);
+  BF8_CHECK(x && maxima && ((uintptr_t)maxima & 255) == 0 &&
+                maxima_bytes >= int8_maxima_bytes(rows, cols, halves),
+            "%s: x and %zu bytes of maxima, 256-byte aligned, must be given (got %zu)", who,
+            int8_maxima_bytes(rows, cols, halves), maxima_bytes);
+  return launch_tiles((const uint16_t*)x, int8_maxima(const_cast<void*>(maxima), rows, cols, halves), out,
+                      row_scale, out_t, col_scale, as_stream(stream));
 }
 
 int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int64_t cols, void* out,

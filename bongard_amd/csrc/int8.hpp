@@ -60,42 +60,39 @@ __device__ __forceinline__ float code_f32(uint32_t w, int e) {
 }
 
 // ---- the maxima that a tensor's scales are made from, as its producer or a pass over it leaves them --------
-// (bf16 keys of magnitudes.) rowpart: [tiles of 512 columns][rows padded to 8], colpart: [strips of rows][cols].
+// (bf16 keys of magnitudes.) rowpart: [row_tiles][rows padded to 8], of 512 columns each, colpart: [strips of
+// `strip` rows][cols].
 struct Int8Maxima {
   int64_t rows, cols;
+  int row_tiles, strip, strips;
   uint16_t *rowpart, *colpart;
 };
 
 __host__ __device__ inline int64_t int8_col_tiles(int64_t cols) { return (cols + 511) / 512; }
 __host__ __device__ inline int64_t int8_row_pad(int64_t rows) { return (rows + 7) / 8 * 8; }
-// Rows of a strip: few strips, as every tile of codes reads its columns' maxima of all of them, but blocks for
-// every CU.
-inline int64_t int8_strip(int64_t rows, int64_t cols) {
-  int64_t s = 256;
-  while (s > 32 && (rows + s - 1) / s * int8_col_tiles(cols) < 1024) s /= 2;
-  return s;
+// The layout for [rows, cols], of `halves` parts side by side (2: d_g and d_u) each with row tiles of its own; ws
+// may be NULL (for the sizes). Strips: few, as every tile of codes reads its columns' maxima of all of them,
+// but blocks for every CU.
+inline Int8Maxima int8_maxima(void* ws, int64_t rows, int64_t cols, int halves = 1) {
+  const int64_t tiles = int8_col_tiles(cols / halves);
+  int s = 256;
+  while (s > 32 && (rows + s - 1) / s * tiles < 1024) s /= 2;
+  Int8Maxima p{rows, cols, (int)(halves * tiles), s, (int)((rows + s - 1) / s), (uint16_t*)ws, nullptr};
+  p.colpart = p.rowpart + ((size_t)p.row_tiles * int8_row_pad(rows) + 127) / 128 * 128;
+  return p;
 }
-inline size_t int8_rowpart_bytes(int64_t rows, int64_t cols) {
-  return ((size_t)int8_col_tiles(cols) * int8_row_pad(rows) * 2 + 255) / 256 * 256;
-}
-inline size_t int8_maxima_bytes(int64_t rows, int64_t cols) {
-  const int64_t s = int8_strip(rows, cols);
-  return int8_rowpart_bytes(rows, cols) + (size_t)((rows + s - 1) / s) * cols * 2;
-}
-inline Int8Maxima int8_maxima(void* ws, int64_t rows, int64_t cols) {
-  return {rows, cols, (uint16_t*)ws, (uint16_t*)((uint8_t*)ws + int8_rowpart_bytes(rows, cols))};
+inline size_t int8_maxima_bytes(int64_t rows, int64_t cols, int halves = 1) {
+  const Int8Maxima p = int8_maxima(nullptr, rows, cols, halves);
+  return (size_t)((uint8_t*)p.colpart - (uint8_t*)p.rowpart) + (size_t)p.strips * cols * 2;
 }
 
-// The maxima of a wave's eight rows (r .. r + 7, zeros past the tensor's) by 512 columns (lane l: columns 8 l ..
-// +7 of column tile tc): into colmax and, the rows', to rowpart. Two rows share a dword; three shuffles
-// leave a pair to each lane of a quad, four more its maximum over the quads.
-__device__ __forceinline__ void int8_strip_maxima(const Int8Maxima& p, const uint4 (&v)[8], uint4& colmax,
-                                                  int64_t r, int tc, int lane) {
+// The maxima of a wave's eight rows r .. r + 7 (zeros past the tensor's) by 512 columns (lane l: columns 8 l ..
+// +7 of column tile tc), row by row: into colmax and, the rows', to rowpart. Two rows share a dword; three
+// shuffles leave a pair to each lane of a quad, four more its maximum over the quads.
+struct Int8Rows {
   uint32_t pair[4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4 a = make_uint4(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu, v[i].z & 0x7FFF7FFFu,
-                               v[i].w & 0x7FFF7FFFu);
+  __device__ __forceinline__ void add(int i, uint4 v, uint4& colmax) {
+    const uint4 a = make_uint4(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu, v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu);
     colmax = make_uint4(pk_max_u16(colmax.x, a.x), pk_max_u16(colmax.y, a.y), pk_max_u16(colmax.z, a.z),
                         pk_max_u16(colmax.w, a.w));
     const uint32_t k = pk_max_u16(pk_max_u16(a.x, a.y), pk_max_u16(a.z, a.w));
@@ -105,18 +102,20 @@ __device__ __forceinline__ void int8_strip_maxima(const Int8Maxima& p, const uin
     else
       pair[i >> 1] = m;
   }
-  const bool odd = lane & 1, high = lane & 2;
-  const uint32_t a = pk_max_u16(odd ? pair[1] : pair[0],
-                                (uint32_t)__shfl_xor((int)(odd ? pair[0] : pair[1]), 1, 64));
-  const uint32_t b = pk_max_u16(odd ? pair[3] : pair[2],
-                                (uint32_t)__shfl_xor((int)(odd ? pair[2] : pair[3]), 1, 64));
-  uint32_t m = pk_max_u16(high ? b : a, (uint32_t)__shfl_xor((int)(high ? a : b), 2, 64));
+  __device__ __forceinline__ void store(const Int8Maxima& p, int64_t r, int tc, int lane) {
+    const bool odd = lane & 1, high = lane & 2;
+    const uint32_t a = pk_max_u16(odd ? pair[1] : pair[0],
+                                  (uint32_t)__shfl_xor((int)(odd ? pair[0] : pair[1]), 1, 64));
+    const uint32_t b = pk_max_u16(odd ? pair[3] : pair[2],
+                                  (uint32_t)__shfl_xor((int)(odd ? pair[2] : pair[3]), 1, 64));
+    uint32_t m = pk_max_u16(high ? b : a, (uint32_t)__shfl_xor((int)(high ? a : b), 2, 64));
 #pragma unroll
-  for (int off = 4; off < 64; off <<= 1) m = pk_max_u16(m, (uint32_t)__shfl_xor((int)m, off, 64));
-  // lane 0: rows 0 and 1, lane 1: 2 and 3, ...
-  if (lane < 4 && r + 2 * lane < int8_row_pad(p.rows))
-    *reinterpret_cast<uint32_t*>(p.rowpart + tc * int8_row_pad(p.rows) + r + 2 * lane) = m;
-}
+    for (int off = 4; off < 64; off <<= 1) m = pk_max_u16(m, (uint32_t)__shfl_xor((int)m, off, 64));
+    // lane 0: rows 0 and 1, lane 1: 2 and 3, ...
+    if (lane < 4)
+      *reinterpret_cast<uint32_t*>(p.rowpart + tc * int8_row_pad(p.rows) + r + 2 * lane) = m;
+  }
+};
 
 // The block's column maxima of strip ts (each wave's in k) to colpart.
 template <int W>

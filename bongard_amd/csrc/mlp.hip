@@ -114,7 +114,8 @@ __global__ __launch_bounds__(kNT) void geglu_fwd_mxi8_kernel(const uint16_t* __r
   }
 }
 
-// geglu_bwd_kernel from the checkpoint: the same chain on the bf16 values that it holds.
+// geglu_bwd_kernel from the checkpoint: the same chain on the bf16 values that it holds. Bound by memory: 4.06
+// bytes an element of H read, 4 written; [4096, 10240] 69 us, [3001, 10240] 50.
 __global__ __launch_bounds__(kNT) void geglu_bwd_mxi8_kernel(const uint16_t* __restrict__ dH,
                                                              const int8_t* __restrict__ gu8,
                                                              const uint8_t* __restrict__ gu8_e,
@@ -143,6 +144,74 @@ __global__ __launch_bounds__(kNT) void geglu_bwd_mxi8_kernel(const uint16_t* __r
     *reinterpret_cast<uint4*>(dGU + at) = make_uint4(dg[0], dg[1], dg[2], dg[3]);
     *reinterpret_cast<uint4*>(dGU + at + I) = make_uint4(du[0], du[1], du[2], du[3]);
   }
+}
+
+// The same where dGU's int8 codes come next: a block takes a strip of rows by 512 columns of H, a wave eight rows
+// at a time (two passes of four), so that the maxima of d_g and d_u fall to it on the way and the pass over dGU
+// that would find them (4 bytes an element of H) is saved: [4096, 10240] with both copies of the codes 157 us,
+// by the kernel above and the ordinary quantizer 168. Alone it is the slower one (73 us there, 10.8 against
+// 5.3 at 64 rows): fewer loads in flight a wave, 2 MB of maxima.
+constexpr int kBwdCols = 512, kBwdRows = 4;
+__global__ __launch_bounds__(kNT, 4) void geglu_bwd_mxi8_maxima_kernel(
+    const uint16_t* __restrict__ dH, const int8_t* __restrict__ gu8, const uint8_t* __restrict__ gu8_e, int64_t I,
+    uint16_t* __restrict__ dGU, Int8Maxima p) {
+  __shared__ __attribute__((aligned(16))) uint16_t ta[kGeluABytes / 2];
+  __shared__ __attribute__((aligned(16))) uint32_t tf[kGeluFBytes / 4];
+  load_gelu_tables<kNT>(ta, tf);
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = p.row_tiles / 2, tc = blockIdx.x % tiles;
+  const int64_t ts = blockIdx.x / tiles, r0 = ts * p.strip;
+  const int64_t c = (int64_t)kBwdCols * tc + 8 * lane;
+  const int left = (int)min((int64_t)p.strip, p.rows - r0);
+  const uint32_t ld = (uint32_t)I, cc = (uint32_t)c;
+  // the lane's offsets in a row of dH, of the codes, of their exponents and of dGU (c >= I: past its end)
+  const uint32_t od = c < I ? 2 * cc : kPastEnd, oq = c < I ? cc : kPastEnd, oe = c < I ? cc >> 5 : kPastEnd;
+  uint4 kg = make_uint4(0u, 0u, 0u, 0u), ku = kg;
+  for (int r = 8 * wid; r < left; r += 8 * (kNT / 64)) {
+    const int64_t at = r0 + r;
+    Int8Rows mg, mu;
+#pragma unroll
+    for (int h = 0; h < 8; h += kBwdRows) {
+      uint4 d[kBwdRows];
+      uint2 g[kBwdRows], u[kBwdRows];
+      uint32_t eg[kBwdRows], eu[kBwdRows];
+#pragma unroll
+      for (int i = 0; i < kBwdRows; ++i) {
+        const int64_t row = at + h + i;
+        const uint32_t n = r + h + i < left ? ld : 0u;  // rows past the tensor's read as zeros
+        d[i] = window_load(window(dH + row * I, 2 * n), od);
+        const Window wq = window(gu8 + row * 2 * I, 2 * n), we = window(gu8_e + row * (I / 16), n / 16);
+        g[i] = window_load8(wq, oq);
+        u[i] = window_load8(wq, oq + ld);
+        eg[i] = window_load1(we, oe);
+        eu[i] = window_load1(we, oe + ld / 32);
+      }
+#pragma unroll
+      for (int i = 0; i < kBwdRows; ++i) {
+        const uint4 gv = mxi8_values8(g[i], mxi8_step(eg[i])), uv = mxi8_values8(u[i], mxi8_step(eu[i]));
+        const uint32_t dhw[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+        const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+        const uint32_t uw[4] = {uv.x, uv.y, uv.z, uv.w};
+        uint32_t dg[4], du[4], m = 0;
+        geglu_bwd8<true>(dhw, gw, uw, ta, tf, dg, du, m);
+        const uint4 vg = make_uint4(dg[0], dg[1], dg[2], dg[3]), vu = make_uint4(du[0], du[1], du[2], du[3]);
+        const Window wo = window(dGU + (at + h + i) * 2 * I, r + h + i < left ? 4 * ld : 0u);
+        window_store(wo, od, vg);
+        window_store(wo, od + 2 * ld, vu);
+        mg.add(h + i, vg, kg);  // (rows past the tensor's: zeros, dH having read as zeros)
+        mu.add(h + i, vu, ku);
+        __builtin_amdgcn_sched_barrier(0);  // row by row: interleaved, the rows' values spill
+      }
+    }
+    mg.store(p, at, tc, lane);
+    mu.store(p, at, tiles + tc, lane);
+  }
+  __syncthreads();
+  uint4(*red)[64] = reinterpret_cast<uint4(*)[64]>(tf);  // the tables have been read
+  int8_column_maxima<kNT / 64>(p, red, kg, ts, c < I ? c : p.cols, wid, lane);
+  __syncthreads();
+  int8_column_maxima<kNT / 64>(p, red, ku, ts, c < I ? I + c : p.cols, wid, lane);
 }
 
 __global__ __launch_bounds__(kNT) void geglu_bwd_kernel(const uint16_t* __restrict__ dH,
@@ -430,13 +499,28 @@ int bf8_geglu_mxint8(const void* GU, int64_t M, int64_t I, void* H, int8_t* GU8,
   return launch_status("geglu_fwd_mxi8_kernel");
 }
 
+size_t bf8_geglu_bwd_mxint8_maxima(int64_t M, int64_t I) {
+  return M > 0 && I > 0 ? int8_maxima_bytes(M, 2 * I, 2) : 0;
+}
+
 int bf8_geglu_bwd_mxint8(const void* dH, const int8_t* GU8, const uint8_t* GU8_exp, int64_t M, int64_t I,
-                         void* dGU, void* stream) {
-  if (const int rc = check_geglu_mxi8("bf8_geglu_bwd_mxint8", dH, dGU, GU8, GU8_exp, M, I)) return rc;
+                         void* dGU, void* maxima, size_t maxima_bytes, void* stream) {
+  const char* who = "bf8_geglu_bwd_mxint8";
+  if (const int rc = check_geglu_mxi8(who, dH, dGU, GU8, GU8_exp, M, I)) return rc;
+  BF8_CHECK(M < (1LL << 31) && I < (1 << 22), "%s: M or I too large", who);
+  BF8_CHECK(!maxima || (((uintptr_t)maxima & 255) == 0 && maxima_bytes >= bf8_geglu_bwd_mxint8_maxima(M, I)),
+            "%s: the maxima need %zu bytes, 256-byte aligned (got %zu)", who,
+            bf8_geglu_bwd_mxint8_maxima(M, I), maxima_bytes);
   if (M == 0 || I == 0) return BF8_OK;
-  hipLaunchKernelGGL(geglu_bwd_mxi8_kernel, dim3((unsigned)bwd_blocks(M, I)), dim3(kNT), 0,
-                     as_stream(stream), (const uint16_t*)dH, GU8, GU8_exp, M, I, (uint16_t*)dGU);
-  return launch_status("geglu_bwd_mxi8_kernel");
+  if (!maxima) {
+    hipLaunchKernelGGL(geglu_bwd_mxi8_kernel, dim3((unsigned)bwd_blocks(M, I)), dim3(kNT), 0, as_stream(stream),
+                       (const uint16_t*)dH, GU8, GU8_exp, M, I, (uint16_t*)dGU);
+    return launch_status("geglu_bwd_mxi8_kernel");
+  }
+  const Int8Maxima p = int8_maxima(maxima, M, 2 * I, 2);
+  hipLaunchKernelGGL(geglu_bwd_mxi8_maxima_kernel, dim3((unsigned)(p.strips * (p.row_tiles / 2))), dim3(kNT), 0,
+                     as_stream(stream), (const uint16_t*)dH, GU8, GU8_exp, I, (uint16_t*)dGU, p);
+  return launch_status("geglu_bwd_mxi8_maxima_kernel");
 }
 
 }  // extern "C"

@@ -692,8 +692,8 @@ class Int8GegluMlpFunction(_Fp8Function):
             dd = ops.gemm_int8(dyq.data_t, dyq.col_scale, h8t, hs)
         if need_dx or need_dgu:
             dH = ops.gemm_int8(dyq.data, dyq.row_scale, d8t, ds)
-            dGU = ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(gu8, gu_exps))
-            dq = ops.quantize_int8(dGU, rowwise=need_dx, colwise=need_dgu)
+            dq = ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(gu8, gu_exps), rowwise=need_dx,
+                                      colwise=need_dgu)
             if need_dx:
                 dx = ops.gemm_int8(dq.data, dq.row_scale, gu8t, gus)
             if need_dgu:

@@ -1561,6 +1561,17 @@ class Int8Tensor:
     cols: int
 
 
+def _new_int8(rows, cols, rowwise, colwise, device):
+    out = scale = out_t = scale_t = None
+    if rowwise:
+        out = torch.empty((rows, cols), dtype=torch.int8, device=device)
+        scale = torch.empty(rows, dtype=torch.float32, device=device)
+    if colwise:
+        out_t = torch.empty((cols, (rows + 15) // 16 * 16), dtype=torch.int8, device=device)
+        scale_t = torch.empty(cols, dtype=torch.float32, device=device)
+    return Int8Tensor(out, scale, out_t, scale_t, rows, cols)
+
+
 @functools.lru_cache(maxsize=4096)
 def _quantize_int8_ws_cached(rows, cols, both):
     return int(_lib.lib().bf8_quantize_int8_workspace(rows, cols, both))
@@ -1577,15 +1588,9 @@ def quantize_int8(x, *, rowwise=True, colwise=False):
     rows, cols = x.shape
     if not (rowwise or colwise):
         raise ValueError(f"{who}: nothing requested")
-    dev = x.device
-    out = scale = out_t = scale_t = ws = None
-    nbytes = 0
-    if rowwise:
-        out = torch.empty((rows, cols), dtype=torch.int8, device=dev)
-        scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    q = _new_int8(rows, cols, rowwise, colwise, x.device)
+    out, scale, out_t, scale_t, ws, nbytes = q.data, q.row_scale, q.data_t, q.col_scale, None, 0
     if colwise:
-        out_t = torch.empty((cols, (rows + 15) // 16 * 16), dtype=torch.int8, device=dev)
-        scale_t = torch.empty(cols, dtype=torch.float32, device=dev)
         nbytes = _quantize_int8_ws_cached(rows, cols, 1 if rowwise else 0)
         if nbytes:
             ws, nbytes = _call_workspace(nbytes, x)
@@ -1596,7 +1601,7 @@ def quantize_int8(x, *, rowwise=True, colwise=False):
         scale_t.fill_(2.0 ** -40 / 127)
     if rowwise and not cols:
         scale.fill_(2.0 ** -40 / 127)
-    return Int8Tensor(out, scale, out_t, scale_t, rows, cols)
+    return q
 
 
 def _int8_matrix(who, **tensors):
@@ -1817,8 +1822,15 @@ def geglu_mxint8(GU):
     return H, q
 
 
-def geglu_bwd_mxint8(dH, gu):
-    """:func:`geglu_bwd` on the values of GU's checkpoint: dGU bf16 [M, 2I]."""
+@functools.lru_cache(maxsize=4096)
+def _geglu_bwd_maxima_cached(M, I):
+    return int(_lib.lib().bf8_geglu_bwd_mxint8_maxima(M, I))
+
+
+def geglu_bwd_mxint8(dH, gu, *, rowwise=False, colwise=False):
+    """:func:`geglu_bwd` on the values of GU's checkpoint: dGU bf16 [M, 2I], or with ``rowwise`` or
+    ``colwise`` that tensor's :func:`quantize_int8` instead (from 1024 rows on by the maxima that the backward's
+    kernel leaves: the same codes and scales)."""
     who = "geglu_bwd_mxint8"
     idx = _index_of(who, dH, gu.data, gu.exps)
     dH = _rows_bf16(dH)
@@ -1826,11 +1838,25 @@ def geglu_bwd_mxint8(dH, gu):
     if I % 32:
         raise ValueError(f"{who}: the intermediate size must be a multiple of 32 (got {I})")
     data, exps = _mxint8_of(who, gu, M, 2 * I)
+    if not (rowwise or colwise):
+        dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
+        if M and I:
+            _call("bf8_geglu_bwd_mxint8", idx, _lib.lib().bf8_geglu_bwd_mxint8, dH.data_ptr(),
+                  data.data_ptr(), exps.data_ptr(), M, I, dGU.data_ptr(), None, 0)
+        return dGU
+    # both copies of dGU's codes, by the maxima and by the quantizer's own pass, us: [512, 2 x 10240] 32.5 and
+    # 31.5, [1500, 2 x 2560] 27.5 and 29.9, [4096, 2 x 10240] 157 and 168
+    if M < 1024 or not I:
+        return quantize_int8(geglu_bwd_mxint8(dH, gu), rowwise=rowwise, colwise=colwise)
     dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
-    if M and I:
-        _call("bf8_geglu_bwd_mxint8", idx, _lib.lib().bf8_geglu_bwd_mxint8, dH.data_ptr(),
-              data.data_ptr(), exps.data_ptr(), M, I, dGU.data_ptr())
-    return dGU
+    L = _lib.lib()
+    ws, nbytes = _call_workspace(_geglu_bwd_maxima_cached(M, I), dH)
+    _call("bf8_geglu_bwd_mxint8", idx, L.bf8_geglu_bwd_mxint8, dH.data_ptr(), data.data_ptr(),
+          exps.data_ptr(), M, I, dGU.data_ptr(), ws.data_ptr(), nbytes)
+    q = _new_int8(M, 2 * I, rowwise, colwise, dH.device)
+    _call("bf8_quantize_int8_maxima_bf16", idx, L.bf8_quantize_int8_maxima_bf16, dGU.data_ptr(), M, 2 * I, 2,
+          _ptr(q.data), _ptr(q.row_scale), _ptr(q.data_t), _ptr(q.col_scale), ws.data_ptr(), nbytes)
+    return q
 
 
 def column_sums(x):

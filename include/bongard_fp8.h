@@ -632,6 +632,12 @@ int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* ou
                            int8_t* out_t, float* col_scale, void* ws, size_t ws_bytes,
                            void* stream);
 
+/* The same codes and scales from the maxima of |x|'s rows and columns that x's producer left
+ * (bf8_geglu_bwd_mxint8's dGU: halves 2), without a pass that looks for them; any cols. */
+int bf8_quantize_int8_maxima_bf16(const void* x, int64_t rows, int64_t cols, int halves, int8_t* out,
+                                  float* row_scale, int8_t* out_t, float* col_scale, const void* maxima,
+                                  size_t maxima_bytes, void* stream);
+
 /* out bf16 [rows, cols] = codes * scale[row] (rounded once). cols % 8 == 0; out 16-byte, codes
  * 8-byte aligned. */
 int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int64_t cols, void* out,
@@ -683,11 +689,14 @@ int bf8_dequant_mxint8(const int8_t* codes, const uint8_t* exponents, int64_t ro
                        void* out, void* stream);
 
 /* bf8_geglu_bf16 (H from GU [M, 2 I]; no amax partials) that writes GU's checkpoint in the same
- * pass, and bf8_geglu_bwd (dGU; no amax partials) on the values of the checkpoint. I % 32 == 0. */
+ * pass, and bf8_geglu_bwd (dGU; no amax partials) on the values of the checkpoint. I % 32 == 0.
+ * maxima, where given: bf8_geglu_bwd_mxint8_maxima(M, I) bytes, 256-byte aligned, which receive the
+ * maxima of dGU's rows and columns for bf8_quantize_int8_maxima_bf16. */
 int bf8_geglu_mxint8(const void* GU, int64_t M, int64_t I, void* H, int8_t* GU8, uint8_t* GU8_exp,
                      void* stream);
+size_t bf8_geglu_bwd_mxint8_maxima(int64_t M, int64_t I);
 int bf8_geglu_bwd_mxint8(const void* dH, const int8_t* GU8, const uint8_t* GU8_exp, int64_t M,
-                         int64_t I, void* dGU, void* stream);
+                         int64_t I, void* dGU, void* maxima, size_t maxima_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * Layer norm of rows (beside the RMSNorm of bongard/fused_mlp.py:25-30; torch's layer_norm), in fp32:

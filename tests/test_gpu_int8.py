@@ -306,7 +306,8 @@ def _gu(M, I, seed, gpu):
     return GU.to(gpu), dH.to(gpu)
 
 
-@pytest.mark.parametrize("M,I", [(1, 32), (31, 96), (64, 640), (257, 384), (2001, 2560)])
+@pytest.mark.parametrize("M,I", [(1, 32), (31, 96), (64, 640), (257, 384), (2001, 2560), (3, 10272), (4100, 544),
+                                 (1024, 32), (1031, 288), (1100, 10272)])
 def test_gated_gelu_from_a_checkpoint(gpu, M, I):
     """H is the gated GELU's, the checkpoint the quantizer's and the gradient the separate backward's at
     the values read back, bit for bit."""
@@ -317,6 +318,13 @@ def test_gated_gelu_from_a_checkpoint(gpu, M, I):
     assert torch.equal(q.data, want.data) and torch.equal(q.exps, want.exps)
     dGU = ops.geglu_bwd_mxint8(dH, q)
     assert torch.equal(dGU, ops.geglu_bwd(dH, ops.dequant_mxint8(q))[0])
+    # its int8 copies (from 1024 rows on by the maxima that the backward leaves)
+    for rowwise, colwise in ((True, True), (True, False), (False, True)):
+        got = ops.geglu_bwd_mxint8(dH, q, rowwise=rowwise, colwise=colwise)
+        want = ops.quantize_int8(dGU, rowwise=rowwise, colwise=colwise)
+        for name in ("data", "row_scale", "data_t", "col_scale"):
+            a, b = getattr(got, name), getattr(want, name)
+            assert (a is None and b is None) or torch.equal(a, b), name
     leaf = GU.clone().requires_grad_()
     h = fused_mlp.gated_gelu(leaf.view(1, M, 2 * I), checkpoint=True)
     h.backward(dH.view(1, M, I))
@@ -351,6 +359,20 @@ def test_gated_gelu_gradient_is_the_difference(gpu):
         got = leaf.grad[:, half * I:(half + 1) * I].cpu().double()
         scale = (v[:, I:] if half == 0 else nn.functional.gelu(v[:, :I], approximate="tanh")) * dH.double()
         assert bool(((got - diff).abs() <= 3 * 2.0 ** -8 * diff.abs() + 2.0 ** -14 * scale.abs() + 2.0 ** -20).all())
+
+
+def test_codes_of_a_nonfinite_gradient(gpu):
+    """Rows and columns of dGU that hold an inf or a NaN: the quantizer's NaN scales and zero codes, also where the
+    backward leaves the maxima."""
+    GU, dH = _gu(1100, 544, 7, gpu)
+    dH[3, 9], dH[1099, 543], dH[700, 64] = float("nan"), float("inf"), -float("inf")
+    _, q = ops.geglu_mxint8(GU)
+    got = ops.geglu_bwd_mxint8(dH, q, rowwise=True, colwise=True)
+    want = ops.quantize_int8(ops.geglu_bwd_mxint8(dH, q), rowwise=True, colwise=True)
+    assert torch.isnan(want.row_scale).nonzero().flatten().tolist() == [3, 700, 1099]
+    for name in ("data", "row_scale", "data_t", "col_scale"):
+        a, b = getattr(got, name), getattr(want, name)
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), name
 
 
 def test_gated_gelu_of_nonfinite_blocks(gpu):

@@ -112,7 +112,7 @@ def _calls(L):
     q, d, g, h = L.bf8_quantize_int8_bf16, L.bf8_dequant_int8, L.bf8_gemm_int8, L.bf8_gemm_geglu_int8
     m, dm, cs = L.bf8_quantize_mxint8_bf16, L.bf8_dequant_mxint8, L.bf8_column_sums_bf16
     f, b = L.bf8_geglu_mxint8, L.bf8_geglu_bwd_mxint8
-    t = L.bf8_linear_int8
+    t, qm = L.bf8_linear_int8, L.bf8_quantize_int8_maxima_bf16
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
     return [
         (q, (p, 4, 12, p, p, null, null, null, 0, null), "cols % 8"),
@@ -168,9 +168,16 @@ def _calls(L):
         (f, (p, 4, 40, p, p, p, null), "I % 32"),
         (f, (p, 4, 64, p, p, null, null), "NULL"),
         (f, (odd, 4, 64, p, p, p, null), "16-byte"),
-        (b, (p, p, p, 4, 24, p, null), "I % 32"),
-        (b, (p, null, p, 4, 32, p, null), "NULL"),
-        (b, (p, odd, p, 4, 32, p, null), "8-byte"),
+        (b, (p, p, p, 4, 24, p, null, 0, null), "I % 32"),
+        (b, (p, null, p, 4, 32, p, null, 0, null), "NULL"),
+        (b, (p, odd, p, 4, 32, p, null, 0, null), "8-byte"),
+        (b, (p, p, p, 4, 32, p, p, 8, null), "maxima need"),
+        (qm, (p, 4, 24, 2, p, p, null, null, p, 1 << 20, null), "cols % 8"),
+        (qm, (p, 4, 32, 3, p, p, null, null, p, 1 << 20, null), "parts"),
+        (qm, (p, 4, 32, 2, p, p, null, null, p, 8, null), "bytes of maxima"),
+        (qm, (p, 4, 32, 2, p, p, null, null, null, 1 << 20, null), "bytes of maxima"),
+        (qm, (p, 4, 32, 2, p, null, null, null, p, 1 << 20, null), "give out"),
+        (qm, (odd, 4, 32, 2, p, p, null, null, p, 1 << 20, null), "16-byte"),
         (cs, (p, 0, 16, p, p, 1 << 20, null), "rows > 0"),
         (cs, (p, 4, 12, p, p, 1 << 20, null), "cols % 8"),
         (cs, (p, 4, 16, null, p, 1 << 20, null), "must be given"),
@@ -211,7 +218,7 @@ def test_sizes_of_nothing():
     assert L.bf8_quantize_mxint8_bf16(null, 0, 64, null, null, null) == 0
     assert L.bf8_dequant_mxint8(null, null, 3, 0, null, null) == 0
     assert L.bf8_geglu_mxint8(null, 0, 32, null, null, null, null) == 0
-    assert L.bf8_geglu_bwd_mxint8(null, null, null, 0, 32, null, null) == 0
+    assert L.bf8_geglu_bwd_mxint8(null, null, null, 0, 32, null, null, 0, null) == 0
     assert L.bf8_layernorm_bf16(null, 0, 64, null, null, 1e-6, null, null, null, null, null, null) == 0
     assert L.bf8_quantize_int8_workspace(0, 64, 0) == 0 and L.bf8_quantize_int8_workspace(3, 64, 0) >= 64 * 6
     assert L.bf8_quantize_int8_workspace(3, 64, 1) == 0 and L.bf8_quantize_int8_workspace(5000, 64, 1) >= 64 * 6
