@@ -198,15 +198,22 @@ constexpr double kSecondLaunchUs = 0.7;
 // matters at few K steps: 9161 x 4176 x 192 on 256x256w8 42.1 us, on 192x128o2 37.4).
 constexpr double kLaterSaves[2] = {0.44, 0.761};
 constexpr double kEmptySaves = 0.145, kOutUsPerMB = 0.143, kOutHidden = 0.175;
+// int8 products cost what FP8's do but for these two (their MFMAs draw more power, so a full chip clocks lower and
+// less of the partials' traffic is hidden). On 5,185 random shapes of the same ranges the picks lose 1.4% on
+// average against the best measured plan, 5% in one of ten, 16% in one of a hundred (of 2e10 products and more
+// 1.0, 4 and 10%); with FP8's two 1.55, 6 and 15% (1.3, 5 and 13%; 2001 x 2560 x 10240 in two pieces 91 us, unsplit
+// 70). Round costs of their own, fitted, won no more.
+constexpr double kI8PartialUsPerMB = 0.54, kI8LaterSaves[2] = {0.3, 0.6};
 
 // Modelled time (us) of a linear plan of C [M, N]. kmajor: as GemmParams::kmajor.
-double linear_cost(const Plan& p, int64_t M, int64_t N, int64_t ksteps, bool mx, int kmajor) {
+double linear_cost(const Plan& p, int64_t M, int64_t N, int64_t ksteps, bool mx, int kmajor, bool i8 = false) {
   // the extra-B-slot twin is costed as the tile it replaces
   const TileInfo& ti = kTiles[p.tile == TILE_256x256w8x ? (int)TILE_256x256w8 : p.tile];
   const RoundCost& rc = mx ? ti.mx_rows : ti.rows;
   const double loaded =
       (double)(std::min<int64_t>(M, ti.bm) + std::min<int64_t>(N, ti.bn)) / (ti.bm + ti.bn);
   const double fill = 1 - kEmptySaves * (1 - loaded);
+  const double later = 1.0 - (i8 ? kI8LaterSaves : kLaterSaves)[ti.occ - 1];
   const double out_mb = 2e-6 * M * N / ((double)p.tiles_m * p.tiles_n);  // of a workgroup
   auto round = [&](int64_t ctas, int64_t steps, bool first, bool writes_out) {
     const double x = (double)std::min<int64_t>(ctas, kNumCus) / kNumCus;
@@ -215,7 +222,7 @@ double linear_cost(const Plan& p, int64_t M, int64_t N, int64_t ksteps, bool mx,
     const double loop = steps * fill * (two ? rc.s2 + (rc.s3 - rc.s2) * y : rc.s0 + (rc.s1 - rc.s0) * x);
     const double fixed = two ? rc.f2 + rc.g2 * y : rc.f1 + rc.g1 * x;
     const double out = writes_out ? kOutUsPerMB * out_mb * ctas - kOutHidden * loop : 0.0;
-    return loop + fixed * (first ? 1.0 : 1.0 - kLaterSaves[ti.occ - 1]) + std::max(out, 0.0);
+    return loop + fixed * (first ? 1.0 : later) + std::max(out, 0.0);
   };
   const int64_t slots = (int64_t)kNumCus * ti.occ;
   const bool tail = p.tail_pieces > 0, split = p.splits > 1;
@@ -230,7 +237,7 @@ double linear_cost(const Plan& p, int64_t M, int64_t N, int64_t ksteps, bool mx,
   if (tail) t += round((tiles - p.full_tiles) * p.tail_pieces, p.kps, false, false);
   if (tail || split)
     t += (kmajor == 3 ? kReduceBothKmajorUs : kReduceUs) + kSecondLaunchUs +
-         kPartialUsPerMB * (double)p.ws_bytes / 1e6;
+         (i8 ? kI8PartialUsPerMB : kPartialUsPerMB) * (double)p.ws_bytes / 1e6;
   return t;
 }
 
@@ -279,21 +286,40 @@ const RoundCost* geglu4_rounds(int tile) {
                                 : nullptr;
 }
 
+// The int8 gated-GELU plans, likewise (their checkpoint's blocks leave no per-tile maxima whose number must not
+// depend on K): least squares over the measured times of 1,250 shapes (M 8 .. 8192, I 128 .. 10240, K 256 .. 10240;
+// with and without the checkpoint, operands repeated and rotated past the L2s); picks on as many others lose 1.0%
+// on average, 3% in one of ten, 16% in one of a hundred; by geglu_cost 4.8, 19 and 49% (155 rows, I 10240, K 384:
+// 128x128 19.7 us, 64x128 9.2). 192x256, the best of one shape in a hundred, is left out.
+constexpr RoundCost kGeglu8_256x256w8 = {0.941, 1.619, 16.008, 2.73};
+constexpr RoundCost kGeglu8_160x256 = {0.937, 1.166, 14.687, 4.991};
+constexpr RoundCost kGeglu8_128x128 = {0.459, 0.576, 8.692, 1.21};
+constexpr RoundCost kGeglu8_64x128 = {0.503, 0.77, 5.526, 0.302, 0.725, 0.75, 6.729, 1.254};
+constexpr double kGeglu8LaterSaves[2] = {0.241, 0.49};
+
+const RoundCost* geglu8_rounds(int tile) {
+  return tile == TILE_256x256w8 ? &kGeglu8_256x256w8
+         : tile == TILE_160x256 ? &kGeglu8_160x256
+         : tile == TILE_128x128 ? &kGeglu8_128x128
+         : tile == TILE_64x128  ? &kGeglu8_64x128
+                                : nullptr;
+}
+
 // Whether MXFP4 has a linear or gated-GELU variant of `tile`: of those that its plans can take.
 bool f4_tile_ok(int tile, bool geglu) {
   return geglu ? geglu4_rounds(tile) != nullptr : kTiles[tile].planned && kTiles[tile].mx;
 }
 
-// Whether int8 has a linear or gated-GELU variant of `tile` (as gemm_kernel_impl.hpp's i8_tile): its
-// checkpoint blocks of 32 columns do not fit the 256x160 tile's halves of 80.
+// Whether int8 has a linear or gated-GELU variant of `tile` (as gemm_kernel_impl.hpp's i8_tile): of those that
+// its plans can take. (Its checkpoint blocks of 32 columns would not fit the 256x160 tile's halves of 80.)
 bool i8_tile_ok(int tile, bool geglu) {
-  if (geglu) return kTiles[tile].planned && kTiles[tile].geglu_rate > 0 && kTiles[tile].bn % 64 == 0;
-  return kTiles[tile].planned || tile == TILE_256x256w8x;
+  return geglu ? geglu8_rounds(tile) != nullptr : kTiles[tile].planned || tile == TILE_256x256w8x;
 }
 
-double geglu4_cost(const Plan& p, int64_t M, int64_t N) {
+double geglu_rounds_cost(const Plan& p, int64_t M, int64_t N, bool i8) {
   const TileInfo& ti = kTiles[p.tile];
-  const RoundCost& rc = *geglu4_rounds(p.tile);
+  const RoundCost& rc = i8 ? *geglu8_rounds(p.tile) : *geglu4_rounds(p.tile);
+  const double later = 1.0 - (i8 ? kGeglu8LaterSaves : kGeglu4LaterSaves)[ti.occ - 1];
   const double loaded =
       (double)(std::min<int64_t>(M, ti.bm) + std::min<int64_t>(N, ti.bn)) / (ti.bm + ti.bn);
   const double steps = p.kps * (1 - kEmptySaves * (1 - loaded));
@@ -303,7 +329,7 @@ double geglu4_cost(const Plan& p, int64_t M, int64_t N) {
     const bool two = ctas > kNumCus;  // occ 2
     const double fixed = two ? rc.f2 + rc.g2 * y : rc.f1 + rc.g1 * x;
     return steps * (two ? rc.s2 + (rc.s3 - rc.s2) * y : rc.s0 + (rc.s1 - rc.s0) * x) +
-           fixed * (first ? 1.0 : 1.0 - kGeglu4LaterSaves[ti.occ - 1]);
+           fixed * (first ? 1.0 : later);
   };
   const int64_t slots = (int64_t)kNumCus * ti.occ, ctas = (int64_t)p.tiles_m * p.tiles_n;
   const int64_t whole = ctas / slots, rest = ctas % slots;
@@ -334,8 +360,8 @@ bool env_override(int& tile, int& splits) {
 }
 
 // Chooses the tile and K split for C[M, N] = A[M, K] . B[N, K]^T. GEGLU plans never split
-// and, but for MXFP4's (f4), depend on (M, N) only, so the per-tile amax partial count is known
-// without K.
+// and, but for MXFP4's (f4) and int8's (i8), depend on (M, N) only, so the per-tile amax partial count
+// is known without K.
 Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, bool mx = false,
                  int kmajor = 0, bool f4 = false, bool i8 = false) {
   const int64_t ksteps = std::max<int64_t>(cdiv(K, kStepBytes), 1);
@@ -353,6 +379,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
     if (p.ws_bytes > ws_avail) p = make_plan(otile, M, N, ksteps, 1);
     return p;
   }
+  const bool coarse = geglu && !f4 && !i8;  // geglu_cost
   Plan best;
   double best_cost = 0;
   bool have = false;
@@ -371,17 +398,17 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
     const bool two_stage = tile == TILE_192x128o2 || tile == TILE_128x128o2;
     const bool two_groups = tile == TILE_128x64k2 || tile == TILE_64x128k2;
     for (int s = 1; s <= (geglu || two_stage || two_groups ? 1 : kMaxSplits); ++s) {
-      const Plan p = make_plan(tile, M, N, geglu && !f4 ? kGegluNominalSteps : ksteps, s);
+      const Plan p = make_plan(tile, M, N, coarse ? kGegluNominalSteps : ksteps, s);
       if (p.splits != s || (s > 1 && p.kps < kMinStepsPerSplit) || p.ws_bytes > ws_avail)
         continue;
       if (two_groups && (int64_t)p.tiles_m * p.tiles_n > kNumCus) continue;
-      const double c = geglu && f4 ? geglu4_cost(p, M, N)
-                       : geglu     ? geglu_cost(p)
-                                   : linear_cost(p, M, N, ksteps, mx, kmajor);
+      const double c = coarse  ? geglu_cost(p)
+                       : geglu ? geglu_rounds_cost(p, M, N, i8)
+                               : linear_cost(p, M, N, ksteps, mx, kmajor, i8);
       // Ties go to the earlier (larger, unsplit) plan. geglu_cost is the coarser model: within 3%
       // the earlier tile was the faster on every shape that differed (M = 4457, I = 2560, K = 10240
       // on 192x256 200.9 us, on 256x256w8 223.5; M = 8340, I = 2048, K = 2560 117.7 and 122.5).
-      if (!have || c < best_cost * (geglu && !f4 ? 0.97 : 0.99)) {
+      if (!have || c < best_cost * (coarse ? 0.97 : 0.99)) {
         best = p;
         best_cost = c;
         have = true;
@@ -389,7 +416,7 @@ Plan choose_plan(int64_t M, int64_t N, int64_t K, bool geglu, size_t ws_avail, b
     }
     Plan tp;
     if (!geglu && make_tail_plan(tile, M, N, ksteps, tp) && tp.ws_bytes <= ws_avail) {
-      const double c = linear_cost(tp, M, N, ksteps, mx, kmajor);
+      const double c = linear_cost(tp, M, N, ksteps, mx, kmajor, i8);
       if (!have || c < best_cost * 0.99) {
         best = tp;
         best_cost = c;

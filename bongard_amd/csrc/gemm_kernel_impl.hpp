@@ -1477,7 +1477,7 @@ constexpr bool i8_tile(int epi) {
   if (std::is_same<T, Tile256x256>::value || std::is_same<T, Tile256x128>::value ||
       std::is_same<T, Tile128x128k2>::value)
     return false;
-  return epi == EPI_LINEAR || T::FN % 2 == 0;
+  return epi == EPI_LINEAR || (T::FN % 2 == 0 && !std::is_same<T, Tile192x256>::value);
 }
 inline int no_i8_tile(int bm, int bn) {
   set_error("gemm: tile %dx%d has no such int8 variant", bm, bn);

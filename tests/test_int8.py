@@ -2,6 +2,7 @@
 the int8, checkpoint and layer-norm entries, before any launch."""
 
 import ctypes
+import re
 from fractions import Fraction
 
 import pytest
@@ -244,6 +245,20 @@ def test_a_named_tile_is_the_plan(monkeypatch, capfd, tile):
         monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", none)
         L.bf8_gemm_int8_workspace(M, N, K)
         assert "bf8 plan gemm" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("M,N,K,tiles,splits", [
+    (2001, 2560, 10240, {"128x128o2", "192x128o2", "256x160", "160x256"}, [1]),  # in two pieces 91 us, unsplit 70-80
+    (4096, 2560, 10240, {"256x160", "256x256w8x"}, [1]),  # 106 us, in two pieces 159
+    (64, 2048, 2560, {"128x64", "128x64k2"}, range(1, 8)),
+])
+def test_planner_picks_int8(monkeypatch, capfd, M, N, K, tiles, splits):
+    """Its partials cost more than FP8's: fewer products run in K pieces."""
+    monkeypatch.delenv("BONGARD_FP8_GEMM_TILE", raising=False)
+    monkeypatch.setenv("BONGARD_FP8_GEMM_DEBUG", "1")
+    _lib.lib().bf8_gemm_int8_workspace(M, N, K)
+    tile, pieces = re.search(r"tile (\S+) splits (\d+)", capfd.readouterr().err).groups()
+    assert tile in tiles and int(pieces) in splits
 
 
 def test_layer_norm_refuses_forward_mode_tangents(monkeypatch):
