@@ -17,10 +17,7 @@ namespace bf8 {
 namespace {
 
 constexpr int kMaxCols = 16384;
-constexpr int64_t kMaxFwdBlocks = 2048;
-// The backward's blocks: those resident at once, as each adds a partial row to the weights' sums.
-constexpr int64_t max_bwd_blocks(int64_t cols) { return cols <= 4096 ? 512 : 256; }
-
+constexpr int64_t kMaxFwdBlocks = 2048, kFewRows = 512;
 struct LayerNorm {
   const uint16_t *x, *w, *b;
   int64_t rows;
@@ -36,7 +33,7 @@ struct LayerNorm {
 };
 
 // Threads of a block whose rows take WPR waves each: four rows of one wave, or one row of more.
-constexpr int block_threads(int wpr) { return 64 * (wpr < 4 ? 4 : wpr); }
+constexpr int block_threads(int wpr) { return wpr == 1 ? 256 : 64 * wpr; }
 
 // Sums of N values over the row's threads: a wave, or the block's waves through LDS, added in order.
 template <int N, int WPR>
@@ -91,6 +88,12 @@ __device__ __forceinline__ void keep_packed(uint4& v) {
   asm volatile("" : "+v"(v.x), "+v"(v.y), "+v"(v.z), "+v"(v.w));
 }
 
+// A row takes WPR waves, a thread V pieces of 8 columns of it. Bound by memory (4 bytes an element, 5.03 with the
+// checkpoint): [18494, 2560] 32 us as a wave a row (35 at a copy's rate; from the memory-side cache in part), with the
+// checkpoint 41 (three waves 33 and 43: a barrier between two sums); [3001, 4104] as three waves 11.3 and 16.1 us
+// (five 13.1, nine 14.9, sixteen 20.7: idle lanes, and fewer rows in flight on a CU); [4096, 8192] as four waves of
+// four pieces 22.9 and 30.5 (eight of two 23.6 and 32.1, sixteen of one 28.8 and 40.1). Few rows take more waves:
+// [64, 2560] as five 3.2 us, as one 3.7.
 template <int V, int WPR, bool CKPT>
 __global__ __launch_bounds__(block_threads(WPR)) void layer_norm_kernel(LayerNorm p) {
   __shared__ float red[2][1][WPR];
@@ -170,18 +173,39 @@ struct Piece<true> {
   uint32_t e;
 };
 
-template <int V, int WPR, bool CKPT>
-__global__ __launch_bounds__(block_threads(WPR)) void layer_norm_bwd_kernel(LayerNorm p) {
-  __shared__ float red[2][WPR];
-  extern __shared__ float4 sums[];  // (WPR 1) two waves' column sums
-  const int t = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
+// A thread's sums of dy n and dy into the block's partial row: t of `threads` of a row.
+template <int V>
+__device__ __forceinline__ void write_sums(const LayerNorm& p, int t, int threads, const float (&aw)[V][8],
+                                           const float (&ab)[V][8]) {
+  float* dst = p.part + (int64_t)blockIdx.x * 2 * p.cols;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int i = t + threads * j;
+    if (i >= p.cols >> 3) continue;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const float(&a)[8] = h < 2 ? aw[j] : ab[j];
+      *reinterpret_cast<float4*>(dst + (h < 2 ? 0 : p.cols) + 8 * i + 4 * (h & 1)) =
+          make_float4(a[4 * (h & 1)], a[4 * (h & 1) + 1], a[4 * (h & 1) + 2], a[4 * (h & 1) + 3]);
+    }
+  }
+}
+
+// Rows of up to 1,536 columns, a wave each: their column sums stay in the wave's registers and the block's four
+// waves add theirs at the end. [20000, 640] 25.5 us with the kernel that adds the partials, [8000, 1536] 21.2 (the
+// kernel below 29.0 and 24.2); from 2,048 columns on a wave's sums and rows leave one wave a SIMD ([18494, 2560] 66,
+// the kernel below 57).
+template <int V, bool CKPT>
+__global__ __launch_bounds__(256) void layer_norm_bwd_kernel(LayerNorm p) {
+  __shared__ float4 sums[2 * V * 4 * 64];  // two waves' column sums
+  const int t = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t first = WPR == 1 ? (int64_t)blockIdx.x * 4 + wid : blockIdx.x;
-  const int64_t stride = WPR == 1 ? (int64_t)gridDim.x * 4 : gridDim.x;
+  const int64_t first = (int64_t)blockIdx.x * 4 + wid;
+  const int64_t stride = (int64_t)gridDim.x * 4;
   const int nvec = p.cols >> 3, blocks = (p.cols + 31) >> 5;
   const float inv = 1.0f / (float)p.cols;
   uint4 w[V];
-  load_row<V, WPR>(row_of(p.w, 0, p.cols), t, w);
+  load_row<V, 1>(row_of(p.w, 0, p.cols), t, w);
   float aw[V][8], ab[V][8];
 #pragma unroll
   for (int j = 0; j < V; ++j)
@@ -190,10 +214,10 @@ __global__ __launch_bounds__(block_threads(WPR)) void layer_norm_bwd_kernel(Laye
   for (int64_t row = first; row < p.rows; row += stride) {
     uint4 dy[V];
     Piece<CKPT> x[V];
-    load_row<V, WPR>(row_of(p.dy, row, p.cols), t, dy);
+    load_row<V, 1>(row_of(p.dy, row, p.cols), t, dy);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int i = t + 64 * WPR * j;
+      const int i = t + 64 * j;
       if constexpr (CKPT) {
         x[j].q = make_uint2(0u, 0u);
         x[j].e = 133u;
@@ -237,8 +261,7 @@ __global__ __launch_bounds__(block_threads(WPR)) void layer_norm_bwd_kernel(Laye
       }
     }
     if (!p.dx) continue;
-    if constexpr (WPR > 1) __syncthreads();  // the row before has read red
-    row_sum<2, WPR>(s, red);
+    row_sum<2, 1>(s, nullptr);
     const float m0 = s[0] * inv, m1 = s[1] * inv;
     const Window dx = row_of(p.dx, row, p.cols);
 #pragma unroll
@@ -251,62 +274,195 @@ __global__ __launch_bounds__(block_threads(WPR)) void layer_norm_bwd_kernel(Laye
       unpack8(w[j], g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) d[e] = r * (fmaf(d[e], g[e], -m0) - n[e] * m1);
-      window_store(dx, 16u * (t + 64 * WPR * j), pack8(d));
+      window_store(dx, 16u * (t + 64 * j), pack8(d));
     }
   }
   if (!p.part) return;
-  auto write_sums = [&]() __attribute__((always_inline)) {
-    float* dst = p.part + (int64_t)blockIdx.x * 2 * p.cols;
+  // the block's four waves add their sums: 2 to 0 and 3 to 1, then 1 to 0
+  auto give = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int i = t + 64 * WPR * j;
-      if (i >= nvec) continue;
+    for (int j = 0; j < V; ++j)
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
         const float(&a)[8] = h < 2 ? aw[j] : ab[j];
-        *reinterpret_cast<float4*>(dst + (h < 2 ? 0 : p.cols) + 8 * i + 4 * (h & 1)) =
+        sums[(to * 4 * V + 4 * j + h) * 64 + t] =
             make_float4(a[4 * (h & 1)], a[4 * (h & 1) + 1], a[4 * (h & 1) + 2], a[4 * (h & 1) + 3]);
       }
-    }
   };
-  if constexpr (WPR > 1) {
-    write_sums();
-  } else {
-    // the block's four waves add their sums: 2 to 0 and 3 to 1, then 1 to 0
-    auto give = [&](int to) __attribute__((always_inline)) {
+  auto take = [&](int from) __attribute__((always_inline)) {
 #pragma unroll
-      for (int j = 0; j < V; ++j)
+    for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const float(&a)[8] = h < 2 ? aw[j] : ab[j];
-          sums[(to * 4 * V + 4 * j + h) * 64 + t] =
-              make_float4(a[4 * (h & 1)], a[4 * (h & 1) + 1], a[4 * (h & 1) + 2], a[4 * (h & 1) + 3]);
-        }
-    };
-    auto take = [&](int from) __attribute__((always_inline)) {
+      for (int h = 0; h < 4; ++h) {
+        float(&a)[8] = h < 2 ? aw[j] : ab[j];
+        const float4 b = sums[(from * 4 * V + 4 * j + h) * 64 + t];
+        a[4 * (h & 1)] += b.x;
+        a[4 * (h & 1) + 1] += b.y;
+        a[4 * (h & 1) + 2] += b.z;
+        a[4 * (h & 1) + 3] += b.w;
+      }
+  };
+  if (wid >= 2) give(wid - 2);
+  __syncthreads();
+  if (wid < 2) take(wid);
+  __syncthreads();
+  if (wid == 1) give(0);
+  __syncthreads();
+  if (wid == 0) {
+    take(0);
+    write_sums<V>(p, t, 64, aw, ab);
+  }
+}
+
+// Sums over the block of N values a thread (2 or 4): a wave's lanes halve them by exchanges until a lane holds
+// one of them, red[wave][N] joins the waves, which are added in order. One barrier: the caller gives a call
+// other LDS than the one before.
+template <int N>
+__device__ __forceinline__ void block_sums(float (&v)[N], float* red) {
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  int n = N, off = 32;
 #pragma unroll
-      for (int j = 0; j < V; ++j)
+  for (; n > 1; n /= 2, off /= 2) {
+    const bool up = lane & off;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          float(&a)[8] = h < 2 ? aw[j] : ab[j];
-          const float4 b = sums[(from * 4 * V + 4 * j + h) * 64 + t];
-          a[4 * (h & 1)] += b.x;
-          a[4 * (h & 1) + 1] += b.y;
-          a[4 * (h & 1) + 2] += b.z;
-          a[4 * (h & 1) + 3] += b.w;
-        }
-    };
-    if (wid >= 2) give(wid - 2);
-    __syncthreads();
-    if (wid < 2) take(wid);
-    __syncthreads();
-    if (wid == 1) give(0);
-    __syncthreads();
-    if (wid == 0) {
-      take(0);
-      write_sums();
+    for (int i = 0; i < n / 2; ++i) {
+      const float give = up ? v[i] : v[i + n / 2], keep = up ? v[i + n / 2] : v[i];
+      v[i] = keep + __shfl_xor(give, off, 64);
     }
   }
+#pragma unroll
+  for (; off >= 1; off /= 2) v[0] += __shfl_xor(v[0], off, 64);
+  constexpr int kLanes = 64 / N;  // that hold the same sum
+  if ((lane & (kLanes - 1)) == 0) red[wid * N + lane / kLanes] = v[0];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = red[i];
+  for (int w = 1; w < waves; ++w)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += red[w * N + i];
+}
+
+// A row of the block: thread t's pieces t, t + blockDim.x.
+template <int V>
+__device__ __forceinline__ void load_block_row(Window w, uint4 (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = window_load(w, 16u * (threadIdx.x + blockDim.x * j));
+}
+
+// R rows of the backward's inputs, x or its checkpoint.
+template <int V, int R, bool CKPT>
+struct BwdRows {
+  uint4 dy[R][V], x[CKPT ? 1 : R][V];
+  uint2 q[CKPT ? R : 1][V];
+  uint32_t e[CKPT ? R : 1][V];
+  float mean[R], rstd[R];
+
+  // rows past the tensor's read as zeros
+  __device__ __forceinline__ void load(const LayerNorm& p, int64_t r0) {
+    const int blocks = (p.cols + 31) >> 5;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int64_t row = r0 + i;
+      const bool in = row < p.rows;
+      load_block_row<V>(row_of(in ? p.dy : nullptr, row, p.cols), dy[i]);
+      if constexpr (CKPT) {
+        const Window wq = row_of(in ? p.x8 : nullptr, row, p.cols, 1);
+        const Window we = row_of(in ? p.x8_e : nullptr, row, blocks, 1);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const uint32_t k = threadIdx.x + blockDim.x * j;
+          q[i][j] = window_load8(wq, 8 * k);
+          e[i][j] = window_load1(we, k >> 2);
+        }
+      } else {
+        load_block_row<V>(row_of(in ? p.x : nullptr, row, p.cols), x[i]);
+      }
+      mean[i] = in ? p.mean[row] : 0.0f;
+      rstd[i] = in ? p.rstd[row] : 0.0f;
+    }
+  }
+
+  __device__ __forceinline__ void norm(int i, int j, float (&n)[8]) {
+    if constexpr (CKPT) {
+      const float step = mxi8_step(e[i][j]);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        n[k] = (code_f32(k < 4 ? q[i][j].x : q[i][j].y, k & 3) * step - mean[i]) * rstd[i];
+    } else {
+      keep_packed(x[i][j]);
+      unpack8(x[i][j], n);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n[k] = (n[k] - mean[i]) * rstd[i];
+    }
+  }
+};
+
+// Wider rows: a block of ceil(cols / 512) waves a row (V 1; V 2 from 8,200 columns on), so that a thread keeps 16 sums
+// a piece and the card 10 or 16 waves a CU. Either R 2 rows between two barriers, or (AHEAD, more than 2,560
+// columns, where one block has a CU) a row, with the next one's loads under its reductions. Bound by memory (6
+// bytes an element, 5.03 from a checkpoint, and 8 bytes a column and block of partials): with the kernel that
+// adds those [18494, 2560] 56.8 us, from a checkpoint 55.7 (AHEAD 61 and 68), [3001, 4104] 26.5 (two rows 29.2),
+// [4096, 8192] 48 (two rows 52), [3000, 16384] 77 (72 from a checkpoint).
+template <int V, int R, bool AHEAD, bool CKPT>
+__global__ __launch_bounds__(1024) void layer_norm_bwd_block_kernel(LayerNorm p) {
+  __shared__ float red[2][16 * 2 * R];
+  const int t = threadIdx.x;
+  const float inv = 1.0f / (float)p.cols;
+  uint4 w[V];
+  load_block_row<V>(row_of(p.w, 0, p.cols), w);
+  float aw[V][8], ab[V][8];
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) aw[j][e] = ab[j][e] = 0.0f;
+  const int64_t stride = (int64_t)gridDim.x * R;
+  BwdRows<V, R, CKPT> in;
+  if (AHEAD) in.load(p, (int64_t)blockIdx.x * R);
+  int odd = 0;
+  for (int64_t r0 = (int64_t)blockIdx.x * R; r0 < p.rows; r0 += stride) {
+    if (!AHEAD) in.load(p, r0);
+    float s[2 * R], n[R][V][8], c[R][V][8];  // sums of c, c n (dy reads as zeros past the row)
+    float r[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      r[i] = in.rstd[i];
+      s[2 * i] = s[2 * i + 1] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float g[8];
+        in.norm(i, j, n[i][j]);
+        unpack8(in.dy[i][j], c[i][j]);
+        keep_packed(w[j]);
+        unpack8(w[j], g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          aw[j][e] = fmaf(c[i][j][e], n[i][j][e], aw[j][e]);
+          ab[j][e] += c[i][j][e];
+          c[i][j][e] *= g[e];
+          s[2 * i] += c[i][j][e];
+          s[2 * i + 1] = fmaf(c[i][j][e], n[i][j][e], s[2 * i + 1]);
+        }
+      }
+    }
+    if (AHEAD) in.load(p, r0 + stride);
+    if (!p.dx) continue;
+    block_sums<2 * R>(s, red[odd]);
+    odd ^= 1;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float m0 = s[2 * i] * inv, m1 = s[2 * i + 1] * inv;
+      const Window dx = row_of(r0 + i < p.rows ? p.dx : nullptr, r0 + i, p.cols);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float d[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d[e] = r[i] * (fmaf(n[i][j][e], -m1, c[i][j][e]) - m0);
+        window_store(dx, 16u * (t + blockDim.x * j), pack8(d));
+      }
+    }
+  }
+  if (!p.part) return;
+  write_sums<V>(p, t, blockDim.x, aw, ab);
 }
 
 // The weight's and the bias' gradients from the blocks' partials: blockIdx.y 0 and 1. A block takes 16
@@ -335,11 +491,20 @@ __global__ __launch_bounds__(kRedNT) void layer_norm_wgrad_kernel(const float* _
   if (g == 0 && col < cols) out[col] = (uint16_t)f32_to_bf16_bits(red[0][lc]);
 }
 
-// Rows up to 2,560 wide take a wave each, wider ones a block of four waves or sixteen.
-constexpr int kWaveCols = 2560;
-int64_t row_blocks(int64_t rows, int cols, int64_t most) {
-  const int64_t b = cols <= kWaveCols ? (rows + 3) / 4 : rows;
-  return std::max<int64_t>(1, std::min(b, most));
+int64_t row_blocks(int64_t rows, int per, int64_t most) {
+  return std::max<int64_t>(1, std::min((rows + per - 1) / per, most));
+}
+
+// The backward's rows and blocks: as many as are resident at once, as each adds a partial row.
+constexpr int kWaveCols = 1536, kTwoRowCols = 2560, kOnePieceCols = 8192;
+int bwd_threads(int64_t cols) {
+  if (cols <= kWaveCols) return 256;
+  const int64_t per_wave = cols <= kOnePieceCols ? 512 : 1024;
+  return 64 * (int)((cols + per_wave - 1) / per_wave);
+}
+int64_t bwd_blocks(int64_t rows, int64_t cols) {
+  if (cols <= kWaveCols) return row_blocks(rows, 4, 512);
+  return cols <= kTwoRowCols ? row_blocks(rows, 2, 512) : row_blocks(rows, 1, 256);
 }
 
 int check_common(const char* who, int64_t rows, int64_t cols, const void* x8, const void* x8_e) {
@@ -350,25 +515,6 @@ int check_common(const char* who, int64_t rows, int64_t cols, const void* x8, co
             "%s: x8 (8-byte aligned) and its block exponents go together", who);
   return BF8_OK;
 }
-
-#define BF8_BY_WIDTH(LAUNCH)                                 \
-  if (cols <= kWaveCols) {                                   \
-    switch ((int)((cols / 8 + 63) / 64)) {                   \
-      case 1: LAUNCH(1, 1); break;                           \
-      case 2: LAUNCH(2, 1); break;                           \
-      case 3: LAUNCH(3, 1); break;                           \
-      case 4: LAUNCH(4, 1); break;                           \
-      default: LAUNCH(5, 1); break;                          \
-    }                                                        \
-  } else {                                                   \
-    if (cols <= 4096) {                                      \
-      LAUNCH(2, 4);                                          \
-    } else if (cols <= 8192) {                               \
-      LAUNCH(1, 16);                                         \
-    } else {                                                 \
-      LAUNCH(2, 16);                                         \
-    }                                                        \
-  }
 
 }  // namespace
 }  // namespace bf8
@@ -391,22 +537,37 @@ int bf8_layernorm_bf16(const void* x, int64_t rows, int64_t cols, const void* we
   p.x = (const uint16_t*)x; p.w = (const uint16_t*)weight; p.b = (const uint16_t*)bias;
   p.rows = rows; p.cols = (int)cols; p.eps = eps;
   p.y = (uint16_t*)y; p.mean = mean; p.rstd = rstd; p.x8 = x8; p.x8_e = x8_exp;
-  const dim3 grid((unsigned)row_blocks(rows, (int)cols, kMaxFwdBlocks));
+  const int pieces = (int)cols / 8;
 #define BF8_LN_FWD(V, W)                                                                               \
-  if (x8)                                                                                              \
-    hipLaunchKernelGGL((layer_norm_kernel<V, W, true>), grid, dim3(block_threads(W)), 0,               \
-                       as_stream(stream), p);                                                          \
-  else                                                                                                 \
-    hipLaunchKernelGGL((layer_norm_kernel<V, W, false>), grid, dim3(block_threads(W)), 0,              \
-                       as_stream(stream), p)
-  BF8_BY_WIDTH(BF8_LN_FWD)
+  {                                                                                                    \
+    const dim3 grid((unsigned)row_blocks(rows, W == 1 ? 4 : 1, kMaxFwdBlocks));                        \
+    if (x8)                                                                                            \
+      hipLaunchKernelGGL((layer_norm_kernel<V, W, true>), grid, dim3(block_threads(W)), 0,             \
+                         as_stream(stream), p);                                                        \
+    else                                                                                               \
+      hipLaunchKernelGGL((layer_norm_kernel<V, W, false>), grid, dim3(block_threads(W)), 0,            \
+                         as_stream(stream), p);                                                        \
+  }
+  // (each is run by the rows it is the narrowest for; few rows of 1,544 .. 2,560 columns: five waves each)
+  if (pieces <= 64) BF8_LN_FWD(1, 1)
+  else if (pieces <= 128) BF8_LN_FWD(2, 1)
+  else if (pieces <= 192) BF8_LN_FWD(3, 1)
+  else if (pieces <= 320 && rows <= kFewRows) BF8_LN_FWD(1, 5)
+  else if (pieces <= 256) BF8_LN_FWD(4, 1)
+  else if (pieces <= 320) BF8_LN_FWD(5, 1)
+  else if (pieces <= 384) BF8_LN_FWD(2, 3)
+  else if (pieces <= 576) BF8_LN_FWD(3, 3)
+  else if (pieces <= 768) BF8_LN_FWD(3, 4)
+  else if (pieces <= 1024) BF8_LN_FWD(4, 4)
+  else if (pieces <= 1536) BF8_LN_FWD(3, 8)
+  else BF8_LN_FWD(4, 8)
 #undef BF8_LN_FWD
   return launch_status("layer_norm_kernel");
 }
 
 size_t bf8_layernorm_bwd_workspace(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0 || cols > kMaxCols) return 0;
-  return (size_t)row_blocks(rows, (int)cols, max_bwd_blocks(cols)) * 2 * (size_t)cols * sizeof(float);
+  return (size_t)bwd_blocks(rows, cols) * 2 * (size_t)cols * sizeof(float);
 }
 
 int bf8_layernorm_bwd_bf16(const void* x, const int8_t* x8, const uint8_t* x8_exp, const void* dy,
@@ -433,16 +594,22 @@ int bf8_layernorm_bwd_bf16(const void* x, const int8_t* x8, const uint8_t* x8_ex
   p.x8 = const_cast<int8_t*>(x8); p.x8_e = const_cast<uint8_t*>(x8_exp);
   p.dy = (const uint16_t*)dy; p.dx = (uint16_t*)dx;
   p.part = wgrad ? (float*)ws : nullptr;
-  const int64_t nb = row_blocks(rows, (int)cols, max_bwd_blocks(cols));
-  const dim3 grid((unsigned)nb);
-#define BF8_LN_BWD(V, W)                                                                               \
-  if (x8)                                                                                              \
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<V, W, true>), grid, dim3(block_threads(W)),              \
-                       W == 1 ? 2 * V * 64 * 16 * sizeof(float) : 0, as_stream(stream), p);            \
-  else                                                                                                 \
-    hipLaunchKernelGGL((layer_norm_bwd_kernel<V, W, false>), grid, dim3(block_threads(W)),             \
-                       W == 1 ? 2 * V * 64 * 16 * sizeof(float) : 0, as_stream(stream), p)
-  BF8_BY_WIDTH(BF8_LN_BWD)
+  const int64_t nb = bwd_blocks(rows, cols);
+  const dim3 grid((unsigned)nb), block(bwd_threads(cols));
+  const hipStream_t st = as_stream(stream);
+#define BF8_LN_BWD(KERNEL, ...)                                                   \
+  {                                                                               \
+    if (x8)                                                                       \
+      hipLaunchKernelGGL((KERNEL<__VA_ARGS__, true>), grid, block, 0, st, p);     \
+    else                                                                          \
+      hipLaunchKernelGGL((KERNEL<__VA_ARGS__, false>), grid, block, 0, st, p);    \
+  }
+  if (cols <= 512) BF8_LN_BWD(layer_norm_bwd_kernel, 1)
+  else if (cols <= 1024) BF8_LN_BWD(layer_norm_bwd_kernel, 2)
+  else if (cols <= kWaveCols) BF8_LN_BWD(layer_norm_bwd_kernel, 3)
+  else if (cols <= kTwoRowCols) BF8_LN_BWD(layer_norm_bwd_block_kernel, 1, 2, false)
+  else if (cols <= kOnePieceCols) BF8_LN_BWD(layer_norm_bwd_block_kernel, 1, 1, true)
+  else BF8_LN_BWD(layer_norm_bwd_block_kernel, 2, 1, true)
 #undef BF8_LN_BWD
   const int rc = launch_status("layer_norm_bwd_kernel");
   if (rc != BF8_OK || !wgrad) return rc;
