@@ -255,4 +255,75 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
   return launch_status("int8_tokens_kernel");
 }
 
+// dy's codes and scales by row and by column, then what the quantization or a product needs.
+namespace {
+int64_t pad16(int64_t rows) { return (rows + 15) / 16 * 16; }
+struct BackwardWs {
+  size_t rows, row_scale, cols, col_scale, rest, bytes;
+};
+BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
+  const int64_t Mp = pad16(M);
+  BackwardWs w{};
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += align256(bytes);
+    return o;
+  };
+  if (dx) {
+    w.rows = take((size_t)M * N);
+    w.row_scale = take((size_t)M * 4);
+  }
+  if (dw) {
+    w.cols = take((size_t)N * Mp);
+    w.col_scale = take((size_t)N * 4);
+  }
+  w.rest = at;
+  size_t rest = dw ? bf8_quantize_int8_workspace(M, N, dx) : 0;
+  if (dx) rest = std::max(rest, bf8_gemm_int8_workspace(M, K, N));
+  if (dw) rest = std::max(rest, bf8_gemm_int8_workspace(N, K, Mp));
+  w.bytes = at + rest;
+  return w;
+}
+}  // namespace
+
+size_t bf8_linear_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int dx, int dw) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return backward_ws(M, N, K, dx != 0, dw != 0).bytes;
+}
+
+int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, const int8_t* Wt,
+                             const float* wt_scale, const int8_t* Xt, const float* xt_scale, void* dx, void* dw,
+                             void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "bf8_linear_int8_backward";
+  BF8_CHECK(M > 0 && N > 0 && K > 0, "%s: empty or negative shape", who);
+  BF8_CHECK(N % 16 == 0 && N <= 32768 && K % 8 == 0 && (!dw || M <= kInt8MaxK),
+            "%s: need N %% 16 == 0, N <= 32768, K %% 8 == 0 and for dw M <= %lld", who, (long long)kInt8MaxK);
+  BF8_CHECK(dx || dw, "%s: nothing requested", who);
+  BF8_CHECK(dy && (!dx || (Wt && wt_scale)) && (!dw || (Xt && xt_scale)), "%s: NULL pointer", who);
+  BF8_CHECK((((uintptr_t)dy | (uintptr_t)Wt | (uintptr_t)wt_scale | (uintptr_t)Xt | (uintptr_t)xt_scale |
+              (uintptr_t)dx | (uintptr_t)dw) & 15) == 0,
+            "%s: every tensor must be 16-byte aligned", who);
+  const int64_t most = std::max(dx ? std::max(M, K) * N : 0, dw ? std::max(N, K) * pad16(M) : 0);
+  BF8_CHECK(M < (1LL << 31) && K < (1LL << 31) && most < (1LL << 31), "%s: operands of 2 GiB and more", who);
+  const BackwardWs w = backward_ws(M, N, K, dx, dw);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
+  int8_t* const base = (int8_t*)ws;
+  int8_t *const rows = dx ? base + w.rows : nullptr, *const cols = dw ? base + w.cols : nullptr;
+  float* const rs = dx ? (float*)(base + w.row_scale) : nullptr;
+  float* const cs = dw ? (float*)(base + w.col_scale) : nullptr;
+  void* const rest = base + w.rest;
+  const size_t rest_bytes = ws_bytes - w.rest;
+  if (const int rc = bf8_quantize_int8_bf16(dy, M, N, rows, rs, cols, cs, rest, rest_bytes, stream)) return rc;
+  if (dx)
+    if (const int rc = bf8_gemm_int8(rows, N, rs, Wt, N, wt_scale, M, K, N, nullptr, dx, BF8_OUT_BF16, K, rest,
+                                     rest_bytes, stream))
+      return rc;
+  if (!dw) return BF8_OK;
+  const int64_t Mp = pad16(M);
+  return bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, N, K, Mp, nullptr, dw, BF8_OUT_BF16, K, rest, rest_bytes,
+                       stream);
+}
+
 }  // extern "C"

@@ -644,11 +644,7 @@ class Int8LinearFunction(_Fp8Function):
         dy = dense_rows(dy)
         dx = dw = None
         if need_dx or need_dw:
-            dyq = ops.quantize_int8(dy, rowwise=need_dx, colwise=need_dw)
-        if need_dx:
-            dx = ops.gemm_int8(dyq.data, dyq.row_scale, w8t, ws)
-        if need_dw:
-            dw = ops.gemm_int8(dyq.data_t, dyq.col_scale, x8t, xs)
+            dx, dw = ops.linear_int8_backward(dy, w8t if need_dx else None, ws, x8t if need_dw else None, xs)
         return dx, dw, ops.column_sums(dy) if need_db else None, None
 
 
@@ -686,12 +682,10 @@ class Int8GegluMlpFunction(_Fp8Function):
     def backward(ctx, dy):
         gu8, gu_exps, x8t, xs, h8t, hs, gu8t, gus, d8t, ds = ctx.saved_tensors
         need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]
-        dyq = ops.quantize_int8(dense_rows(dy), rowwise=need_dx or need_dgu, colwise=need_dd)
-        dx = dgu = dd = None
-        if need_dd:
-            dd = ops.gemm_int8(dyq.data_t, dyq.col_scale, h8t, hs)
+        dx = dgu = None
+        dH, dd = ops.linear_int8_backward(dense_rows(dy), d8t if need_dx or need_dgu else None, ds,
+                                          h8t if need_dd else None, hs)
         if need_dx or need_dgu:
-            dH = ops.gemm_int8(dyq.data, dyq.row_scale, d8t, ds)
             dq = ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(gu8, gu_exps), rowwise=need_dx,
                                       colwise=need_dgu)
             if need_dx:

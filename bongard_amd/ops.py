@@ -1713,6 +1713,46 @@ def linear_int8(x, w, w_scale, *, bias=None, out_dtype=torch.bfloat16):
     return out if len(shape) == 2 else out.view(*shape[:-1], N)
 
 
+@functools.lru_cache(maxsize=4096)
+def _linear_int8_backward_ws_cached(M, N, K, dx, dw):
+    return int(_lib.lib().bf8_linear_int8_backward_workspace(M, N, K, dx, dw))
+
+
+def linear_int8_backward(dy, w_t=None, w_t_scale=None, x_t=None, x_t_scale=None):
+    """Gradients ``(dx, dw)`` of an int8 linear for bf16 ``dy`` [M, N] in one call: ``dy`` quantized by token
+    for dx [M, K], the product with ``w_t`` [K, N] (W's columnwise codes, scales ``w_t_scale`` [K]), and by
+    channel for dw [N, K], the product with ``x_t`` [K, M rounded up to 16] (x's, ``x_t_scale`` [K]). Without
+    ``w_t`` (``x_t``) dx (dw) is None. The values are :func:`quantize_int8`'s and :func:`gemm_int8`'s. N a
+    multiple of 16, K of 8."""
+    who = "linear_int8_backward"
+    idx = _index_of(who, dy, w_t, w_t_scale, x_t, x_t_scale)
+    dy = _rows_bf16(dy)
+    M, N = dy.shape
+    if w_t is None and x_t is None:
+        raise ValueError(f"{who}: nothing requested")
+    K = (x_t if w_t is None else w_t).shape[0]
+    for name, t, scale, cols in (("w_t", w_t, w_t_scale, N), ("x_t", x_t, x_t_scale, (M + 15) // 16 * 16)):
+        if t is None:
+            continue
+        if t.dtype is not torch.int8 or t.shape != (K, cols) or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} must be contiguous int8 [{K}, {cols}] (got {t.dtype} "
+                             f"{tuple(t.shape)})")
+        if scale is None or scale.dtype is not torch.float32 or scale.shape != (K,) or not scale.is_contiguous():
+            raise ValueError(f"{who}: {name}_scale must be contiguous float32 [{K}]")
+    dx = None if w_t is None else torch.empty((M, K), dtype=torch.bfloat16, device=dy.device)
+    dw = None if x_t is None else torch.empty((N, K), dtype=torch.bfloat16, device=dy.device)
+    if not (M and N and K):  # sums of nothing
+        for t in (dx, dw):
+            if t is not None:
+                t.zero_()
+        return dx, dw
+    L = _lib.lib()
+    ws, nbytes = _call_workspace(_linear_int8_backward_ws_cached(M, N, K, dx is not None, dw is not None), dy)
+    _call("bf8_linear_int8_backward", idx, L.bf8_linear_int8_backward, dy.data_ptr(), M, N, K, _ptr(w_t),
+          _ptr(w_t_scale), _ptr(x_t), _ptr(x_t_scale), _ptr(dx), _ptr(dw), ws.data_ptr(), nbytes)
+    return dx, dw
+
+
 @dataclass
 class MxInt8Tensor:
     """An 8-bit checkpoint of a bf16 tensor [rows, cols]: ``data`` int8 [rows, cols] and ``exps`` uint8

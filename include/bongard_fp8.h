@@ -661,6 +661,17 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
                     int64_t N, int64_t K, const void* bias, void* C, int out_dtype, int64_t ldc,
                     void* ws, size_t ws_bytes, void* stream);
 
+/* The backward of a linear layer in int8 from dy bf16 [M, N]: dy quantized by row and by column as
+ * bf8_quantize_int8_bf16 does, then dx [M, K] = dy . Wt^T (Wt int8 [K, N], the columnwise copy of W, scales
+ * wt_scale [K]) and dw [N, K] = dy^T . Xt^T (Xt int8 [K, M rounded up to 16], the columnwise copy of x,
+ * xt_scale [K]), the products bf8_gemm_int8's; bf16. dx or dw may be NULL (with its operand). N a multiple
+ * of 16, 32768 at most, K of 8; M, N, K > 0, for dw M 133120 at most. ws:
+ * bf8_linear_int8_backward_workspace(M, N, K, dx?, dw?) bytes, 256-byte aligned. */
+size_t bf8_linear_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int dx, int dw);
+int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, const int8_t* Wt,
+                             const float* wt_scale, const int8_t* Xt, const float* xt_scale, void* dx,
+                             void* dw, void* ws, size_t ws_bytes, void* stream);
+
 /* The gate/up product of int8 operands X [M, K] and W [2 I, K] (gate rows then up rows) with the
  * gated GELU (TEMLP's chain, bongard/te_linear.py:98-103): H bf16 [M, I], and where GU8 is given
  * the checkpoint of the bf16 pre-activations [M, 2 I] as bf8_quantize_mxint8_bf16 writes it.

@@ -466,6 +466,33 @@ def test_linear_function(gpu, M, N, K):
     assert bool(((leaves[2].grad.cpu().double() - want).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 16, 8), (17, 32, 264), (333, 4112, 40), (1000, 1024, 512), (2049, 64, 2048),
+                                   (64, 8208, 72)])
+def test_linear_backward_is_its_parts(gpu, M, N, K):
+    """Both gradients in one call and each alone: the quantizer's copies of dy through the products, bit for bit."""
+    x, w, dy = (_x(*s, 7, False).to(gpu) for s in ((M, K), (N, K), (M, N)))
+    xq, wq = (ops.quantize_int8(t, rowwise=False, colwise=True) for t in (x, w))
+    q = ops.quantize_int8(dy, colwise=True)
+    dx = ops.gemm_int8(q.data, q.row_scale, wq.data_t, wq.col_scale)
+    dw = ops.gemm_int8(q.data_t, q.col_scale, xq.data_t, xq.col_scale)
+    wt, xt = (wq.data_t, wq.col_scale), (xq.data_t, xq.col_scale)
+    got = ops.linear_int8_backward(dy, *wt, *xt)
+    assert torch.equal(got[0], dx) and torch.equal(got[1], dw)
+    wide = torch.zeros(M, N + 8, dtype=BF16, device=gpu)[:, 8:].copy_(dy)  # (its rows are copied)
+    got = ops.linear_int8_backward(wide, *wt)
+    assert torch.equal(got[0], dx) and got[1] is None
+    got = ops.linear_int8_backward(dy, x_t=xt[0], x_t_scale=xt[1])
+    assert got[0] is None and torch.equal(got[1], dw)
+    with pytest.raises(ValueError, match="w_t must be"):
+        ops.linear_int8_backward(dy, wq.data_t[:, :-16] if N > 16 else wq.data_t.t(), wt[1])
+    with pytest.raises(ValueError, match="x_t_scale"):
+        ops.linear_int8_backward(dy, *wt, xt[0], None)
+    with pytest.raises(ValueError, match="nothing requested"):
+        ops.linear_int8_backward(dy)
+    dx, dw = ops.linear_int8_backward(dy[:0], *wt, xt[0][:, :0].contiguous(), xt[1])
+    assert dx.shape == (0, K) and not bool(dw.any()) and dw.shape == (N, K)
+
+
 def test_linear_gradients_are_the_differences(gpu):
     """On whole values up to 127 with a 127 in every row and column the layer is exactly bilinear:
     y(x + d) - y(x) is what the gradient says."""

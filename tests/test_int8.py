@@ -115,7 +115,21 @@ def _calls(L):
     f, b = L.bf8_geglu_mxint8, L.bf8_geglu_bwd_mxint8
     t, qm = L.bf8_linear_int8, L.bf8_quantize_int8_maxima_bf16
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
+    lb, mb = L.bf8_linear_int8_backward, 1 << 20
     return [
+        (lb, (p, 0, 16, 16, p, p, p, p, p, p, p, mb, null), "empty"),
+        (lb, (p, 4, 24, 16, p, p, p, p, p, p, p, mb, null), "N % 16"),
+        (lb, (p, 4, 32784, 16, p, p, p, p, p, p, p, mb, null), "32768"),
+        (lb, (p, 4, 16, 12, p, p, p, p, p, p, p, mb, null), "K % 8"),
+        (lb, (p, 133121, 16, 16, p, p, p, p, p, p, p, mb, null), "133120"),
+        (lb, (p, 4, 16, 16, p, p, p, p, null, null, p, mb, null), "nothing requested"),
+        (lb, (p, 4, 16, 16, null, p, p, p, p, p, p, mb, null), "NULL"),
+        (lb, (p, 4, 16, 16, p, p, p, null, p, p, p, mb, null), "NULL"),
+        (lb, (p, 4, 16, 16, p, p, p, odd, p, p, p, mb, null), "16-byte"),
+        (lb, (p, 66000, 32768, 16, p, p, null, null, p, null, p, mb, null), "2 GiB"),
+        (lb, (p, 100000, 32768, 16, p, p, p, p, p, p, p, mb, null), "2 GiB"),
+        (lb, (p, 4, 16, 16, p, p, p, p, p, p, p, 64, null), "workspace needs"),
+        (lb, (p, 4, 16, 16, p, p, p, p, p, p, null, 0, null), "workspace needs"),
         (q, (p, 4, 12, p, p, null, null, null, 0, null), "cols % 8"),
         (q, (p, 4, 32776, p, p, null, null, null, 0, null), "32768"),
         (q, (p, -1, 16, p, p, null, null, null, 0, null), "bad shape"),
