@@ -628,6 +628,9 @@ class Int8LinearFunction(_Fp8Function):
     def forward(ctx, x, weight, bias, wq):
         need_dx, need_dw = _forward_needs(ctx, 2)
         _check_int8("int8 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
+        if wq is not None and not (need_dx or need_dw):  # (the same product; few tokens take one kernel)
+            ctx.save_for_backward(None, None, None, None)
+            return ops.linear_int8(dense_rows(x), wq.data, wq.row_scale, bias=bias)
         xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dw)
         if wq is None or (need_dx and wq.data_t is None):
             wq = quantize_weight_int8(weight, transpose=need_dx)
@@ -663,6 +666,8 @@ class Int8GegluMlpFunction(_Fp8Function):
         need_dx, need_dgu, need_dd = _forward_needs(ctx, 3)
         keep = need_dx or need_dgu
         _check_int8("int8 gated MLP", x.shape[-1], *([w_down.shape[0]] if keep or need_dd else []))
+        if gu_q is not None and down_q is not None and not (keep or need_dd):
+            return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
         xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dgu)
         if gu_q is None or (need_dx and gu_q.data_t is None):
             gu_q = quantize_weight_int8(w_gu, transpose=need_dx)

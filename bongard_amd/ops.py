@@ -1834,15 +1834,40 @@ def gemm_geglu_int8(x, x_scale, w, w_scale, intermediate, *, keep_gu=False):
     return H, gu
 
 
+def linear_geglu_int8(x, w, w_scale):
+    """A gate/up projection of int8 weights in serving with the gated GELU: H bf16 [..., I] of bf16 x [..., K]
+    quantized by token in the call and W as codes [2I, K] (gate rows then up rows) under ``w_scale`` [2I], as
+    :func:`gemm_geglu_int8` computes it. I a multiple of 128. No gradients
+    (:class:`bongard_amd.linear.Int8GegluMlpFunction` has them)."""
+    who = "linear_geglu_int8"
+    idx = _index_of(who, x, w, w_scale)
+    _int8_matrix(who, w=w)
+    shape = x.shape
+    N, K = w.shape
+    if shape[-1] != K:
+        raise ValueError(f"{who}: inner dims differ ({shape[-1]} vs {K})")
+    if N % 256 or K == 0:
+        raise ValueError(f"{who}: the intermediate size must be a multiple of 128 and K not 0 (got {tuple(w.shape)})")
+    I = N // 2
+    w_scale = _int8_scale(who, "w_scale", w_scale, N)
+    x = _rows_bf16(x)
+    M = x.shape[0]
+    out = torch.empty((M, I), dtype=torch.bfloat16, device=x.device)
+    if M and I:
+        L, ws = _lib.lib(), None
+        ws_bytes = L.bf8_linear_geglu_int8_workspace(M, I, K)
+        if ws_bytes:
+            ws, ws_bytes = _call_workspace(ws_bytes, x)
+        _call("bf8_linear_geglu_int8", idx, L.bf8_linear_geglu_int8, x.data_ptr(), w.data_ptr(), w.stride(0),
+              w_scale.data_ptr(), M, I, K, out.data_ptr(), _ptr(ws), ws_bytes)
+    return out if len(shape) == 2 else out.view(*shape[:-1], I)
+
+
 def geglu_mlp_int8(x, w_gu, w_gu_scale, w_down, w_down_scale):
     """The gated MLP of int8 weights in serving: bf16 x [..., K], W_gu as codes [2I, K] (gate rows then
     up rows) and W_down [N, I], each with its scales; x and the activation are quantized by token in the
     call. No gradients (:class:`bongard_amd.linear.Int8GegluMlpFunction` has them)."""
-    shape = x.shape
-    q = quantize_int8(x)
-    H, _ = gemm_geglu_int8(q.data, q.row_scale, w_gu, w_gu_scale, w_gu.shape[0] // 2)
-    y = linear_int8(H, w_down, w_down_scale)
-    return y if len(shape) == 2 else y.view(*shape[:-1], y.shape[-1])
+    return linear_int8(linear_geglu_int8(x, w_gu, w_gu_scale), w_down, w_down_scale)
 
 
 def geglu_mxint8(GU):

@@ -661,6 +661,13 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
                     int64_t N, int64_t K, const void* bias, void* C, int out_dtype, int64_t ldc,
                     void* ws, size_t ws_bytes, void* stream);
 
+/* The gate/up projection of int8 weights W [2 I, K] (gate rows then up rows) on bf16 x [M, K] with the gated
+ * GELU: x quantized by row, then bf8_gemm_geglu_int8's H (few rows take one kernel). I a multiple of 128, K of
+ * 16, 32768 at most. ws: bf8_linear_geglu_int8_workspace(M, I, K) bytes, 256-byte aligned. */
+size_t bf8_linear_geglu_int8_workspace(int64_t M, int64_t I, int64_t K);
+int bf8_linear_geglu_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_scale, int64_t M,
+                          int64_t I, int64_t K, void* H, void* ws, size_t ws_bytes, void* stream);
+
 /* The backward of a linear layer in int8 from dy bf16 [M, N]: dy quantized by row and by column as
  * bf8_quantize_int8_bf16 does, then dx [M, K] = dy . Wt^T (Wt int8 [K, N], the columnwise copy of W, scales
  * wt_scale [K]) and dw [N, K] = dy^T . Xt^T (Xt int8 [K, M rounded up to 16], the columnwise copy of x,

@@ -269,6 +269,33 @@ def test_linear_of_no_tokens_and_wide_rows_of_weights(gpu):
         _check_product(y, ref, ref, F32)
 
 
+@pytest.mark.parametrize("M", [1, 2, 5, 16, 17, 32, 33, 200])
+@pytest.mark.parametrize("I,K", [(128, 16), (256, 1792), (10240, 2560), (128, 8208), (384, 272)])
+def test_tokens_through_a_gated_projection(gpu, M, I, K):
+    """The gated product of the quantizer's codes, bit for bit, whichever kernel runs it: small and large gates, zeros,
+    a token of inf."""
+    x, w = _x(M, K, M + I, spread=False), _x(2 * I, K, K, spread=False)
+    w[:I] *= torch.logspace(-6, 2, I)[:, None].to(BF16)
+    w[3] = 0
+    wq = ops.quantize_int8(w.to(gpu))
+    for bad in (False, True):
+        if bad:
+            x[M - 1, K // 2] = float("inf")
+        q = ops.quantize_int8(x.to(gpu))
+        want, _ = ops.gemm_geglu_int8(q.data, q.row_scale, wq.data, wq.row_scale, I)
+        got = ops.linear_geglu_int8(x.to(gpu).view(M, 1, K), wq.data, wq.row_scale)
+        assert tuple(got.shape) == (M, 1, I)
+        assert torch.equal(got.view(M, I).view(torch.int16), want.view(torch.int16))
+        assert bool(torch.isnan(got[M - 1]).all()) == bad
+    wide = torch.full((2 * I, K + 16), 99, dtype=torch.int8, device=gpu)
+    wide[:, :K] = wq.data
+    assert torch.equal(ops.linear_geglu_int8(x[:M - 1].to(gpu), wide[:, :K], wq.row_scale), want[:M - 1])
+    with pytest.raises(ValueError, match="multiple of 128"):
+        ops.linear_geglu_int8(x.to(gpu), wq.data[:64], wq.row_scale[:64])
+    with pytest.raises(ValueError, match="inner dims"):
+        ops.linear_geglu_int8(x.to(gpu)[:, :8], wq.data, wq.row_scale)
+
+
 # ---- checkpoints -------------------------------------------------------------------------------
 def _check_ckpt(q, x):
     codes, e = i8.checkpoint(x)
@@ -464,6 +491,25 @@ def test_linear_function(gpu, M, N, K):
     want = dy.double().sum(0)
     tol = 2.0 ** -8 * want.abs() + (M + 64) * 2.0 ** -24 * dy.double().abs().sum(0)
     assert bool(((leaves[2].grad.cpu().double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("M", [1, 20, 100])
+def test_functions_without_gradients(gpu, M):
+    """Under no_grad with cached weights few tokens take the kernels of serving: the values of the forward that
+    keeps for a backward. A bias that alone is trained has its gradient."""
+    x, w, w_gu, w_d = (_x(*s, 7, False).to(gpu) for s in ((M, 256), (96, 256), (512, 256), (64, 256)))
+    bias = _x(1, 96, 4, False)[0].to(gpu).requires_grad_()
+    wq, gq, dq = (linear.quantize_weight_int8(t) for t in (w, w_gu, w_d))
+    leaf = x.clone().requires_grad_()
+    want = linear.Int8LinearFunction.apply(leaf, w, bias, wq)
+    mlp = linear.Int8GegluMlpFunction.apply(leaf, w_gu, w_d, gq, dq, 256)
+    with torch.no_grad():
+        assert torch.equal(linear.Int8LinearFunction.apply(leaf, w, bias, wq), want)
+        assert torch.equal(linear.Int8GegluMlpFunction.apply(leaf, w_gu, w_d, gq, dq, 256), mlp)
+    y = linear.Int8LinearFunction.apply(x, w, bias, wq)
+    assert torch.equal(y, want)
+    y.backward(torch.ones_like(y))
+    assert torch.equal(bias.grad, torch.full_like(bias, M))
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 16, 8), (17, 32, 264), (333, 4112, 40), (1000, 1024, 512), (2049, 64, 2048),

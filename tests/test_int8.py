@@ -116,7 +116,16 @@ def _calls(L):
     t, qm = L.bf8_linear_int8, L.bf8_quantize_int8_maxima_bf16
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
     lb, mb = L.bf8_linear_int8_backward, 1 << 20
+    lg = L.bf8_linear_geglu_int8
     return [
+        (lg, (p, p, 32, p, 4, 64, 32, p, null, 0, null), "I % 128"),
+        (lg, (p, p, 24, p, 4, 128, 24, p, null, 0, null), "K % 16"),
+        (lg, (p, p, 32784, p, 4, 128, 32784, p, null, 0, null), "32768"),
+        (lg, (p, p, 16, p, 4, 128, 32, p, null, 0, null), "row stride"),
+        (lg, (odd, p, 32, p, 4, 128, 32, p, null, 0, null), "16-byte"),
+        (lg, (p, null, 32, p, 4, 128, 32, p, null, 0, null), "NULL"),
+        (lg, (p, p, 32, p, 4, 128, 0, p, null, 0, null), "K == 0"),
+        (lg, (p, p, 32, p, 40, 128, 32, p, null, 0, null), "workspace needs"),
         (lb, (p, 0, 16, 16, p, p, p, p, p, p, p, mb, null), "empty"),
         (lb, (p, 4, 24, 16, p, p, p, p, p, p, p, mb, null), "N % 16"),
         (lb, (p, 4, 32784, 16, p, p, p, p, p, p, p, mb, null), "32768"),
