@@ -24,8 +24,10 @@ constexpr int kStep = 64;        // K bytes of an MFMA
 // workgroup a CU, 20 us at I 10240, K 2560 instead of 15).
 constexpr int kAheadLinear = 5, kAheadGated = 3;
 constexpr int kMaxTokens = 32;
-constexpr int64_t kMaxCodes = 57344;  // LDS bytes of the tokens' codes (two workgroups a CU)
-constexpr int64_t kMaxBlocks = 2 * kNumCus;
+// LDS bytes of the tokens' codes up to which one kernel is the faster: linear 32 x 2560 x 2560 10.1 us (quantizer and
+// GEMM 13.8), 8 x 2560 x 10240 16.0 (20.5), but 16 x 10240 x 6144 27.3 (23.1); gated 12 x 10240 x 10240 40 (52), but
+// 32 x 20480 x 4096 37 (31).
+constexpr int64_t kMaxCodes = 81920, kMaxCodesGated = 122880;
 
 struct Tokens {
   const uint16_t* x;  // [M, K]
@@ -88,10 +90,13 @@ __global__ __launch_bounds__(kNT, 4) void int8_tokens_kernel(Tokens p) {
     if (!GATED && p.bias) wb = *reinterpret_cast<const uint2*>(p.bias + n);
   };
   // the tokens' codes: `share` waves a token, the row's 16-byte vectors spread over their lanes; the next
-  // token's first kHold of a lane are loaded before this one's maximum is known
-  const int share = p.M >= 5 ? 1 : p.M >= 3 ? 2 : p.M == 2 ? 4 : 8;
-  const int nvec = p.K >> 3, first = 64 * (wid & (share - 1)) + lane;
+  // token's first kHold of a lane are loaded before this one's maximum is known. More waves share a long row: one
+  // each takes 8 x 2560 x 10240 from 16 to 19 us
   constexpr int kHold = 5;
+  const int nvec = p.K >> 3;
+  int share = p.M >= 5 ? 1 : p.M >= 3 ? 2 : p.M == 2 ? 4 : 8;
+  while (share < kWaves && nvec > 64 * kHold * share) share *= 2;
+  const int first = 64 * (wid & (share - 1)) + lane;
   auto row = [&](int t) __attribute__((always_inline)) {
     return window(p.x + (int64_t)t * p.K, t < p.M ? 2u * p.K : 0u);
   };
@@ -236,10 +241,22 @@ __global__ __launch_bounds__(kNT, 4) void int8_tokens_kernel(Tokens p) {
 }
 
 int64_t token_steps(int64_t K) { return (K + kStep - 1) / kStep; }
-bool one_kernel(int64_t M, int64_t K) {
-  return M <= kMaxTokens && M * token_steps(K) * kStep <= kMaxCodes;
+int64_t code_bytes(int64_t M, int64_t K) { return M * token_steps(K) * kStep; }
+bool one_kernel(int64_t M, int64_t K, bool gated) {
+  return M <= kMaxTokens && code_bytes(M, K) <= (gated ? kMaxCodesGated : kMaxCodes);
 }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// LDS bytes of a workgroup: the codes, the waves' sums, the table.
+int64_t lds_bytes(const Tokens& p, bool gated) {
+  return code_bytes(p.M, p.K) + (p.M <= 16 ? 8352 : 16544) + (gated ? kGeluABytes : 0);
+}
+// Two workgroups a CU; one where the LDS holds no second and a long row's quantization takes more than the evener
+// share of the groups gives back (8 x 10240 x 10240 30.9 us, by twice the workgroups 37.6; 32 x 10240 x 2560 17.0
+// and 15.4).
+int64_t max_blocks(const Tokens& p, bool gated) {
+  return 2 * lds_bytes(p, gated) > 160 * 1024 && p.K >= 4096 ? kNumCus : 2 * kNumCus;
+}
 
 // What a split of K over `split` waves costs beside what all of them do (us): on the busiest CU its one or two
 // workgroups, which quantize the tokens each, and the sets of groups that they take one after another, by their
@@ -248,7 +265,7 @@ int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // waves as there are steps for, 10% and 62% (1 x 8192 x 1024: 6.2 us, in four 5.3; 16 x 20480 x 2560: 14.9, in four
 // 15.1, in two 17.5).
 double split_cost(const Tokens& p, int split, bool gated) {
-  const int64_t sets = cdiv(p.groups, kWaves / split), blocks = std::min(sets, kMaxBlocks);
+  const int64_t sets = cdiv(p.groups, kWaves / split), blocks = std::min(sets, max_blocks(p, gated));
   const bool two = blocks > kNumCus;
   const int64_t on_cu = cdiv(sets, blocks) + (two ? cdiv(sets - kNumCus, blocks) : 0);
   const int64_t batches = cdiv(cdiv(p.steps, split), gated ? kAheadGated : kAheadLinear);
@@ -274,8 +291,8 @@ Tokens tokens(const void* x, const int8_t* W, int64_t ldw, const float* w_scale,
   }
   return p;
 }
-dim3 token_grid(const Tokens& p) {
-  return dim3((unsigned)std::min<int64_t>(cdiv(p.groups, kWaves / p.split), kMaxBlocks));
+dim3 token_grid(const Tokens& p, bool gated) {
+  return dim3((unsigned)std::min<int64_t>(cdiv(p.groups, kWaves / p.split), max_blocks(p, gated)));
 }
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
@@ -287,7 +304,7 @@ using namespace bf8;
 extern "C" {
 
 size_t bf8_linear_int8_workspace(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || one_kernel(M, K)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || one_kernel(M, K, false)) return 0;
   return align256((size_t)M * K) + align256((size_t)M * 4) + bf8_gemm_int8_workspace(M, N, K);
 }
 
@@ -309,7 +326,7 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
   if (M == 0 || N == 0) return BF8_OK;
   BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
   BF8_CHECK(x && W && w_scale && C, "%s: NULL pointer", who);
-  if (!one_kernel(M, K)) {
+  if (!one_kernel(M, K, false)) {
     const size_t head = align256((size_t)M * K) + align256((size_t)M * 4);
     BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= head,
               "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who,
@@ -325,12 +342,12 @@ int bf8_linear_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_
   const bool f32 = out_dtype == BF8_OUT_F32;
   const auto kernel = M <= 16 ? (f32 ? int8_tokens_kernel<1, true> : int8_tokens_kernel<1, false>)
                               : (f32 ? int8_tokens_kernel<2, true> : int8_tokens_kernel<2, false>);
-  hipLaunchKernelGGL(kernel, token_grid(p), dim3(kNT), (size_t)p.M * p.steps * kStep, as_stream(stream), p);
+  hipLaunchKernelGGL(kernel, token_grid(p, false), dim3(kNT), (size_t)p.M * p.steps * kStep, as_stream(stream), p);
   return launch_status("int8_tokens_kernel");
 }
 
 size_t bf8_linear_geglu_int8_workspace(int64_t M, int64_t I, int64_t K) {
-  if (M <= 0 || I <= 0 || K <= 0 || one_kernel(M, K)) return 0;
+  if (M <= 0 || I <= 0 || K <= 0 || one_kernel(M, K, true)) return 0;
   return align256((size_t)M * K) + align256((size_t)M * 4);
 }
 
@@ -348,7 +365,7 @@ int bf8_linear_geglu_int8(const void* x, const int8_t* W, int64_t ldw, const flo
   if (M == 0 || I == 0) return BF8_OK;
   BF8_CHECK(K > 0, "%s: K == 0 is not supported", who);
   BF8_CHECK(x && W && w_scale && H, "%s: NULL pointer", who);
-  if (!one_kernel(M, K)) {
+  if (!one_kernel(M, K, true)) {
     const size_t need = bf8_linear_geglu_int8_workspace(M, I, K);
     BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= need,
               "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, need, ws_bytes);
@@ -359,7 +376,7 @@ int bf8_linear_geglu_int8(const void* x, const int8_t* W, int64_t ldw, const flo
   }
   const Tokens p = tokens(x, W, ldw, w_scale, M, I, K, nullptr, H, I, true);
   const auto kernel = M <= 16 ? int8_tokens_kernel<1, false, true> : int8_tokens_kernel<2, false, true>;
-  hipLaunchKernelGGL(kernel, token_grid(p), dim3(kNT), (size_t)p.M * p.steps * kStep, as_stream(stream), p);
+  hipLaunchKernelGGL(kernel, token_grid(p, true), dim3(kNT), (size_t)p.M * p.steps * kStep, as_stream(stream), p);
   return launch_status("int8_tokens_kernel(gated)");
 }
 

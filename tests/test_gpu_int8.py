@@ -240,7 +240,8 @@ def test_product_special_rows(gpu):
 
 
 @pytest.mark.parametrize("M", [1, 2, 3, 5, 8, 15, 16, 17, 31, 32, 33, 64, 65])
-@pytest.mark.parametrize("N,K", [(2048, 2560), (40, 16), (2560, 10240), (1032, 272), (8, 4112)])
+@pytest.mark.parametrize("N,K", [(2048, 2560), (40, 16), (2560, 10240), (1032, 272), (8, 4112), (4104, 5120),
+                                 (200, 20496), (6160, 640)])
 def test_tokens_through_a_linear(gpu, M, N, K):
     """x quantized in the call: the product of the quantizer's codes, whichever kernel runs it."""
     x, b = _x(M, K, M + K), _operand(N, K, N, gpu, spread=False)
@@ -269,8 +270,9 @@ def test_linear_of_no_tokens_and_wide_rows_of_weights(gpu):
         _check_product(y, ref, ref, F32)
 
 
-@pytest.mark.parametrize("M", [1, 2, 5, 16, 17, 32, 33, 200])
-@pytest.mark.parametrize("I,K", [(128, 16), (256, 1792), (10240, 2560), (128, 8208), (384, 272)])
+@pytest.mark.parametrize("M", [1, 2, 5, 15, 16, 17, 32, 33, 200])
+@pytest.mark.parametrize("I,K", [(128, 16), (256, 1792), (10240, 2560), (128, 8208), (384, 272), (4608, 4096),
+                                 (128, 20496)])
 def test_tokens_through_a_gated_projection(gpu, M, I, K):
     """The gated product of the quantizer's codes, bit for bit, whichever kernel runs it: small and large gates, zeros,
     a token of inf."""
