@@ -610,9 +610,19 @@ def _check_int8(who, *dims):
                          f"(got {list(dims)})")
 
 
+# An int8 weight gradient sums a term for each token in int32: * 127^2 < 2^31.
+_INT8_MAX_TOKENS = 133120
+
+
+def _check_int8_tokens(who, rows):
+    if rows > _INT8_MAX_TOKENS:
+        raise ValueError(f"{who}: a weight gradient takes {_INT8_MAX_TOKENS} tokens at most (got {rows})")
+
+
 class Int8LinearFunction(_Fp8Function):
     """y = x @ W^T (+ b) with every tensor in 8-bit integers, one scale for each token or channel
-    (gradients included; round to nearest even), sums exact in int32; x: bf16 [M, K], any M; W [N, K],
+    (gradients included; round to nearest even), sums exact in int32; x: bf16 [M, K], any M (133120 at most
+    where W's gradient is asked for); W [N, K],
     K a multiple of 16, N of 8 (of 16 for gradients). ``wq``: a cached int8 weight
     (:func:`quantize_weight_int8`) or None.
 
@@ -628,6 +638,8 @@ class Int8LinearFunction(_Fp8Function):
     def forward(ctx, x, weight, bias, wq):
         need_dx, need_dw = _forward_needs(ctx, 2)
         _check_int8("int8 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
+        if need_dw:
+            _check_int8_tokens("int8 linear", x.shape[0])
         if wq is not None and not (need_dx or need_dw):  # (the same product; few tokens take one kernel)
             ctx.save_for_backward(None, None, None, None)
             return ops.linear_int8(dense_rows(x), wq.data, wq.row_scale, bias=bias)
@@ -656,8 +668,8 @@ class Int8GegluMlpFunction(_Fp8Function):
     (:class:`Int8LinearFunction`'s granularity) and the pre-activations kept for the backward as an
     8-bit checkpoint, half the bytes of bf16: the gate/up product with the gated GELU and the checkpoint
     in its epilogue, the down product; backward through dH, the gelu chain on the checkpoint's values and
-    the dgrad/wgrad products. x: bf16 [M, K], any M; w_gu [2I, K], w_down [K_out, I], K and K_out
-    multiples of 16, I of 128. ``gu_q`` / ``down_q``: optional cached int8 weights. TEMLP / FusedMLP under
+    the dgrad/wgrad products. x: bf16 [M, K], any M (133120 at most where a weight's gradient is asked
+    for); w_gu [2I, K], w_down [K_out, I], K and K_out multiples of 16, I of 128. ``gu_q`` / ``down_q``: optional cached int8 weights. TEMLP / FusedMLP under
     'int8' (bongard/te_linear.py:98-103, bongard/fused_mlp.py:25-33 for the chain)."""
 
     @staticmethod
@@ -666,6 +678,8 @@ class Int8GegluMlpFunction(_Fp8Function):
         need_dx, need_dgu, need_dd = _forward_needs(ctx, 3)
         keep = need_dx or need_dgu
         _check_int8("int8 gated MLP", x.shape[-1], *([w_down.shape[0]] if keep or need_dd else []))
+        if need_dgu or need_dd:
+            _check_int8_tokens("int8 gated MLP", x.shape[0])
         if gu_q is not None and down_q is not None and not (keep or need_dd):
             return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
         xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dgu)

@@ -1723,7 +1723,7 @@ def linear_int8_backward(dy, w_t=None, w_t_scale=None, x_t=None, x_t_scale=None)
     for dx [M, K], the product with ``w_t`` [K, N] (W's columnwise codes, scales ``w_t_scale`` [K]), and by
     channel for dw [N, K], the product with ``x_t`` [K, M rounded up to 16] (x's, ``x_t_scale`` [K]). Without
     ``w_t`` (``x_t``) dx (dw) is None. The values are :func:`quantize_int8`'s and :func:`gemm_int8`'s. N a
-    multiple of 16, K of 8."""
+    multiple of 16, K of 8; for dw M at most 133120."""
     who = "linear_int8_backward"
     idx = _index_of(who, dy, w_t, w_t_scale, x_t, x_t_scale)
     dy = _rows_bf16(dy)
@@ -1731,14 +1731,19 @@ def linear_int8_backward(dy, w_t=None, w_t_scale=None, x_t=None, x_t_scale=None)
     if w_t is None and x_t is None:
         raise ValueError(f"{who}: nothing requested")
     K = (x_t if w_t is None else w_t).shape[0]
-    for name, t, scale, cols in (("w_t", w_t, w_t_scale, N), ("x_t", x_t, x_t_scale, (M + 15) // 16 * 16)):
+
+    def operand(name, t, scale, cols):
         if t is None:
-            continue
-        if t.dtype is not torch.int8 or t.shape != (K, cols) or not t.is_contiguous():
-            raise ValueError(f"{who}: {name} must be contiguous int8 [{K}, {cols}] (got {t.dtype} "
-                             f"{tuple(t.shape)})")
-        if scale is None or scale.dtype is not torch.float32 or scale.shape != (K,) or not scale.is_contiguous():
-            raise ValueError(f"{who}: {name}_scale must be contiguous float32 [{K}]")
+            return None, None
+        if t.dtype is not torch.int8 or t.shape != (K, cols):
+            raise ValueError(f"{who}: {name} must be int8 [{K}, {cols}] (got {t.dtype} {tuple(t.shape)})")
+        if scale is None:
+            raise ValueError(f"{who}: {name} needs {name}_scale")
+        t = t.contiguous()
+        return t if t.data_ptr() % 16 == 0 else t.clone(), _int8_scale(who, f"{name}_scale", scale, K)
+
+    w_t, w_t_scale = operand("w_t", w_t, w_t_scale, N)
+    x_t, x_t_scale = operand("x_t", x_t, x_t_scale, (M + 15) // 16 * 16)
     dx = None if w_t is None else torch.empty((M, K), dtype=torch.bfloat16, device=dy.device)
     dw = None if x_t is None else torch.empty((N, K), dtype=torch.bfloat16, device=dy.device)
     if not (M and N and K):  # sums of nothing

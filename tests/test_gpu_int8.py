@@ -531,9 +531,15 @@ def test_linear_backward_is_its_parts(gpu, M, N, K):
     assert torch.equal(got[0], dx) and got[1] is None
     got = ops.linear_int8_backward(dy, x_t=xt[0], x_t_scale=xt[1])
     assert got[0] is None and torch.equal(got[1], dw)
+    far = torch.empty(K + 1, device=gpu)[1:].copy_(wt[1])  # (off its alignment)
+    rows = torch.zeros(K, N + 16, dtype=torch.int8, device=gpu)[:, 16:].copy_(wt[0])
+    got = ops.linear_int8_backward(dy, rows, far, x_t_scale=far)
+    assert torch.equal(got[0], dx) and got[1] is None
     with pytest.raises(ValueError, match="w_t must be"):
-        ops.linear_int8_backward(dy, wq.data_t[:, :-16] if N > 16 else wq.data_t.t(), wt[1])
-    with pytest.raises(ValueError, match="x_t_scale"):
+        ops.linear_int8_backward(dy, wq.data_t[:, :-8], wt[1])
+    with pytest.raises(ValueError, match="w_t_scale"):
+        ops.linear_int8_backward(dy, wt[0], wt[1][1:])
+    with pytest.raises(ValueError, match="x_t needs x_t_scale"):
         ops.linear_int8_backward(dy, *wt, xt[0], None)
     with pytest.raises(ValueError, match="nothing requested"):
         ops.linear_int8_backward(dy)

@@ -231,6 +231,17 @@ def test_entries_refuse_before_any_launch():
         assert told.startswith(fn.__name__ + ":") and message in told, (message, told)
 
 
+def test_a_weight_gradient_of_too_many_tokens():
+    """More terms than an int32 sum holds are refused where the forward could still be told."""
+    x, w = torch.empty(133121, 16, dtype=torch.bfloat16), torch.empty(16, 16, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="133120 tokens"):
+        linear.Int8LinearFunction.apply(x, w, None, None)
+    down = torch.empty(16, 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="133120 tokens"):
+        linear.Int8GegluMlpFunction.apply(x, torch.empty(256, 16, dtype=torch.bfloat16, requires_grad=True), down,
+                                          None, None, 128)
+
+
 def test_sizes_of_nothing():
     """Empty calls return without a launch or a pointer; the workspaces of nothing are empty."""
     L = _lib.lib()
