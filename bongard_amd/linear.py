@@ -643,9 +643,11 @@ class Int8LinearFunction(_Fp8Function):
         if wq is not None and not (need_dx or need_dw):  # (the same product; few tokens take one kernel)
             ctx.save_for_backward(None, None, None, None)
             return ops.linear_int8(dense_rows(x), wq.data, wq.row_scale, bias=bias)
-        xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dw)
         if wq is None or (need_dx and wq.data_t is None):
-            wq = quantize_weight_int8(weight, transpose=need_dx)
+            y, *saved = ops.linear_int8_forward(x, weight, bias=bias, keep_x=need_dw, keep_w=need_dx)
+            ctx.save_for_backward(*saved)
+            return y
+        xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dw)
         y = ops.gemm_int8(xq.data, xq.row_scale, wq.data, wq.row_scale, bias=bias)
         ctx.save_for_backward(xq.data_t, xq.col_scale, wq.data_t if need_dx else None,
                               wq.col_scale if need_dx else None)

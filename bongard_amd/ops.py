@@ -1714,6 +1714,43 @@ def linear_int8(x, w, w_scale, *, bias=None, out_dtype=torch.bfloat16):
 
 
 @functools.lru_cache(maxsize=4096)
+def _linear_int8_forward_ws_cached(M, N, K, keep_x, keep_w):
+    return int(_lib.lib().bf8_linear_int8_forward_workspace(M, N, K, keep_x, keep_w))
+
+
+def linear_int8_forward(x, w, *, bias=None, keep_x=False, keep_w=False):
+    """The training forward of an int8 linear in one call: ``(y, x_t, x_t_scale, w_t, w_t_scale)``, y bf16 [M, N]
+    of bf16 x [M, K] and w [N, K], both quantized by row, and with ``keep_x`` (``keep_w``) the columnwise codes
+    and scales that :func:`linear_int8_backward` takes (else None). The values are :func:`quantize_int8`'s and
+    :func:`gemm_int8`'s. K a multiple of 16, N of 8."""
+    who = "linear_int8_forward"
+    idx = _index_of(who, x, w, bias)
+    x, w = _rows_bf16(x), _rows_bf16(w)
+    M, K = x.shape
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"{who}: inner dims differ ({K} vs {w.shape[1]})")
+    if bias is not None:
+        bias = _linear_bias(who, bias, N)
+    if not (M and N and K):  # nothing to launch, or an empty sum
+        xq, wq = quantize_int8(x, colwise=keep_x), quantize_int8(w, colwise=keep_w)
+        y = gemm_int8(xq.data, xq.row_scale, wq.data, wq.row_scale, bias=bias)
+        return y, xq.data_t, xq.col_scale, wq.data_t, wq.col_scale
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    x_t = x_t_scale = w_t = w_t_scale = None
+    if keep_x:
+        x_t = torch.empty((K, (M + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        x_t_scale = torch.empty(K, dtype=torch.float32, device=x.device)
+    if keep_w:
+        w_t = torch.empty((K, (N + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+        w_t_scale = torch.empty(K, dtype=torch.float32, device=x.device)
+    ws, nbytes = _call_workspace(_linear_int8_forward_ws_cached(M, N, K, keep_x, keep_w), x)
+    _call("bf8_linear_int8_forward", idx, _lib.lib().bf8_linear_int8_forward, x.data_ptr(), w.data_ptr(), M, N, K,
+          _ptr(bias), y.data_ptr(), _ptr(x_t), _ptr(x_t_scale), _ptr(w_t), _ptr(w_t_scale), ws.data_ptr(), nbytes)
+    return y, x_t, x_t_scale, w_t, w_t_scale
+
+
+@functools.lru_cache(maxsize=4096)
 def _linear_int8_backward_ws_cached(M, N, K, dx, dw):
     return int(_lib.lib().bf8_linear_int8_backward_workspace(M, N, K, dx, dw))
 

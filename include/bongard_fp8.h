@@ -668,6 +668,16 @@ size_t bf8_linear_geglu_int8_workspace(int64_t M, int64_t I, int64_t K);
 int bf8_linear_geglu_int8(const void* x, const int8_t* W, int64_t ldw, const float* w_scale, int64_t M,
                           int64_t I, int64_t K, void* H, void* ws, size_t ws_bytes, void* stream);
 
+/* The training forward of a linear layer in int8: C bf16 [M, N] = x . W^T (+ bias) of bf16 x [M, K] and
+ * W [N, K], both quantized by row as bf8_quantize_int8_bf16 does, and where given their columnwise copies
+ * Xt [K, M rounded up to 16] and Wt [K, N rounded up to 16] with scales [K] for the backward. K a multiple
+ * of 16, 32768 at most, N of 8; M, N, K > 0. ws: bf8_linear_int8_forward_workspace(M, N, K, Xt?, Wt?) bytes,
+ * 256-byte aligned. */
+size_t bf8_linear_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int keep_x, int keep_w);
+int bf8_linear_int8_forward(const void* x, const void* W, int64_t M, int64_t N, int64_t K, const void* bias,
+                            void* C, int8_t* Xt, float* xt_scale, int8_t* Wt, float* wt_scale, void* ws,
+                            size_t ws_bytes, void* stream);
+
 /* The backward of a linear layer in int8 from dy bf16 [M, N]: dy quantized by row and by column as
  * bf8_quantize_int8_bf16 does, then dx [M, K] = dy . Wt^T (Wt int8 [K, N], the columnwise copy of W, scales
  * wt_scale [K]) and dw [N, K] = dy^T . Xt^T (Xt int8 [K, M rounded up to 16], the columnwise copy of x,

@@ -515,11 +515,28 @@ def test_functions_without_gradients(gpu, M):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 16, 8), (17, 32, 264), (333, 4112, 40), (1000, 1024, 512), (2049, 64, 2048),
-                                   (64, 8208, 72)])
-def test_linear_backward_is_its_parts(gpu, M, N, K):
-    """Both gradients in one call and each alone: the quantizer's copies of dy through the products, bit for bit."""
+                                   (64, 8208, 72), (37, 272, 80), (1100, 4112, 2576)])
+def test_linear_calls_are_their_parts(gpu, M, N, K):
+    """The forward in one call, both gradients in one and each alone: the quantizer's copies through the products, bit
+    for bit."""
     x, w, dy = (_x(*s, 7, False).to(gpu) for s in ((M, K), (N, K), (M, N)))
     xq, wq = (ops.quantize_int8(t, rowwise=False, colwise=True) for t in (x, w))
+    if K % 16 == 0:  # the forward, with either copy, both and none
+        rows = [ops.quantize_int8(t) for t in (x, w)]
+        bias = _x(1, N, 4, False)[0].to(gpu)
+        want = ops.gemm_int8(rows[0].data, rows[0].row_scale, rows[1].data, rows[1].row_scale, bias=bias)
+        for keep_x, keep_w in ((True, True), (True, False), (False, True), (False, False)):
+            y, *kept = ops.linear_int8_forward(x, w, bias=bias, keep_x=keep_x, keep_w=keep_w)
+            assert torch.equal(y, want)
+            for got, q, keep in ((kept[:2], xq, keep_x), (kept[2:], wq, keep_w)):
+                if keep:
+                    assert torch.equal(got[0], q.data_t) and torch.equal(got[1], q.col_scale)
+                else:
+                    assert got == [None, None]
+        y, *kept = ops.linear_int8_forward(x[:0], w, keep_x=True, keep_w=True)
+        assert y.shape == (0, N) and kept[0].shape == (K, 0) and torch.equal(kept[2], wq.data_t)
+        with pytest.raises(ValueError, match="inner dims"):
+            ops.linear_int8_forward(x, w[:, :-16])
     q = ops.quantize_int8(dy, colwise=True)
     dx = ops.gemm_int8(q.data, q.row_scale, wq.data_t, wq.col_scale)
     dw = ops.gemm_int8(q.data_t, q.col_scale, xq.data_t, xq.col_scale)

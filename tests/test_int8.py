@@ -116,8 +116,17 @@ def _calls(L):
     t, qm = L.bf8_linear_int8, L.bf8_quantize_int8_maxima_bf16
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
     lb, mb = L.bf8_linear_int8_backward, 1 << 20
-    lg = L.bf8_linear_geglu_int8
+    lg, lf = L.bf8_linear_geglu_int8, L.bf8_linear_int8_forward
     return [
+        (lf, (p, p, 0, 16, 16, null, p, p, p, p, p, p, mb, null), "empty"),
+        (lf, (p, p, 4, 16, 24, null, p, p, p, p, p, p, mb, null), "K % 16"),
+        (lf, (p, p, 4, 12, 16, null, p, p, p, p, p, p, mb, null), "N % 8"),
+        (lf, (p, p, 4, 16, 32784, null, p, p, p, p, p, p, mb, null), "32768"),
+        (lf, (p, p, 4, 16, 16, null, p, p, null, p, p, p, mb, null), "NULL"),
+        (lf, (p, null, 4, 16, 16, null, p, p, p, p, p, p, mb, null), "NULL"),
+        (lf, (p, p, 4, 16, 16, null, p, p, odd, p, p, p, mb, null), "16-byte"),
+        (lf, (p, p, 70000, 16, 32768, null, p, p, p, p, p, p, mb, null), "2 GiB"),
+        (lf, (p, p, 4, 16, 16, null, p, p, p, p, p, p, 64, null), "workspace needs"),
         (lg, (p, p, 32, p, 4, 64, 32, p, null, 0, null), "I % 128"),
         (lg, (p, p, 24, p, 4, 128, 24, p, null, 0, null), "K % 16"),
         (lg, (p, p, 32784, p, 4, 128, 32784, p, null, 0, null), "32768"),
