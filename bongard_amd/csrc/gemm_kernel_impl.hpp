@@ -186,7 +186,9 @@ __device__ __forceinline__ v16f mfma(v8i a, v8i b, v16f c) {
 }
 
 // The int8 form: the 64 bytes of a sub-step are two 32x32x32 MFMAs, one for each 16-byte half of the
-// fragments (as for bf16; together they take an FP8 MFMA's time). Sums are exact.
+// fragments (as for bf16; together they take an FP8 MFMA's time). Sums are exact. Bound by power on a full chip: codes
+// of normal numbers 8192^3 468 us (2.35 POP/s), of zeros 320 (3.43); 4096 x 20480 x 2560 192-219 us by box, 2001 x 2560
+// x 10240 69-72.
 template <int FA, int FB>
 __device__ __forceinline__ v16i mfma(v8i a, v8i b, v16i c) {
   static_assert(FA == kFmtInt8 && FB == kFmtInt8, "int8 GEMMs take two int8 operands");
@@ -535,7 +537,8 @@ __device__ __forceinline__ void scaled_h_epilogue(const GemmParams& p, const uin
 
 // int8 gated-GELU epilogue: the wave's staged pre-activations (ROWS rows x CH*8 bf16 columns, first row
 // gm0, first column n0 of [M, 2I]) as checkpoint blocks of 32 along the rows (int8.hpp), a group of four
-// lanes a block.
+// lanes a block. 4096 x 20480 x 2560 takes 192-205 us without it and 239-246 with: its stores 22-26 (84 MB), the
+// conversions the rest.
 template <int ROWS, int CH>
 __device__ __forceinline__ void mxi8_gu_epilogue(const GemmParams& p, const uint8_t* wbuf, int lane,
                                                  int gm0, int n0) {

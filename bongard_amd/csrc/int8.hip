@@ -53,7 +53,8 @@ __device__ __forceinline__ uint32_t group_max(uint32_t m) {
 // Rows [blockIdx.x * strip, + strip) of x, one row per TPR threads at a time (strip is a multiple of the
 // kNT / TPR rows taken at once, so every group runs the same number of steps). Thread tl of a group holds
 // the row's 16-byte vectors tl, tl + TPR, ... (V of them); the next row's are loaded before this
-// row's maximum is known.
+// row's maximum is known. Bound by memory (2 B read, 1 written an element): [4096, 10240] 22.0 us, [20480, 2560]
+// 27.2 (5.7-5.8 TB/s), [64, 2560] 3.2.
 template <int TPR, int V>
 __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restrict__ x, int64_t rows,
                                                        int cols, int64_t strip,
@@ -98,7 +99,8 @@ __global__ __launch_bounds__(kNT) void int8_row_kernel(const uint16_t* __restric
 }
 
 // The maxima of strips of rows (a multiple of 32) by 512 columns, a block each: lane l of a wave holds
-// columns 8 l .. +7 of the tile, the waves take eight rows at a time by turns.
+// columns 8 l .. +7 of the tile, the waves take eight rows at a time by turns. Bound by memory (2 B an element):
+// [20480, 2560] 22.8 us, [4096, 10240] 21.8 (4.6 and 3.8 TB/s).
 __global__ __launch_bounds__(kTileNT) void int8_maxima_kernel(const uint16_t* __restrict__ x,
                                                               Int8Maxima p) {
   __shared__ uint4 red[kTileNT / 64][64];
@@ -125,7 +127,9 @@ __global__ __launch_bounds__(kTileNT) void int8_maxima_kernel(const uint16_t* __
 // of them take the tiles (strips) by turns. Each wave casts 32 rows of all 128 columns: lane l holds columns
 // 8 (l & 15) .. +7 of the rows 4 k + l / 16, k < 8; the columnwise codes meet in LDS and each wave turns 32
 // columns of all 128 rows, so that every store instruction writes whole 128-byte lines. Rows past the
-// tensor's are zeros in out_t [cols, ld].
+// tensor's are zeros in out_t [cols, ld]. Bound by memory (2 B read, 1 written an element and copy, x in part from
+// the memory-side cache): both copies of [4096, 20480] 70 us, [20480, 2560] 43, [4096, 10240] 33 (4.8-5.1 TB/s). Tiles
+// of 256 rows measured level.
 template <bool ROWS, bool COLS>
 __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* __restrict__ x, Int8Maxima p,
                                                             int64_t ld,
@@ -221,7 +225,8 @@ __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* _
 // Both copies of up to 128 R rows. Blocks [0, row_blocks) are int8_row_kernel's of eight rows each (TPR 64, V
 // vectors a lane). Of the others each takes 32 columns of all rows: four lanes a row (8 columns each), 128 rows
 // a step, R steps held in registers; the columns' maxima by packed 16-bit maxima over lanes and waves, the
-// codes turned in LDS, 1,024 rows at a time.
+// codes turned in LDS, 1,024 rows at a time. Bound by latency: [64, 2560] 4.1 us, [500, 2560] 6.7 (two passes over
+// tiles, as below it 1,024 rows, 11.3).
 constexpr int kPairCols = 32, kPairPitch = kPairCols / 4 + 1, kPairStage = 8;  // stage: steps of 128 rows
 template <int V, int R>
 __global__ __launch_bounds__(kNT) void int8_pair_kernel(const uint16_t* __restrict__ x, int rows, int cols,
@@ -316,7 +321,8 @@ __global__ __launch_bounds__(kNT) void int8_pair_kernel(const uint16_t* __restri
   }
 }
 
-// bf16 [rows, cols] of codes [rows, cols] and a scale a row, 8 values a thread.
+// bf16 [rows, cols] of codes [rows, cols] and a scale a row, 8 values a thread. Bound by memory: [20480, 2560] 24.9 us
+// (6.3 TB/s), [64, 2560] 2.3.
 __global__ __launch_bounds__(256) void int8_dequant_kernel(const int8_t* __restrict__ q,
                                                            const float* __restrict__ scale,
                                                            int64_t rows, int64_t cols,
@@ -336,7 +342,8 @@ __global__ __launch_bounds__(256) void int8_dequant_kernel(const int8_t* __restr
 }
 
 // Checkpoint blocks of 32 along the rows of x: four lanes of 8 values a block (per_row of them a row, a
-// multiple of four; past the row they hold zeros).
+// multiple of four; past the row they hold zeros). Bound by memory: [20480, 2560] 31.1 us (5.1 TB/s), its read-back
+// 25.9 (6.2).
 __global__ __launch_bounds__(256) void mxi8_kernel(const uint16_t* __restrict__ x, int64_t rows,
                                                    int64_t cols, int64_t per_row,
                                                    int8_t* __restrict__ out,
@@ -365,7 +372,8 @@ __global__ __launch_bounds__(256) void mxi8_dequant_kernel(const int8_t* __restr
 }
 
 // Sums of columns: block (x, y) adds rows y, y + gridDim.y, .. (eight of them a step, of 256 columns) in
-// fp32 into part[y][cols]; column_finish_kernel adds the parts in order.
+// fp32 into part[y][cols]; column_finish_kernel adds the parts in order. Bound by memory, of few rows by the two
+// launches: [20480, 2560] 29.4 us (3.6 TB/s), [500, 2560] 8.8.
 constexpr int kSumCols = 256;
 constexpr int64_t kSumStrips = 64;
 int64_t sum_strips(int64_t rows) { return std::min<int64_t>((rows + 7) / 8, kSumStrips); }
@@ -447,7 +455,7 @@ int launch_tiles(const uint16_t* x, const Int8Maxima& p, int8_t* out, float* row
 
 int launch_pair(const uint16_t* x, int rows, int cols, int8_t* out, float* row_scale, int8_t* out_t,
                 float* col_scale, hipStream_t s) {
-  const int row_blocks = (rows + 7) / 8, v = (cols / 8 + 63) / 64;
+  const int row_blocks = out ? (rows + 7) / 8 : 0, v = (cols / 8 + 63) / 64;
   const dim3 grid((unsigned)(row_blocks + (cols + kPairCols - 1) / kPairCols));
   const auto run = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kNT), 0, s, x, rows, cols, row_blocks, out, row_scale, out_t,
@@ -506,6 +514,8 @@ int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* ou
     BF8_CHECK(ws && ws_bytes >= bf8_quantize_int8_workspace(rows, cols, 0) && ((uintptr_t)ws & 255) == 0,
               "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who,
               bf8_quantize_int8_workspace(rows, cols, 0), ws_bytes);
+  if (out_t && pair_fits(rows, cols))  // (the columnwise copy alone: 64 x 2560 4.1 us, in two launches 6.4)
+    return launch_pair(xs, (int)rows, (int)cols, nullptr, nullptr, out_t, col_scale, s);
   if (!out_t) {
     if (cols <= 4096)
       launch_rows<64>(xs, rows, (int)cols, out, row_scale, s);

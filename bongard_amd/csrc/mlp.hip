@@ -85,7 +85,8 @@ __global__ __launch_bounds__(kNT) void geglu_fwd_kernel(const uint16_t* __restri
 }
 
 // The same, and GU's checkpoint: blocks of 32 codes along its rows (gu8 [M, 2I], gu8_e [M, 2I / 32],
-// I % 32 == 0), a group of four lanes a block of gates and one of ups.
+// I % 32 == 0), a group of four lanes a block of gates and one of ups. Bound by memory (4 B read, 4.06 written an
+// element of H): [4096, 10240] 64.6 us (5.2 TB/s), [3001, 10240] 41.6.
 __global__ __launch_bounds__(kNT) void geglu_fwd_mxi8_kernel(const uint16_t* __restrict__ GU, int64_t M,
                                                              int64_t I, uint16_t* __restrict__ H,
                                                              int8_t* __restrict__ gu8,
