@@ -731,6 +731,47 @@ def test_layer_together_in_a_graph(gpu):
                 assert torch.equal(a, b), f"replay {rep}, result {k}"
 
 
+def test_decoding_and_a_long_batch_in_a_graph(gpu):
+    """Serving of 1, 20 and 100 tokens (one kernel, one kernel a product, the quantizer and the GEMM) through a norm, a
+    projection and the MLP, and the MLP's training at rows whose gradient leaves its maxima, captured and replayed
+    on new inputs beside eager work: every replay gives the eager bits."""
+    H, I = 256, 512
+    torch.manual_seed(2)
+    w, w_gu, w_d, nw = ((torch.randn(*s, device=gpu) * 0.05).to(BF16) for s in ((H, H), (2 * I, H), (H, I), (H,)))
+    q, gq, dq = (linear.quantize_weight_int8(t) for t in (w, w_gu, w_d))
+
+    def serve(x):
+        n = ops.linear_int8(fused_mlp.layer_norm(x, nw), q.data, q.row_scale)
+        return [n, ops.geglu_mlp_int8(n, gq.data, gq.row_scale, dq.data, dq.row_scale)]
+
+    def train(x):
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_() for t in (x, w_gu, w_d)]
+            y = linear.Int8GegluMlpFunction.apply(*leaves, None, None, I)
+            return [y.detach(), *torch.autograd.grad(y, leaves, x)]
+    graphs = []
+    for M, f in ((1, serve), (20, serve), (100, serve), (1100, train)):
+        x = torch.randn(M, H, device=gpu).to(BF16)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            f(x)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = f(x)
+        graphs.append((graph, x, f, outs))
+    for rep in range(3):
+        for graph, x, f, outs in graphs:
+            x.copy_(torch.randn_like(x))
+            want = [t.clone() for t in f(x)]
+            graph.replay()
+            torch.cuda.synchronize()
+            for k, (a, b) in enumerate(zip(outs, want)):
+                assert torch.equal(a, b), f"replay {rep} of {x.shape[0]} rows, result {k}"
+
+
 def test_two_graphs_at_once(gpu):
     """Calls with a workspace (a product in K pieces, columns' scales, the norm's backward, sums of
     columns) captured into two graphs, replayed side by side on two streams: neither touches the other's."""
