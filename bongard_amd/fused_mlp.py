@@ -135,16 +135,20 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps, checkpoint):
-        y, mean, rstd, q = _ops.layernorm(x, weight, bias, eps, want_stats=True, checkpoint=checkpoint)
-        ctx.save_for_backward(*((q.data, q.exps) if checkpoint else (x, None)), weight, mean, rstd)
+        y, stats, q = _ops._layernorm(x, weight, bias, eps, True, checkpoint)
+        ctx.save_for_backward(*((q.data, q.exps) if checkpoint else (x, None)), weight, stats)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_linear._once_differentiable
     def backward(ctx, dy):
-        x, exps, weight, mean, rstd = ctx.saved_tensors
-        grads = _ops.layernorm_backward(x if exps is None else _ops.MxInt8Tensor(x, exps), dy, weight, mean,
-                                        rstd, needs=ctx.needs_input_grad[:3])
+        x, exps, weight, stats = ctx.saved_tensors
+        weight = _ops._norm_weight("layernorm_backward", "weight", weight, dy.shape[-1])
+        rows = _ops._rows_bf16(dy)
+        x, data = (_ops._rows_bf16(x), None) if exps is None else (None, x)
+        mean = stats.data_ptr()
+        grads = _ops._layernorm_backward(rows.get_device(), dy.shape, x, data, exps, rows, weight, mean,
+                                         mean + 4 * rows.shape[0], ctx.needs_input_grad[:3])
         return (*grads, None, None)
 
 

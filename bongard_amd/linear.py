@@ -21,6 +21,7 @@ bongard/float8_training.py:16-22, te.Linear under TELinear.forward
 bongard/fused_mlp.py:62-79).
 """
 
+import functools
 import threading
 from dataclasses import dataclass
 from typing import Optional
@@ -40,6 +41,17 @@ class QuantizedWeight:
 
     q: ops.Fp8Tensor
     version: int
+
+
+def _once_differentiable(backward):
+    """``once_differentiable`` where the gradients' own graph is recorded; where it is not, the backward as it is
+    (4 us of host time less)."""
+    once = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
 
 
 class _Fp8Function(torch.autograd.Function):
@@ -654,14 +666,15 @@ class Int8LinearFunction(_Fp8Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         x8t, xs, w8t, ws = ctx.saved_tensors
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
-        dy = dense_rows(dy)
         dx = dw = None
         if need_dx or need_dw:
-            dx, dw = ops.linear_int8_backward(dy, w8t if need_dx else None, ws, x8t if need_dw else None, xs)
+            dy = ops._rows_bf16(dy)
+            dx, dw = ops._linear_int8_backward(dy.get_device(), dy, (w8t if need_dx else x8t).shape[0],
+                                               w8t if need_dx else None, ws, x8t if need_dw else None, xs)
         return dx, dw, ops.column_sums(dy) if need_db else None, None
 
 
@@ -699,7 +712,7 @@ class Int8GegluMlpFunction(_Fp8Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dy):
         gu8, gu_exps, x8t, xs, h8t, hs, gu8t, gus, d8t, ds = ctx.saved_tensors
         need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]
@@ -730,9 +743,11 @@ class GegluCheckpointFunction(_Fp8Function):
         return H
 
     @staticmethod
-    @once_differentiable
+    @_once_differentiable
     def backward(ctx, dH):
-        return ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(*ctx.saved_tensors))
+        data, exps = ctx.saved_tensors
+        dH = ops._rows_bf16(dH)
+        return ops._geglu_bwd_mxint8(dH.get_device(), dH, data, exps)
 
 
 def mlp_forward(x, w_gu, w_down, gu_q, down_q, intermediate, split_scales, scaling, x_amax,

@@ -1781,6 +1781,12 @@ def linear_int8_backward(dy, w_t=None, w_t_scale=None, x_t=None, x_t_scale=None)
 
     w_t, w_t_scale = operand("w_t", w_t, w_t_scale, N)
     x_t, x_t_scale = operand("x_t", x_t, x_t_scale, (M + 15) // 16 * 16)
+    return _linear_int8_backward(idx, dy, K, w_t, w_t_scale, x_t, x_t_scale)
+
+
+def _linear_int8_backward(idx, dy, K, w_t, w_t_scale, x_t, x_t_scale):
+    """:func:`linear_int8_backward` of what its checks or the forward's have seen."""
+    M, N = dy.shape
     dx = None if w_t is None else torch.empty((M, K), dtype=torch.bfloat16, device=dy.device)
     dw = None if x_t is None else torch.empty((N, K), dtype=torch.bfloat16, device=dy.device)
     if not (M and N and K):  # sums of nothing
@@ -1788,9 +1794,8 @@ def linear_int8_backward(dy, w_t=None, w_t_scale=None, x_t=None, x_t_scale=None)
             if t is not None:
                 t.zero_()
         return dx, dw
-    L = _lib.lib()
     ws, nbytes = _call_workspace(_linear_int8_backward_ws_cached(M, N, K, dx is not None, dw is not None), dy)
-    _call("bf8_linear_int8_backward", idx, L.bf8_linear_int8_backward, dy.data_ptr(), M, N, K, _ptr(w_t),
+    _call("bf8_linear_int8_backward", idx, _lib.lib().bf8_linear_int8_backward, dy.data_ptr(), M, N, K, _ptr(w_t),
           _ptr(w_t_scale), _ptr(x_t), _ptr(x_t_scale), _ptr(dx), _ptr(dw), ws.data_ptr(), nbytes)
     return dx, dw
 
@@ -1934,6 +1939,16 @@ def _geglu_bwd_maxima_cached(M, I):
     return int(_lib.lib().bf8_geglu_bwd_mxint8_maxima(M, I))
 
 
+def _geglu_bwd_mxint8(idx, dH, data, exps):
+    """:func:`geglu_bwd_mxint8` of what its checks or the forward's have seen."""
+    M, I = dH.shape
+    dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
+    if M and I:
+        _call("bf8_geglu_bwd_mxint8", idx, _lib.lib().bf8_geglu_bwd_mxint8, dH.data_ptr(),
+              data.data_ptr(), exps.data_ptr(), M, I, dGU.data_ptr(), None, 0)
+    return dGU
+
+
 def geglu_bwd_mxint8(dH, gu, *, rowwise=False, colwise=False):
     """:func:`geglu_bwd` on the values of GU's checkpoint: dGU bf16 [M, 2I], or with ``rowwise`` or
     ``colwise`` that tensor's :func:`quantize_int8` instead (from 1024 rows on by the maxima that the backward's
@@ -1946,11 +1961,7 @@ def geglu_bwd_mxint8(dH, gu, *, rowwise=False, colwise=False):
         raise ValueError(f"{who}: the intermediate size must be a multiple of 32 (got {I})")
     data, exps = _mxint8_of(who, gu, M, 2 * I)
     if not (rowwise or colwise):
-        dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
-        if M and I:
-            _call("bf8_geglu_bwd_mxint8", idx, _lib.lib().bf8_geglu_bwd_mxint8, dH.data_ptr(),
-                  data.data_ptr(), exps.data_ptr(), M, I, dGU.data_ptr(), None, 0)
-        return dGU
+        return _geglu_bwd_mxint8(idx, dH, data, exps)
     # both copies of dGU's codes, by the maxima and by the quantizer's own pass, us: [512, 2 x 10240] 32.5 and
     # 31.5, [1500, 2 x 2560] 27.5 and 29.9, [4096, 2 x 10240] 157 and 168
     if M < 1024 or not I:
@@ -1990,6 +2001,13 @@ def layernorm(x, weight, bias, eps, *, want_stats=False, checkpoint=False):
     eps) (else None); ``checkpoint``: the :class:`MxInt8Tensor` of x, written in the same pass (else
     None). cols: a multiple of 8, 16384 at most. No gradients
     (:func:`bongard_amd.fused_mlp.layer_norm` has them)."""
+    y, stats, q = _layernorm(x, weight, bias, eps, want_stats, checkpoint)
+    mean, rstd = (None, None) if stats is None else stats.unbind(0)
+    return y, mean, rstd, q
+
+
+def _layernorm(x, weight, bias, eps, want_stats, checkpoint):
+    """:func:`layernorm` with the statistics as one tensor [2, rows]: ``(y, statistics, checkpoint)``."""
     who = "layernorm"
     idx = _index_of(who, x, weight, bias)
     shape = x.shape
@@ -1998,16 +2016,18 @@ def layernorm(x, weight, bias, eps, *, want_stats=False, checkpoint=False):
     x = _rows_bf16(x)
     rows, cols = x.shape
     y = torch.empty_like(x)
-    mean = rstd = q = None
+    stats = mean = rstd = q = None
     if want_stats:
-        mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     if checkpoint:
         q = _new_mxint8(rows, cols, x.device)
     if rows:
         _call("bf8_layernorm_bf16", idx, _lib.lib().bf8_layernorm_bf16, x.data_ptr(), rows, cols,
-              weight.data_ptr(), _ptr(bias), eps, y.data_ptr(), _ptr(mean), _ptr(rstd),
+              weight.data_ptr(), _ptr(bias), eps, y.data_ptr(), mean, rstd,
               q.data.data_ptr() if checkpoint else None, q.exps.data_ptr() if checkpoint else None)
-    return y if len(shape) == 2 else y.view(shape), mean, rstd, q
+    return y if len(shape) == 2 else y.view(shape), stats, q
 
 
 @functools.lru_cache(maxsize=4096)
@@ -2036,8 +2056,17 @@ def layernorm_backward(x, dy, weight, mean, rstd, *, needs=(True, True, True)):
         if t.dtype is not torch.float32 or t.shape != (rows,) or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be contiguous float32 [{rows}] (got {t.dtype} "
                              f"{tuple(t.shape)})")
+    return _layernorm_backward(idx, shape, x, data if q else None, exps if q else None, dy, weight, mean.data_ptr(),
+                               rstd.data_ptr(), needs)
+
+
+def _layernorm_backward(idx, shape, x, data, exps, dy, weight, mean, rstd, needs):
+    """:func:`layernorm_backward` of what its checks or the forward's have seen: contiguous and aligned tensors (x
+    unread where ``data`` is given), the statistics' addresses."""
+    rows, cols = dy.shape
     dx = torch.empty_like(dy) if needs[0] else None
-    dw, db = (torch.empty_like(weight) if n else None for n in needs[1:])
+    dw = torch.empty_like(weight) if needs[1] else None
+    db = torch.empty_like(weight) if needs[2] else None
     if rows == 0:
         for g in (dw, db):
             if g is not None:
@@ -2047,9 +2076,8 @@ def layernorm_backward(x, dy, weight, mean, rstd, *, needs=(True, True, True)):
         if needs[1] or needs[2]:
             ws, nbytes = _call_workspace(_layernorm_ws_cached(rows, cols), dy)
         _call("bf8_layernorm_bwd_bf16", idx, _lib.lib().bf8_layernorm_bwd_bf16,
-              None if q else x.data_ptr(), data.data_ptr() if q else None, exps.data_ptr() if q else None,
-              dy.data_ptr(), rows, cols, weight.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(dx),
-              _ptr(dw), _ptr(db), _ptr(ws), nbytes)
+              x.data_ptr() if data is None else None, _ptr(data), _ptr(exps), dy.data_ptr(), rows, cols,
+              weight.data_ptr(), mean, rstd, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes)
     if dx is not None and len(shape) != 2:
         dx = dx.view(shape)
     return dx, dw, db
