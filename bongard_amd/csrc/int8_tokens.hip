@@ -383,124 +383,4 @@ int bf8_linear_geglu_int8(const void* x, const int8_t* W, int64_t ldw, const flo
   return launch_status("int8_tokens_kernel(gated)");
 }
 
-// The row copies of x and W, then what the quantizations or the product need.
-namespace {
-struct ForwardWs {
-  size_t x, x_scale, w, w_scale, rest, bytes;
-};
-ForwardWs forward_ws(int64_t M, int64_t N, int64_t K, bool keep_x, bool keep_w) {
-  ForwardWs f{};
-  f.x_scale = align256((size_t)M * K);
-  f.w = f.x_scale + align256((size_t)M * 4);
-  f.w_scale = f.w + align256((size_t)N * K);
-  f.rest = f.w_scale + align256((size_t)N * 4);
-  size_t rest = bf8_gemm_int8_workspace(M, N, K);
-  if (keep_x) rest = std::max(rest, bf8_quantize_int8_workspace(M, K, 1));
-  if (keep_w) rest = std::max(rest, bf8_quantize_int8_workspace(N, K, 1));
-  f.bytes = f.rest + rest;
-  return f;
-}
-}  // namespace
-
-size_t bf8_linear_int8_forward_workspace(int64_t M, int64_t N, int64_t K, int keep_x, int keep_w) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return forward_ws(M, N, K, keep_x != 0, keep_w != 0).bytes;
-}
-
-int bf8_linear_int8_forward(const void* x, const void* W, int64_t M, int64_t N, int64_t K, const void* bias,
-                            void* C, int8_t* Xt, float* xt_scale, int8_t* Wt, float* wt_scale, void* ws,
-                            size_t ws_bytes, void* stream) {
-  const char* who = "bf8_linear_int8_forward";
-  BF8_CHECK(M > 0 && N > 0 && K > 0, "%s: empty or negative shape", who);
-  BF8_CHECK(K % 16 == 0 && K <= 32768 && N % 8 == 0, "%s: need K %% 16 == 0, K <= 32768 and N %% 8 == 0", who);
-  BF8_CHECK(x && W && C && (Xt == nullptr) == (xt_scale == nullptr) && (Wt == nullptr) == (wt_scale == nullptr),
-            "%s: NULL pointer", who);
-  BF8_CHECK((((uintptr_t)x | (uintptr_t)W | (uintptr_t)C | (uintptr_t)Xt | (uintptr_t)xt_scale | (uintptr_t)Wt |
-              (uintptr_t)wt_scale) & 15) == 0 && ((uintptr_t)bias & 7) == 0,
-            "%s: every tensor must be 16-byte (bias 8-byte) aligned", who);
-  BF8_CHECK(M < (1LL << 31) && N < (1LL << 31) && std::max(M, N) * K < (1LL << 31),
-            "%s: operands of 2 GiB and more", who);
-  const ForwardWs f = forward_ws(M, N, K, Xt, Wt);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= f.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, f.bytes, ws_bytes);
-  int8_t* const base = (int8_t*)ws;
-  float *const xs = (float*)(base + f.x_scale), *const wsc = (float*)(base + f.w_scale);
-  void* const rest = base + f.rest;
-  const size_t rest_bytes = ws_bytes - f.rest;
-  if (const int rc = bf8_quantize_int8_bf16(x, M, K, base, xs, Xt, xt_scale, rest, rest_bytes, stream)) return rc;
-  if (const int rc = bf8_quantize_int8_bf16(W, N, K, base + f.w, wsc, Wt, wt_scale, rest, rest_bytes, stream)) return rc;
-  return bf8_gemm_int8(base, K, xs, base + f.w, K, wsc, M, N, K, bias, C, BF8_OUT_BF16, N, rest, rest_bytes, stream);
-}
-
-// dy's codes and scales by row and by column, then what the quantization or a product needs.
-namespace {
-int64_t pad16(int64_t rows) { return (rows + 15) / 16 * 16; }
-struct BackwardWs {
-  size_t rows, row_scale, cols, col_scale, rest, bytes;
-};
-BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
-  const int64_t Mp = pad16(M);
-  BackwardWs w{};
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    const size_t o = at;
-    at += align256(bytes);
-    return o;
-  };
-  if (dx) {
-    w.rows = take((size_t)M * N);
-    w.row_scale = take((size_t)M * 4);
-  }
-  if (dw) {
-    w.cols = take((size_t)N * Mp);
-    w.col_scale = take((size_t)N * 4);
-  }
-  w.rest = at;
-  size_t rest = dw ? bf8_quantize_int8_workspace(M, N, dx) : 0;
-  if (dx) rest = std::max(rest, bf8_gemm_int8_workspace(M, K, N));
-  if (dw) rest = std::max(rest, bf8_gemm_int8_workspace(N, K, Mp));
-  w.bytes = at + rest;
-  return w;
-}
-}  // namespace
-
-size_t bf8_linear_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int dx, int dw) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  return backward_ws(M, N, K, dx != 0, dw != 0).bytes;
-}
-
-int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, const int8_t* Wt,
-                             const float* wt_scale, const int8_t* Xt, const float* xt_scale, void* dx, void* dw,
-                             void* ws, size_t ws_bytes, void* stream) {
-  const char* who = "bf8_linear_int8_backward";
-  BF8_CHECK(M > 0 && N > 0 && K > 0, "%s: empty or negative shape", who);
-  BF8_CHECK(N % 16 == 0 && N <= 32768 && K % 8 == 0 && (!dw || M <= kInt8MaxK),
-            "%s: need N %% 16 == 0, N <= 32768, K %% 8 == 0 and for dw M <= %lld", who, (long long)kInt8MaxK);
-  BF8_CHECK(dx || dw, "%s: nothing requested", who);
-  BF8_CHECK(dy && (!dx || (Wt && wt_scale)) && (!dw || (Xt && xt_scale)), "%s: NULL pointer", who);
-  BF8_CHECK((((uintptr_t)dy | (uintptr_t)Wt | (uintptr_t)wt_scale | (uintptr_t)Xt | (uintptr_t)xt_scale |
-              (uintptr_t)dx | (uintptr_t)dw) & 15) == 0,
-            "%s: every tensor must be 16-byte aligned", who);
-  const int64_t most = std::max(dx ? std::max(M, K) * N : 0, dw ? std::max(N, K) * pad16(M) : 0);
-  BF8_CHECK(M < (1LL << 31) && K < (1LL << 31) && most < (1LL << 31), "%s: operands of 2 GiB and more", who);
-  const BackwardWs w = backward_ws(M, N, K, dx, dw);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
-  int8_t* const base = (int8_t*)ws;
-  int8_t *const rows = dx ? base + w.rows : nullptr, *const cols = dw ? base + w.cols : nullptr;
-  float* const rs = dx ? (float*)(base + w.row_scale) : nullptr;
-  float* const cs = dw ? (float*)(base + w.col_scale) : nullptr;
-  void* const rest = base + w.rest;
-  const size_t rest_bytes = ws_bytes - w.rest;
-  if (const int rc = bf8_quantize_int8_bf16(dy, M, N, rows, rs, cols, cs, rest, rest_bytes, stream)) return rc;
-  if (dx)
-    if (const int rc = bf8_gemm_int8(rows, N, rs, Wt, N, wt_scale, M, K, N, nullptr, dx, BF8_OUT_BF16, K, rest,
-                                     rest_bytes, stream))
-      return rc;
-  if (!dw) return BF8_OK;
-  const int64_t Mp = pad16(M);
-  return bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, N, K, Mp, nullptr, dw, BF8_OUT_BF16, K, rest, rest_bytes,
-                       stream);
-}
-
 }  // extern "C"

@@ -705,6 +705,7 @@ class Int8GegluMlpFunction(_Fp8Function):
             down_q = quantize_weight_int8(w_down, transpose=keep)
         hq = ops.quantize_int8(H, rowwise=True, colwise=need_dd)
         y = ops.gemm_int8(hq.data, hq.row_scale, down_q.data, down_q.row_scale)
+        ctx.shapes = x.shape, w_gu.shape, w_down.shape
         ctx.save_for_backward(*((gu.data, gu.exps) if keep else (None, None)), xq.data_t, xq.col_scale,
                               hq.data_t, hq.col_scale, gu_q.data_t if need_dx else None,
                               gu_q.col_scale if need_dx else None, down_q.data_t if keep else None,
@@ -714,19 +715,13 @@ class Int8GegluMlpFunction(_Fp8Function):
     @staticmethod
     @_once_differentiable
     def backward(ctx, dy):
-        gu8, gu_exps, x8t, xs, h8t, hs, gu8t, gus, d8t, ds = ctx.saved_tensors
-        need_dx, need_dgu, need_dd = ctx.needs_input_grad[:3]
-        dx = dgu = None
-        dH, dd = ops.linear_int8_backward(dense_rows(dy), d8t if need_dx or need_dgu else None, ds,
-                                          h8t if need_dd else None, hs)
-        if need_dx or need_dgu:
-            dq = ops.geglu_bwd_mxint8(dH, ops.MxInt8Tensor(gu8, gu_exps), rowwise=need_dx,
-                                      colwise=need_dgu)
-            if need_dx:
-                dx = ops.gemm_int8(dq.data, dq.row_scale, gu8t, gus)
-            if need_dgu:
-                dgu = ops.gemm_int8(dq.data_t, dq.col_scale, x8t, xs)
-        return dx, dgu, dd, None, None, None
+        needs = ctx.needs_input_grad[:3]
+        if not dy.shape[0]:
+            grads = [torch.zeros(s, dtype=torch.bfloat16, device=dy.device) if n else None
+                     for n, s in zip(needs, ctx.shapes)]
+        else:
+            grads = ops._geglu_mlp_int8_backward(dy, ctx.shapes[0][1], ctx.shapes[2][1], needs, *ctx.saved_tensors)
+        return (*grads, None, None, None)
 
 
 class GegluCheckpointFunction(_Fp8Function):

@@ -1935,6 +1935,27 @@ def geglu_mxint8(GU):
 
 
 @functools.lru_cache(maxsize=4096)
+def _geglu_mlp_int8_backward_ws_cached(*args):
+    return int(_lib.lib().bf8_geglu_mlp_int8_backward_workspace(*args))
+
+
+def _geglu_mlp_int8_backward(dy, K, I, needs, gu8, gu_exps, x_t, x_t_scale, h_t, h_t_scale, gu_t, gu_t_scale, down_t,
+                             down_t_scale):
+    """Gradients ``(dx, dW_gu, dW_down)`` (those of ``needs``, the others None) of the gated int8 MLP for bf16 dy
+    [M, N], M > 0, from the columnwise codes and the checkpoint that its forward kept:
+    :func:`linear_int8_backward` on H and W_down, :func:`geglu_bwd_mxint8`, the products with x and W_gu."""
+    dy = _rows_bf16(dy)
+    M, N = dy.shape
+    dx, dgu, dd = (torch.empty(shape, dtype=torch.bfloat16, device=dy.device) if n else None
+                   for n, shape in zip(needs, ((M, K), (2 * I, K), (N, I))))
+    ws, nbytes = _call_workspace(_geglu_mlp_int8_backward_ws_cached(M, K, I, N, *needs), dy)
+    _call("bf8_geglu_mlp_int8_backward", dy.get_device(), _lib.lib().bf8_geglu_mlp_int8_backward, dy.data_ptr(), M, K,
+          I, N, _ptr(gu8), _ptr(gu_exps), _ptr(x_t), _ptr(x_t_scale), _ptr(h_t), _ptr(h_t_scale), _ptr(gu_t),
+          _ptr(gu_t_scale), _ptr(down_t), _ptr(down_t_scale), _ptr(dx), _ptr(dgu), _ptr(dd), ws.data_ptr(), nbytes)
+    return dx, dgu, dd
+
+
+@functools.lru_cache(maxsize=4096)
 def _geglu_bwd_maxima_cached(M, I):
     return int(_lib.lib().bf8_geglu_bwd_mxint8_maxima(M, I))
 

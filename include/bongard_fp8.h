@@ -697,6 +697,22 @@ int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, cons
                         int64_t ldw, const float* w_scale, int64_t M, int64_t I, int64_t K, void* H,
                         int8_t* GU8, uint8_t* GU8_exp, void* stream);
 
+/* The backward of the gated MLP in int8 from dy bf16 [M, N]: dH [M, I] and dW_down [N, I] as
+ * bf8_linear_int8_backward (Wt_down [I, N] and Ht [I, M rounded up to 16], the columnwise copies of W_down and
+ * H, with scales [I]), dGU [M, 2 I] from the checkpoint GU8 [M, 2 I] with GU8_exp as bf8_geglu_bwd_mxint8, then
+ * dx [M, K] and dW_gu [2 I, K] (Wt_gu [K, 2 I] and Xt [K, M rounded up to 16], scales [K]); bf16. Any of dx,
+ * dW_gu and dW_down may be NULL with the operands that it alone needs. I a multiple of 32, 16384 at most, N of
+ * 16, 32768 at most, K of 8; for a weight's gradient M 133120 at most. ws:
+ * bf8_geglu_mlp_int8_backward_workspace(M, K, I, N, dx?, dW_gu?, dW_down?) bytes, 256-byte aligned. */
+size_t bf8_geglu_mlp_int8_backward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int dx, int dgu,
+                                             int dd);
+int bf8_geglu_mlp_int8_backward(const void* dy, int64_t M, int64_t K, int64_t I, int64_t N,
+                                const int8_t* GU8, const uint8_t* GU8_exp, const int8_t* Xt,
+                                const float* xt_scale, const int8_t* Ht, const float* ht_scale,
+                                const int8_t* Wt_gu, const float* wt_gu_scale, const int8_t* Wt_down,
+                                const float* wt_down_scale, void* dx, void* dW_gu, void* dW_down, void* ws,
+                                size_t ws_bytes, void* stream);
+
 /* out bf16 [cols] = the sum over rows of x [rows, cols], in fp32 and a fixed order (the gradient of
  * a bias). cols % 8 == 0, x 16-byte aligned; ws: bf8_column_sums_workspace(rows, cols) bytes, 16-byte
  * aligned. rows > 0. */

@@ -593,7 +593,7 @@ def test_linear_gradients_are_the_differences(gpu):
         assert abs(diff - told) <= slack and diff != 0
 
 
-@pytest.mark.parametrize("M,K,I", [(1, 32, 128), (37, 96, 256), (512, 256, 384)])
+@pytest.mark.parametrize("M,K,I", [(1, 32, 128), (37, 96, 256), (512, 256, 384), (1023, 48, 128), (1100, 320, 640)])
 def test_mlp_function_is_its_ops(gpu, M, K, I):
     x, w_gu, w_d, dy = _mlp_inputs(M, K, I, 5, gpu)
     leaves = [t.requires_grad_() for t in (x, w_gu, w_d)]
@@ -618,6 +618,11 @@ def test_mlp_function_is_its_ops(gpu, M, K, I):
         one = [t.detach().requires_grad_(i == k) for k, t in enumerate(leaves)]
         (g,) = torch.autograd.grad(linear.Int8GegluMlpFunction.apply(*one, None, None, I), one[i], dy)
         assert torch.equal(g, grads[i])
+    none = torch.empty(0, K, dtype=BF16, device=gpu, requires_grad=True)
+    y = linear.Int8GegluMlpFunction.apply(none, w_gu, w_d, None, None, I)
+    grads = torch.autograd.grad(y, [none, w_gu, w_d], dy[:0])
+    assert y.shape == dy[:0].shape and [g.shape for g in grads] == [none.shape, w_gu.shape, w_d.shape]
+    assert not any(bool(g.any()) for g in grads)
 
 
 class _Mlp(nn.Module):

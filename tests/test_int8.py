@@ -117,7 +117,18 @@ def _calls(L):
     n, nb = L.bf8_layernorm_bf16, L.bf8_layernorm_bwd_bf16
     lb, mb = L.bf8_linear_int8_backward, 1 << 20
     lg, lf = L.bf8_linear_geglu_int8, L.bf8_linear_int8_forward
+    gb, kept, big = L.bf8_geglu_mlp_int8_backward, (p,) * 10, 1 << 30
     return [
+        (gb, (p, 0, 16, 32, 16, *kept, p, p, p, p, big, null), "empty"),
+        (gb, (p, 4, 16, 24, 16, *kept, p, p, p, p, big, null), "I % 32"),
+        (gb, (p, 4, 16, 16416, 16, *kept, p, p, p, p, big, null), "16384"),
+        (gb, (p, 4, 16, 32, 24, *kept, p, p, p, p, big, null), "N % 16"),
+        (gb, (p, 4, 12, 32, 16, *kept, p, p, p, p, big, null), "K % 8"),
+        (gb, (p, 4, 16, 32, 16, *kept, null, null, null, p, big, null), "nothing requested"),
+        (gb, (p, 4, 16, 32, 16, null, *kept[1:], p, p, p, p, big, null), "NULL"),
+        (gb, (p, 4, 16, 32, 16, *kept[:2], null, *kept[3:], null, p, null, p, big, null), "NULL"),
+        (gb, (p, 133121, 16, 32, 16, *kept, p, p, p, p, big, null), "133120"),
+        (gb, (p, 4, 16, 32, 16, *kept, p, p, p, p, 64, null), "workspace needs"),
         (lf, (p, p, 0, 16, 16, null, p, p, p, p, p, p, mb, null), "empty"),
         (lf, (p, p, 4, 16, 24, null, p, p, p, p, p, p, mb, null), "K % 16"),
         (lf, (p, p, 4, 12, 16, null, p, p, p, p, p, p, mb, null), "N % 8"),
