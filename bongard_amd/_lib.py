@@ -170,6 +170,10 @@ SIGNATURES = {
     "bf8_linear_int8_backward_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
     "bf8_linear_int8_backward": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                          c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "bf8_geglu_mlp_int8_forward_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int]),
+    "bf8_geglu_mlp_int8_forward": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                           c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "bf8_geglu_mlp_int8_backward_workspace": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int, c_int,
                                                          c_int]),
     "bf8_geglu_mlp_int8_backward": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p,

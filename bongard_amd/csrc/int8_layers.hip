@@ -1,5 +1,5 @@
-// A layer's pass in 8-bit integers as one call: the training forward and backward of a linear and the backward of the
-// gated MLP, as the quantizer's, the products' and the gated GELU's own entries in turn on one workspace (from
+// A layer's pass in 8-bit integers as one call: the training forward and backward of a linear and of the gated
+// MLP, as the quantizer's, the products' and the gated GELU's own entries in turn on one workspace (from
 // Python each of those is 10 us of host time, in the autograd engine's thread up to twice that: 500 x 2048 x 2560
 // trained 171 us as six calls, 118 as two).
 #include <hip/hip_runtime.h>
@@ -63,6 +63,26 @@ BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
   size_t rest = dw ? bf8_quantize_int8_workspace(M, N, dx) : 0;
   if (dx) rest = std::max(rest, bf8_gemm_int8_workspace(M, K, N));
   if (dw) rest = std::max(rest, bf8_gemm_int8_workspace(N, K, Mp));
+  w.bytes = w.rest + rest;
+  return w;
+}
+
+// x's and H's row copies, H (bf16), and what the quantizations or the down product need.
+struct MlpForwardWs {
+  size_t x, x_scale, h, h8, h_scale, rest, bytes;
+};
+MlpForwardWs mlp_forward_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool keep_x, bool keep_h) {
+  MlpForwardWs w{};
+  Parts p;
+  w.x = p.take((size_t)M * K);
+  w.x_scale = p.take((size_t)M * 4);
+  w.h = p.take((size_t)M * I * 2);
+  w.h8 = p.take((size_t)M * I);
+  w.h_scale = p.take((size_t)M * 4);
+  w.rest = p.at;
+  size_t rest = bf8_gemm_int8_workspace(M, N, I);
+  if (keep_x) rest = std::max(rest, bf8_quantize_int8_workspace(M, K, 1));
+  if (keep_h) rest = std::max(rest, bf8_quantize_int8_workspace(M, I, 1));
   w.bytes = w.rest + rest;
   return w;
 }
@@ -172,6 +192,37 @@ int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, co
   if (!dw) return BF8_OK;
   const int64_t Mp = pad16(M);
   return bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, N, K, Mp, nullptr, dw, BF8_OUT_BF16, K, rest, rest_bytes,
+                       stream);
+}
+
+size_t bf8_geglu_mlp_int8_forward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int keep_x, int keep_h) {
+  if (M <= 0 || K <= 0 || I <= 0 || N <= 0) return 0;
+  return mlp_forward_ws(M, K, I, N, keep_x != 0, keep_h != 0).bytes;
+}
+
+int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, int64_t N, const int8_t* W_gu,
+                               const float* w_gu_scale, const int8_t* W_down, const float* w_down_scale, void* Y,
+                               int8_t* GU8, uint8_t* GU8_exp, int8_t* Xt, float* xt_scale, int8_t* Ht,
+                               float* ht_scale, void* ws, size_t ws_bytes, void* stream) {
+  const char* who = "bf8_geglu_mlp_int8_forward";
+  BF8_CHECK(M > 0 && K > 0 && I > 0 && N > 0, "%s: empty or negative shape", who);
+  BF8_CHECK(K % 16 == 0 && K <= 32768 && I % 128 == 0 && I <= 32768 && N % 8 == 0 && M < (1LL << 31),
+            "%s: need K %% 16 == 0, I %% 128 == 0, both 32768 at most, and N %% 8 == 0", who);
+  BF8_CHECK(x && W_gu && w_gu_scale && W_down && w_down_scale && Y && (GU8 == nullptr) == (GU8_exp == nullptr) &&
+                (Xt == nullptr) == (xt_scale == nullptr) && (Ht == nullptr) == (ht_scale == nullptr),
+            "%s: NULL pointer", who);
+  const MlpForwardWs w = mlp_forward_ws(M, K, I, N, Xt, Ht);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
+  uint8_t* const base = (uint8_t*)ws;
+  int8_t *const x8 = (int8_t*)base + w.x, *const h8 = (int8_t*)base + w.h8;
+  float *const xs = (float*)(base + w.x_scale), *const hs = (float*)(base + w.h_scale);
+  void *const H = base + w.h, *const rest = base + w.rest;
+  const size_t rest_bytes = ws_bytes - w.rest;
+  if (const int rc = bf8_quantize_int8_bf16(x, M, K, x8, xs, Xt, xt_scale, rest, rest_bytes, stream)) return rc;
+  if (const int rc = bf8_gemm_geglu_int8(x8, K, xs, W_gu, K, w_gu_scale, M, I, K, H, GU8, GU8_exp, stream)) return rc;
+  if (const int rc = bf8_quantize_int8_bf16(H, M, I, h8, hs, Ht, ht_scale, rest, rest_bytes, stream)) return rc;
+  return bf8_gemm_int8(h8, I, hs, W_down, I, w_down_scale, M, N, I, nullptr, Y, BF8_OUT_BF16, N, rest, rest_bytes,
                        stream);
 }
 

@@ -697,19 +697,16 @@ class Int8GegluMlpFunction(_Fp8Function):
             _check_int8_tokens("int8 gated MLP", x.shape[0])
         if gu_q is not None and down_q is not None and not (keep or need_dd):
             return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
-        xq = ops.quantize_int8(dense_rows(x), rowwise=True, colwise=need_dgu)
         if gu_q is None or (need_dx and gu_q.data_t is None):
             gu_q = quantize_weight_int8(w_gu, transpose=need_dx)
-        H, gu = ops.gemm_geglu_int8(xq.data, xq.row_scale, gu_q.data, gu_q.row_scale, I, keep_gu=keep)
         if down_q is None or (keep and down_q.data_t is None):
             down_q = quantize_weight_int8(w_down, transpose=keep)
-        hq = ops.quantize_int8(H, rowwise=True, colwise=need_dd)
-        y = ops.gemm_int8(hq.data, hq.row_scale, down_q.data, down_q.row_scale)
         ctx.shapes = x.shape, w_gu.shape, w_down.shape
-        ctx.save_for_backward(*((gu.data, gu.exps) if keep else (None, None)), xq.data_t, xq.col_scale,
-                              hq.data_t, hq.col_scale, gu_q.data_t if need_dx else None,
-                              gu_q.col_scale if need_dx else None, down_q.data_t if keep else None,
-                              down_q.col_scale if keep else None)
+        if not x.shape[0]:  # nothing to launch (its gradients are zeros)
+            return x.new_empty((0, w_down.shape[0]), dtype=torch.bfloat16)
+        y, *kept = ops._geglu_mlp_int8_forward(x, I, gu_q, down_q, keep, need_dgu, need_dd)
+        ctx.save_for_backward(*kept, gu_q.data_t if need_dx else None, gu_q.col_scale if need_dx else None,
+                              down_q.data_t if keep else None, down_q.col_scale if keep else None)
         return y
 
     @staticmethod

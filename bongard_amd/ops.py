@@ -1935,6 +1935,38 @@ def geglu_mxint8(GU):
 
 
 @functools.lru_cache(maxsize=4096)
+def _geglu_mlp_int8_forward_ws_cached(*args):
+    return int(_lib.lib().bf8_geglu_mlp_int8_forward_workspace(*args))
+
+
+def _geglu_mlp_int8_forward(x, I, gu_q, down_q, keep_gu, keep_x, keep_h):
+    """The gated int8 MLP of bf16 x [M, K], M > 0, and the rowwise copies of its weights, in one call: ``(y, checkpoint
+    codes, its exponents, x_t, x_t_scale, h_t, h_t_scale)``, None where not kept. The values are
+    :func:`quantize_int8`'s, :func:`gemm_geglu_int8`'s and :func:`gemm_int8`'s."""
+    who = "geglu_mlp_int8_forward"
+    idx = _index_of(who, x, gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
+    x = _rows_bf16(x)
+    M, K = x.shape
+    N = down_q.rows
+    if (gu_q.rows, gu_q.cols, down_q.cols) != (2 * I, K, I):
+        raise ValueError(f"{who}: weights [{gu_q.rows}, {gu_q.cols}] and [{N}, {down_q.cols}] for x [..., {K}] and the "
+                         f"intermediate size {I}")
+    weights = [t.contiguous() for t in (gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)]
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    gu = _new_mxint8(M, 2 * I, x.device) if keep_gu else None
+    copies = [None] * 4
+    for at, keep, n in ((0, keep_x, K), (2, keep_h, I)):
+        if keep:
+            copies[at] = torch.empty((n, (M + 15) // 16 * 16), dtype=torch.int8, device=x.device)
+            copies[at + 1] = torch.empty(n, dtype=torch.float32, device=x.device)
+    ws, nbytes = _call_workspace(_geglu_mlp_int8_forward_ws_cached(M, K, I, N, keep_x, keep_h), x)
+    data, exps = (gu.data, gu.exps) if keep_gu else (None, None)
+    _call("bf8_geglu_mlp_int8_forward", idx, _lib.lib().bf8_geglu_mlp_int8_forward, x.data_ptr(), M, K, I, N,
+          *(t.data_ptr() for t in weights), y.data_ptr(), _ptr(data), _ptr(exps), *(_ptr(t) for t in copies), ws.data_ptr(), nbytes)
+    return (y, data, exps, *copies)
+
+
+@functools.lru_cache(maxsize=4096)
 def _geglu_mlp_int8_backward_ws_cached(*args):
     return int(_lib.lib().bf8_geglu_mlp_int8_backward_workspace(*args))
 

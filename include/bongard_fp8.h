@@ -697,6 +697,18 @@ int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, cons
                         int64_t ldw, const float* w_scale, int64_t M, int64_t I, int64_t K, void* H,
                         int8_t* GU8, uint8_t* GU8_exp, void* stream);
 
+/* The training forward of the gated MLP in int8: Y bf16 [M, N] of bf16 x [M, K] and the row copies of W_gu
+ * [2 I, K] (gate rows then up rows) and W_down [N, I], x and H quantized by row, and where given the checkpoint
+ * of the pre-activations as bf8_gemm_geglu_int8's and the columnwise copies Xt [K, M rounded up to 16] and Ht
+ * [I, M rounded up to 16] with scales [K] and [I]. K a multiple of 16, I of 128, 32768 at most, N of 8. ws:
+ * bf8_geglu_mlp_int8_forward_workspace(M, K, I, N, Xt?, Ht?) bytes, 256-byte aligned. */
+size_t bf8_geglu_mlp_int8_forward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int keep_x,
+                                            int keep_h);
+int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, int64_t N, const int8_t* W_gu,
+                               const float* w_gu_scale, const int8_t* W_down, const float* w_down_scale,
+                               void* Y, int8_t* GU8, uint8_t* GU8_exp, int8_t* Xt, float* xt_scale,
+                               int8_t* Ht, float* ht_scale, void* ws, size_t ws_bytes, void* stream);
+
 /* The backward of the gated MLP in int8 from dy bf16 [M, N]: dH [M, I] and dW_down [N, I] as
  * bf8_linear_int8_backward (Wt_down [I, N] and Ht [I, M rounded up to 16], the columnwise copies of W_down and
  * H, with scales [I]), dGU [M, 2 I] from the checkpoint GU8 [M, 2 I] with GU8_exp as bf8_geglu_bwd_mxint8, then

@@ -118,7 +118,16 @@ def _calls(L):
     lb, mb = L.bf8_linear_int8_backward, 1 << 20
     lg, lf = L.bf8_linear_geglu_int8, L.bf8_linear_int8_forward
     gb, kept, big = L.bf8_geglu_mlp_int8_backward, (p,) * 10, 1 << 30
+    gf, w4 = L.bf8_geglu_mlp_int8_forward, (p,) * 4
     return [
+        (gf, (p, 0, 16, 128, 16, *w4, p, p, p, p, p, p, p, p, big, null), "empty"),
+        (gf, (p, 4, 24, 128, 16, *w4, p, p, p, p, p, p, p, p, big, null), "K % 16"),
+        (gf, (p, 4, 16, 96, 16, *w4, p, p, p, p, p, p, p, p, big, null), "I % 128"),
+        (gf, (p, 4, 16, 128, 12, *w4, p, p, p, p, p, p, p, p, big, null), "N % 8"),
+        (gf, (p, 4, 16, 128, 16, *w4, null, p, p, p, p, p, p, p, big, null), "NULL"),
+        (gf, (p, 4, 16, 128, 16, *w4, p, p, null, p, p, p, p, p, big, null), "NULL"),
+        (gf, (p, 4, 16, 128, 16, *w4, p, p, p, p, p, p, null, p, big, null), "NULL"),
+        (gf, (p, 4, 16, 128, 16, *w4, p, p, p, p, p, p, p, p, 64, null), "workspace needs"),
         (gb, (p, 0, 16, 32, 16, *kept, p, p, p, p, big, null), "empty"),
         (gb, (p, 4, 16, 24, 16, *kept, p, p, p, p, big, null), "I % 32"),
         (gb, (p, 4, 16, 16416, 16, *kept, p, p, p, p, big, null), "16384"),
