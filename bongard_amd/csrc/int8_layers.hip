@@ -185,14 +185,15 @@ int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, co
   void* const rest = base + w.rest;
   const size_t rest_bytes = ws_bytes - w.rest;
   if (const int rc = bf8_quantize_int8_bf16(dy, M, N, rows, rs, cols, cs, rest, rest_bytes, stream)) return rc;
-  if (dx)
-    if (const int rc = bf8_gemm_int8(rows, N, rs, Wt, N, wt_scale, M, K, N, nullptr, dx, BF8_OUT_BF16, K, rest,
+  const int64_t Mp = pad16(M);
+  if (dw)
+    if (const int rc = bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, N, K, Mp, nullptr, dw, BF8_OUT_BF16, K, rest,
                                      rest_bytes, stream))
       return rc;
-  if (!dw) return BF8_OK;
-  const int64_t Mp = pad16(M);
-  return bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, N, K, Mp, nullptr, dw, BF8_OUT_BF16, K, rest, rest_bytes,
-                       stream);
+  // (dx last: what reads it next finds it in the caches)
+  return dx ? bf8_gemm_int8(rows, N, rs, Wt, N, wt_scale, M, K, N, nullptr, dx, BF8_OUT_BF16, K, rest, rest_bytes,
+                            stream)
+            : BF8_OK;
 }
 
 size_t bf8_geglu_mlp_int8_forward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int keep_x, int keep_h) {
@@ -269,14 +270,14 @@ int bf8_geglu_mlp_int8_backward(const void* dy, int64_t M, int64_t K, int64_t I,
                                                             stream)
                             : bf8_quantize_int8_bf16(dGU, M, 2 * I, rows, rs, cols, cs, rest, rest_bytes, stream))
     return rc;
-  if (dx)
-    if (const int rc = bf8_gemm_int8(rows, 2 * I, rs, Wt_gu, 2 * I, wt_gu_scale, M, K, 2 * I, nullptr, dx,
-                                     BF8_OUT_BF16, K, rest, rest_bytes, stream))
-      return rc;
-  if (!dW_gu) return BF8_OK;
   const int64_t Mp = pad16(M);
-  return bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, 2 * I, K, Mp, nullptr, dW_gu, BF8_OUT_BF16, K, rest,
-                       rest_bytes, stream);
+  if (dW_gu)
+    if (const int rc = bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, 2 * I, K, Mp, nullptr, dW_gu, BF8_OUT_BF16, K,
+                                     rest, rest_bytes, stream))
+      return rc;
+  return dx ? bf8_gemm_int8(rows, 2 * I, rs, Wt_gu, 2 * I, wt_gu_scale, M, K, 2 * I, nullptr, dx, BF8_OUT_BF16, K,
+                            rest, rest_bytes, stream)
+            : BF8_OK;
 }
 
 }  // extern "C"

@@ -697,10 +697,10 @@ class Int8GegluMlpFunction(_Fp8Function):
             _check_int8_tokens("int8 gated MLP", x.shape[0])
         if gu_q is not None and down_q is not None and not (keep or need_dd):
             return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
-        if gu_q is None or (need_dx and gu_q.data_t is None):
-            gu_q = quantize_weight_int8(w_gu, transpose=need_dx)
         if down_q is None or (keep and down_q.data_t is None):
             down_q = quantize_weight_int8(w_down, transpose=keep)
+        if gu_q is None or (need_dx and gu_q.data_t is None):  # (last: its codes are read first)
+            gu_q = quantize_weight_int8(w_gu, transpose=need_dx)
         ctx.shapes = x.shape, w_gu.shape, w_down.shape
         if not x.shape[0]:  # nothing to launch (its gradients are zeros)
             return x.new_empty((0, w_down.shape[0]), dtype=torch.bfloat16)
