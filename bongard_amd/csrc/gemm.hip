@@ -15,6 +15,7 @@
 #include <cstring>
 
 #include "gemm_kernel.hpp"
+#include "int8.hpp"
 
 namespace bf8 {
 namespace {
@@ -1327,7 +1328,21 @@ int bf8_gemm_int8(const int8_t* A, int64_t lda, const float* a_scale, const int8
 int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
                         const float* w_scale, int64_t M, int64_t I, int64_t K, void* H, int8_t* GU8,
                         uint8_t* GU8_exp, void* stream) {
-  const char* who = "bf8_gemm_geglu_int8";
+  return gemm_geglu_int8("bf8_gemm_geglu_int8", X, ldx, x_scale, W, ldw, w_scale, M, I, K, H, GU8, GU8_exp, nullptr,
+                         stream);
+}
+
+}  // extern "C"
+
+namespace bf8 {
+
+bool geglu_int8_leaves_maxima(int64_t M, int64_t I, int64_t K) {
+  return kept_plan(kFmtInt8, M, 2 * I, K, true, 0).tile == TILE_256x256w8;
+}
+
+int gemm_geglu_int8(const char* who, const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
+                    const float* w_scale, int64_t M, int64_t I, int64_t K, void* H, int8_t* GU8, uint8_t* GU8_exp,
+                    const Int8Maxima* hm, void* stream) {
   BF8_CHECK(M >= 0 && I >= 0 && K >= 0, "%s: negative shape", who);
   BF8_CHECK(I % 128 == 0, "%s: I must be a multiple of 128 (got %lld)", who, (long long)I);
   BF8_CHECK(K % 16 == 0 && K <= kInt8MaxK, "%s: need K %% 16 == 0 and K <= %lld (got %lld)", who,
@@ -1345,7 +1360,12 @@ int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, cons
   p.C = H; p.ldc = I;
   p.gu8 = GU8; p.gu8_e = GU8_exp;
   const Plan pl = kept_plan(kFmtInt8, M, 2 * I, K, true, 0);
+  if (hm) {
+    BF8_CHECK(pl.tile == TILE_256x256w8, "%s: no maxima of H under this plan", who);
+    p.h_rowpart = hm->rowpart;
+    p.h_colpart = hm->colpart;
+  }
   return launch_plan(pl, p, EPI_GEGLU, BF8_OUT_BF16, kFmtInt8, kFmtInt8, nullptr, as_stream(stream));
 }
 
-}  // extern "C"
+}  // namespace bf8

@@ -50,6 +50,7 @@ struct GemmParams {
   uint16_t* GU;
   int8_t* gu8;     // int8 GEGLU: the pre-activations as blocks of 32 codes (int8.hpp) [M, 2I] instead of
   uint8_t* gu8_e;  // GU, with their bytes [M, 2I / 32]
+  uint16_t *h_rowpart, *h_colpart;  // int8 GEGLU on 256x256w8: H's maxima (int8_tile_maxima), or NULL
   uint32_t* partials;     // GEGLU: one amax key of |H| per tile
   // GEGLU with H quantized in the epilogue (C, the bf16 H, may then be NULL). h8: e4m3
   // [M, I]; h8t (optional, needs M % 32 == 0): e4m3 H^T [I, M]. MX: E8M0 block scales
@@ -145,5 +146,12 @@ using Tile128x128k2 = GemmTile<2, 2, 2, 2, 2, 1, 2>;
 template <class T>
 int launch_gemm_tile(const GemmParams& p, int epi, int out_dtype, int fmt_a, int fmt_b,
                      hipStream_t stream, bool mx);
+
+// bf8_gemm_geglu_int8, H's maxima in tiles left in hm (NULL: none). Only where the plan for that shape leaves them.
+struct Int8Maxima;
+bool geglu_int8_leaves_maxima(int64_t M, int64_t I, int64_t K);
+int gemm_geglu_int8(const char* who, const int8_t* X, int64_t ldx, const float* x_scale, const int8_t* W, int64_t ldw,
+                    const float* w_scale, int64_t M, int64_t I, int64_t K, void* H, int8_t* GU8, uint8_t* GU8_exp,
+                    const Int8Maxima* hm, void* stream);
 
 }  // namespace bf8

@@ -559,6 +559,43 @@ __device__ __forceinline__ void mxi8_gu_epilogue(const GemmParams& p, const uint
   }
 }
 
+// The maxima of H for its int8 codes (Int8Maxima, int8.hpp) on the eight-wave tile: a wave's 128 rows by 32 columns,
+// 16 rows a step (four lanes a row, 8 columns each). The rows' meet in LDS over the four waves beside each other,
+// the columns' stay in registers: a strip of 128 rows each. The pass over H that would find them is saved: of 22 us at
+// 4096 x 10240 ten stay saved, the product 1-2 longer and the codes' pass 9, which reads H from memory then.
+struct TileMaxima {
+  uint16_t* rows;  // (LDS) the wave's of [4][256]
+  uint4 cols;
+  __device__ __forceinline__ void add(uint4 d, int row, int lane) {
+    const uint4 a = make_uint4(d.x & 0x7FFF7FFFu, d.y & 0x7FFF7FFFu, d.z & 0x7FFF7FFFu, d.w & 0x7FFF7FFFu);
+    cols = make_uint4(pk_max_u16(cols.x, a.x), pk_max_u16(cols.y, a.y), pk_max_u16(cols.z, a.z),
+                      pk_max_u16(cols.w, a.w));
+    const uint32_t m = quad_max(absmax16(d));
+    if ((lane & 3) == 0) rows[row] = (uint16_t)m;
+  }
+  // n0: the tile's first column; every thread t of the block calls it
+  __device__ __forceinline__ void store(const GemmParams& p, int m0, int n0, int wave_m0, int lane, int t) {
+#pragma unroll
+    for (int off = 4; off < 64; off <<= 1)
+      cols = make_uint4(pk_max_u16(cols.x, (uint32_t)__shfl_xor((int)cols.x, off, 64)),
+                        pk_max_u16(cols.y, (uint32_t)__shfl_xor((int)cols.y, off, 64)),
+                        pk_max_u16(cols.z, (uint32_t)__shfl_xor((int)cols.z, off, 64)),
+                        pk_max_u16(cols.w, (uint32_t)__shfl_xor((int)cols.w, off, 64)));
+    const int wn = t >> 7, strip = (m0 + wave_m0) >> 7;  // (waves go down the rows first)
+    if (lane < 4 && m0 + wave_m0 < p.M)
+      *reinterpret_cast<uint4*>(p.h_colpart + (int64_t)strip * p.I + n0 + 32 * wn + 8 * lane) = cols;
+    const uint16_t* const all = rows - 256 * wn - wave_m0;
+    __syncthreads();
+    const int64_t pad = int8_row_pad(p.M);
+    if (t < 128 && m0 + 2 * t < pad) {
+      uint32_t k = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) k = pk_max_u16(k, reinterpret_cast<const uint32_t*>(all + 256 * w)[t]);
+      *reinterpret_cast<uint32_t*>(p.h_rowpart + (int64_t)(n0 >> 7) * pad + m0 + 2 * t) = k;
+    }
+  }
+};
+
 // The operand fragments of one MFMA sub-step as 16-byte halves, in the order the MFMAs
 // of the sub-step consume them: b0, a0 .. a(FM-1), b1 .. b(FN-1).
 template <int NH>
@@ -1441,6 +1478,14 @@ gemm_kernel(GemmParams p) {
       uint16_t* dst = pass == 0 ? reinterpret_cast<uint16_t*>(p.C) : p.GU;
       const int64_t ld = pass == 0 ? p.ldc : 2 * (int64_t)p.I;
       const int coff = pass == 2 ? p.I : 0;
+      constexpr bool kMaxima = I8 && pass == 0 && NW == 8 && BM == 256 && BN == 256;
+      TileMaxima h_maxima;
+      if constexpr (kMaxima) {
+        static_assert(ROWS == 128 && CH == 4 && kGeluA32Bytes + NW * ROWS * CH * 16 + 2048 <= NS * kStage,
+                      "the rows' maxima fit past the staging");
+        h_maxima.rows = reinterpret_cast<uint16_t*>(smem + kGeluA32Bytes + NW * ROWS * CH * 16) + 256 * wn + wave_m0;
+        h_maxima.cols = make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll 4
       for (int it = 0; it < ROWS * CH / 64; ++it) {
         const int idx = it * 64 + lane;
@@ -1448,6 +1493,12 @@ gemm_kernel(GemmParams p) {
         const uint4 d = stage_get<CH>(wbuf, row, c);
         const int gm = m0 + wave_m0 + row;
         if (gm < p.M) store_bf16x8(dst + (int64_t)gm * ld + coff + wave_h0 + c * 8, d, ld);
+        if constexpr (kMaxima) {
+          if (p.h_rowpart) h_maxima.add(gm < p.M ? d : make_uint4(0u, 0u, 0u, 0u), row, lane);
+        }
+      }
+      if constexpr (kMaxima) {
+        if (p.h_rowpart) h_maxima.store(p, m0, n0, wave_m0, lane, t);
       }
     };
     // Eight-wave tiles store the pre-activations kept for the backward first, so their

@@ -480,6 +480,11 @@ int launch_pair(const uint16_t* x, int rows, int cols, int8_t* out, float* row_s
 }
 
 }  // namespace
+
+int int8_codes_of_maxima(const uint16_t* x, const Int8Maxima& p, int8_t* out, float* row_scale, int8_t* out_t,
+                         float* col_scale, hipStream_t s) {
+  return launch_tiles(x, p, out, row_scale, out_t, col_scale, s);
+}
 }  // namespace bf8
 
 using namespace bf8;

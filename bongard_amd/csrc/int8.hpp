@@ -85,6 +85,19 @@ inline size_t int8_maxima_bytes(int64_t rows, int64_t cols, int halves = 1) {
   const Int8Maxima p = int8_maxima(nullptr, rows, cols, halves);
   return (size_t)((uint8_t*)p.colpart - (uint8_t*)p.rowpart) + (size_t)p.strips * cols * 2;
 }
+// The layout that the gated product's 256 x 128 tiles of H leave, by 128 x 128: row tiles of 128 columns.
+inline Int8Maxima int8_tile_maxima(void* ws, int64_t rows, int64_t cols) {
+  Int8Maxima p{rows, cols, (int)(cols / 128), 128, (int)((rows + 127) / 128), (uint16_t*)ws, nullptr};
+  p.colpart = p.rowpart + ((size_t)p.row_tiles * int8_row_pad(rows) + 127) / 128 * 128;
+  return p;
+}
+inline size_t int8_tile_maxima_bytes(int64_t rows, int64_t cols) {
+  const Int8Maxima p = int8_tile_maxima(nullptr, rows, cols);
+  return (size_t)((uint8_t*)p.colpart - (uint8_t*)p.rowpart) + (size_t)p.strips * cols * 2;
+}
+// The codes of x from its maxima (bf8_quantize_int8_maxima_bf16 without its checks).
+int int8_codes_of_maxima(const uint16_t* x, const Int8Maxima& p, int8_t* out, float* row_scale, int8_t* out_t,
+                         float* col_scale, hipStream_t s);
 
 // The maxima of a wave's eight rows r .. r + 7 (zeros past the tensor's) by 512 columns (lane l: columns 8 l ..
 // +7 of column tile tc), row by row: into colmax and, the rows', to rowpart. Two rows share a dword; three

@@ -82,7 +82,7 @@ MlpForwardWs mlp_forward_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool kee
   w.rest = p.at;
   size_t rest = bf8_gemm_int8_workspace(M, N, I);
   if (keep_x) rest = std::max(rest, bf8_quantize_int8_workspace(M, K, 1));
-  if (keep_h) rest = std::max(rest, bf8_quantize_int8_workspace(M, I, 1));
+  if (keep_h) rest = std::max({rest, bf8_quantize_int8_workspace(M, I, 1), int8_tile_maxima_bytes(M, I)});
   w.bytes = w.rest + rest;
   return w;
 }
@@ -221,8 +221,15 @@ int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, i
   void *const H = base + w.h, *const rest = base + w.rest;
   const size_t rest_bytes = ws_bytes - w.rest;
   if (const int rc = bf8_quantize_int8_bf16(x, M, K, x8, xs, Xt, xt_scale, rest, rest_bytes, stream)) return rc;
-  if (const int rc = bf8_gemm_geglu_int8(x8, K, xs, W_gu, K, w_gu_scale, M, I, K, H, GU8, GU8_exp, stream)) return rc;
-  if (const int rc = bf8_quantize_int8_bf16(H, M, I, h8, hs, Ht, ht_scale, rest, rest_bytes, stream)) return rc;
+  // both copies of H by the maxima that the product leaves, where it does
+  const bool maxima = Ht && geglu_int8_leaves_maxima(M, I, K);
+  const Int8Maxima hm = int8_tile_maxima(rest, M, I);
+  if (const int rc = gemm_geglu_int8(who, x8, K, xs, W_gu, K, w_gu_scale, M, I, K, H, GU8, GU8_exp,
+                                     maxima ? &hm : nullptr, stream))
+    return rc;
+  if (const int rc = maxima ? int8_codes_of_maxima((const uint16_t*)H, hm, h8, hs, Ht, ht_scale, as_stream(stream))
+                            : bf8_quantize_int8_bf16(H, M, I, h8, hs, Ht, ht_scale, rest, rest_bytes, stream))
+    return rc;
   return bf8_gemm_int8(h8, I, hs, W_down, I, w_down_scale, M, N, I, nullptr, Y, BF8_OUT_BF16, N, rest, rest_bytes,
                        stream);
 }

@@ -625,6 +625,30 @@ def test_mlp_function_is_its_ops(gpu, M, K, I):
     assert not any(bool(g.any()) for g in grads)
 
 
+@pytest.mark.parametrize("tile", ["256x256w8", "128x128", ""])
+@pytest.mark.parametrize("M,K,I", [(1, 32, 128), (129, 96, 256), (513, 256, 384), (1100, 320, 640)])
+def test_copies_of_h_in_the_mlps_forward(gpu, monkeypatch, tile, M, K, I):
+    """H's columnwise codes and the result from the maxima that the eight-wave tile leaves, and where none does: the
+    quantizer's of the product's H, a token of inf among them."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    x, w_gu, w_d, _ = _mlp_inputs(M, K, I, 6, gpu)
+    for bad in (False, True):
+        if bad:
+            x[M // 2, 3] = float("inf")
+        xq, gq, dq = (ops.quantize_int8(t) for t in (x, w_gu, w_d))
+        H, gu = ops.gemm_geglu_int8(xq.data, xq.row_scale, gq.data, gq.row_scale, I, keep_gu=True)
+        hq = ops.quantize_int8(H, colwise=True)
+        want = ops.gemm_int8(hq.data, hq.row_scale, dq.data, dq.row_scale)
+        y, gu8, exps, x_t, x_s, h_t, h_s = ops._geglu_mlp_int8_forward(x, I, gq, dq, True, False, True)
+        assert x_t is None and x_s is None
+        same = lambda a, b: torch.equal(a.view(torch.uint8), b.view(torch.uint8))  # noqa: E731
+        assert same(y, want) and same(gu8, gu.data) and same(exps, gu.exps)
+        assert torch.equal(h_t, hq.data_t) and same(h_s, hq.col_scale)
+        assert bool(torch.isnan(h_s).all()) == bad
+        y, *kept = ops._geglu_mlp_int8_forward(x, I, gq, dq, False, False, False)
+        assert same(y, want) and kept == [None] * 6
+
+
 class _Mlp(nn.Module):
     def __init__(self, hidden, inter):
         super().__init__()
