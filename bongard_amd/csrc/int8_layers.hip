@@ -24,9 +24,10 @@ struct Parts {
   }
 };
 
-// The row copies of x and W, then what the quantizations or the product need.
+// The row copies of x and W, then what the quantizations or the product need. (least: without the product's, which runs
+// a plan that needs less where less is there.)
 struct ForwardWs {
-  size_t x, x_scale, w, w_scale, rest, bytes;
+  size_t x, x_scale, w, w_scale, rest, least, bytes;
 };
 ForwardWs forward_ws(int64_t M, int64_t N, int64_t K, bool keep_x, bool keep_w) {
   ForwardWs f{};
@@ -36,16 +37,17 @@ ForwardWs forward_ws(int64_t M, int64_t N, int64_t K, bool keep_x, bool keep_w) 
   f.w = p.take((size_t)N * K);
   f.w_scale = p.take((size_t)N * 4);
   f.rest = p.at;
-  size_t rest = bf8_gemm_int8_workspace(M, N, K);
+  size_t rest = 0;
   if (keep_x) rest = std::max(rest, bf8_quantize_int8_workspace(M, K, 1));
   if (keep_w) rest = std::max(rest, bf8_quantize_int8_workspace(N, K, 1));
-  f.bytes = f.rest + rest;
+  f.least = f.rest + rest;
+  f.bytes = f.rest + std::max(rest, bf8_gemm_int8_workspace(M, N, K));
   return f;
 }
 
 // dy's codes and scales by row and by column, then what the quantization or a product needs.
 struct BackwardWs {
-  size_t rows, row_scale, cols, col_scale, rest, bytes;
+  size_t rows, row_scale, cols, col_scale, rest, least, bytes;
 };
 BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
   const int64_t Mp = pad16(M);
@@ -61,6 +63,7 @@ BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
   }
   w.rest = p.at;
   size_t rest = dw ? bf8_quantize_int8_workspace(M, N, dx) : 0;
+  w.least = w.rest + rest;
   if (dx) rest = std::max(rest, bf8_gemm_int8_workspace(M, K, N));
   if (dw) rest = std::max(rest, bf8_gemm_int8_workspace(N, K, Mp));
   w.bytes = w.rest + rest;
@@ -69,7 +72,7 @@ BackwardWs backward_ws(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
 
 // x's and H's row copies, H (bf16), and what the quantizations or the down product need.
 struct MlpForwardWs {
-  size_t x, x_scale, h, h8, h_scale, rest, bytes;
+  size_t x, x_scale, h, h8, h_scale, rest, least, bytes;
 };
 MlpForwardWs mlp_forward_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool keep_x, bool keep_h) {
   MlpForwardWs w{};
@@ -80,10 +83,11 @@ MlpForwardWs mlp_forward_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool kee
   w.h8 = p.take((size_t)M * I);
   w.h_scale = p.take((size_t)M * 4);
   w.rest = p.at;
-  size_t rest = bf8_gemm_int8_workspace(M, N, I);
+  size_t rest = 0;
   if (keep_x) rest = std::max(rest, bf8_quantize_int8_workspace(M, K, 1));
   if (keep_h) rest = std::max({rest, bf8_quantize_int8_workspace(M, I, 1), int8_tile_maxima_bytes(M, I)});
-  w.bytes = w.rest + rest;
+  w.least = w.rest + rest;
+  w.bytes = w.rest + std::max(rest, bf8_gemm_int8_workspace(M, N, I));
   return w;
 }
 
@@ -91,7 +95,7 @@ MlpForwardWs mlp_forward_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool kee
 // their maxima and the products need.
 constexpr int64_t kMaximaRows = 1024;  // (as the gated backward's codes alone: from here on by the maxima it leaves)
 struct MlpWs {
-  size_t dh, linear, dgu, rows, row_scale, cols, col_scale, rest, bytes;
+  size_t dh, linear, dgu, rows, row_scale, cols, col_scale, rest, least, bytes;
 };
 MlpWs mlp_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool dx, bool dgu, bool dd) {
   MlpWs w{};
@@ -99,8 +103,9 @@ MlpWs mlp_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool dx, bool dgu, bool
   const bool dh = dx || dgu;
   if (dh) w.dh = p.take((size_t)M * I * 2);
   w.linear = p.at;
-  const size_t linear = bf8_linear_int8_backward_workspace(M, N, I, dh, dd);
-  w.bytes = w.linear + linear;
+  const BackwardWs linear = backward_ws(M, N, I, dh, dd);
+  w.least = w.linear + linear.least;
+  w.bytes = w.linear + linear.bytes;
   if (!dh) return w;
   w.dgu = p.take((size_t)M * 2 * I * 2);
   if (dx) {
@@ -113,6 +118,7 @@ MlpWs mlp_ws(int64_t M, int64_t K, int64_t I, int64_t N, bool dx, bool dgu, bool
   }
   w.rest = p.at;
   size_t rest = M >= kMaximaRows ? bf8_geglu_bwd_mxint8_maxima(M, I) : dgu ? bf8_quantize_int8_workspace(M, 2 * I, dx) : 0;
+  w.least = std::max(w.least, w.rest + rest);
   if (dx) rest = std::max(rest, bf8_gemm_int8_workspace(M, K, 2 * I));
   if (dgu) rest = std::max(rest, bf8_gemm_int8_workspace(2 * I, K, pad16(M)));
   w.bytes = std::max(w.bytes, w.rest + rest);
@@ -145,8 +151,8 @@ int bf8_linear_int8_forward(const void* x, const void* W, int64_t M, int64_t N, 
   BF8_CHECK(M < (1LL << 31) && N < (1LL << 31) && std::max(M, N) * K < (1LL << 31),
             "%s: operands of 2 GiB and more", who);
   const ForwardWs f = forward_ws(M, N, K, Xt, Wt);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= f.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, f.bytes, ws_bytes);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= f.least,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, f.least, ws_bytes);
   int8_t* const base = (int8_t*)ws;
   float *const xs = (float*)(base + f.x_scale), *const wsc = (float*)(base + f.w_scale);
   void* const rest = base + f.rest;
@@ -176,8 +182,8 @@ int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, co
   const int64_t most = std::max(dx ? std::max(M, K) * N : 0, dw ? std::max(N, K) * pad16(M) : 0);
   BF8_CHECK(M < (1LL << 31) && K < (1LL << 31) && most < (1LL << 31), "%s: operands of 2 GiB and more", who);
   const BackwardWs w = backward_ws(M, N, K, dx, dw);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.least,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.least, ws_bytes);
   int8_t* const base = (int8_t*)ws;
   int8_t *const rows = dx ? base + w.rows : nullptr, *const cols = dw ? base + w.cols : nullptr;
   float* const rs = dx ? (float*)(base + w.row_scale) : nullptr;
@@ -213,8 +219,8 @@ int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, i
                 (Xt == nullptr) == (xt_scale == nullptr) && (Ht == nullptr) == (ht_scale == nullptr),
             "%s: NULL pointer", who);
   const MlpForwardWs w = mlp_forward_ws(M, K, I, N, Xt, Ht);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.least,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.least, ws_bytes);
   uint8_t* const base = (uint8_t*)ws;
   int8_t *const x8 = (int8_t*)base + w.x, *const h8 = (int8_t*)base + w.h8;
   float *const xs = (float*)(base + w.x_scale), *const hs = (float*)(base + w.h_scale);
@@ -256,8 +262,8 @@ int bf8_geglu_mlp_int8_backward(const void* dy, int64_t M, int64_t K, int64_t I,
   BF8_CHECK(!(dW_gu || dW_down) || M <= kInt8MaxK, "%s: for a weight's gradient M is %lld at most", who,
             (long long)kInt8MaxK);
   const MlpWs w = mlp_ws(M, K, I, N, dx, dW_gu, dW_down);
-  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.bytes,
-            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.bytes, ws_bytes);
+  BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.least,
+            "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.least, ws_bytes);
   uint8_t* const base = (uint8_t*)ws;
   void* const dH = dh ? base + w.dh : nullptr;
   if (const int rc = bf8_linear_int8_backward(dy, M, N, I, Wt_down, wt_down_scale, Ht, ht_scale, dH, dW_down,

@@ -625,6 +625,25 @@ def test_mlp_function_is_its_ops(gpu, M, K, I):
     assert not any(bool(g.any()) for g in grads)
 
 
+def test_a_plan_named_after_a_layer_has_run(gpu, monkeypatch):
+    """The products of a layer's calls are as asked for by then, or without the K pieces that the workspace cannot
+    hold: the same values."""
+    M, K, I = 140, 1152, 1280
+    x, w_gu, w_d, dy = _mlp_inputs(M, K, I, 8, gpu)
+    leaves = [t.requires_grad_() for t in (x, w_gu, w_d)]
+
+    def f():
+        y = linear.Int8LinearFunction.apply(leaves[0], leaves[1], None, None)
+        z = linear.Int8GegluMlpFunction.apply(*leaves, None, None, I)
+        return [y, z, *torch.autograd.grad(y, leaves[:2], torch.ones_like(y)), *torch.autograd.grad(z, leaves, dy)]
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", "256x256w8")
+    want = f()
+    for tile in ("128x64:8", "64x128:4", "", "256x256w8:2"):
+        monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+        for a, b in zip(f(), want):
+            assert torch.equal(a, b), tile
+
+
 @pytest.mark.parametrize("tile", ["256x256w8", "128x128", ""])
 @pytest.mark.parametrize("M,K,I", [(1, 32, 128), (129, 96, 256), (513, 256, 384), (1100, 320, 640)])
 def test_copies_of_h_in_the_mlps_forward(gpu, monkeypatch, tile, M, K, I):
