@@ -631,11 +631,22 @@ def _check_int8_tokens(who, rows):
         raise ValueError(f"{who}: a weight gradient takes {_INT8_MAX_TOKENS} tokens at most (got {rows})")
 
 
-class Int8LinearFunction(_Fp8Function):
+class _Int8Function(_Fp8Function):
+    """Base of the int8 functions, which see x as rows: [M, K] of x [..., K], and give y [..., N]."""
+
+    @classmethod
+    def apply(cls, x, *args):
+        if x.dim() == 2:
+            return super().apply(x, *args)
+        y = super().apply(x.reshape(-1, x.shape[-1]), *args)
+        return y.view(*x.shape[:-1], y.shape[-1])
+
+
+class Int8LinearFunction(_Int8Function):
     """y = x @ W^T (+ b) with every tensor in 8-bit integers, one scale for each token or channel
-    (gradients included; round to nearest even), sums exact in int32; x: bf16 [M, K], any M (133120 at most
-    where W's gradient is asked for); W [N, K],
-    K a multiple of 16, N of 8 (of 16 for gradients). ``wq``: a cached int8 weight
+    (gradients included; round to nearest even), sums exact in int32; x: bf16 [..., K], any number of rows
+    (133120 at most where W's gradient is asked for); W [N, K],
+    K a multiple of 16, N of 8 (of 16 for gradients). ``wq``: a cached int8 copy of W
     (:func:`quantize_weight_int8`) or None.
 
       forward  y  = X8 . W8^T           scales by token and by output channel
@@ -678,13 +689,14 @@ class Int8LinearFunction(_Fp8Function):
         return dx, dw, ops.column_sums(dy) if need_db else None, None
 
 
-class Int8GegluMlpFunction(_Fp8Function):
+class Int8GegluMlpFunction(_Int8Function):
     """The gated MLP of :class:`Fp8GegluMlpFunction` with every product in 8-bit integers
     (:class:`Int8LinearFunction`'s granularity) and the pre-activations kept for the backward as an
     8-bit checkpoint, half the bytes of bf16: the gate/up product with the gated GELU and the checkpoint
     in its epilogue, the down product; backward through dH, the gelu chain on the checkpoint's values and
-    the dgrad/wgrad products. x: bf16 [M, K], any M (133120 at most where a weight's gradient is asked
-    for); w_gu [2I, K], w_down [K_out, I], K and K_out multiples of 16, I of 128. ``gu_q`` / ``down_q``: optional cached int8 weights. TEMLP / FusedMLP under
+    the dgrad/wgrad products. x: bf16 [..., K], any number of rows (133120 at most where a weight's
+    gradient is asked for); w_gu [2I, K], w_down [K_out, I], K and K_out multiples of 16, I of 128. ``gu_q`` /
+    ``down_q``: optional cached int8 copies of the weights. TEMLP / FusedMLP under
     'int8' (bongard/te_linear.py:98-103, bongard/fused_mlp.py:25-33 for the chain)."""
 
     @staticmethod

@@ -969,3 +969,29 @@ def test_refusals(gpu):
         ops.geglu_bwd_mxint8(x, ops.quantize_mxint8(x))
     with pytest.raises(ValueError, match="checkpoint must be"):
         ops.dequant_mxint8(ops.MxInt8Tensor(q.data, q.data))
+
+
+@pytest.mark.parametrize("shape", [(3, 7, 32), (1, 300, 32), (32,), (0, 4, 32)])
+def test_functions_of_batched_rows(gpu, shape):
+    """x of any number of dimensions: the values and the gradients of its rows, in its shape (x longer than K among
+    them, whose rows the backward must not take for K)."""
+    I, N = 128, 48
+    M = torch.Size(shape[:-1]).numel()
+    x = _x(M + 1, 32, 1, False)[:M].to(gpu).view(shape)
+    w, w_gu, w_d = (_x(*s, 7, False).to(gpu) for s in ((N, 32), (2 * I, 32), (N, I)))
+    copies = [linear.quantize_weight_int8(t) for t in (w, w_gu, w_d)]
+    for cached in (False, True):
+        wq, gq, dq = copies if cached else (None,) * 3
+        for f, weights in ((lambda t, a: linear.Int8LinearFunction.apply(t, a, None, wq), (w,)),
+                           (lambda t, a, b: linear.Int8GegluMlpFunction.apply(t, a, b, gq, dq, I), (w_gu, w_d))):
+            leaves = [t.detach().requires_grad_() for t in (x, *weights)]
+            rows = [t.detach().requires_grad_() for t in (x.reshape(-1, 32), *weights)]
+            y, want = f(*leaves), f(*rows)
+            assert y.shape == (*shape[:-1], N) and torch.equal(y.reshape(-1, N), want)
+            dy = torch.ones_like(want)
+            got = torch.autograd.grad(y, leaves, dy.view(y.shape))
+            for a, b in zip(got, torch.autograd.grad(want, rows, dy)):
+                assert torch.equal(a.reshape(b.shape), b)
+            assert got[0].shape == x.shape
+            with torch.no_grad():
+                assert torch.equal(f(*leaves), y)

@@ -335,3 +335,32 @@ def test_layer_norm_refuses_forward_mode_tangents(monkeypatch):
                 dual = forward_ad.make_dual(args[name], torch.ones_like(args[name]))
                 with pytest.raises(NotImplementedError, match="jvp"):
                     fused_mlp.layer_norm(**{**args, name: dual})
+
+
+def _copy_of(rows, cols):
+    """An int8 weight's cached copies, as the functions take them."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.int8)  # noqa: E731
+    return ops.Int8Tensor(z(rows, cols), torch.ones(rows), z(cols, (rows + 15) // 16 * 16), torch.ones(cols), rows, cols)
+
+
+def test_functions_see_x_as_rows(monkeypatch):
+    """x of any number of dimensions reaches the int8 calls as [M, K] and its gradient comes back in its shape: the
+    backward's K is x's last size, not its second."""
+    seen = []
+
+    def forward(x, I, gu_q, down_q, *keep):
+        seen.append(tuple(x.shape))
+        return (torch.zeros(x.shape[0], down_q.rows, dtype=torch.bfloat16), *[None] * 6)
+
+    def backward(dy, K, I, needs, *kept):
+        seen.append((dy.reshape(-1, dy.shape[-1]).shape[0], K, I))
+        return torch.ones(dy.reshape(-1, dy.shape[-1]).shape[0], K, dtype=torch.bfloat16), None, None
+    monkeypatch.setattr(ops, "_geglu_mlp_int8_forward", forward)
+    monkeypatch.setattr(ops, "_geglu_mlp_int8_backward", backward)
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    for shape in ((6, 32), (2, 3, 32), (1, 64, 32), (32,), (2, 1, 2, 32)):
+        rows, x = z(*shape).numel() // 32, z(*shape).requires_grad_()
+        y = linear.Int8GegluMlpFunction.apply(x, z(256, 32), z(16, 128), _copy_of(256, 32), _copy_of(16, 128), 128)
+        assert y.shape == (*shape[:-1], 16)
+        y.backward(torch.ones_like(y))
+        assert x.grad.shape == x.shape and seen[-2:] == [(rows, 32), (rows, 32, 128)]
