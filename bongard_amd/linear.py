@@ -642,6 +642,12 @@ class _Int8Function(_Fp8Function):
         return y.view(*x.shape[:-1], y.shape[-1])
 
 
+def _check_int8_weight(who, name, q, weight):
+    """A cached copy is of the weight's size: the backward's sizes are the weight's."""
+    if q is not None and (q.rows, q.cols) != tuple(weight.shape):
+        raise ValueError(f"{who}: {name} is the copy of a weight [{q.rows}, {q.cols}], the weight is {list(weight.shape)}")
+
+
 class Int8LinearFunction(_Int8Function):
     """y = x @ W^T (+ b) with every tensor in 8-bit integers, one scale for each token or channel
     (gradients included; round to nearest even), sums exact in int32; x: bf16 [..., K], any number of rows
@@ -666,6 +672,7 @@ class Int8LinearFunction(_Int8Function):
         if wq is not None and not (need_dx or need_dw):  # (the same product; few tokens take one kernel)
             ctx.save_for_backward(None, None, None, None)
             return ops.linear_int8(dense_rows(x), wq.data, wq.row_scale, bias=bias)
+        _check_int8_weight("int8 linear", "wq", wq, weight)
         if wq is None or (need_dx and wq.data_t is None):
             y, *saved = ops.linear_int8_forward(x, weight, bias=bias, keep_x=need_dw, keep_w=need_dx)
             ctx.save_for_backward(*saved)
@@ -709,6 +716,11 @@ class Int8GegluMlpFunction(_Int8Function):
             _check_int8_tokens("int8 gated MLP", x.shape[0])
         if gu_q is not None and down_q is not None and not (keep or need_dd):
             return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
+        if w_gu.shape != (2 * I, x.shape[1]) or w_down.shape[1] != I:
+            raise ValueError(f"int8 gated MLP: weights {list(w_gu.shape)} and {list(w_down.shape)} for x [..., {x.shape[1]}] "
+                             f"and the intermediate size {I}")
+        _check_int8_weight("int8 gated MLP", "gu_q", gu_q, w_gu)
+        _check_int8_weight("int8 gated MLP", "down_q", down_q, w_down)
         if down_q is None or (keep and down_q.data_t is None):
             down_q = quantize_weight_int8(w_down, transpose=keep)
         if gu_q is None or (need_dx and gu_q.data_t is None):  # (last: its codes are read first)

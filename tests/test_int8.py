@@ -343,6 +343,26 @@ def _copy_of(rows, cols):
     return ops.Int8Tensor(z(rows, cols), torch.ones(rows), z(cols, (rows + 15) // 16 * 16), torch.ones(cols), rows, cols)
 
 
+def test_weights_and_their_copies_must_fit():
+    """The backward's sizes are the weights' and x's, its operands the cached copies: others would run it past their
+    ends. Refused by the forward, before any tensor is read."""
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, requires_grad=True)  # noqa: E731
+    x, w = z(4, 32), z(48, 32)
+    for q in (_copy_of(64, 32), _copy_of(48, 16), _copy_of(32, 48)):
+        with pytest.raises(ValueError, match="wq is the copy"):
+            linear.Int8LinearFunction.apply(x, w, None, q)
+    gu, down = z(256, 32), z(16, 128)
+    apply = linear.Int8GegluMlpFunction.apply
+    for args in ((z(512, 32), down, None, None), (gu, z(16, 256), None, None), (z(256, 64), down, None, None),
+                 (gu, z(16, 256), _copy_of(256, 32), _copy_of(16, 128))):
+        with pytest.raises(ValueError, match="intermediate size 128"):
+            apply(x, *args, 128)
+    with pytest.raises(ValueError, match="gu_q is the copy"):
+        apply(x, gu, down, _copy_of(512, 32), _copy_of(16, 128), 128)
+    with pytest.raises(ValueError, match="down_q is the copy"):
+        apply(x, gu, down, _copy_of(256, 32), _copy_of(32, 128), 128)
+
+
 def test_functions_see_x_as_rows(monkeypatch):
     """x of any number of dimensions reaches the int8 calls as [M, K] and its gradient comes back in its shape: the
     backward's K is x's last size, not its second."""
