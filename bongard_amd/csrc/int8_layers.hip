@@ -261,6 +261,15 @@ int bf8_geglu_mlp_int8_backward(const void* dy, int64_t M, int64_t K, int64_t I,
             "%s: NULL pointer", who);
   BF8_CHECK(!(dW_gu || dW_down) || M <= kInt8MaxK, "%s: for a weight's gradient M is %lld at most", who,
             (long long)kInt8MaxK);
+  // (here, and not by the products that read them, before which most of the work is done)
+  BF8_CHECK((((uintptr_t)dy | (uintptr_t)Xt | (uintptr_t)xt_scale | (uintptr_t)Ht | (uintptr_t)ht_scale |
+              (uintptr_t)Wt_gu | (uintptr_t)wt_gu_scale | (uintptr_t)Wt_down | (uintptr_t)wt_down_scale |
+              (uintptr_t)dx | (uintptr_t)dW_gu | (uintptr_t)dW_down) & 15) == 0 && ((uintptr_t)GU8 & 7) == 0,
+            "%s: every tensor must be 16-byte (GU8 8-byte) aligned", who);
+  const int64_t Mp = pad16(M);
+  const int64_t most = std::max({dh ? std::max(M, I) * N : 0, dW_down ? std::max(N, I) * Mp : 0,
+                                 dx ? std::max(M, K) * 2 * I : 0, dW_gu ? std::max(2 * I, K) * Mp : 0});
+  BF8_CHECK(K < (1LL << 31) && most < (1LL << 31), "%s: operands of 2 GiB and more", who);
   const MlpWs w = mlp_ws(M, K, I, N, dx, dW_gu, dW_down);
   BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.least,
             "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.least, ws_bytes);
@@ -283,7 +292,6 @@ int bf8_geglu_mlp_int8_backward(const void* dy, int64_t M, int64_t K, int64_t I,
                                                             stream)
                             : bf8_quantize_int8_bf16(dGU, M, 2 * I, rows, rs, cols, cs, rest, rest_bytes, stream))
     return rc;
-  const int64_t Mp = pad16(M);
   if (dW_gu)
     if (const int rc = bf8_gemm_int8(cols, Mp, cs, Xt, Mp, xt_scale, 2 * I, K, Mp, nullptr, dW_gu, BF8_OUT_BF16, K,
                                      rest, rest_bytes, stream))

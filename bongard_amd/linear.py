@@ -631,6 +631,19 @@ def _check_int8_tokens(who, rows):
         raise ValueError(f"{who}: a weight gradient takes {_INT8_MAX_TOKENS} tokens at most (got {rows})")
 
 
+def _check_int8_backward(who, M, K, N, dx, dw):
+    """The sizes of a linear that its backward (``bf8_linear_int8_backward``) takes, for its forward to refuse the
+    others: rows that the quantizer takes, operands below 2 GiB, for ``dw`` no more tokens than a sum holds."""
+    if dw:
+        _check_int8_tokens(who, M)
+    if N > 32768 and (dx or dw):
+        raise ValueError(f"{who}: gradients take 32768 output features at most (got {N})")
+    padded = (M + 15) // 16 * 16
+    most = max(max(M, K) * N if dx else 0, max(N, K) * padded if dw else 0)
+    if most >= 1 << 31:
+        raise ValueError(f"{who}: gradients take operands below 2 GiB (a tensor of {most} codes for {M} rows)")
+
+
 class _Int8Function(_Fp8Function):
     """Base of the int8 functions, which see x as rows: [M, K] of x [..., K], and give y [..., N]."""
 
@@ -650,9 +663,9 @@ def _check_int8_weight(who, name, q, weight):
 
 class Int8LinearFunction(_Int8Function):
     """y = x @ W^T (+ b) with every tensor in 8-bit integers, one scale for each token or channel
-    (gradients included; round to nearest even), sums exact in int32; x: bf16 [..., K], any number of rows
-    (133120 at most where W's gradient is asked for); W [N, K],
-    K a multiple of 16, N of 8 (of 16 for gradients). ``wq``: a cached int8 copy of W
+    (gradients included; round to nearest even), sums exact in int32; x: bf16 [..., K], any number of rows;
+    W [N, K], K a multiple of 16, 32768 at most, N of 8 (for gradients: of 16, 32768 at most). Gradients take
+    operands (x, y, W) of less than 2^31 elements, W's 133120 rows at most. ``wq``: a cached int8 copy of W
     (:func:`quantize_weight_int8`) or None.
 
       forward  y  = X8 . W8^T           scales by token and by output channel
@@ -667,8 +680,8 @@ class Int8LinearFunction(_Int8Function):
     def forward(ctx, x, weight, bias, wq):
         need_dx, need_dw = _forward_needs(ctx, 2)
         _check_int8("int8 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
-        if need_dw:
-            _check_int8_tokens("int8 linear", x.shape[0])
+        if need_dx or need_dw:
+            _check_int8_backward("int8 linear", *x.shape, weight.shape[0], need_dx, need_dw)
         if wq is not None and not (need_dx or need_dw):  # (the same product; few tokens take one kernel)
             ctx.save_for_backward(None, None, None, None)
             return ops.linear_int8(dense_rows(x), wq.data, wq.row_scale, bias=bias)
@@ -701,9 +714,10 @@ class Int8GegluMlpFunction(_Int8Function):
     (:class:`Int8LinearFunction`'s granularity) and the pre-activations kept for the backward as an
     8-bit checkpoint, half the bytes of bf16: the gate/up product with the gated GELU and the checkpoint
     in its epilogue, the down product; backward through dH, the gelu chain on the checkpoint's values and
-    the dgrad/wgrad products. x: bf16 [..., K], any number of rows (133120 at most where a weight's
-    gradient is asked for); w_gu [2I, K], w_down [K_out, I], K and K_out multiples of 16, I of 128. ``gu_q`` /
-    ``down_q``: optional cached int8 copies of the weights. TEMLP / FusedMLP under
+    the dgrad/wgrad products. x: bf16 [..., K], any number of rows; w_gu [2I, K], w_down
+    [K_out, I], K and K_out multiples of 16, 32768 at most, I of 128, 32768 at most (for gradients 16384). Gradients
+    take operands (x, [gate | up], y, the weights) of less than 2^31 elements, the weights' 133120 rows at most.
+    ``gu_q`` / ``down_q``: optional cached int8 copies of the weights. TEMLP / FusedMLP under
     'int8' (bongard/te_linear.py:98-103, bongard/fused_mlp.py:25-33 for the chain)."""
 
     @staticmethod
@@ -712,8 +726,12 @@ class Int8GegluMlpFunction(_Int8Function):
         need_dx, need_dgu, need_dd = _forward_needs(ctx, 3)
         keep = need_dx or need_dgu
         _check_int8("int8 gated MLP", x.shape[-1], *([w_down.shape[0]] if keep or need_dd else []))
-        if need_dgu or need_dd:
-            _check_int8_tokens("int8 gated MLP", x.shape[0])
+        if keep or need_dd:  # the down projection's backward, then the gate/up projection's
+            if I > 16384:
+                raise ValueError(f"int8 gated MLP: gradients take an intermediate size of 16384 at most (got {I})")
+            M, K = x.shape
+            _check_int8_backward("int8 gated MLP", M, I, w_down.shape[0], keep, need_dd)
+            _check_int8_backward("int8 gated MLP", M, K, 2 * I, need_dx, need_dgu)
         if gu_q is not None and down_q is not None and not (keep or need_dd):
             return ops.geglu_mlp_int8(dense_rows(x), gu_q.data, gu_q.row_scale, down_q.data, down_q.row_scale)
         if w_gu.shape != (2 * I, x.shape[1]) or w_down.shape[1] != I:

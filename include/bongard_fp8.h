@@ -682,7 +682,7 @@ int bf8_linear_int8_forward(const void* x, const void* W, int64_t M, int64_t N, 
  * bf8_quantize_int8_bf16 does, then dx [M, K] = dy . Wt^T (Wt int8 [K, N], the columnwise copy of W, scales
  * wt_scale [K]) and dw [N, K] = dy^T . Xt^T (Xt int8 [K, M rounded up to 16], the columnwise copy of x,
  * xt_scale [K]), the products bf8_gemm_int8's; bf16. dx or dw may be NULL (with its operand). N a multiple
- * of 16, 32768 at most, K of 8; M, N, K > 0, for dw M 133120 at most. ws:
+ * of 16, 32768 at most, K of 8; M, N, K > 0, for dw M 133120 at most; operands below 2 GiB. ws:
  * bf8_linear_int8_backward_workspace(M, N, K, dx?, dw?) bytes, 256-byte aligned. */
 size_t bf8_linear_int8_backward_workspace(int64_t M, int64_t N, int64_t K, int dx, int dw);
 int bf8_linear_int8_backward(const void* dy, int64_t M, int64_t N, int64_t K, const int8_t* Wt,
@@ -714,7 +714,7 @@ int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, i
  * H, with scales [I]), dGU [M, 2 I] from the checkpoint GU8 [M, 2 I] with GU8_exp as bf8_geglu_bwd_mxint8, then
  * dx [M, K] and dW_gu [2 I, K] (Wt_gu [K, 2 I] and Xt [K, M rounded up to 16], scales [K]); bf16. Any of dx,
  * dW_gu and dW_down may be NULL with the operands that it alone needs. I a multiple of 32, 16384 at most, N of
- * 16, 32768 at most, K of 8; for a weight's gradient M 133120 at most. ws:
+ * 16, 32768 at most, K of 8; for a weight's gradient M 133120 at most; operands below 2 GiB. ws:
  * bf8_geglu_mlp_int8_backward_workspace(M, K, I, N, dx?, dW_gu?, dW_down?) bytes, 256-byte aligned. */
 size_t bf8_geglu_mlp_int8_backward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int dx, int dgu,
                                              int dd);

@@ -384,3 +384,88 @@ def test_functions_see_x_as_rows(monkeypatch):
         assert y.shape == (*shape[:-1], 16)
         y.backward(torch.ones_like(y))
         assert x.grad.shape == x.shape and seen[-2:] == [(rows, 32), (rows, 32, 128)]
+
+
+def _refusal(entry, *args):
+    """What an entry says of sizes and no memory: nothing of the sizes where it is the workspace that it misses."""
+    L = _lib.lib()
+    assert getattr(L, entry)(*args) == 1
+    told = L.bf8_last_error().decode()
+    return None if "workspace needs" in told else told
+
+
+def _ctypes(flags, *given):
+    p, null = ctypes.c_void_p(4096), ctypes.c_void_p(0)
+    return [p if flags[k] else null for k in given]
+
+
+SIZES = [(4, 32, 32768), (4, 32, 32784), (104857, 2560, 20480), (104858, 2560, 20480), (104848, 2560, 20480),
+         (133120, 32, 16128), (133120, 32, 16144), (133121, 32, 32), (66000, 32784, 32), (65535, 16, 32768),
+         (65536, 16, 32768), (65519, 16, 32768), (1, 65536, 32768), (1, 65520, 32768), (16384, 131072, 16)]
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are no memory: the host checks alone")
+@pytest.mark.parametrize("dx,dw", [(True, False), (False, True), (True, True)])
+def test_a_linears_forward_refuses_what_its_backward_does(dx, dw):
+    """The same sizes on both sides of every limit: rows, features, tokens, 2 GiB."""
+    seen = set()
+    for M, K, N in SIZES:
+        told = _refusal("bf8_linear_int8_backward", ctypes.c_void_p(4096), M, N, K, *_ctypes((dx, dw), 0, 0, 1, 1, 0, 1),
+                        ctypes.c_void_p(4096), 64, ctypes.c_void_p(0))
+        try:
+            linear._check_int8_backward("layer", M, K, N, dx, dw)
+            assert told is None, (M, K, N, told)
+        except ValueError as e:
+            assert told is not None, (M, K, N, e)
+        seen.add(told is None)
+    assert seen == {True, False}
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are no memory: the host checks alone")
+@pytest.mark.parametrize("needs", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1), (1, 0, 1), (0, 1, 1)])
+def test_a_gated_mlps_forward_refuses_what_its_backward_does(monkeypatch, needs):
+    """As its autograd function checks: intermediate sizes, output features, tokens, [gate | up] of 2 GiB."""
+    monkeypatch.setattr(linear, "_check_int8_weight", lambda *a: None)
+    z = lambda r, c, n: torch.empty(1, 1, dtype=torch.bfloat16).expand(r, c).requires_grad_(bool(n))  # noqa: E731
+    seen = set()
+    for M, K, I, N in [(4, 16, 16384, 16), (4, 16, 16512, 16), (4, 16, 128, 32768), (4, 16, 128, 32784),
+                       (104848, 16, 10240, 16), (104849, 16, 10240, 16), (104858, 16, 10240, 16), (133120, 16, 128, 16),
+                       (133121, 16, 128, 16), (65536, 16, 256, 32768), (65520, 16, 256, 32768)]:
+        dh = needs[0] or needs[1]
+        flags = (dh, needs[1], needs[2], needs[0])
+        told = _refusal("bf8_geglu_mlp_int8_backward", ctypes.c_void_p(4096), M, K, I, N,
+                        *_ctypes(flags, 0, 0, 1, 1, 2, 2, 3, 3, 0, 0, 3, 1, 2), ctypes.c_void_p(4096), 64,
+                        ctypes.c_void_p(0))
+        args = z(M, K, needs[0]), z(2 * I, K, needs[1]), z(N, I, needs[2])
+        try:
+            linear.Int8GegluMlpFunction.apply(*args, None, None, I)
+        except ValueError as e:
+            assert told is not None and "gradient" in str(e), (M, K, I, N, e)
+        except RuntimeError:  # (past the checks: these tensors are on no GPU)
+            assert told is None, (M, K, I, N, told)
+        with torch.no_grad(), pytest.raises(RuntimeError):
+            linear.Int8GegluMlpFunction.apply(*args, None, None, I)
+        seen.add(told is None)
+    assert seen == {True, False}
+
+
+@pytest.mark.parametrize("M,N", [(4, 32784), (104858, 20480)])
+def test_an_int8_linear_refuses_in_its_forward(M, N):
+    z = lambda r, c: torch.empty(1, 1, dtype=torch.bfloat16).expand(r, c)  # noqa: E731
+    with pytest.raises(ValueError, match="gradients take"):
+        linear.Int8LinearFunction.apply(z(M, 2560).requires_grad_(), z(N, 2560), None, None)
+    with torch.no_grad(), pytest.raises(RuntimeError):  # (past the checks)
+        linear.Int8LinearFunction.apply(z(M, 2560).requires_grad_(), z(N, 2560), None, None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are no memory: the host checks alone")
+def test_a_gated_mlps_backward_refuses_before_its_first_launch():
+    """Sizes and alignments that only its last products read."""
+    p, odd, null = ctypes.c_void_p(4096), ctypes.c_void_p(4100), ctypes.c_void_p(0)
+    f, big = _lib.lib().bf8_geglu_mlp_int8_backward, 1 << 40
+    for M, args, message in ((104864, [p] * 13, "2 GiB"), (65536, [p] * 13, None),
+                             *((4, [p] * k + [odd] + [p] * (12 - k), "aligned") for k in range(13) if k != 1)):
+        I = 10240
+        assert f(p, M, 16, I, 16, *args, p, 64 if message is None else big, null) == 1
+        told = _lib.lib().bf8_last_error().decode()
+        assert told.startswith("bf8_geglu_mlp_int8_backward:") and (message or "workspace needs") in told, (M, told)
