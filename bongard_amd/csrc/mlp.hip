@@ -411,7 +411,7 @@ int64_t bf8_geglu_partials_elementwise(int64_t M, int64_t I) { return bwd_blocks
 int bf8_geglu_bf16(const void* GU, int64_t M, int64_t I, void* H, uint32_t* partials,
                    void* stream) {
   BF8_CHECK(M >= 0 && I >= 8 && I % 8 == 0, "bf8_geglu_bf16: need I %% 8 == 0 (I=%lld)", (long long)I);
-  BF8_CHECK(GU && H && partials, "bf8_geglu_bf16: NULL pointer");
+  BF8_CHECK(partials && (M == 0 || (GU && H)), "bf8_geglu_bf16: NULL pointer");  // (no rows: partials of 0)
   BF8_CHECK((((uintptr_t)GU | (uintptr_t)H) & 15) == 0,
             "bf8_geglu_bf16: pointers must be 16-byte aligned");
   const int64_t nb = bwd_blocks(M, I);
@@ -425,7 +425,7 @@ int64_t bf8_geglu_bwd_partials(int64_t M, int64_t I) { return bwd_blocks(M, I); 
 int bf8_geglu_bwd(const void* dH, const void* GU, int64_t M, int64_t I, void* dGU,
                   uint32_t* partials, void* stream) {
   BF8_CHECK(M >= 0 && I >= 8 && I % 8 == 0, "bf8_geglu_bwd: need I %% 8 == 0 (I=%lld)", (long long)I);
-  BF8_CHECK(dH && GU && dGU && partials, "bf8_geglu_bwd: NULL pointer");
+  BF8_CHECK(partials && (M == 0 || (dH && GU && dGU)), "bf8_geglu_bwd: NULL pointer");
   BF8_CHECK((((uintptr_t)dH | (uintptr_t)GU | (uintptr_t)dGU) & 15) == 0,
             "bf8_geglu_bwd: pointers must be 16-byte aligned");
   const int64_t nb = bwd_blocks(M, I);

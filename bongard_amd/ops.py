@@ -844,7 +844,7 @@ def geglu(GU, *, partials=None):
     _require_gpu(GU)
     if GU.dtype != torch.bfloat16 or GU.dim() != 2 or GU.shape[1] % 2:
         raise ValueError(f"geglu: GU must be bf16 [M, 2I] (got {GU.dtype} {tuple(GU.shape)})")
-    GU = GU.contiguous()
+    GU = _rows_bf16(GU)
     M, I = GU.shape[0], GU.shape[1] // 2
     L = _lib.lib()
     H = torch.empty((M, I), dtype=torch.bfloat16, device=GU.device)
@@ -869,9 +869,9 @@ def geglu_bwd(dH, GU, *, partials=None):
     per-block amax partials of |dGU| (for ``cast_partials`` or a delayed scaler;
     ``partials``: an optional caller-owned buffer)."""
     _require_gpu(dH, GU)
-    dH = dH.contiguous()
+    dH = _rows_bf16(dH)
     M, I = dH.shape
-    GU = _gu_operand("geglu_bwd", GU, M, I)
+    GU = _rows_bf16(_gu_operand("geglu_bwd", GU, M, I))
     L = _lib.lib()
     dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
     count = int(L.bf8_geglu_bwd_partials(M, I))

@@ -995,3 +995,42 @@ def test_functions_of_batched_rows(gpu, shape):
             assert got[0].shape == x.shape
             with torch.no_grad():
                 assert torch.equal(f(*leaves), y)
+
+
+@pytest.mark.parametrize("checkpoint", [False, True])
+@pytest.mark.parametrize("lead", [(5,), (0,), (2, 3), (0, 3), (2, 0)])
+def test_gated_gelu_of_no_rows_and_of_any_alignment(gpu, checkpoint, lead):
+    """Recorded or not, an empty batch and pre-activations (and their gradient) whose storage starts off 16 bytes."""
+    I = 64
+    n = torch.Size(lead).numel()
+    GU, dH = _x(n + 1, 2 * I, 3, False)[:n], _x(n + 1, I, 4, False)[:n]
+
+    def off(t, shape):
+        for k in (1, 4):
+            store = torch.zeros(t.numel() + 8, dtype=BF16, device=gpu)
+            yield store[k:k + t.numel()].copy_(t.flatten()).view(shape)
+    want = ops.geglu(GU.to(gpu))[0] if n else torch.empty(0, I, dtype=BF16, device=gpu)
+    for gu, dh in zip(off(GU, (*lead, 2 * I)), off(dH, (*lead, I))):
+        with torch.no_grad():
+            h = fused_mlp.gated_gelu(gu, checkpoint=checkpoint)
+        assert h.shape == (*lead, I) and torch.equal(h.reshape(n, I), want)
+        leaf = gu.detach().requires_grad_()
+        assert leaf.data_ptr() == gu.data_ptr()
+        h = fused_mlp.gated_gelu(leaf, checkpoint=checkpoint)
+        assert torch.equal(h.detach().reshape(n, I), want)
+        (grad,) = torch.autograd.grad(h, leaf, dh)
+        assert grad.shape == leaf.shape
+        if n:
+            held = ops.dequant_mxint8(ops.quantize_mxint8(GU.to(gpu))) if checkpoint else GU.to(gpu)
+            assert torch.equal(grad.reshape(n, 2 * I), ops.geglu_bwd(dH.to(gpu), held)[0])
+
+
+def test_elementwise_gated_gelu_of_no_rows_leaves_maxima_of_zero(gpu):
+    """No rows through the plain entries: partials of 0 that a cast may read."""
+    none = torch.empty(0, 128, dtype=BF16, device=gpu)
+    parts = torch.full((4,), 7, dtype=torch.int32, device=gpu)
+    H, p = ops.geglu(none, partials=parts)
+    assert tuple(H.shape) == (0, 64) and not bool(p.any())
+    parts.fill_(7)
+    dGU, p = ops.geglu_bwd(H, none, partials=parts)
+    assert tuple(dGU.shape) == (0, 128) and not bool(p.any())
