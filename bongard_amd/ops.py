@@ -855,8 +855,7 @@ def geglu(GU, *, partials=None):
         if partials.numel() < count or partials.dtype != torch.int32:
             raise ValueError(f"geglu: partials must be int32 with >= {count} entries")
         parts = partials[:count]
-    _lib.check(L.bf8_geglu_bf16(_ptr(GU), M, I, _ptr(H), _ptr(parts), _stream(GU.device)),
-               "bf8_geglu_bf16")
+    _call("bf8_geglu_bf16", GU.get_device(), L.bf8_geglu_bf16, _ptr(GU), M, I, _ptr(H), _ptr(parts))
     return H, parts
 
 
@@ -881,8 +880,7 @@ def geglu_bwd(dH, GU, *, partials=None):
         if partials.numel() < count or partials.dtype != torch.int32:
             raise ValueError(f"geglu_bwd: partials must be int32 with >= {count} entries")
         parts = partials[:count]
-    _lib.check(L.bf8_geglu_bwd(_ptr(dH), _ptr(GU), M, I, _ptr(dGU), _ptr(parts),
-                               _stream(dH.device)), "bf8_geglu_bwd")
+    _call("bf8_geglu_bwd", dH.get_device(), L.bf8_geglu_bwd, _ptr(dH), _ptr(GU), M, I, _ptr(dGU), _ptr(parts))
     return dGU, parts
 
 

@@ -1034,3 +1034,24 @@ def test_elementwise_gated_gelu_of_no_rows_leaves_maxima_of_zero(gpu):
     parts.fill_(7)
     dGU, p = ops.geglu_bwd(H, none, partials=parts)
     assert tuple(dGU.shape) == (0, 128) and not bool(p.any())
+
+
+def test_gated_gelu_launches_on_its_tensors_device(gpu, monkeypatch):
+    """Where another device is the current one, the tensors' is made it for the launch, with a checkpoint and without."""
+    real, made = ops.torch.cuda.device, []
+
+    def device(idx):
+        made.append(idx)
+        return real(idx)
+    GU, dH = _gu(4, 64, 1, gpu)
+    monkeypatch.setattr(ops.torch.cuda, "device", device)
+    for checkpoint in (False, True):
+        leaf = GU.detach().requires_grad_()
+        monkeypatch.setattr(ops.torch._C, "_cuda_getDevice", lambda: 7)
+        h = fused_mlp.gated_gelu(leaf, checkpoint=checkpoint)
+        assert made == [0]
+        torch.autograd.grad(h, leaf, dH)
+        assert made == [0, 0]
+        monkeypatch.undo()
+        monkeypatch.setattr(ops.torch.cuda, "device", device)
+        made.clear()
