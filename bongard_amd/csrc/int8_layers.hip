@@ -218,6 +218,14 @@ int bf8_geglu_mlp_int8_forward(const void* x, int64_t M, int64_t K, int64_t I, i
   BF8_CHECK(x && W_gu && w_gu_scale && W_down && w_down_scale && Y && (GU8 == nullptr) == (GU8_exp == nullptr) &&
                 (Xt == nullptr) == (xt_scale == nullptr) && (Ht == nullptr) == (ht_scale == nullptr),
             "%s: NULL pointer", who);
+  // (here, and not by what reads them: H's copies are written by one of two quantizations, and most of the work is done
+  // before the down product)
+  BF8_CHECK((((uintptr_t)x | (uintptr_t)W_gu | (uintptr_t)w_gu_scale | (uintptr_t)W_down | (uintptr_t)w_down_scale |
+              (uintptr_t)Y | (uintptr_t)Xt | (uintptr_t)xt_scale | (uintptr_t)Ht | (uintptr_t)ht_scale) & 15) == 0 &&
+                ((uintptr_t)GU8 & 7) == 0,
+            "%s: every tensor must be 16-byte (GU8 8-byte) aligned", who);
+  BF8_CHECK(N < (1LL << 31) && std::max(M, 2 * I) * K < (1LL << 31) && std::max(M, N) * I < (1LL << 31),
+            "%s: operands of 2 GiB and more", who);
   const MlpForwardWs w = mlp_forward_ws(M, K, I, N, Xt, Ht);
   BF8_CHECK(ws && ((uintptr_t)ws & 255) == 0 && ws_bytes >= w.least,
             "%s: workspace needs %zu bytes, 256-byte aligned (got %zu)", who, w.least, ws_bytes);

@@ -700,7 +700,8 @@ int bf8_gemm_geglu_int8(const int8_t* X, int64_t ldx, const float* x_scale, cons
 /* The training forward of the gated MLP in int8: Y bf16 [M, N] of bf16 x [M, K] and the row copies of W_gu
  * [2 I, K] (gate rows then up rows) and W_down [N, I], x and H quantized by row, and where given the checkpoint
  * of the pre-activations as bf8_gemm_geglu_int8's and the columnwise copies Xt [K, M rounded up to 16] and Ht
- * [I, M rounded up to 16] with scales [K] and [I]. K a multiple of 16, I of 128, 32768 at most, N of 8. ws:
+ * [I, M rounded up to 16] with scales [K] and [I]. K a multiple of 16, I of 128, 32768 at most, N of 8; operands
+ * below 2 GiB; GU8 8-byte, every other tensor but GU8_exp 16-byte aligned. ws:
  * bf8_geglu_mlp_int8_forward_workspace(M, K, I, N, Xt?, Ht?) bytes, 256-byte aligned. */
 size_t bf8_geglu_mlp_int8_forward_workspace(int64_t M, int64_t K, int64_t I, int64_t N, int keep_x,
                                             int keep_h);

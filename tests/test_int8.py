@@ -469,3 +469,23 @@ def test_a_gated_mlps_backward_refuses_before_its_first_launch():
         assert f(p, M, 16, I, 16, *args, p, 64 if message is None else big, null) == 1
         told = _lib.lib().bf8_last_error().decode()
         assert told.startswith("bf8_geglu_mlp_int8_backward:") and (message or "workspace needs") in told, (M, told)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses that are no memory: the host checks alone")
+@pytest.mark.parametrize("tile", ["", "256x256w8"])
+def test_a_gated_mlps_forward_refuses_before_its_first_launch(monkeypatch, tile):
+    """Whichever plan runs the products: H's columnwise codes off 16 bytes (one of two quantizations writes them),
+    operands of 2 GiB that only the down product reads."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    L = _lib.lib()
+    p, odd, null = ctypes.c_void_p(4096), ctypes.c_void_p(4100), ctypes.c_void_p(0)
+    f, big = L.bf8_geglu_mlp_int8_forward, 1 << 40
+    # (W_gu, its scale, W_down, its scale, Y, GU8, its exponents, Xt, its scale, Ht, its scale)
+    cases = [(4, 128, 16, [p] * k + [odd] + [p] * (10 - k), "aligned") for k in range(11) if k != 6]
+    cases += [(4, 128, 16, [p] * 11, None), (65536, 32768, 16, [p] * 11, "2 GiB"), (65535, 32768, 16, [p] * 11, None),
+              (4, 32768, 65536, [p] * 11, "2 GiB"), (4, 32768, 65528, [p] * 11, None)]
+    for M, I, N, args, message in cases:
+        assert f(p, M, 16, I, N, *args, p, big if message else 64, null) == 1
+        told = L.bf8_last_error().decode()
+        assert told.startswith("bf8_geglu_mlp_int8_forward:") and (message or "workspace needs") in told, (M, N, told)
+    assert f(odd, 4, 16, 128, 16, *[p] * 11, p, big, null) == 1 and "aligned" in L.bf8_last_error().decode()
