@@ -1618,7 +1618,7 @@ def _int8_scale(who, name, t, rows):
 
 
 def dequant_int8(q, *, transpose=False):
-    """The values of an :class:`Int8Tensor` as bf16 [rows, cols] (code times scale, rounded once), or with
+    """The values of an :class:`Int8Tensor` as bf16 [rows, cols] (the fp32 product of code and scale, rounded), or with
     ``transpose`` those of its columnwise copy, [cols, rows] (a view of rows padded to 16 where rows
     is not a multiple)."""
     who = "dequant_int8"
@@ -1628,6 +1628,7 @@ def dequant_int8(q, *, transpose=False):
     idx = _index_of(who, codes, scale)
     _int8_matrix(who, codes=codes)
     codes = codes.contiguous()
+    codes = codes if codes.data_ptr() % 8 == 0 else codes.clone()
     rows, cols = codes.shape
     scale = _int8_scale(who, "scale", scale, rows)
     out = torch.empty((rows, cols), dtype=torch.bfloat16, device=codes.device)

@@ -638,7 +638,7 @@ int bf8_quantize_int8_maxima_bf16(const void* x, int64_t rows, int64_t cols, int
                                   float* row_scale, int8_t* out_t, float* col_scale, const void* maxima,
                                   size_t maxima_bytes, void* stream);
 
-/* out bf16 [rows, cols] = codes * scale[row] (rounded once). cols % 8 == 0; out 16-byte, codes
+/* out bf16 [rows, cols] = codes * scale[row] (in fp32, then rounded). cols % 8 == 0; out 16-byte, codes
  * 8-byte aligned. */
 int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int64_t cols, void* out,
                      void* stream);

@@ -1055,3 +1055,16 @@ def test_gated_gelu_launches_on_its_tensors_device(gpu, monkeypatch):
         monkeypatch.undo()
         monkeypatch.setattr(ops.torch.cuda, "device", device)
         made.clear()
+
+
+def test_read_back_of_codes_off_their_alignment(gpu):
+    """Codes whose storage starts anywhere, as the other entries take them."""
+    q = ops.quantize_int8(_x(20, 64, 1).to(gpu), colwise=True)
+    for k in (1, 4, 7):
+        store = torch.zeros(20 * 64 + 8, dtype=torch.int8, device=gpu)
+        off = store[k:k + 20 * 64].copy_(q.data.flatten()).view(20, 64)
+        got = ops.dequant_int8(ops.Int8Tensor(off, q.row_scale, None, None, 20, 64))
+        assert torch.equal(got, ops.dequant_int8(q))
+        off = store[k:k + 32 * 32].copy_(q.data_t[:32].flatten()).view(32, 32)
+        got = ops.dequant_int8(ops.Int8Tensor(None, None, off, q.col_scale[:32], 20, 32), transpose=True)
+        assert torch.equal(got, ops.dequant_int8(q, transpose=True)[:32])
