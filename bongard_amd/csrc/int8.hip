@@ -225,16 +225,16 @@ __global__ __launch_bounds__(kTileNT, 4) void int8_tile_kernel(const uint16_t* _
 // Both copies of up to 128 R rows. Blocks [0, row_blocks) are int8_row_kernel's of eight rows each (TPR 64, V
 // vectors a lane). Of the others each takes 32 columns of all rows: four lanes a row (8 columns each), 128 rows
 // a step, R steps held in registers; the columns' maxima by packed 16-bit maxima over lanes and waves, the
-// codes turned in LDS, 1,024 rows at a time. Bound by latency: [64, 2560] 4.1 us, [500, 2560] 6.7 (two passes over
+// codes turned in LDS. Bound by latency: [64, 2560] 4.1 us, [500, 2560] 6.7 (two passes over
 // tiles, as below it 1,024 rows, 11.3).
-constexpr int kPairCols = 32, kPairPitch = kPairCols / 4 + 1, kPairStage = 8;  // stage: steps of 128 rows
+constexpr int kPairCols = 32, kPairPitch = kPairCols / 4 + 1;
 template <int V, int R>
 __global__ __launch_bounds__(kNT) void int8_pair_kernel(const uint16_t* __restrict__ x, int rows, int cols,
                                                         int row_blocks, int8_t* __restrict__ out,
                                                         float* __restrict__ row_scale,
                                                         int8_t* __restrict__ out_t,
                                                         float* __restrict__ col_scale) {
-  __shared__ uint32_t stage[(R < kPairStage ? R : kPairStage) * 128 * kPairPitch];
+  __shared__ uint32_t stage[R * 128 * kPairPitch];
   __shared__ uint4 top[kNT / 64][4];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
   if ((int)blockIdx.x < row_blocks) {
@@ -293,31 +293,25 @@ __global__ __launch_bounds__(kNT) void int8_pair_kernel(const uint16_t* __restri
     reinterpret_cast<float4*>(col_scale + c)[1] = make_float4(scale[4], scale[5], scale[6], scale[7]);
   }
 #pragma unroll
-  for (int i0 = 0; i0 < R; i0 += kPairStage) {
-    if (i0) __syncthreads();
+  for (int i = 0; i < R; ++i) {
+    const uint2 q = int8_codes8(v[i], mult);
+    uint32_t* d = stage + (128 * i + rl) * kPairPitch + 2 * cg;
+    d[0] = q.x;
+    d[1] = q.y;
+  }
+  __syncthreads();
+  // a thread turns 16 rows of 4 columns: 8 pieces of rows a step of 128, 8 groups of columns
+  for (int it = threadIdx.x; it < R * 64; it += kNT) {
+    const int r = (it & (8 * R - 1)) * 16, g = it / (8 * R);
+    if (r >= rows || c0 + 4 * g >= cols) continue;
+    uint32_t d[16];
 #pragma unroll
-    for (int i = i0; i < R && i < i0 + kPairStage; ++i) {
-      const uint2 q = int8_codes8(v[i], mult);
-      uint32_t* d = stage + (128 * (i - i0) + rl) * kPairPitch + 2 * cg;
-      d[0] = q.x;
-      d[1] = q.y;
-    }
-    __syncthreads();
-    // a thread turns 16 rows of 4 columns: 8 pieces of rows a step of 128, 8 groups of columns
-    constexpr int kSteps = R < kPairStage ? R : kPairStage;
-    for (int it = threadIdx.x; it < kSteps * 64; it += kNT) {
-      const int rg = (it & (8 * kSteps - 1)) * 16, g = it / (8 * kSteps);
-      const int r = 128 * i0 + rg;
-      if (r >= rows || c0 + 4 * g >= cols) continue;
-      uint32_t d[16];
+    for (int i = 0; i < 16; ++i) d[i] = stage[(r + i) * kPairPitch + g];
+    uint4 tq[4];
+    transpose_4x16(d, tq);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) d[i] = stage[(rg + i) * kPairPitch + g];
-      uint4 tq[4];
-      transpose_4x16(d, tq);
-#pragma unroll
-      for (int cc = 0; cc < 4; ++cc)
-        *reinterpret_cast<uint4*>(out_t + (int64_t)(c0 + 4 * g + cc) * ld + r) = tq[cc];
-    }
+    for (int cc = 0; cc < 4; ++cc)
+      *reinterpret_cast<uint4*>(out_t + (int64_t)(c0 + 4 * g + cc) * ld + r) = tq[cc];
   }
 }
 

@@ -624,8 +624,9 @@ int bf8_rmsnorm_residual_bwd_bf16(const void* h, const void* out, const void* do
  * codes 0 (its products are NaN).
  * out: [rows, cols] with row_scale [rows]; out_t: the columns' copy [cols, R], R = rows rounded up
  * to 16 (zeros past the rows), with col_scale [cols]; each optional (at least one). cols % 8 == 0 and
- * <= 32768. out_t needs ws: bf8_quantize_int8_workspace(rows, cols) bytes, 256-byte aligned. x
- * and out_t 16-byte, out 8-byte aligned.
+ * <= 32768. out_t needs ws: bf8_quantize_int8_workspace(rows, cols, both) bytes, 256-byte aligned, where
+ * both says whether out is written too (few rows of both copies need none; of out_t alone they do). x,
+ * out_t and col_scale 16-byte, out 8-byte aligned.
  * ------------------------------------------------------------------------------- */
 size_t bf8_quantize_int8_workspace(int64_t rows, int64_t cols, int both);
 int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* out, float* row_scale,
@@ -633,7 +634,8 @@ int bf8_quantize_int8_bf16(const void* x, int64_t rows, int64_t cols, int8_t* ou
                            void* stream);
 
 /* The same codes and scales from the maxima of |x|'s rows and columns that x's producer left
- * (bf8_geglu_bwd_mxint8's dGU: halves 2), without a pass that looks for them; any cols. */
+ * (bf8_geglu_bwd_mxint8's dGU: halves 2), without a pass that looks for them. cols % (8 * halves) == 0 and
+ * < 2^24; maxima 256-byte, the others aligned as above. */
 int bf8_quantize_int8_maxima_bf16(const void* x, int64_t rows, int64_t cols, int halves, int8_t* out,
                                   float* row_scale, int8_t* out_t, float* col_scale, const void* maxima,
                                   size_t maxima_bytes, void* stream);
