@@ -1068,3 +1068,21 @@ def test_read_back_of_codes_off_their_alignment(gpu):
         off = store[k:k + 32 * 32].copy_(q.data_t[:32].flatten()).view(32, 32)
         got = ops.dequant_int8(ops.Int8Tensor(None, None, off, q.col_scale[:32], 20, 32), transpose=True)
         assert torch.equal(got, ops.dequant_int8(q, transpose=True)[:32])
+
+
+@pytest.mark.parametrize("tile,has", [("256x256w8", True), ("160x256", True), ("64x128", True), ("128x128", True),
+                                      ("192x256", False)])
+@pytest.mark.parametrize("M,K,I", [(1, 16, 128), (290, 544, 640)])
+def test_gated_product_runs_the_tile_that_is_named(gpu, monkeypatch, capfd, tile, has, M, K, I):
+    """A named tile is the one that runs where it has a gated int8 variant (192x256 has none: the plan's own choice,
+    which is printed where it is made), and gives the product's H and checkpoint."""
+    monkeypatch.setenv("BONGARD_FP8_GEMM_TILE", tile)
+    monkeypatch.setenv("BONGARD_FP8_GEMM_DEBUG", "1")
+    x, w, _, _ = _mlp_inputs(M, K, I, 7, gpu)
+    xq, wq = ops.quantize_int8(x), ops.quantize_int8(w)
+    capfd.readouterr()
+    H, gu = ops.gemm_geglu_int8(xq.data, xq.row_scale, wq.data, wq.row_scale, I, keep_gu=True)
+    assert ("bf8 plan geglu" in capfd.readouterr().err) == (not has)
+    GU = ops.gemm_int8(xq.data, xq.row_scale, wq.data, wq.row_scale)
+    want = ops.quantize_mxint8(GU)
+    assert torch.equal(H, ops.geglu(GU)[0]) and torch.equal(gu.data, want.data) and torch.equal(gu.exps, want.exps)
