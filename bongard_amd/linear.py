@@ -679,6 +679,7 @@ class Int8LinearFunction(_Int8Function):
     @staticmethod
     def forward(ctx, x, weight, bias, wq):
         need_dx, need_dw = _forward_needs(ctx, 2)
+        ctx.bias_shape = None if bias is None else bias.shape
         _check_int8("int8 linear", x.shape[-1], *([weight.shape[0]] if need_dx or need_dw else []))
         if need_dx or need_dw:
             _check_int8_backward("int8 linear", *x.shape, weight.shape[0], need_dx, need_dw)
@@ -706,7 +707,7 @@ class Int8LinearFunction(_Int8Function):
             dy = ops._rows_bf16(dy)
             dx, dw = ops._linear_int8_backward(dy.get_device(), dy, (w8t if need_dx else x8t).shape[0],
                                                w8t if need_dx else None, ws, x8t if need_dw else None, xs)
-        return dx, dw, ops.column_sums(dy) if need_db else None, None
+        return dx, dw, ops.column_sums(dy).view(ctx.bias_shape) if need_db else None, None
 
 
 class Int8GegluMlpFunction(_Int8Function):

@@ -1086,3 +1086,14 @@ def test_gated_product_runs_the_tile_that_is_named(gpu, monkeypatch, capfd, tile
     GU = ops.gemm_int8(xq.data, xq.row_scale, wq.data, wq.row_scale)
     want = ops.quantize_mxint8(GU)
     assert torch.equal(H, ops.geglu(GU)[0]) and torch.equal(gu.data, want.data) and torch.equal(gu.exps, want.exps)
+
+
+@pytest.mark.parametrize("shape", [(48,), (1, 48)])
+def test_a_bias_of_any_shape_has_its_gradient(gpu, shape):
+    """The forward takes N values; their gradient comes back in the bias' shape, with others and alone."""
+    x, w, dy = (_x(*s, 7, False).to(gpu) for s in ((20, 32), (48, 32), (20, 48)))
+    bias = _x(1, 48, 3, False).to(gpu).view(shape).requires_grad_()
+    for leaf in (x.clone().requires_grad_(), x):
+        linear.Int8LinearFunction.apply(leaf, w, bias, None).backward(dy)
+        assert bias.grad.shape == shape and torch.equal(bias.grad.flatten(), ops.column_sums(dy))
+        bias.grad = None
