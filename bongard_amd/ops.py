@@ -2003,8 +2003,8 @@ def _geglu_bwd_mxint8(idx, dH, data, exps):
 
 def geglu_bwd_mxint8(dH, gu, *, rowwise=False, colwise=False):
     """:func:`geglu_bwd` on the values of GU's checkpoint: dGU bf16 [M, 2I], or with ``rowwise`` or
-    ``colwise`` that tensor's :func:`quantize_int8` instead (from 1024 rows on by the maxima that the backward's
-    kernel leaves: the same codes and scales)."""
+    ``colwise`` that tensor's :func:`quantize_int8` instead (from 1024 rows on, and where its rows are too wide for
+    that, by the maxima that the backward's kernel leaves: the same codes and scales)."""
     who = "geglu_bwd_mxint8"
     idx = _index_of(who, dH, gu.data, gu.exps)
     dH = _rows_bf16(dH)
@@ -2016,7 +2016,7 @@ def geglu_bwd_mxint8(dH, gu, *, rowwise=False, colwise=False):
         return _geglu_bwd_mxint8(idx, dH, data, exps)
     # both copies of dGU's codes, by the maxima and by the quantizer's own pass, us: [512, 2 x 10240] 32.5 and
     # 31.5, [1500, 2 x 2560] 27.5 and 29.9, [4096, 2 x 10240] 157 and 168
-    if M < 1024 or not I:
+    if M < 1024 and I <= 16384 or not (M and I):
         return quantize_int8(geglu_bwd_mxint8(dH, gu), rowwise=rowwise, colwise=colwise)
     dGU = torch.empty((M, 2 * I), dtype=torch.bfloat16, device=dH.device)
     L = _lib.lib()

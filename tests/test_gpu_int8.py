@@ -1097,3 +1097,18 @@ def test_a_bias_of_any_shape_has_its_gradient(gpu, shape):
         linear.Int8LinearFunction.apply(leaf, w, bias, None).backward(dy)
         assert bias.grad.shape == shape and torch.equal(bias.grad.flatten(), ops.column_sums(dy))
         bias.grad = None
+
+
+@pytest.mark.parametrize("M", [0, 1, 37, 1030])
+def test_codes_of_a_wide_gradient(gpu, M):
+    """Rows of dGU wider than the quantizer takes: the oracle's codes and scales whatever the number of rows."""
+    I = 16416
+    GU, dH = _gu(M + 1, I, 5, gpu)
+    _, q = ops.geglu_mxint8(GU[:M])
+    dGU = ops.geglu_bwd_mxint8(dH[:M], q)
+    got = ops.geglu_bwd_mxint8(dH[:M], q, rowwise=True, colwise=True)
+    assert tuple(got.data.shape) == (M, 2 * I) and tuple(got.data_t.shape) == (2 * I, (M + 15) // 16 * 16)
+    if M:
+        _check(got, dGU.cpu(), True, True)
+        for rowwise, colwise in ((True, False), (False, True)):
+            _check(ops.geglu_bwd_mxint8(dH[:M], q, rowwise=rowwise, colwise=colwise), dGU.cpu(), rowwise, colwise)
