@@ -151,7 +151,7 @@ __global__ __launch_bounds__(kNT) void geglu_bwd_mxi8_kernel(const uint16_t* __r
 // at a time (two passes of four), so that the maxima of d_g and d_u fall to it on the way and the pass over dGU
 // that would find them (4 bytes an element of H) is saved: [4096, 10240] with both copies of the codes 157 us,
 // by the kernel above and the ordinary quantizer 168. Alone it is the slower one (73 us there, 10.8 against
-// 5.3 at 64 rows): fewer loads in flight a wave, 2 MB of maxima.
+// 5.3 at 64 rows): fewer loads in flight a wave, 2 MB of maxima, 48 bytes a lane in scratch.
 constexpr int kBwdCols = 512, kBwdRows = 4;
 __global__ __launch_bounds__(kNT, 4) void geglu_bwd_mxi8_maxima_kernel(
     const uint16_t* __restrict__ dH, const int8_t* __restrict__ gu8, const uint8_t* __restrict__ gu8_e, int64_t I,

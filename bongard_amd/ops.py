@@ -1648,7 +1648,8 @@ def _linear_bias(who, bias, N):
 def gemm_int8(a, a_scale, b, b_scale, *, bias=None, out_dtype=torch.bfloat16, out=None):
     """``C = a_scale[:, None] * b_scale * (A @ B.T) (+ bias)`` of int8 codes A [M, K] and B [N, K] with
     fp32 scales [M] and [N] (as :func:`quantize_int8` writes them) on the int8 MFMA; the sums are exact in
-    int32. K a multiple of 16, 133120 at most, N of 8; C bf16 or fp32."""
+    int32. K a multiple of 16, 133120 at most (131056 for codes of -128, which no quantizer here writes), N of 8;
+    C bf16 or fp32. The scales' product is formed first, in fp32: past its range C is inf, or NaN where the sum is 0."""
     who = "gemm_int8"
     idx = _index_of(who, a, a_scale, b, b_scale, bias, out)
     _int8_matrix(who, a=a, b=b)

@@ -646,7 +646,8 @@ int bf8_dequant_int8(const int8_t* codes, const float* scale, int64_t rows, int6
                      void* stream);
 
 /* C[m, n] = a_scale[m] * b_scale[n] * sum_k A[m, k] B[n, k] (+ bias[n]), the sum exact in int32: A
- * [M, K] and B [N, K] row-major, K and row strides multiples of 16, K <= 133120, N % 8 == 0; bias
+ * [M, K] and B [N, K] row-major, K and row strides multiples of 16, K <= 133120 (131056 for codes of
+ * -128, which no quantizer here writes), N % 8 == 0; a_scale * b_scale is formed first, in fp32; bias
  * bf16 [N] or NULL; C bf16 or fp32. Operands and scales 16-byte aligned. ws:
  * bf8_gemm_int8_workspace(M, N, K) bytes, 256-byte aligned (less, or none, runs a plan that needs
  * less). */

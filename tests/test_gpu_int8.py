@@ -1112,3 +1112,15 @@ def test_codes_of_a_wide_gradient(gpu, M):
         _check(got, dGU.cpu(), True, True)
         for rowwise, colwise in ((True, False), (False, True)):
             _check(ops.geglu_bwd_mxint8(dH[:M], q, rowwise=rowwise, colwise=colwise), dGU.cpu(), rowwise, colwise)
+
+
+def test_product_of_codes_of_minus_128(gpu):
+    """No quantizer writes them; their sums stay exact up to K 131,056 (* 128^2 < 2^31)."""
+    M, N, K = 8, 16, 131056
+    a = torch.full((M, K), -128, dtype=torch.int8, device=gpu)
+    b = torch.full((N, K), -128, dtype=torch.int8, device=gpu)
+    b[1::2] = 127
+    one = torch.ones(N, device=gpu)
+    y = ops.gemm_int8(a, one[:M], b, one, out_dtype=F32).cpu().double()
+    want = torch.where(torch.arange(N) % 2 == 0, 128.0, -127.0).double() * 128 * K
+    assert bool(((y - want).abs() <= 2.0 ** -24 * want.abs()).all())
