@@ -1,7 +1,7 @@
 // A layer's pass in 8-bit integers as one call: the training forward and backward of a linear and of the gated
 // MLP, as the quantizer's, the products' and the gated GELU's own entries in turn on one workspace (from
 // Python each of those is 10 us of host time, in the autograd engine's thread up to twice that: 500 x 2048 x 2560
-// trained 171 us as six calls, 118-129 as two, by box).
+// trained 171 us as six calls, 118-129 as two, by machine).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -508,7 +508,7 @@ int bf8_geglu_bwd_mxint8(const void* dH, const int8_t* GU8, const uint8_t* GU8_e
                          void* dGU, void* maxima, size_t maxima_bytes, void* stream) {
   const char* who = "bf8_geglu_bwd_mxint8";
   if (const int rc = check_geglu_mxi8(who, dH, dGU, GU8, GU8_exp, M, I)) return rc;
-  BF8_CHECK(M < (1LL << 31) && I < (1 << 22), "%s: M or I too large", who);
+  BF8_CHECK(!maxima || (M < (1LL << 31) && I < (1 << 22)), "%s: M or I too large", who);
   BF8_CHECK(!maxima || (((uintptr_t)maxima & 255) == 0 && maxima_bytes >= bf8_geglu_bwd_mxint8_maxima(M, I)),
             "%s: the maxima need %zu bytes, 256-byte aligned (got %zu)", who,
             bf8_geglu_bwd_mxint8_maxima(M, I), maxima_bytes);

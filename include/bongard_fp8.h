@@ -751,7 +751,7 @@ int bf8_dequant_mxint8(const int8_t* codes, const uint8_t* exponents, int64_t ro
 /* bf8_geglu_bf16 (H from GU [M, 2 I]; no amax partials) that writes GU's checkpoint in the same
  * pass, and bf8_geglu_bwd (dGU; no amax partials) on the values of the checkpoint. I % 32 == 0.
  * maxima, where given: bf8_geglu_bwd_mxint8_maxima(M, I) bytes, 256-byte aligned, which receive the
- * maxima of dGU's rows and columns for bf8_quantize_int8_maxima_bf16. */
+ * maxima of dGU's rows and columns for bf8_quantize_int8_maxima_bf16 (M < 2^31, I < 2^22). */
 int bf8_geglu_mxint8(const void* GU, int64_t M, int64_t I, void* H, int8_t* GU8, uint8_t* GU8_exp,
                      void* stream);
 size_t bf8_geglu_bwd_mxint8_maxima(int64_t M, int64_t I);

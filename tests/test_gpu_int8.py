@@ -1124,3 +1124,15 @@ def test_product_of_codes_of_minus_128(gpu):
     y = ops.gemm_int8(a, one[:M], b, one, out_dtype=F32).cpu().double()
     want = torch.where(torch.arange(N) % 2 == 0, 128.0, -127.0).double() * 128 * K
     assert bool(((y - want).abs() <= 2.0 ** -24 * want.abs()).all())
+
+
+def test_gated_gelu_of_the_widest_rows(gpu):
+    """Rows of 2^22 and more, which the forward takes, have their gradient."""
+    I = (1 << 22) + 32
+    g = torch.Generator(device=gpu).manual_seed(0)
+    GU, dH = (torch.randn(1, n, generator=g, device=gpu).to(BF16) for n in (2 * I, I))
+    leaf = GU.clone().requires_grad_()
+    fused_mlp.gated_gelu(leaf, checkpoint=True).backward(dH)
+    assert torch.equal(leaf.grad, ops.geglu_bwd(dH, ops.dequant_mxint8(ops.quantize_mxint8(GU)))[0])
+    with pytest.raises(_lib.Fp8LibError, match="too large"):
+        ops.geglu_bwd_mxint8(dH, ops.quantize_mxint8(GU), rowwise=True)
